@@ -301,12 +301,12 @@ def exact(c, seed):
                 position = torch.arange(lengths[b] - new[b], lengths[b])
                 at, slot = table[b][position // c["page"]].long().to(DEVICE), (position % c["page"]).to(DEVICE)
                 if scales is not None:
-                    top = x.abs().amax(-1)
-                    power = torch.ceil(torch.log2(top / 448))
-                    power = power - (top <= 448 * 2.0 ** (power - 1)).double() + (top > 448 * 2.0 ** power).double()
-                    scale = torch.where(top > 0, 2.0 ** power, 1.0)
+                    powers = torch.tensor([2.0 ** e for e in range(-126, 121)], dtype=torch.float64, device=DEVICE)
+                    top = x.abs().amax(-1)               # the least power with top <= 448 * power; rows of zeros have 1
+                    scale = torch.where(top > 0, powers[torch.searchsorted(448 * powers, top)], 1.0)
                     y = x / scale[..., None]
-                    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+                    power = powers[torch.searchsorted(powers, y.abs().clamp(min=2.0 ** -6), right=True) - 1]
+                    step = power / 8                     # four bits of what lies between two powers, or of the least normal one
                     x = torch.round(y / step) * step     # to the even one of two
                     scales[half][at, slot] = scale
                 pages[half][at, slot] = x
