@@ -53,8 +53,9 @@ extern "C" {
  * 7: mhip_attn_bwd_chunks, mhip_attn_bwd_group.
  * 8: mhip_attn_fwd_blocks takes the number of chunks of a result; mhip_attn_fwd_chain.
  * 9: mhip_attn_bwd_take.
- * 10: mhip_attn_fwd_tile, mhip_attn_bwd_chunks_plan. */
-#define MHIP_ABI_VERSION 10
+ * 10: mhip_attn_fwd_tile, mhip_attn_bwd_chunks_plan.
+ * 11: mhip_paged_cache_write, mhip_paged_cache_read, mhip_paged_attn_workspace_bytes, mhip_paged_attn_fwd. */
+#define MHIP_ABI_VERSION 11
 int         mhip_abi_version(void);   /* the MHIP_ABI_VERSION the library was built with */
 int         mhip_version(void);
 /* Optional: per-device set-up the entry points otherwise do on their first call on a device (today: the address
@@ -330,6 +331,64 @@ int mhip_unpack(const float* buf, void* out, float* lse, int B, int Sq, int Hq, 
  * dst = (acc ? acc : 0) + float(block), n elements, block in bf16; dst may alias acc.
  */
 int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_t n, void* stream);
+
+/*
+ * A paged K/V cache (no counterpart in the reference, whose chunks are dense): the keys and values of many sequences of any
+ * length in pages of page_size rows.  k_cache and v_cache are (pages, page_size, Hkv, D) with the element strides c_sp, c_ss,
+ * c_sh (the same for both, D contiguous, c_ss >= D), MHIP_BF16 or MHIP_E4M3; e4m3 rows have one fp32 scale each, k_scales and
+ * v_scales (pages, page_size, Hkv) with the strides s_sp, s_ss, s_sh, and stand for code * scale (NULL for MHIP_BF16).
+ * Key j of sequence b is row j % page_size of page page_table[b * t_sb + j / page_size]; lengths[b] counts its keys, the new
+ * tokens' among them, which are the last ones.  An entry outside [0, pages) is a page that is not here (freed, not yet given,
+ * or another rank's): nobody sees its keys, rows written to it are dropped, rows read from it are zeros.  New tokens lie in
+ * tensors (B, n, heads, D), or, with `starts` (B + 1 whole numbers that do not fall), packed as (T, heads, D): rows starts[b] up
+ * to starts[b + 1] are sequence b's, rows outside of all of them are neither read nor written.  Without starts T is B * n.
+ * page_table, lengths and starts are DEVICE arrays of int32, read when the kernels run (a captured graph follows them); a length
+ * counts as one from 0 to table_pages * page_size, a start as one from 0 to T.
+ * page_size: a multiple of 16, table_pages * page_size < 2^31, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
+ * multiple of 8 (MHIP_E4M3: of 16) up to 128.  Bases and rows on 16 bytes.
+ */
+
+/*
+ * The new tokens' keys and values (bf16) into their rows of the cache.  MHIP_E4M3: a row x gets the scale s = 2^e, the least
+ * power of two from 2^-126 on with max|x| <= 448 s (1 if all of x is zero), and the codes round-to-nearest-even e4m3fn(x / s); a
+ * row with an infinity or a NaN gets the scale NaN.  Two new tokens of a call must not lie in one row of the cache
+ * (sequences that share the page they write to): which of them stays is not defined.
+ */
+int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+                           const int* page_table, const int* lengths, const int* starts,
+                           int B, int n, int T, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
+                           int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                           int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                           int dtype, void* stream);
+
+/*
+ * Rows begin .. begin + rows - 1 of every sequence as a dense bf16 chunk: out (2, B, rows, Hkv, D), keys and values, element
+ * strides o_half, o_sb, o_ss, o_sh.  Rows past a sequence's end are zeros.  e4m3 rows are rounded once, and what
+ * mhip_paged_cache_write wrote comes back exactly (down to the least numbers of bf16).
+ */
+int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+                          const int* page_table, const int* lengths, void* out,
+                          int B, int begin, int rows, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
+                          int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                          int64_t o_half, int64_t o_sb, int64_t o_ss, int64_t o_sh, int dtype, void* stream);
+
+/*
+ * Attention of the new tokens over the cache, which holds their own keys too: q (bf16), out (bf16) as new tokens with Hq heads,
+ * out = softmax(scale * q k^T) v, lse fp32 (B, Hq, n) contiguous, packed (Hq, T), natural logarithm.  MHIP_MASK_CAUSAL: new token i
+ * of n sees keys j <= lengths[b] - n + i; MHIP_MASK_NONE: all of them.  Rows that see no key get out = 0, lse = -inf, so
+ * results over different pages of a sequence (other entries -1) merge as those of different chunks do.  A key a row does not see has
+ * no part in its result, whatever the cache holds there.  most_new: with starts, about how many new tokens a sequence has at most;
+ * it chooses the form of the kernels, results are right whatever it says.  `workspace`: 16-byte aligned,
+ * mhip_paged_attn_workspace_bytes(most_new or n, Hq, Hkv, D) bytes of device memory; calls that overlap in time need one each.
+ */
+int64_t mhip_paged_attn_workspace_bytes(int most_new, int Hq, int Hkv, int D);
+int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+                        const int* page_table, const int* lengths, const int* starts, void* out, float* lse,
+                        int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
+                        int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                        int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                        int64_t o_sb, int64_t o_ss, int64_t o_sh,
+                        float softmax_scale, int mask, int dtype, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

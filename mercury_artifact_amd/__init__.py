@@ -15,6 +15,7 @@ from .lazy import LazyLse, LazyOut, update_out_and_lse_lazy
 from .merge import (LocalGroup, _update_out_and_lse, add_collective, flash_reduce, get_default_args,
                     grad_accumulate, merge_into, merge_many, pack_block, unpack_into, update_out_and_lse,
                     update_out_and_lse_collective)
+from .paged import paged_attn_fwd, paged_cache, paged_cache_read, paged_cache_write
 from .ring import (flash_attn_backward, flash_attn_expose_reduce, flash_attn_expose_reduce_q_ring,
                    flash_attn_pack_kv,
                    flash_attn_pack_split_kv, fp8_pack_split_kv, gqa_pack_kv, quantize_e4m3,

@@ -19,7 +19,7 @@ import torch
 # MERCURY_HIP_LIB is a deployment option: the path of the built library when it is not kept next to the package.
 _BUILT = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("MERCURY_HIP_LIB") or os.path.join(_BUILT, "libmercury_hip.so")
-ABI_VERSION = 10     # MHIP_ABI_VERSION of include/mercury_hip.h the signatures below were written against
+ABI_VERSION = 11     # MHIP_ABI_VERSION of include/mercury_hip.h the signatures below were written against
 
 
 class _NoHost:
@@ -84,6 +84,10 @@ _SIGNATURES = {
     "mhip_unpack": (c_int, [_P] * 3 + [_I] * 4 + [_P]),
     "mhip_grad_accumulate": (c_int, [_P] * 3 + [_L, _P]),
     "mhip_quantize_e4m3": (c_int, [_P, _I, _L, _P, _P, _P, _P]),
+    "mhip_paged_cache_write": (c_int, [_P] * 9 + [_I] * 8 + [_L] * 13 + [_I, _P]),
+    "mhip_paged_cache_read": (c_int, [_P] * 7 + [_I] * 8 + [_L] * 11 + [_I, _P]),
+    "mhip_paged_attn_workspace_bytes": (c_int64, [_I] * 4),
+    "mhip_paged_attn_fwd": (c_int, [_P] * 10 + [_I] * 10 + [_L] * 13 + [_F, _I, _I, _P, _P]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

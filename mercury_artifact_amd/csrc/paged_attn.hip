@@ -1,0 +1,596 @@
+// Attention of new tokens over a paged K/V cache: out = softmax(scale * q k^T) v and lse, keys and values read where they lie.
+//
+// The query heads that share a K/V head and the new tokens of a sequence are the rows of one product, so that a key is read
+// once for all of them: rows r = token * G + head of the group.
+//
+// paged_attn_few: bound by memory (each byte of the cache feeds as many multiply-adds as there are rows).
+//   work       : a unit is 128 keys of one (sequence, K/V head, tile of rows).  The units of all sequences, counted by every
+//                workgroup from the lengths in device memory, are dealt out evenly and in order to one workgroup per CU: a
+//                long sequence beside short ones, or alone, keeps all CUs reading, without the host knowing a length.  A
+//                workgroup whose share ends inside an item leaves a partial result, and paged_attn_join adds those up.
+//   wavefront  : every fourth tile of 32 keys is its own, in a ring of 32 KB of LDS filled by copies that do not pass through
+//                registers (buffer_load ... lds): no barrier in the loop, and 64 to 128 KB in flight on a CU, where 25 bytes
+//                a nanosecond times the latency of a microsecond asks for 25 KB.
+//   S^T = K Q^T: v_mfma_f32_16x16x32_bf16 with A = K rows from LDS and B = Q rows in registers: lane (ln, lg) then holds
+//                keys 4 lg .. +3 of both halves of a tile for row ln, softmax is lane-local but for two exchanges.
+//   O^T = V^T P^T: the same lane's P is the B operand, and the transposing LDS reads fetch V^T in its key order.
+//   e4m3       : codes are exact in bf16 (v_cvt_scalef32_pk_bf16_fp8); a key's scale multiplies its score, a value's scale
+//                its weight, in fp32.  Rounding P to bf16 (2^-9 of each weight at most) is the only rounding before the last.
+#include "paged.hpp"
+
+#include <math.h>
+
+namespace mhip {
+namespace {
+
+typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i32x2;
+
+constexpr int kWaves = 4;
+constexpr int kKeys = 32;                  // keys of a tile, one wavefront's
+constexpr int kUnit = kWaves * kKeys;      // and of a unit of work
+constexpr int kRing = 32768;               // bytes of K and V tiles of a wavefront
+constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
+constexpr int kWorkgroups = 256;           // one per CU
+
+struct AttnParams {
+  PagedGeom g;
+  const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
+  int64_t c_sp, c_ss, c_sh;                // of the cache, bytes
+  int64_t s_sp, s_ss, s_sh;                // of the scales, elements
+  const uint16_t* q; uint16_t* out; float* lse;
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, l_sb, l_sh;
+  int Hq, Hkv, G, D, causal;
+  float scale_log2;
+  Divisor by_group, by_heads, by_new;
+  float* part_o; f32x2* part_ml;           // partial results: two slots of each workgroup
+};
+
+struct Item { int rts; int64_t steps; };   // row tiles of a sequence and K/V head, units of each
+template <int ROWS>
+__device__ __forceinline__ Item item_of(const AttnParams& p, const PagedSeq& s) {
+  Item it;
+  it.rts = (s.n * p.G + ROWS - 1) / ROWS;
+  it.steps = s.len > kUnit ? (s.len + kUnit - 1) / kUnit : 1;
+  return it;
+}
+template <int ROWS, bool UNIFORM>
+__device__ __forceinline__ int64_t units_of(const AttnParams& p, int b) {
+  const Item it = item_of<ROWS>(p, paged_seq<UNIFORM>(p.g, b));
+  return it.steps * it.rts * p.Hkv;
+}
+
+// The units before each lane's run of sequences, and of all of them.
+struct Plan {
+  int per;                   // sequences of a lane
+  int64_t before, mine, total;
+};
+template <int ROWS>
+__device__ __forceinline__ Plan plan_of(const AttnParams& p, int lane) {
+  Plan plan;
+  plan.per = (p.g.B + 63) / 64;
+  plan.mine = 0;
+  for (int j = 0; j < plan.per; ++j)
+    if (lane * plan.per + j < p.g.B) plan.mine += units_of<ROWS, false>(p, lane * plan.per + j);
+  int64_t sum = plan.mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t below = __shfl_up((long long)sum, off);
+    if (lane >= off) sum += below;
+  }
+  plan.before = sum - plan.mine;
+  plan.total = __shfl((long long)sum, 63);
+  return plan;
+}
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+template <int ROWB>
+__device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks of LDS rows of ROWB bytes
+  return ROWB == 256 ? lds_row_swizzle_16(row) : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+template <bool E4M3, int COLS, int NR>
+__global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParams p) {
+  constexpr int ROWS = 16 * NR;
+  constexpr int kSize = E4M3 ? 1 : 2;
+  constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
+  constexpr int kChunks = ROWB / 16;
+  constexpr int kCopyRows = 1024 / ROWB;               // rows of one copy instruction
+  constexpr int kCopies = 16 / kCopyRows;              // and instructions of half a tile
+  constexpr int kTileBytes = kKeys * ROWB;
+  constexpr int kStages = kRing / (2 * kTileBytes);
+  constexpr int kStage = 2 * kTileBytes + (E4M3 ? 256 : 0);      // K, V, 32 scales of each
+  constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
+  constexpr int KB = COLS / 32, DB = COLS / 16;
+  constexpr int kRegion = kStages * kStage;
+  static_assert(ROWS * COLS * 4 <= kRegion, "a wavefront's O takes the place of its ring");
+  static_assert(kStages * (nK + nV) < 64, "copies in flight are counted in 6 bits");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kWaves * kRegion];
+  __shared__ f32x2 stats[kWaves][ROWS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+
+  // ---- this workgroup's share ------------------------------------------------------------------------------
+  // (workgroups of one XCD take neighbouring shares)
+  const int w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const Plan plan = plan_of<ROWS>(p, lane);
+  const int64_t total = uniform64(plan.total);
+  const int64_t shares = total < (int64_t)gridDim.x ? total : gridDim.x;
+  if (w >= shares) return;
+  int64_t lo = total * w / shares;
+  const int64_t hi = total * (w + 1) / shares;
+  const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= plan.before && lo < plan.before + plan.mine));
+  int b = owner * plan.per;
+  int64_t pos = lo - uniform64(__shfl((long long)plan.before, owner));     // inside sequence b
+  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<ROWS, true>(p, b)); ++b) pos -= u;
+
+  // ---- what does not change from segment to segment -----------------------------------------------------------
+  const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const uint32_t ring = lds_smem + wave * kRegion;
+  int voff[kCopies];
+#pragma unroll
+  for (int u = 0; u < kCopies; ++u) {
+    const int row = u * kCopyRows + lane / kChunks, chunk = (lane % kChunks) ^ swizzle<ROWB>(row);
+    voff[u] = chunk * 16 < p.D * kSize ? (int)(row * p.c_ss) + chunk * 16 : kNoColumn;
+  }
+  // K operand: 16 bytes of row ln; in e4m3 they serve two k-steps of 32 columns
+  constexpr int KR = E4M3 ? KB / 2 : KB;               // 16-byte reads of a K row
+  int k_a[KR];
+#pragma unroll
+  for (int i = 0; i < KR; ++i) k_a[i] = (int)ring + ln * ROWB + (((4 * i + lg) ^ swizzle<ROWB>(ln)) << 4);
+  // V^T operand: keys 4 lg .. +3 of both halves of the tile, one column of a strip of 16 per lane.  bf16: within 16 lanes lane s
+  // supplies the address of columns 4 (s % 4) .. +3 of row s / 4 and receives column s; e4m3: of columns 8 (s % 2) .. +7 of row s / 2.
+  int v_a[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    if (E4M3) {
+      const int r8 = ln >> 1, row = (r8 & 3) + 4 * lg + 16 * (r8 >> 2);
+      v_a[db] = (int)ring + kTileBytes + row * ROWB + ((db ^ swizzle<ROWB>(row & 15)) << 4) + (ln & 1) * 8;
+    } else {
+      const int row = 4 * lg + (ln >> 2);
+      v_a[db] = (int)ring + kTileBytes + row * ROWB + (((2 * db + ((ln & 3) >> 1)) ^ swizzle<ROWB>(row)) << 4) + (ln & 1) * 8;
+    }
+  }
+  typedef __attribute__((address_space(3))) bf16x4* lds_bf16x4;
+  typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
+  typedef __attribute__((address_space(3))) const u32x4* lds_u32x4;
+  typedef __attribute__((address_space(3))) const f32x4* lds_f32x4;
+  auto codes_to_bf16 = [](uint32_t a, uint32_t c) -> bf16x8 {
+    const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
+    const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true);
+    return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+  };
+  auto read_v = [&](int db, int stage_at) -> bf16x8 {
+    if constexpr (E4M3) {
+      const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(uintptr_t)(uint32_t)(v_a[db] + stage_at));
+      return codes_to_bf16((uint32_t)c[0], (uint32_t)c[1]);
+    } else {
+      const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + stage_at));
+      const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + stage_at + 16 * ROWB));
+      return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  auto mfma = [](const bf16x8& x, const bf16x8& y, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); };
+
+  for (;;) {
+    const PagedSeq s = paged_seq<true>(p.g, b);
+    const Item it = item_of<ROWS>(p, s);
+    const int64_t item = pos / it.steps;
+    const int first = (int)(pos - item * it.steps);
+    const int64_t left = hi - lo;
+    const int count = (int)(it.steps - first < left ? it.steps - first : left);
+    const int hk = (int)(item / it.rts), rt = (int)(item - (int64_t)hk * it.rts);
+    const int row0 = rt * ROWS;
+    const int rows = s.n * p.G - row0 < ROWS ? s.n * p.G - row0 : ROWS;
+
+    // ---- Q rows: B operand of S^T, lane (ln, lg) holds 8 columns of row ln, in the order of the K operand's ----------
+    bf16x8 qf[NR][KB];
+    int lim[NR];                                       // keys that the row sees
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = r * 16 + ln;
+      int of_group;
+      const int token = p.by_group.quotient(row0 + (row < rows ? row : 0), of_group);
+      const uint16_t* src = p.q + b * p.q_sb + (int64_t)(s.start + token) * p.q_ss + (hk * p.G + of_group) * p.q_sh;
+      lim[r] = p.causal ? clamped(s.len - s.n + token + 1, 0, s.len) : s.len;
+#pragma unroll
+      for (int ks = 0; ks < KB; ++ks) {
+        const int col = E4M3 ? (ks >> 1) * 64 + lg * 16 + (ks & 1) * 8 : ks * 32 + lg * 8;
+        qf[r][ks] = bf16x8{};
+        if (row < rows && col < p.D) qf[r][ks] = *reinterpret_cast<const bf16x8*>(src + col);
+      }
+    }
+    // keys that all rows see, and that some row sees
+    const int seen_first = p.causal ? clamped(s.len - s.n + p.by_group.quotient(row0) + 1, 0, s.len) : s.len;
+    const int seen_last = p.causal ? clamped(s.len - s.n + p.by_group.quotient(row0 + rows - 1) + 1, 0, s.len) : s.len;
+
+    // ---- copies of tile t of this wavefront, 16 keys (of one page) at a time -----------------------------------------
+    const int* table = p.g.table + b * p.g.t_sb;
+    auto key_of = [&](int t) { return ((first + t) * kWaves + wave) * kKeys; };
+    int page[2], slot[2], held[2];                     // of the tile whose copies go out next
+    auto look_up = [&](int t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = key_of(t) + 16 * h;
+        held[h] = t < count ? clamped(seen_last - key, 0, 16) : 0;
+        page[h] = -1;
+        slot[h] = 0;
+        if (held[h] > 0) page[h] = uniform_load(table, p.g.by_page.quotient(key, slot[h]));
+      }
+    };
+    uint32_t gone = 0;                                 // two bits of each stage: that half of its tile is not here
+    auto settle = [&](int stage) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool here = page[h] >= 0 && page[h] < p.g.pages;
+        if (!here) held[h] = 0;
+        gone = (gone & ~(1u << (2 * stage + h))) | (here ? 0u : 1u << (2 * stage + h));
+      }
+    };
+    auto copy = [&](const uint8_t* base, int at) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* from = base + (held[h] > 0 ? page[h] * p.c_sp + slot[h] * p.c_ss + hk * p.c_sh : 0);
+        const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * p.c_ss + p.D * kSize) : 0u);
+#pragma unroll
+        for (int u = 0; u < kCopies; ++u) copy16_to_lds(rs, ring + at + h * 16 * ROWB + u * 1024, voff[u], 0);
+      }
+    };
+    auto copy_k = [&](int stage) {
+      if constexpr (E4M3) {
+        const int h = (lane >> 4) & 1, row = ln < held[h] ? ln : held[h] - 1;
+        const float* at = (lane >> 5 ? p.v_scales : p.k_scales) + (page[h] * p.s_sp + (slot[h] + row) * p.s_ss + hk * p.s_sh);
+        copy4_to_lds(held[h] > 0 ? static_cast<const void*>(at) : p.q, ring + stage * kStage + 2 * kTileBytes);
+      }
+      copy(p.k, stage * kStage);
+    };
+    auto copy_v = [&](int stage) { copy(p.v, stage * kStage + kTileBytes); };
+
+    f32x4 o[DB][NR];
+    float m[NR], l[NR];                                // maximum (times scale * log2 e), this lane's share of the sum
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db][r] = f32x4{};
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(qf[r][ks]));      // loaded before the first copy goes out
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < kStages; ++t) {
+      look_up(t);
+      settle(t);
+      copy_k(t);
+      copy_v(t);
+    }
+    look_up(kStages);
+
+    for (int t = 0; t < count; ++t) {
+      const int stage = t % kStages, at = stage * kStage, key0 = key_of(t);
+      const uint32_t hidden = gone >> (2 * stage) & 3u;
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(nV + (kStages - 1) * (nK + nV)) : "memory");     // K of tile t is there
+      f32x4 sc[2][NR];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+          const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
+#pragma unroll
+          for (int e = 0; e < KB / KR; ++e) {
+            const bf16x8 kf = E4M3 ? codes_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
+            const int ks = E4M3 ? 2 * i + e : i;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) sc[kb][r] = mfma(kf, qf[r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
+          }
+        }
+      f32x4 k_scale[2], v_scale[2];
+      if constexpr (E4M3)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          k_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + kb * 64 + lg * 16);
+          v_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + 128 + kb * 64 + lg * 16);
+          asm volatile("" : "+v"(k_scale[kb]), "+v"(v_scale[kb]));
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the tile has been read: its place can be filled
+      settle(stage);
+      copy_k(stage);
+
+      // ---- softmax --------------------------------------------------------------------------------------------
+      const bool cut = key0 + kKeys > seen_first;                // some row does not see some key
+      u32x4 pw[NR], seen[NR];
+      bool moved = false;
+      float alpha[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[kb][r][j] *= E4M3 ? p.scale_log2 * k_scale[kb][j] : p.scale_log2;
+        if (cut || hidden) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (key0 + 16 * kb + 4 * lg + j >= lim[r] || (hidden >> kb & 1)) sc[kb][r][j] = -INFINITY;
+        }
+        float top = sc[0][r][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[kb][r][j]);
+        top = fmaxf(quad_max(top), m[r]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        alpha[r] = fast_exp2(m[r] - ref);
+        moved = moved || !(m[r] == top);
+        m[r] = top;
+        float x[8], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = fast_exp2(sc[i >> 2][r][i & 3] - ref);
+          sum += x[i];
+        }
+        l[r] = l[r] * alpha[r] + sum;
+        if constexpr (E4M3)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+      }
+      if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db][r] *= alpha[r];
+      }
+
+      // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(nK + (kStages - 1) * (nK + nV)) : "memory");     // V of tile t is there
+      if (!(cut && seen_first < seen_last)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const bf16x8 vf = read_v(db, at);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
+        }
+      } else {
+        // A value that is no number, seen by some rows only: zero in the product, and counted for the rows that see it in
+        // products of their own (+inf, -inf and NaN), since 0 * NaN would reach the others.
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            seen[r][i] = (sc[i >> 1][r][2 * (i & 1)] == -INFINITY ? 0u : 0x3f80u) | (sc[i >> 1][r][2 * (i & 1) + 1] == -INFINITY ? 0u : 0x3f800000u);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u32x4 vf = __builtin_bit_cast(u32x4, read_v(db, at));
+          u32x4 fine, up, down, none;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            fine[i] = up[i] = down[i] = none[i] = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t x = vf[i] >> (16 * h) & 0xffffu, one = 0x3f80u << (16 * h);
+              if ((x & 0x7f80u) != 0x7f80u) fine[i] |= x << (16 * h);
+              else if (x == 0x7f80u) up[i] |= one;
+              else if (x == 0xff80u) down[i] |= one;
+              else none[i] |= one;
+            }
+          }
+          const bool odd = ((up[0] | up[1] | up[2] | up[3]) | (down[0] | down[1] | down[2] | down[3]) | (none[0] | none[1] | none[2] | none[3])) != 0;
+          const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            o[db][r] = mfma(__builtin_bit_cast(bf16x8, fine), __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
+            if (any) {
+              const bf16x8 of = __builtin_bit_cast(bf16x8, seen[r]);
+              const f32x4 u = mfma(__builtin_bit_cast(bf16x8, up), of, f32x4{}), d = mfma(__builtin_bit_cast(bf16x8, down), of, f32x4{});
+              const f32x4 n = mfma(__builtin_bit_cast(bf16x8, none), of, f32x4{});
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (u[j] > 0.f) o[db][r][j] += INFINITY;
+                if (d[j] > 0.f) o[db][r][j] -= INFINITY;
+                if (n[j] > 0.f) o[db][r][j] = __builtin_nanf("");
+              }
+            }
+          }
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      copy_v(stage);
+      look_up(t + kStages + 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // copies past the last tile
+
+    // ---- the wavefronts' shares meet -------------------------------------------------------------------------------
+    unsigned char* region = smem + wave * kRegion;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float sum = quad_sum(l[r]);
+      if (lg == 0) stats[wave][r * 16 + ln] = f32x2{m[r], sum};
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        *reinterpret_cast<f32x4*>(region + (r * 16 + ln) * (COLS * 4) + (((db * 4 + lg) ^ ln) << 4)) = o[db][r];
+    }
+    __syncthreads();
+    const bool whole = count == it.steps;
+    const int64_t slot_of = 2 * (int64_t)w + (first == 0 ? 1 : 0);
+#pragma unroll
+    for (int i = 0; i < ROWS * COLS / 4 / (kWaves * 64); ++i) {
+      const int unit = i * (kWaves * 64) + threadIdx.x;
+      const int row = unit / (COLS / 4), c4 = unit % (COLS / 4);
+      if (row >= rows) continue;
+      f32x2 st[kWaves];
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) {
+        st[v] = stats[v][row];
+        top = fmaxf(top, st[v][0]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 acc{};
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) {
+        const float weight = fast_exp2(st[v][0] - ref);
+        sum += st[v][1] * weight;
+        acc += *reinterpret_cast<const f32x4*>(smem + v * kRegion + row * (COLS * 4) + ((c4 ^ (row & 15)) << 4)) * weight;
+      }
+      if (whole) {
+        int of_group;
+        const int token = s.start + p.by_group.quotient(row0 + row, of_group), head = hk * p.G + of_group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (c4 * 4 < p.D)
+          *reinterpret_cast<u32x2*>(p.out + b * p.o_sb + token * p.o_ss + head * p.o_sh + c4 * 4) =
+              u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+        if (c4 == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+      } else {
+        *reinterpret_cast<f32x4*>(p.part_o + (slot_of * ROWS + row) * COLS + c4 * 4) = acc;
+        if (c4 == 0) p.part_ml[slot_of * ROWS + row] = f32x2{top, sum};
+      }
+    }
+
+    lo += count;
+    pos += count;
+    if (lo >= hi) break;
+    if (pos >= it.steps * it.rts * p.Hkv) {
+      pos = 0;
+      for (++b; b + 1 < p.g.B && units_of<ROWS, true>(p, b) == 0;) ++b;
+    }
+    __syncthreads();
+  }
+}
+
+// The partial results of every row whose item several workgroups shared: one wavefront a row, two columns a lane.
+template <int COLS, int ROWS>
+__global__ __launch_bounds__(256) void paged_attn_join(const AttnParams p, int64_t n_rows, int workgroups) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= n_rows) return;
+  int head, i = 0, b;
+  const int t = __builtin_amdgcn_readfirstlane(p.by_heads.quotient((int)id, head));
+  head = __builtin_amdgcn_readfirstlane(head);
+  if (p.g.starts) b = paged_owner<64>(p.g, t, lane);
+  else b = p.by_new.quotient(t, i);
+  b = __builtin_amdgcn_readfirstlane(b);
+  if (b >= p.g.B) return;
+  const PagedSeq s = paged_seq<true>(p.g, b);
+  if (p.g.starts) i = t - s.start;
+  if (i < 0 || i >= s.n) return;
+  const Plan plan = plan_of<ROWS>(p, lane);
+  const int64_t total = uniform64(plan.total);
+  int64_t before = uniform64(__shfl((long long)plan.before, b / plan.per));
+  for (int c = b / plan.per * plan.per; c < b; ++c) before += units_of<ROWS, true>(p, c);
+  const Item it = item_of<ROWS>(p, s);
+  int of_group;
+  const int hk = p.by_group.quotient(head, of_group);
+  const int r = i * p.G + of_group, rt = r / ROWS, row = r % ROWS;
+  const int64_t u0 = before + ((int64_t)hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
+  const int64_t shares = total < workgroups ? total : workgroups;
+  const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
+  if (w0 == w1) return;                                // one workgroup had all of it
+  auto slot_row = [&](int w) { return (2 * (int64_t)w + (w == w0 ? 1 : 0)) * ROWS + row; };
+  float top = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, p.part_ml[slot_row(w)][0]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float ref = top == -INFINITY ? 0.f : top;
+  const int col = lane * 2;
+  float sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) {
+    const f32x2 ml = p.part_ml[slot_row(w)];
+    const float weight = fast_exp2(ml[0] - ref);
+    sum += ml[1] * weight;
+    if (col < COLS) {
+      const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_o + slot_row(w) * COLS + col);
+      a0 += x[0] * weight;
+      a1 += x[1] * weight;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int token = s.start + i;
+  if (col < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
+  if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+}
+
+// Tiles of 16, 32 or 64 rows: the least that holds the rows of a sequence with `most` new tokens.
+int row_blocks(int G, int64_t most) { return G * most <= 16 ? 1 : G * most <= 32 ? 2 : 4; }
+
+template <bool E4M3, int COLS, int NR>
+void launch_few(const AttnParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR>), dim3(kWorkgroups), dim3(kWaves * 64), 0, st, p);
+  const int64_t n_rows = (int64_t)p.g.T * p.Hq;
+  hipLaunchKernelGGL((paged_attn_join<COLS, 16 * NR>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p, n_rows, kWorkgroups);
+}
+template <bool E4M3, int COLS>
+void launch_rows(const AttnParams& p, int blocks, hipStream_t st) {
+  if (blocks == 1) launch_few<E4M3, COLS, 1>(p, st);
+  else if (blocks == 2) launch_few<E4M3, COLS, 2>(p, st);
+  else launch_few<E4M3, COLS, 4>(p, st);
+}
+
+}  // namespace
+}  // namespace mhip
+
+using namespace mhip;
+
+extern "C" int64_t mhip_paged_attn_workspace_bytes(int most_new, int Hq, int Hkv, int D) {
+  if (most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
+  if (D <= 0 || D > 128) return MHIP_EHEADDIM;
+  const int64_t rows = 16 * row_blocks(Hq / Hkv, most_new);
+  return 2 * kWorkgroups * rows * ((D <= 64 ? 64 : 128) + 2) * 4;
+}
+
+extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+                                   const int* page_table, const int* lengths, const int* starts, void* out, float* lse,
+                                   int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
+                                   int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                                   int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                                   int64_t o_sb, int64_t o_ss, int64_t o_sh,
+                                   float softmax_scale, int mask, int dtype, void* workspace, void* stream) {
+  AttnParams p{};
+  if (B < 0 || n < 0 || T < 0 || most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
+  if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) return MHIP_EINVAL;
+  if (mask != MHIP_MASK_NONE && mask != MHIP_MASK_CAUSAL) return MHIP_EINVAL;
+  if (!starts && (int64_t)B * n > 0x7fffffff) return MHIP_EUNSUPPORTED;
+  if (!starts) { T = B * n; most_new = n; }
+  if (int code = paged_geometry(p.g, page_table, lengths, starts, t_sb, B, n, T, pages, page_size, table_pages)) return code;
+  if (int code = paged_cache_fits(k_cache, v_cache, k_scales, v_scales, pages, Hkv, D, c_sp, c_ss, c_sh, dtype)) return code;
+  if (T == 0 || B == 0) return MHIP_OK;
+  if (!q || !out || !lse || !workspace) return MHIP_EINVAL;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3u)) return MHIP_EALIGN;
+  for (int64_t s : {q_sb, q_ss, q_sh, o_sb, o_ss, o_sh})
+    if (s % 8 != 0) return MHIP_EALIGN;
+  if ((int64_t)T * Hq >= (int64_t(1) << 31) - 64) return MHIP_EUNSUPPORTED;
+  const int size = dtype == MHIP_E4M3 ? 1 : 2;
+  p.k = static_cast<const uint8_t*>(k_cache); p.v = static_cast<const uint8_t*>(v_cache);
+  p.k_scales = k_scales; p.v_scales = v_scales;
+  p.c_sp = c_sp * size; p.c_ss = c_ss * size; p.c_sh = c_sh * size;
+  p.s_sp = s_sp; p.s_ss = s_ss; p.s_sh = s_sh;
+  p.q = static_cast<const uint16_t*>(q); p.out = static_cast<uint16_t*>(out); p.lse = lse;
+  p.q_sb = starts ? 0 : q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
+  p.o_sb = starts ? 0 : o_sb; p.o_ss = o_ss; p.o_sh = o_sh;
+  p.l_sb = starts ? 0 : (int64_t)Hq * n; p.l_sh = starts ? T : n;
+  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D;
+  p.causal = mask == MHIP_MASK_CAUSAL;
+  p.scale_log2 = softmax_scale * kLog2e;
+  p.by_group = Divisor(p.G); p.by_heads = Divisor(Hq); p.by_new = Divisor(n);
+  const int blocks = row_blocks(p.G, most_new);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)kWorkgroups * 16 * blocks * (D <= 64 ? 64 : 128));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == MHIP_E4M3) {
+    if (D <= 64) launch_rows<true, 64>(p, blocks, st);
+    else launch_rows<true, 128>(p, blocks, st);
+  } else {
+    if (D <= 64) launch_rows<false, 64>(p, blocks, st);
+    else launch_rows<false, 128>(p, blocks, st);
+  }
+  return launch_status();
+}
