@@ -13,7 +13,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.hip", "attn_fwd.hip", "attn_fwd_fp8.hip", "attn_bwd.hip", "lse_merge.hip", "quantize.hip",
-           "paged_cache.hip", "paged_attn.hip"]
+           "paged_cache.hip", "paged_attn.hip", "paged_attn_chunk.hip"]
 LIB = os.path.join(HERE, "libmercury_hip.so")
 HOST = os.path.join(HERE, "_mercury_host.so")
 # -packed-fp32-ops off: keep the compiler from forming v_pk_{add,mul,fma}_f32.

@@ -16,9 +16,7 @@
 //   O^T = V^T P^T: the same lane's P is the B operand, and the transposing LDS reads fetch V^T in its key order.
 //   e4m3       : codes are exact in bf16 (v_cvt_scalef32_pk_bf16_fp8); a key's scale multiplies its score, a value's scale
 //                its weight, in fp32.  Rounding P to bf16 (2^-9 of each weight at most) is the only rounding before the last.
-#include "paged.hpp"
-
-#include <math.h>
+#include "paged_attn.hpp"
 
 namespace mhip {
 namespace {
@@ -31,30 +29,18 @@ constexpr int kUnit = kWaves * kKeys;      // and of a unit of work
 constexpr int kRing = 32768;               // bytes of K and V tiles of a wavefront
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
 constexpr int kWorkgroups = 256;           // one per CU
-
-struct AttnParams {
-  PagedGeom g;
-  const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
-  int64_t c_sp, c_ss, c_sh;                // of the cache, bytes
-  int64_t s_sp, s_ss, s_sh;                // of the scales, elements
-  const uint16_t* q; uint16_t* out; float* lse;
-  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, l_sb, l_sh;
-  int Hq, Hkv, G, D, causal;
-  float scale_log2;
-  Divisor by_group, by_heads, by_new;
-  float* part_o; f32x2* part_ml;           // partial results: two slots of each workgroup
-};
+constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
 struct Item { int rts; int64_t steps; };   // row tiles of a sequence and K/V head, units of each
 template <int ROWS>
-__device__ __forceinline__ Item item_of(const AttnParams& p, const PagedSeq& s) {
+__device__ __forceinline__ Item item_of(const PagedAttn& p, const PagedSeq& s) {
   Item it;
-  it.rts = (s.n * p.G + ROWS - 1) / ROWS;
+  it.rts = s.n * p.G <= p.few_rows ? (s.n * p.G + ROWS - 1) / ROWS : 0;
   it.steps = s.len > kUnit ? (s.len + kUnit - 1) / kUnit : 1;
   return it;
 }
 template <int ROWS, bool UNIFORM>
-__device__ __forceinline__ int64_t units_of(const AttnParams& p, int b) {
+__device__ __forceinline__ int64_t units_of(const PagedAttn& p, int b) {
   const Item it = item_of<ROWS>(p, paged_seq<UNIFORM>(p.g, b));
   return it.steps * it.rts * p.Hkv;
 }
@@ -65,7 +51,7 @@ struct Plan {
   int64_t before, mine, total;
 };
 template <int ROWS>
-__device__ __forceinline__ Plan plan_of(const AttnParams& p, int lane) {
+__device__ __forceinline__ Plan plan_of(const PagedAttn& p, int lane) {
   Plan plan;
   plan.per = (p.g.B + 63) / 64;
   plan.mine = 0;
@@ -81,18 +67,13 @@ __device__ __forceinline__ Plan plan_of(const AttnParams& p, int lane) {
   plan.total = __shfl((long long)sum, 63);
   return plan;
 }
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
-}
-
 template <int ROWB>
 __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks of LDS rows of ROWB bytes
   return ROWB == 256 ? lds_row_swizzle_16(row) : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
 template <bool E4M3, int COLS, int NR>
-__global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParams p) {
+__global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn p) {
   constexpr int ROWS = 16 * NR;
   constexpr int kSize = E4M3 ? 1 : 2;
   constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
@@ -304,7 +285,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParam
 
       // ---- softmax --------------------------------------------------------------------------------------------
       const bool cut = key0 + kKeys > seen_first;                // some row does not see some key
-      u32x4 pw[NR], seen[NR];
+      u32x4 pw[NR];
       bool moved = false;
       float alpha[NR];
 #pragma unroll
@@ -360,45 +341,26 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParam
           for (int r = 0; r < NR; ++r) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
         }
       } else {
-        // A value that is no number, seen by some rows only: zero in the product, and counted for the rows that see it in
-        // products of their own (+inf, -inf and NaN), since 0 * NaN would reach the others.
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            seen[r][i] = (sc[i >> 1][r][2 * (i & 1)] == -INFINITY ? 0u : 0x3f80u) | (sc[i >> 1][r][2 * (i & 1) + 1] == -INFINITY ? 0u : 0x3f800000u);
+        // (some rows do not see some of the keys: see finite_part)
+        uint32_t odd = 0;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const u32x4 vf = __builtin_bit_cast(u32x4, read_v(db, at));
-          u32x4 fine, up, down, none;
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, finite_part(__builtin_bit_cast(u32x4, read_v(db, at)), odd));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            fine[i] = up[i] = down[i] = none[i] = 0;
+          for (int r = 0; r < NR; ++r) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t x = vf[i] >> (16 * h) & 0xffffu, one = 0x3f80u << (16 * h);
-              if ((x & 0x7f80u) != 0x7f80u) fine[i] |= x << (16 * h);
-              else if (x == 0x7f80u) up[i] |= one;
-              else if (x == 0xff80u) down[i] |= one;
-              else none[i] |= one;
+          for (int db = 0; db < DB; ++db) {
+            const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, at))));
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              const f32x4 counts = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[r])), f32x4{});
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[db][r][j] = with_odd(o[db][r][j], counts[j]);
             }
-          }
-          const bool odd = ((up[0] | up[1] | up[2] | up[3]) | (down[0] | down[1] | down[2] | down[3]) | (none[0] | none[1] | none[2] | none[3])) != 0;
-          const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            o[db][r] = mfma(__builtin_bit_cast(bf16x8, fine), __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
-            if (any) {
-              const bf16x8 of = __builtin_bit_cast(bf16x8, seen[r]);
-              const f32x4 u = mfma(__builtin_bit_cast(bf16x8, up), of, f32x4{}), d = mfma(__builtin_bit_cast(bf16x8, down), of, f32x4{});
-              const f32x4 n = mfma(__builtin_bit_cast(bf16x8, none), of, f32x4{});
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (u[j] > 0.f) o[db][r][j] += INFINITY;
-                if (d[j] > 0.f) o[db][r][j] -= INFINITY;
-                if (n[j] > 0.f) o[db][r][j] = __builtin_nanf("");
-              }
-            }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
@@ -446,7 +408,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParam
         const int token = s.start + p.by_group.quotient(row0 + row, of_group), head = hk * p.G + of_group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         if (c4 * 4 < p.D)
-          *reinterpret_cast<u32x2*>(p.out + b * p.o_sb + token * p.o_ss + head * p.o_sh + c4 * 4) =
+          *reinterpret_cast<u32x2*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + c4 * 4) =
               u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
         if (c4 == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
       } else {
@@ -466,73 +428,52 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const AttnParam
   }
 }
 
-// The partial results of every row whose item several workgroups shared: one wavefront a row, two columns a lane.
+// The rows that several workgroups shared, a wavefront each.
 template <int COLS, int ROWS>
-__global__ __launch_bounds__(256) void paged_attn_join(const AttnParams p, int64_t n_rows, int workgroups) {
+__global__ __launch_bounds__(256) void paged_attn_few_join(const PagedAttn p, int64_t n_rows, int workgroups) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= n_rows) return;
-  int head, i = 0, b;
-  const int t = __builtin_amdgcn_readfirstlane(p.by_heads.quotient((int)id, head));
-  head = __builtin_amdgcn_readfirstlane(head);
-  if (p.g.starts) b = paged_owner<64>(p.g, t, lane);
-  else b = p.by_new.quotient(t, i);
-  b = __builtin_amdgcn_readfirstlane(b);
-  if (b >= p.g.B) return;
-  const PagedSeq s = paged_seq<true>(p.g, b);
-  if (p.g.starts) i = t - s.start;
-  if (i < 0 || i >= s.n) return;
+  RowOf x;
+  if (id >= n_rows || !row_of(p, (int)id, lane, x) || x.s.n * p.G > p.few_rows) return;
+  const int rt = x.r / ROWS, row = x.r % ROWS;
   const Plan plan = plan_of<ROWS>(p, lane);
   const int64_t total = uniform64(plan.total);
-  int64_t before = uniform64(__shfl((long long)plan.before, b / plan.per));
-  for (int c = b / plan.per * plan.per; c < b; ++c) before += units_of<ROWS, true>(p, c);
-  const Item it = item_of<ROWS>(p, s);
-  int of_group;
-  const int hk = p.by_group.quotient(head, of_group);
-  const int r = i * p.G + of_group, rt = r / ROWS, row = r % ROWS;
-  const int64_t u0 = before + ((int64_t)hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
+  int64_t before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
+  for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, true>(p, c);
+  const Item it = item_of<ROWS>(p, x.s);
+  const int64_t u0 = before + ((int64_t)x.hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
   const int64_t shares = total < workgroups ? total : workgroups;
   const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
   if (w0 == w1) return;                                // one workgroup had all of it
-  auto slot_row = [&](int w) { return (2 * (int64_t)w + (w == w0 ? 1 : 0)) * ROWS + row; };
-  float top = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, p.part_ml[slot_row(w)][0]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float ref = top == -INFINITY ? 0.f : top;
-  const int col = lane * 2;
-  float sum = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const f32x2 ml = p.part_ml[slot_row(w)];
-    const float weight = fast_exp2(ml[0] - ref);
-    sum += ml[1] * weight;
-    if (col < COLS) {
-      const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_o + slot_row(w) * COLS + col);
-      a0 += x[0] * weight;
-      a1 += x[1] * weight;
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int token = s.start + i;
-  if (col < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
-  if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+  join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.token, x.head);
 }
 
 // Tiles of 16, 32 or 64 rows: the least that holds the rows of a sequence with `most` new tokens.
-int row_blocks(int G, int64_t most) { return G * most <= 16 ? 1 : G * most <= 32 ? 2 : 4; }
+int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int64_t few_bytes(int64_t rows, int D) { return 2 * kWorkgroups * 16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4; }
 
 template <bool E4M3, int COLS, int NR>
-void launch_few(const AttnParams& p, hipStream_t st) {
+void launch_few(PagedAttn p, hipStream_t st) {
+  p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)kWorkgroups * 16 * NR * COLS);
   hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR>), dim3(kWorkgroups), dim3(kWaves * 64), 0, st, p);
   const int64_t n_rows = (int64_t)p.g.T * p.Hq;
-  hipLaunchKernelGGL((paged_attn_join<COLS, 16 * NR>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p, n_rows, kWorkgroups);
+  hipLaunchKernelGGL((paged_attn_few_join<COLS, 16 * NR>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p, n_rows, kWorkgroups);
 }
 template <bool E4M3, int COLS>
-void launch_rows(const AttnParams& p, int blocks, hipStream_t st) {
+void launch_rows(const PagedAttn& p, int64_t rows, hipStream_t st) {
+  const int blocks = row_blocks(rows);
   if (blocks == 1) launch_few<E4M3, COLS, 1>(p, st);
   else if (blocks == 2) launch_few<E4M3, COLS, 2>(p, st);
   else launch_few<E4M3, COLS, 4>(p, st);
+}
+void launch(const PagedAttn& p, bool e4m3, int64_t rows, hipStream_t st) {
+  if (e4m3) {
+    if (p.D <= 64) launch_rows<true, 64>(p, rows, st);
+    else launch_rows<true, 128>(p, rows, st);
+  } else {
+    if (p.D <= 64) launch_rows<false, 64>(p, rows, st);
+    else launch_rows<false, 128>(p, rows, st);
+  }
 }
 
 }  // namespace
@@ -543,8 +484,8 @@ using namespace mhip;
 extern "C" int64_t mhip_paged_attn_workspace_bytes(int most_new, int Hq, int Hkv, int D) {
   if (most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
   if (D <= 0 || D > 128) return MHIP_EHEADDIM;
-  const int64_t rows = 16 * row_blocks(Hq / Hkv, most_new);
-  return 2 * kWorkgroups * rows * ((D <= 64 ? 64 : 128) + 2) * 4;
+  const int64_t rows = (int64_t)most_new * (Hq / Hkv), few = few_bytes(rows, D), chunk = rows > kFewRows ? paged_attn_chunk_bytes(D) : 0;
+  return few > chunk ? few : chunk;
 }
 
 extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
@@ -554,7 +495,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
                                    int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
                                    int64_t o_sb, int64_t o_ss, int64_t o_sh,
                                    float softmax_scale, int mask, int dtype, void* workspace, void* stream) {
-  AttnParams p{};
+  PagedAttn p{};
   if (B < 0 || n < 0 || T < 0 || most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
   if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) return MHIP_EINVAL;
   if (mask != MHIP_MASK_NONE && mask != MHIP_MASK_CAUSAL) return MHIP_EINVAL;
@@ -579,18 +520,20 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   p.l_sb = starts ? 0 : (int64_t)Hq * n; p.l_sh = starts ? T : n;
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D;
   p.causal = mask == MHIP_MASK_CAUSAL;
+  p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * kLog2e;
   p.by_group = Divisor(p.G); p.by_heads = Divisor(Hq); p.by_new = Divisor(n);
-  const int blocks = row_blocks(p.G, most_new);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)kWorkgroups * 16 * blocks * (D <= 64 ? 64 : 128));
+  const int64_t rows = (int64_t)most_new * p.G;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == MHIP_E4M3) {
-    if (D <= 64) launch_rows<true, 64>(p, blocks, st);
-    else launch_rows<true, 128>(p, blocks, st);
+  if (rows <= kFewRows) {                  // (a sequence with more rows all the same is several tiles of them)
+    p.few_rows = 0x7fffffff;
+    launch(p, dtype == MHIP_E4M3, rows, st);
   } else {
-    if (D <= 64) launch_rows<false, 64>(p, blocks, st);
-    else launch_rows<false, 128>(p, blocks, st);
+    // Packed sequences may be of either kind: two pairs of launches, one after the other on the stream, share the workspace.
+    p.few_rows = starts ? kFewRows : -1;
+    if (starts) launch(p, dtype == MHIP_E4M3, rows, st);
+    paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st);
   }
   return launch_status();
 }

@@ -1,0 +1,116 @@
+// What the two forms of attention over a paged cache share: the arguments, and the last step of rows that several workgroups shared.
+#pragma once
+
+#include "paged.hpp"
+
+#include <math.h>
+
+namespace mhip {
+
+struct PagedAttn {
+  PagedGeom g;
+  const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
+  int64_t c_sp, c_ss, c_sh;                // of the cache, bytes
+  int64_t s_sp, s_ss, s_sh;                // of the scales, elements
+  const uint16_t* q; uint16_t* out; float* lse;
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, l_sb, l_sh;
+  int Hq, Hkv, G, D, causal;
+  float scale, scale_log2;
+  Divisor by_group, by_heads, by_new;
+  int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
+  float* part_o; f32x2* part_ml;           // partial results
+};
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+// Values that are no numbers, in a tile of which some rows do not see some keys: 0 * NaN would reach rows that do not see the key.
+// They are zeros in the product with P then, and a product of odd_marks with seen_marks counts for every row and column how many
+// it sees of each kind: +inf in ones, -inf in 128s, NaN in 16384s (at most 64 keys; all of it exact).
+__device__ __forceinline__ u32x4 finite_part(const u32x4& v, uint32_t& odd) {
+  u32x4 fine;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = (v[i] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u, hi = (v[i] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+    fine[i] = v[i] & ~(lo | hi);
+    odd |= lo | hi;
+  }
+  return fine;
+}
+__device__ __forceinline__ u32x4 odd_marks(const u32x4& v) {
+  u32x4 marks;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    auto mark = [](uint32_t x) {       // 1, 128 and 16384 in bf16
+      return (x & 0x7f80u) != 0x7f80u ? 0u : x & 0x7fu ? 0x4680u : x & 0x8000u ? 0x4300u : 0x3f80u;
+    };
+    marks[i] = mark(v[i] & 0xffffu) | mark(v[i] >> 16) << 16;
+  }
+  return marks;
+}
+__device__ __forceinline__ u32x4 seen_marks(const u32x4& p) {
+  u32x4 marks;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) marks[i] = (p[i] & 0x7fffu ? 0x3f80u : 0u) | (p[i] & 0x7fff0000u ? 0x3f800000u : 0u);
+  return marks;
+}
+__device__ __forceinline__ float with_odd(float o, float counts) {
+  const int n = (int)counts;
+  if (n >= 16384) return __builtin_nanf("");
+  if (n & 127) o += INFINITY;
+  if (n >> 7) o -= INFINITY;
+  return o;
+}
+
+// One row from its partial results, the slot of number k at at(k): a wavefront, two columns a lane.
+template <int COLS, class At>
+__device__ __forceinline__ void join_row(const PagedAttn& p, int lane, int n_parts, At at, int b, int token, int head) {
+  float top = -INFINITY;
+  for (int k = lane; k < n_parts; k += 64) top = fmaxf(top, p.part_ml[at(k)][0]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float ref = top == -INFINITY ? 0.f : top;
+  const int col = lane * 2;
+  float sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < n_parts; ++k) {
+    const f32x2 ml = p.part_ml[at(k)];
+    const float weight = fast_exp2(ml[0] - ref);
+    sum += ml[1] * weight;
+    if (col < COLS) {
+      const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_o + at(k) * COLS + col);
+      a0 += x[0] * weight;
+      a1 += x[1] * weight;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (col < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
+  if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+}
+
+// The row of q that number `id` of all T * Hq stands for: its sequence, and the row's number there.  False where there is none.
+struct RowOf { int b, head, hk, r, token; PagedSeq s; };
+__device__ __forceinline__ bool row_of(const PagedAttn& p, int id, int lane, RowOf& x) {
+  int i = 0;
+  const int t = __builtin_amdgcn_readfirstlane(p.by_heads.quotient(id, x.head));
+  x.head = __builtin_amdgcn_readfirstlane(x.head);
+  if (p.g.starts) x.b = paged_owner<64>(p.g, t, lane);
+  else x.b = p.by_new.quotient(t, i);
+  x.b = __builtin_amdgcn_readfirstlane(x.b);
+  if (x.b >= p.g.B) return false;
+  x.s = paged_seq<true>(p.g, x.b);
+  if (p.g.starts) i = t - x.s.start;
+  if (i < 0 || i >= x.s.n) return false;
+  int of_group;
+  x.hk = p.by_group.quotient(x.head, of_group);
+  x.r = i * p.G + of_group;
+  x.token = x.s.start + i;
+  return true;
+}
+
+int64_t paged_attn_chunk_bytes(int D);
+void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
+
+}  // namespace mhip

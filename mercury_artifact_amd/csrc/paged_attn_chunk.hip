@@ -1,0 +1,625 @@
+// Attention of many new tokens over a paged K/V cache: more rows than paged_attn_few takes (rows r = token * G + head of the group).
+//
+// Bound by the matrix pipes (and the board's power), as the block forward: a key tile feeds 256 rows, 256 multiply-adds for each
+// byte read.  The structure is that of attn_fwd.hip on 16 x 16 MFMA tiles:
+//   workgroup  = 256 rows of one (sequence, K/V head): 8 wavefronts x 32 rows, one workgroup per CU, two wavefronts per SIMD
+//   main loop  = 64-key tiles, K and V rings of four stages in LDS, rows of 256 bytes with XOR-swizzled 16-byte chunks
+//   S^T = K Q^T, O^T = V^T P^T with the lane's own P as B operand; the reference score of a row is its first tile's maximum and
+//                moves only when a later sum would overflow
+//   ping-pong  : the matrix phase of wavefronts 0-3 runs beside the vector phase of wavefronts 4-7 and the other way round
+// and what the pages change:
+//   copies     : a wavefront copies 8 rows of each tile, which lie in one page; the table's entries are read through the scalar cache
+//                at the start of a vector phase and used at its end, when nothing else waits on that counter
+//   e4m3       : a wavefront's 8 rows of codes come through registers, requested one tile ahead, and go into LDS as bf16 rows
+//                times their scale, exact for a power of two: converted once by one wavefront, not by all eight
+//   pieces     : where the items are few, or one is long, several workgroups share an item's keys (cut_of) and a second kernel
+//                joins their partial results
+#include "paged_attn.hpp"
+
+namespace mhip {
+namespace {
+
+constexpr int kBM = 256;                   // rows of a workgroup: 8 wavefronts of 32
+constexpr int kBN = 64;                    // keys of a tile
+constexpr int kTileLds = kBN * 256;        // a K or V tile in LDS, rows of 256 bytes
+constexpr int kRingStages = 4;
+constexpr int kVRing = kRingStages * kTileLds;
+constexpr int kParts = 512;                // partial results there is room for
+constexpr float kPieceCost = 12.f;         // what a piece costs besides its tiles, in tiles
+
+// How the items (sequence, K/V head, tile of rows) are cut into pieces of their keys, one workgroup each: all alike where the
+// sequences are, in proportion to their lengths where they are not, so that `want` pieces of equal length would do.
+struct Cut { int64_t want, total; };       // S of a sequence: steps * want / total, at least 1
+struct Pieces { int rts, parts; int64_t steps; };     // tiles of rows, pieces of each, 64-key steps
+__device__ __forceinline__ Pieces chunk_items(const PagedAttn& p, const PagedSeq& s) {
+  Pieces c;
+  c.rts = s.n * p.G > p.few_rows ? (s.n * p.G + kBM - 1) / kBM : 0;
+  c.steps = s.len > kBN ? (s.len + kBN - 1) / kBN : 1;
+  c.parts = 1;
+  return c;
+}
+__device__ __forceinline__ Pieces chunk_pieces(const PagedAttn& p, const PagedSeq& s, const Cut& cut) {
+  Pieces c = chunk_items(p, s);
+  if (c.rts > 0) {
+    const int64_t parts = c.steps * cut.want / cut.total, most = c.steps / 4;
+    c.parts = (int)(parts < most ? parts : most);
+    if (c.parts < 1) c.parts = 1;
+  }
+  return c;
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+  return x;
+}
+__device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane) {
+  const int per = (p.g.B + 63) / 64;
+  long long steps = 0, items = 0;
+  for (int j = 0; j < per; ++j)
+    if (lane * per + j < p.g.B) {
+      const Pieces c = chunk_items(p, paged_seq<false>(p.g, lane * per + j));
+      items += c.rts;
+      steps += c.rts * c.steps;
+    }
+  Cut cut;
+  items = uniform64(wave_sum(items)) * p.Hkv;
+  cut.total = uniform64(wave_sum(steps)) * p.Hkv;
+  cut.want = items < kParts ? items : kParts;            // pieces of items in several: at most so many
+  if (items > 0 && items < kParts) {
+    // the number of pieces that takes the least rounds of 256 workgroups times their length; lane l tries so many to an item
+    const int unit = items < 4 ? 4 / (int)items : 1, parts = (lane + 1) * unit;
+    const float mean = (float)cut.total / (float)items;
+    const int rounds = (int)((items * parts + 255) / 256);
+    float time = rounds * (mean / parts + kPieceCost) + (parts > 1 ? kPieceCost : 0.f);
+    if (parts > 1 && items * parts > kParts) time = INFINITY;
+    if (lane == 0 && unit > 1) time = mean + kPieceCost;           // (stands for one piece)
+    float best = time;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = fminf(best, __shfl_xor(best, off));
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(time == best));
+    cut.want = items * (at == 0 ? 1 : (at + 1) * unit);
+  }
+  return cut;
+}
+// Pieces (and those of items in more than one) before each lane's run of sequences.
+struct Layout { int per; int64_t before, mine, slots_before; };
+__device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, int lane) {
+  Layout y;
+  y.per = (p.g.B + 63) / 64;
+  y.mine = 0;
+  int64_t slots = 0;
+  for (int j = 0; j < y.per; ++j)
+    if (lane * y.per + j < p.g.B) {
+      const Pieces c = chunk_pieces(p, paged_seq<false>(p.g, lane * y.per + j), cut);
+      const int64_t n = (int64_t)p.Hkv * c.rts * c.parts;
+      y.mine += n;
+      if (c.parts > 1) slots += n;
+    }
+  int64_t sum = y.mine, sum_slots = slots;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t a = __shfl_up((long long)sum, off), b = __shfl_up((long long)sum_slots, off);
+    if (lane >= off) { sum += a; sum_slots += b; }
+  }
+  y.before = sum - y.mine;
+  y.slots_before = sum_slots - slots;
+  return y;
+}
+// piece i of a sequence: K/V heads fastest (eight of them: one to an XCD's L2), then the row tiles, the last (longest) first
+struct Piece { int part, rt, hk; };
+__device__ __forceinline__ Piece piece_of(const Pieces& c, int Hkv, int64_t i) {
+  Piece x;
+  const int64_t of_part = (int64_t)c.rts * Hkv;
+  x.part = (int)(i / of_part);
+  const int rest = (int)(i - x.part * of_part);
+  x.rt = c.rts - 1 - rest / Hkv;
+  x.hk = rest % Hkv;
+  return x;
+}
+__device__ __forceinline__ int64_t piece_number(const Pieces& c, int Hkv, int part, int rt, int hk) {
+  return ((int64_t)part * c.rts + (c.rts - 1 - rt)) * Hkv + hk;
+}
+
+constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
+constexpr int kFragDepth = 4;              // LDS operand reads in flight ahead of the MFMAs
+constexpr int kOStride = 136;              // epilogue staging of O, bf16 elements per row
+
+template <bool E4M3, int COLS>
+__global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
+  constexpr int KB = COLS / 32, DB = COLS / 16;        // k-steps of S^T, blocks of O^T
+  constexpr int MB = kBN / 16, kSteps = kBN / 32;      // key blocks of S^T, k-steps of O^T
+  constexpr int kSlotsS = MB * KB, kSlotsO = kSteps * DB;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * kVRing];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+  const bool group_b = wave >= 4;
+
+  // ---- this workgroup's piece --------------------------------------------------------------------------------
+  const Cut cut = cut_of(p, lane);
+  if (cut.total == 0) return;
+  const Layout y = layout_of(p, cut, lane);
+  const int64_t id = blockIdx.x;
+  const uint64_t owners = __builtin_amdgcn_ballot_w64(id >= y.before && id < y.before + y.mine);
+  if (owners == 0) return;                             // past the last piece
+  const int owner = __builtin_ctzll(owners);
+  int b = owner * y.per;
+  int64_t pos = id - uniform64(__shfl((long long)y.before, owner)), slot0 = uniform64(__shfl((long long)y.slots_before, owner));
+  PagedSeq s = paged_seq<true>(p.g, b);
+  Pieces c = chunk_pieces(p, s, cut);
+  for (int64_t n; b + 1 < p.g.B && pos >= (n = (int64_t)p.Hkv * c.rts * c.parts);) {
+    pos -= n;
+    if (c.parts > 1) slot0 += n;
+    s = paged_seq<true>(p.g, ++b);
+    c = chunk_pieces(p, s, cut);
+  }
+  const Piece piece = piece_of(c, p.Hkv, pos);
+  const int hk = piece.hk, row0 = piece.rt * kBM;
+  const int rows = s.n * p.G - row0 < kBM ? s.n * p.G - row0 : kBM;
+  auto sees = [&](int row) {                           // keys that a row sees
+    return p.causal ? clamped(s.len - s.n + p.by_group.quotient(row) + 1, 0, s.len) : s.len;
+  };
+  const int seen_last = sees(row0 + rows - 1);
+  const int64_t steps = (seen_last + kBN - 1) / kBN;
+  const int t0 = (int)(steps * piece.part / c.parts), ntiles = (int)(steps * (piece.part + 1) / c.parts) - t0;
+  // of the wavefront's rows (those past the last repeat it): the least
+  const int my_row0 = row0 + wave * 32;
+  const int seen_first = sees(my_row0 < row0 + rows ? my_row0 : row0 + rows - 1);
+
+  // ---- Q rows: B operand of S^T, lane (ln, lg) holds 8 columns of rows ln and 16 + ln --------------------------------
+  bf16x8 qf[2][KB];
+  int lim[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = my_row0 + r * 16 + ln, real = row < row0 + rows ? row : row0 + rows - 1;
+    int of_group;
+    const int token = p.by_group.quotient(real, of_group);
+    lim[r] = p.causal ? clamped(s.len - s.n + token + 1, 0, s.len) : s.len;
+    const uint16_t* src = p.q + b * p.q_sb + (int64_t)(s.start + token) * p.q_ss + (hk * p.G + of_group) * p.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < KB; ++ks) {
+      const int col = ks * 32 + lg * 8;
+      qf[r][ks] = bf16x8{};
+      if (col < p.D) qf[r][ks] = *reinterpret_cast<const bf16x8*>(src + col);
+    }
+  }
+
+  // ---- tiles into LDS -----------------------------------------------------------------------------------------------
+  const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const uint32_t lds_rows = lds_smem + wave * 2048;    // the wavefront's 8 rows of a stage
+  const int* table = p.g.table + b * p.g.t_sb;
+  // Entries of the four quarters of a tile, 16 keys (of one page) each; the wavefront's rows are in quarter wave / 2.
+  // gone: four bits of each of the last eight tiles, that its quarters are not here.
+  struct Rows { int page, slot, held; };
+  uint32_t gone = 0;
+  auto look_up = [&](int t) {
+    const int key = (t0 + t) * kBN;
+    int entry[4], slot[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      entry[h] = -1;
+      slot[h] = 0;
+      if (t < ntiles && key + 16 * h < seen_last) entry[h] = uniform_load(table, p.g.by_page.quotient(key + 16 * h, slot[h]));
+    }
+    uint32_t bits = 0;
+    Rows x{-1, 0, 0};
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const bool here = entry[h] >= 0 && entry[h] < p.g.pages;
+      bits |= here ? 0u : 1u << h;
+      if (h == wave >> 1) {
+        x.page = entry[h];
+        x.slot = slot[h] + 8 * (wave & 1);
+        x.held = here ? clamped(seen_last - (key + 8 * wave), 0, 8) : 0;
+      }
+    }
+    gone = (gone & ~(15u << (4 * (t & 7)))) | bits << (4 * (t & 7));
+    return x;
+  };
+  int voff[2];                                         // bf16: of copy instruction u, 4 rows each
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = 4 * u + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(8 * wave + row);
+    voff[u] = chunk * 8 < p.D ? (int)(row * p.c_ss) + chunk * 16 : kNoColumn;
+  }
+  auto copy_rows = [&](const uint8_t* base, const Rows& x, uint32_t to) {
+    const uint8_t* from = base + (x.held > 0 ? x.page * p.c_sp + x.slot * p.c_ss + hk * p.c_sh : 0);
+    const u32x4 rs = rsrc_words(from, x.held > 0 ? (uint32_t)((x.held - 1) * p.c_ss + p.D * 2) : 0u);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) copy16_to_lds(rs, to + u * 1024, voff[u], 0);
+  };
+  // e4m3: lane l takes codes 16 (l % 8) .. +15 of row l / 8
+  const int row8 = lane >> 3, col16 = (lane & 7) * 16;
+  struct Codes { u32x4 w; float scale; };
+  auto request = [&](const uint8_t* base, const float* scales, const Rows& x) {
+    Codes k{u32x4{}, 0.f};
+    if (row8 < x.held && col16 < p.D) {
+      k.w = *reinterpret_cast<const u32x4*>(base + x.page * p.c_sp + (int64_t)(x.slot + row8) * p.c_ss + hk * p.c_sh + col16);
+      k.scale = scales[x.page * p.s_sp + (int64_t)(x.slot + row8) * p.s_ss + hk * p.s_sh];
+    }
+    return k;
+  };
+  typedef __attribute__((address_space(3))) u32x4* lds_u32x4;
+  auto put = [&](const Codes& k, uint32_t to) {
+    u32x4 lo, hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], false), z = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], true);
+      const uint32_t w0 = pack_bf16(x[0] * k.scale, x[1] * k.scale), w1 = pack_bf16(z[0] * k.scale, z[1] * k.scale);
+      if (i < 2) { lo[2 * i] = w0; lo[2 * i + 1] = w1; } else { hi[2 * i - 4] = w0; hi[2 * i - 3] = w1; }
+    }
+    const int swz = lds_row_swizzle(8 * wave + row8), chunk = (lane & 7) * 2;
+    *(lds_u32x4)(uintptr_t)(to + row8 * 256 + ((chunk ^ swz) << 4)) = lo;
+    *(lds_u32x4)(uintptr_t)(to + row8 * 256 + (((chunk + 1) ^ swz) << 4)) = hi;
+  };
+
+  // ---- operands from LDS (addresses inside the stage that is read next move on in place) --------------------------------
+  int k_a[KB];                                         // + mb * 16 rows
+#pragma unroll
+  for (int ks = 0; ks < KB; ++ks) k_a[ks] = (int)lds_smem + ln * 256 + (((4 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
+  int v_a[DB];                                         // + t * 32 rows
+  {
+    const int row = 4 * lg + (ln >> 2);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      v_a[db] = (int)lds_smem + kVRing + row * 256 + (((2 * db + ((ln & 3) >> 1)) ^ lds_row_swizzle(row)) << 4) + (ln & 1) * 8;
+  }
+  typedef __attribute__((address_space(3))) bf16x4* lds_bf16x4;
+  typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8;
+  auto read_k = [&](int mb, int ks) -> bf16x8 { return *(lds_bf16x8)(uintptr_t)(uint32_t)(k_a[ks] + mb * 4096); };
+  auto read_v = [&](int db, int t) -> bf16x8 {
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + t * 8192));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + t * 8192 + 4096));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto stage_step = [](int t) { return (t + 1) % kRingStages == 0 ? -(kRingStages - 1) * kTileLds : kTileLds; };
+
+  // ---- softmax state and products -------------------------------------------------------------------------------------
+  f32x4 o_acc[DB][2], sc[MB][2];
+  u32x4 pw[kSteps][2];                                 // P^T of the current tile
+  float m_ref[2] = {}, nmsc[2] = {}, l_run[2] = {}, rs[2] = {};
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o_acc[i][0] = o_acc[i][1] = f32x4{};
+  constexpr float kTrigger = 1048576.f, kSlack = 14.f, kMost = 0x1.fffffep127f;
+  float scale_log2 = p.scale_log2;
+  asm volatile("" : "+s"(scale_log2));
+  auto mfma = [](const bf16x8& x, const bf16x8& z, const f32x4& a) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, z, a, 0, 0, 0); };
+  auto s_mfma = [&](int mb, int ks, const bf16x8& kf) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) sc[mb][r] = mfma(kf, qf[r][ks], ks == 0 ? f32x4{} : sc[mb][r]);
+  };
+  auto o_mfma = [&](int db, int t, const bf16x8& vf) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) o_acc[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[t][r]), o_acc[db][r]);
+  };
+  auto cuts = [&](int t) { return (t0 + t + 1) * kBN > seen_first; };      // some row of the wavefront does not see some key
+  auto sm_mask = [&](int t) {
+    const uint32_t bits = gone >> (4 * (t & 7)) & 15u;
+    if (cuts(t) || bits) {
+      const int kv0 = (t0 + t) * kBN;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (kv0 + mb * 16 + lg * 4 + j >= lim[r] || (bits >> mb & 1)) sc[mb][r][j] = -INFINITY;
+    }
+  };
+  auto sm_pair = [&](int idx) {
+    const int t = idx >> 3, r = (idx >> 2) & 1, d = idx & 3, mb = 2 * t + (d >> 1), e = 2 * (d & 1);
+    const float x0 = fast_exp2(__builtin_fmaf(sc[mb][r][e], scale_log2, nmsc[r]));
+    const float x1 = fast_exp2(__builtin_fmaf(sc[mb][r][e + 1], scale_log2, nmsc[r]));
+    if (t == 0 && d == 0) rs[r] = x0 + x1; else rs[r] += x0 + x1;
+    uint32_t w = pack_bf16(x0, x1);
+    asm volatile("" : "+v"(w), "+v"(rs[r]));           // keeps the pair where it is written
+    pw[t][r][d] = w;
+  };
+  constexpr int kPairs = kBN / 4;
+  auto sm_exps = [&]() {
+#pragma unroll
+    for (int idx = 0; idx < kPairs; ++idx) sm_pair(idx);
+  };
+  auto sm_fix = [&](bool first) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float mx = sc[0][r][0];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, sc[mb][r][j]);
+      mx = quad_max(mx);
+      const float grown = (mx - m_ref[r]) * scale_log2;
+      const bool move = first || grown > kSlack;
+      if (!first) {
+        const float alpha = move ? fast_exp2(-grown) : 1.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o_acc[db][r] *= alpha;
+        l_run[r] *= alpha;
+      }
+      if (move) m_ref[r] = first ? fmaxf(mx, -kMost) : mx;
+      nmsc[r] = fminf(-m_ref[r] * scale_log2, kMost);
+    }
+  };
+  constexpr int kEarlyPairs = 2;
+  auto sm_tile = [&]() {
+#pragma unroll
+    for (int idx = kEarlyPairs; idx < kPairs; ++idx) sm_pair(idx);
+    if (__builtin_amdgcn_ballot_w64(!(rs[0] + rs[1] < kTrigger)) != 0) {
+      sm_fix(false);
+      sm_exps();
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) l_run[r] += rs[r];
+  };
+  // O^T of a tile that cuts (see finite_part).
+  auto pv_cut = [&]() __attribute__((always_inline)) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < kSlotsO; ++i) {
+      o_mfma(i % DB, i / DB, __builtin_bit_cast(bf16x8, finite_part(__builtin_bit_cast(u32x4, read_v(i % DB, i / DB)), odd)));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      f32x4 counts[2] = {};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, t))));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) counts[r] = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[t][r])), counts[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o_acc[db][r][j] = with_odd(o_acc[db][r][j], counts[r][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // Matrix phase of tile t: S^T(t+1) and O^T += V^T(t) P^T(t), operands kFragDepth reads ahead.
+  auto read_frag = [&](int i) -> bf16x8 {
+    if (i < kSlotsS) return read_k(i % MB, i / MB);
+    return read_v((i - kSlotsS) % DB, (i - kSlotsS) / DB);
+  };
+  bf16x8 frag[kFragDepth];
+  auto first_frags = [&]() {
+#pragma unroll
+    for (int i = 0; i < kFragDepth; ++i) frag[i] = read_frag(i);
+  };
+  auto early_slot = [](int idx) { return kSlotsS + DB + idx * (kSlotsO - DB) / kEarlyPairs; };
+  auto matrix_phase = [&](int t) __attribute__((always_inline)) {
+    const int k_step = stage_step(t + 1), v_step = stage_step(t);
+#pragma unroll
+    for (int i = 0; i < kSlotsS + kSlotsO; ++i) {
+      if (i < kSlotsS) s_mfma(i % MB, i / MB, frag[i % kFragDepth]);
+      else o_mfma((i - kSlotsS) % DB, (i - kSlotsS) / DB, frag[i % kFragDepth]);
+      if (i + kFragDepth < kSlotsS + kSlotsO) frag[i % kFragDepth] = read_frag(i + kFragDepth);
+      if (i >= kSlotsS && i < kSlotsS + KB) k_a[i - kSlotsS] += k_step;            // the last K read went out before slot kSlotsS
+      if (i >= kSlotsS + kSlotsO - kFragDepth) {                                   // and the last V read by here
+#pragma unroll
+        for (int e = 0; e < DB; ++e)
+          if (e % kFragDepth == i - (kSlotsS + kSlotsO - kFragDepth)) v_a[e] += v_step;
+      }
+      if (i == kSlotsS) sm_mask(t + 1);
+#pragma unroll
+      for (int idx = 0; idx < kEarlyPairs; ++idx)
+        if (early_slot(idx) == i) sm_pair(idx);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // the same where tile t cuts
+  auto matrix_phase_cut = [&](int t) __attribute__((always_inline)) {
+    pv_cut();
+#pragma unroll
+    for (int i = 0; i < kSlotsS; ++i) {
+      s_mfma(i % MB, i / MB, read_k(i % MB, i / MB));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const int k_step = stage_step(t + 1), v_step = stage_step(t);
+#pragma unroll
+    for (int ks = 0; ks < KB; ++ks) k_a[ks] += k_step;
+#pragma unroll
+    for (int e = 0; e < DB; ++e) v_a[e] += v_step;
+    sm_mask(t + 1);
+#pragma unroll
+    for (int idx = 0; idx < kEarlyPairs; ++idx) sm_pair(idx);
+  };
+
+  if (ntiles > 0) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(qf[r][ks]));      // loaded before the first copy goes out
+    // Tiles 0 .. 3 of K and 0 .. 2 of V; in the loop K(t + 4) and V(t + 3) follow, whose places tile t's matrix phase and the one
+    // before it were the last to read.  Codes that pass through registers are requested one tile before they are put there.
+    Rows next_v, next_k;                               // bf16: V(t + 3); e4m3: whose codes are in registers
+    Codes ck, cv;
+    if constexpr (!E4M3) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const Rows x = look_up(t);
+        copy_rows(p.k, x, lds_rows + t * kTileLds);
+        if (t < 3) copy_rows(p.v, x, lds_rows + kVRing + t * kTileLds);
+        next_v = x;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+      Codes k[4], v[3];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const Rows x = look_up(t);
+        k[t] = request(p.k, p.k_scales, x);
+        if (t < 3) v[t] = request(p.v, p.v_scales, x);
+        next_v = x;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        put(k[t], lds_rows + t * kTileLds);
+        if (t < 3) put(v[t], lds_rows + kVRing + t * kTileLds);
+      }
+      cv = request(p.v, p.v_scales, next_v);
+      next_k = look_up(4);
+      ck = request(p.k, p.k_scales, next_k);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < KB; ++ks) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) s_mfma(mb, ks, read_k(mb, ks));
+      k_a[ks] += kTileLds;
+    }
+    sm_mask(0);
+    sm_fix(true);
+    sm_exps();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) l_run[r] = rs[r];
+    __syncthreads();                                   // K(0) has been read by all
+    if (ntiles > 1) first_frags();
+    if (group_b) __builtin_amdgcn_s_barrier();
+    // vector phase of tile t: softmax of tile t + 1 and the copies ahead
+    auto vector_phase = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) asm volatile("" : "+v"(sc[0][r]), "+v"(sc[MB - 1][r]));   // keeps the exponentials behind the barrier
+      if constexpr (!E4M3) {
+        const Rows x = look_up(t + 4);
+        sm_tile();
+        copy_rows(p.k, x, lds_rows + (t & 3) * kTileLds);
+        copy_rows(p.v, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
+        next_v = x;
+        if (t + 2 < ntiles) first_frags();
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");          // the four copies of one tile ago are done
+      } else {
+        const Rows x = look_up(t + 5);
+        sm_tile();
+        put(ck, lds_rows + (t & 3) * kTileLds);
+        put(cv, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
+        cv = request(p.v, p.v_scales, next_k);
+        ck = request(p.k, p.k_scales, x);
+        next_k = x;
+        if (t + 2 < ntiles) first_frags();
+      }
+    };
+    // Tiles that all rows see whole, then those that cut (of the workgroup, whose wavefronts keep step).
+    const int whole = clamped(sees(row0) / kBN - t0, 0, ntiles - 1);
+    int t = 0;
+    for (; t < whole; ++t) {
+      __builtin_amdgcn_s_setprio(2);
+      matrix_phase(t);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_s_barrier();
+      vector_phase(t);
+      __builtin_amdgcn_s_barrier();
+    }
+    for (; t + 1 < ntiles; ++t) {
+      matrix_phase_cut(t);
+      __builtin_amdgcn_s_barrier();
+      vector_phase(t);
+      __builtin_amdgcn_s_barrier();
+    }
+    pv_cut();
+    if (!group_b) __builtin_amdgcn_s_barrier();
+  }
+
+  // ---- epilogue -----------------------------------------------------------------------------------------------------
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // copies past the last tile
+  __syncthreads();                                     // every wavefront is done with K and V
+  if (c.parts > 1) {
+    const int64_t at = (slot0 + pos) * kBM + wave * 32;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float l_tot = quad_sum(l_run[r]);
+      if (wave * 32 + r * 16 + ln >= rows) continue;
+      const int64_t row = at + r * 16 + ln;
+      if (lg == 0) p.part_ml[row] = f32x2{l_tot == 0.f ? -INFINITY : m_ref[r] * scale_log2, l_tot};
+#pragma unroll
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(p.part_o + row * COLS + db * 16 + lg * 4) = o_acc[db][r];
+    }
+    return;
+  }
+  unsigned char* os = smem + wave * (32 * kOStride * 2);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float l_tot = quad_sum(l_run[r]), inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+    const int row = my_row0 + r * 16 + ln;
+    if (lg == 0 && row < row0 + rows) {
+      int of_group;
+      const int token = s.start + p.by_group.quotient(row, of_group);
+      p.lse[b * p.l_sb + (hk * p.G + of_group) * p.l_sh + token] = l_tot == 0.f ? -INFINITY : __builtin_fmaf(fast_log2(l_tot), kLn2, m_ref[r] * p.scale);
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      u32x2 w;
+      w[0] = pack_bf16(o_acc[db][r][0] * inv, o_acc[db][r][1] * inv);
+      w[1] = pack_bf16(o_acc[db][r][2] * inv, o_acc[db][r][3] * inv);
+      *reinterpret_cast<u32x2*>(os + (r * 16 + ln) * (kOStride * 2) + (db * 16 + lg * 4) * 2) = w;
+    }
+  }
+  __syncthreads();
+  const int chunk = lane & 15;
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int r = (lane >> 4) + 4 * it, row = my_row0 + r;
+    if (row < row0 + rows && chunk * 8 < p.D) {
+      int of_group;
+      const int token = s.start + p.by_group.quotient(row, of_group);
+      *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + (hk * p.G + of_group) * p.o_sh + chunk * 8) =
+          *reinterpret_cast<const u32x4*>(os + r * (kOStride * 2) + chunk * 16);
+    }
+  }
+}
+
+// The rows that several workgroups shared, a wavefront each; a wavefront does eight, so that it counts the pieces once for them.
+constexpr int kJoinRows = 8;
+template <int COLS>
+__global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kJoinRows;
+  const Cut cut = cut_of(p, lane);
+  if (cut.total == 0) return;
+  const Layout y = layout_of(p, cut, lane);
+  for (int k = 0; k < kJoinRows; ++k) {
+    RowOf x;
+    if (id0 + k >= n_rows) return;
+    if (!row_of(p, (int)(id0 + k), lane, x)) continue;
+    const Pieces c = chunk_pieces(p, x.s, cut);
+    if (c.rts == 0 || c.parts == 1) continue;
+    int64_t before = uniform64(__shfl((long long)y.slots_before, x.b / y.per));
+    for (int e = x.b / y.per * y.per; e < x.b; ++e) {
+      const Pieces d = chunk_pieces(p, paged_seq<true>(p.g, e), cut);
+      if (d.parts > 1) before += (int64_t)p.Hkv * d.rts * d.parts;
+    }
+    const int64_t first = before + piece_number(c, p.Hkv, 0, x.r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
+    const int row = x.r % kBM;
+    join_row<COLS>(p, lane, c.parts, [&](int part) { return (first + part * step) * kBM + row; }, x.b, x.token, x.head);
+  }
+}
+
+template <bool E4M3, int COLS>
+void launch(const PagedAttn& p, hipStream_t st) {
+  const int64_t n_rows = (int64_t)p.g.T * p.Hq, rows = (int64_t)p.g.T * p.G;
+  const int64_t items = p.Hkv * (p.g.starts ? rows / kBM + p.g.B : p.g.B * (((int64_t)p.g.n * p.G + kBM - 1) / kBM));
+  hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)(items + kParts)), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((paged_attn_chunk_join<COLS>), dim3((unsigned)((n_rows + 4 * kJoinRows - 1) / (4 * kJoinRows))), dim3(256), 0, st, p, n_rows);
+}
+template <bool E4M3>
+void launch(const PagedAttn& p, hipStream_t st) {
+  if (p.D <= 64) launch<E4M3, 64>(p, st);
+  else if (p.D <= 96) launch<E4M3, 96>(p, st);
+  else launch<E4M3, 128>(p, st);
+}
+
+}  // namespace
+
+int64_t paged_attn_chunk_bytes(int D) { return (int64_t)kParts * kBM * ((D <= 64 ? 64 : D <= 96 ? 96 : 128) + 2) * 4; }
+void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
+  PagedAttn q = p;
+  q.part_ml = reinterpret_cast<f32x2*>(q.part_o + (int64_t)kParts * kBM * (p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128));
+  if (e4m3) launch<true>(q, stream);
+  else launch<false>(q, stream);
+}
+
+}  // namespace mhip
