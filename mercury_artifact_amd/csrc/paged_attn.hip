@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
 #pragma unroll
   for (int u = 0; u < kCopies; ++u) {
     const int row = u * kCopyRows + lane / kChunks, chunk = (lane % kChunks) ^ swizzle<ROWB>(row);
-    voff[u] = chunk * 16 < p.D * kSize ? (int)(row * p.c_ss) + chunk * 16 : kNoColumn;
+    voff[u] = chunk * 16 < p.D * kSize ? row * (int)p.c_ss16 * 16 + chunk * 16 : kNoColumn;
   }
   // K operand: 16 bytes of row ln; in e4m3 they serve two k-steps of 32 columns
   constexpr int KR = E4M3 ? KB / 2 : KB;               // 16-byte reads of a K row
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
     auto copy = [&](const uint8_t* base, int at) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t* from = base + (held[h] > 0 ? page[h] * p.c_sp + slot[h] * p.c_ss + hk * p.c_sh : 0);
-        const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * p.c_ss + p.D * kSize) : 0u);
+        const uint8_t* from = base + (held[h] > 0 ? row_offset(p, page[h], slot[h]) + hk * p.c_sh : 0);
+        const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * (int)p.c_ss16 * 16 + p.D * kSize) : 0u);
 #pragma unroll
         for (int u = 0; u < kCopies; ++u) copy16_to_lds(rs, ring + at + h * 16 * ROWB + u * 1024, voff[u], 0);
       }
@@ -510,9 +510,11 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
     if (s % 8 != 0) return MHIP_EALIGN;
   if ((int64_t)T * Hq >= (int64_t(1) << 31) - 64) return MHIP_EUNSUPPORTED;
   const int size = dtype == MHIP_E4M3 ? 1 : 2;
+  // places are counted in 16 bytes: 32 bits for a page, and for the rows of one
+  if (c_sp < 0 || c_sp * size / 16 > 0xffffffffll || c_ss * size / 16 * page_size > 0xffffffffll) return MHIP_EUNSUPPORTED;
   p.k = static_cast<const uint8_t*>(k_cache); p.v = static_cast<const uint8_t*>(v_cache);
   p.k_scales = k_scales; p.v_scales = v_scales;
-  p.c_sp = c_sp * size; p.c_ss = c_ss * size; p.c_sh = c_sh * size;
+  p.c_sp16 = (uint32_t)(c_sp * size / 16); p.c_ss16 = (uint32_t)(c_ss * size / 16); p.c_sh = c_sh * size;
   p.s_sp = s_sp; p.s_ss = s_ss; p.s_sh = s_sh;
   p.q = static_cast<const uint16_t*>(q); p.out = static_cast<uint16_t*>(out); p.lse = lse;
   p.q_sb = starts ? 0 : q_sb; p.q_ss = q_ss; p.q_sh = q_sh;

@@ -10,7 +10,8 @@ namespace mhip {
 struct PagedAttn {
   PagedGeom g;
   const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
-  int64_t c_sp, c_ss, c_sh;                // of the cache, bytes
+  uint32_t c_sp16, c_ss16;                 // strides of the cache from page to page and slot to slot, in 16 bytes,
+  int64_t c_sh;                            // and from head to head, bytes
   int64_t s_sp, s_ss, s_sh;                // of the scales, elements
   const uint16_t* q; uint16_t* out; float* lse;
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, l_sb, l_sh;
@@ -62,6 +63,19 @@ __device__ __forceinline__ float with_odd(float o, float counts) {
   if (n & 127) o += INFINITY;
   if (n >> 7) o -= INFINITY;
   return o;
+}
+
+// The arguments once more, read from memory where this stands: values that only the end of a kernel needs would otherwise stay in
+// (or move in and out of) scalar registers through its main loop.
+__device__ __forceinline__ PagedAttn arguments_again() {
+  auto at = (__attribute__((address_space(4))) const PagedAttn*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const PagedAttn*)at;
+}
+
+// Where row `slot` of a page begins, from the first row of the cache.
+__device__ __forceinline__ int64_t row_offset(const PagedAttn& p, int page, int slot) {
+  return (int64_t)(((uint64_t)(uint32_t)page * p.c_sp16 + (uint64_t)((uint32_t)slot * p.c_ss16)) << 4);
 }
 
 // One row from its partial results, the slot of number k at at(k): a wavefront, two columns a lane.

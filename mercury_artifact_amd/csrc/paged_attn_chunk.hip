@@ -189,31 +189,43 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const uint32_t lds_rows = lds_smem + wave * 2048;    // the wavefront's 8 rows of a stage
   const int* table = p.g.table + b * p.g.t_sb;
-  // Entries of the four quarters of a tile, 16 keys (of one page) each; the wavefront's rows are in quarter wave / 2.
+  // The four quarters of a tile, 16 keys (of one page) each; the wavefront's rows are in quarter wave / 2.  A look-up reads their
+  // table entries (of keys past the last one the last one's), settle() uses them.
   // gone: four bits of each of the last eight tiles, that its quarters are not here.
-  struct Rows { int page, slot, held; };
+  struct Entries { int page[4], slot; };               // slot: of the wavefront's own quarter
+  struct Rows { int64_t at; int page, slot, held, bytes; };      // at: from the first row of the head; bytes: of the rows there are
   uint32_t gone = 0;
+  const int last_entry = seen_last > 0 ? p.g.by_page.quotient(seen_last - 1) : 0;
   auto look_up = [&](int t) {
-    const int key = (t0 + t) * kBN;
-    int entry[4], slot[4];
+    Entries e;
+    int slot, index = p.g.by_page.quotient((t0 + t) * kBN, slot);
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      entry[h] = -1;
-      slot[h] = 0;
-      if (t < ntiles && key + 16 * h < seen_last) entry[h] = uniform_load(table, p.g.by_page.quotient(key + 16 * h, slot[h]));
+      e.page[h] = uniform_load(table, index < last_entry ? index : last_entry);
+      if (h == wave >> 1) e.slot = slot + 8 * (wave & 1);
+      slot += 16;
+      if (slot >= p.g.page) { slot = 0; ++index; }
     }
+    return e;
+  };
+  const int row_step = (int)p.c_ss16 * 16, row_tail = p.D * 2 - row_step;        // (bf16)
+  auto settle = [&](int t, Entries e) {
+    asm volatile("" : "+s"(e.page[0]), "+s"(e.page[1]), "+s"(e.page[2]), "+s"(e.page[3]));      // waited for here
     uint32_t bits = 0;
-    Rows x{-1, 0, 0};
+    Rows x{0, 0, e.slot, 0, 0};
+    const int left = seen_last - ((t0 + t) * kBN + 8 * wave), held = left < 8 ? left : 8;
+    const bool some = t < ntiles && left > 0;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const bool here = entry[h] >= 0 && entry[h] < p.g.pages;
+      const bool here = (uint32_t)e.page[h] < (uint32_t)p.g.pages;
       bits |= here ? 0u : 1u << h;
-      if (h == wave >> 1) {
-        x.page = entry[h];
-        x.slot = slot[h] + 8 * (wave & 1);
-        x.held = here ? clamped(seen_last - (key + 8 * wave), 0, 8) : 0;
+      if (h == wave >> 1 && here && some) {
+        x.page = e.page[h];
+        x.held = held;
+        x.bytes = held * row_step + row_tail;
       }
     }
+    x.at = row_offset(p, x.page, x.slot);
     gone = (gone & ~(15u << (4 * (t & 7)))) | bits << (4 * (t & 7));
     return x;
   };
@@ -221,21 +233,22 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = 4 * u + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(8 * wave + row);
-    voff[u] = chunk * 8 < p.D ? (int)(row * p.c_ss) + chunk * 16 : kNoColumn;
+    voff[u] = chunk * 8 < p.D ? row * (int)p.c_ss16 * 16 + chunk * 16 : kNoColumn;
   }
-  auto copy_rows = [&](const uint8_t* base, const Rows& x, uint32_t to) {
-    const uint8_t* from = base + (x.held > 0 ? x.page * p.c_sp + x.slot * p.c_ss + hk * p.c_sh : 0);
-    const u32x4 rs = rsrc_words(from, x.held > 0 ? (uint32_t)((x.held - 1) * p.c_ss + p.D * 2) : 0u);
+  const uint8_t* k_head = p.k + hk * p.c_sh;
+  const uint8_t* v_head = p.v + hk * p.c_sh;
+  auto copy_rows = [&](const uint8_t* head, const Rows& x, uint32_t to) {
+    const u32x4 rs = rsrc_words(head + x.at, (uint32_t)x.bytes);
 #pragma unroll
     for (int u = 0; u < 2; ++u) copy16_to_lds(rs, to + u * 1024, voff[u], 0);
   };
   // e4m3: lane l takes codes 16 (l % 8) .. +15 of row l / 8
   const int row8 = lane >> 3, col16 = (lane & 7) * 16;
   struct Codes { u32x4 w; float scale; };
-  auto request = [&](const uint8_t* base, const float* scales, const Rows& x) {
+  auto request = [&](const uint8_t* head, const float* scales, const Rows& x) {
     Codes k{u32x4{}, 0.f};
     if (row8 < x.held && col16 < p.D) {
-      k.w = *reinterpret_cast<const u32x4*>(base + x.page * p.c_sp + (int64_t)(x.slot + row8) * p.c_ss + hk * p.c_sh + col16);
+      k.w = *reinterpret_cast<const u32x4*>(head + x.at + row8 * (int)p.c_ss16 * 16 + col16);
       k.scale = scales[x.page * p.s_sp + (int64_t)(x.slot + row8) * p.s_ss + hk * p.s_sh];
     }
     return k;
@@ -441,9 +454,9 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const Rows x = look_up(t);
-        copy_rows(p.k, x, lds_rows + t * kTileLds);
-        if (t < 3) copy_rows(p.v, x, lds_rows + kVRing + t * kTileLds);
+        const Rows x = settle(t, look_up(t));
+        copy_rows(k_head, x, lds_rows + t * kTileLds);
+        if (t < 3) copy_rows(v_head, x, lds_rows + kVRing + t * kTileLds);
         next_v = x;
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -451,9 +464,9 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       Codes k[4], v[3];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const Rows x = look_up(t);
-        k[t] = request(p.k, p.k_scales, x);
-        if (t < 3) v[t] = request(p.v, p.v_scales, x);
+        const Rows x = settle(t, look_up(t));
+        k[t] = request(k_head, p.k_scales, x);
+        if (t < 3) v[t] = request(v_head, p.v_scales, x);
         next_v = x;
       }
 #pragma unroll
@@ -461,9 +474,9 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
         put(k[t], lds_rows + t * kTileLds);
         if (t < 3) put(v[t], lds_rows + kVRing + t * kTileLds);
       }
-      cv = request(p.v, p.v_scales, next_v);
-      next_k = look_up(4);
-      ck = request(p.k, p.k_scales, next_k);
+      cv = request(v_head, p.v_scales, next_v);
+      next_k = settle(4, look_up(4));
+      ck = request(k_head, p.k_scales, next_k);
     }
     __syncthreads();
 #pragma unroll
@@ -485,20 +498,22 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) asm volatile("" : "+v"(sc[0][r]), "+v"(sc[MB - 1][r]));   // keeps the exponentials behind the barrier
       if constexpr (!E4M3) {
-        const Rows x = look_up(t + 4);
+        const Entries e = look_up(t + 4);
         sm_tile();
-        copy_rows(p.k, x, lds_rows + (t & 3) * kTileLds);
-        copy_rows(p.v, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
+        const Rows x = settle(t + 4, e);
+        copy_rows(k_head, x, lds_rows + (t & 3) * kTileLds);
+        copy_rows(v_head, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
         next_v = x;
         if (t + 2 < ntiles) first_frags();
         asm volatile("s_waitcnt vmcnt(4)" ::: "memory");          // the four copies of one tile ago are done
       } else {
-        const Rows x = look_up(t + 5);
+        const Entries e = look_up(t + 5);
         sm_tile();
+        const Rows x = settle(t + 5, e);
         put(ck, lds_rows + (t & 3) * kTileLds);
         put(cv, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
-        cv = request(p.v, p.v_scales, next_k);
-        ck = request(p.k, p.k_scales, x);
+        cv = request(v_head, p.v_scales, next_k);
+        ck = request(k_head, p.k_scales, x);
         next_k = x;
         if (t + 2 < ntiles) first_frags();
       }
@@ -526,6 +541,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 
   // ---- epilogue -----------------------------------------------------------------------------------------------------
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // copies past the last tile
+  const PagedAttn a = arguments_again();
   __syncthreads();                                     // every wavefront is done with K and V
   if (c.parts > 1) {
     const int64_t at = (slot0 + pos) * kBM + wave * 32;
@@ -534,9 +550,9 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       const float l_tot = quad_sum(l_run[r]);
       if (wave * 32 + r * 16 + ln >= rows) continue;
       const int64_t row = at + r * 16 + ln;
-      if (lg == 0) p.part_ml[row] = f32x2{l_tot == 0.f ? -INFINITY : m_ref[r] * scale_log2, l_tot};
+      if (lg == 0) a.part_ml[row] = f32x2{l_tot == 0.f ? -INFINITY : m_ref[r] * scale_log2, l_tot};
 #pragma unroll
-      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(p.part_o + row * COLS + db * 16 + lg * 4) = o_acc[db][r];
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part_o + row * COLS + db * 16 + lg * 4) = o_acc[db][r];
     }
     return;
   }
@@ -547,8 +563,8 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     const int row = my_row0 + r * 16 + ln;
     if (lg == 0 && row < row0 + rows) {
       int of_group;
-      const int token = s.start + p.by_group.quotient(row, of_group);
-      p.lse[b * p.l_sb + (hk * p.G + of_group) * p.l_sh + token] = l_tot == 0.f ? -INFINITY : __builtin_fmaf(fast_log2(l_tot), kLn2, m_ref[r] * p.scale);
+      const int token = s.start + a.by_group.quotient(row, of_group);
+      a.lse[b * a.l_sb + (hk * a.G + of_group) * a.l_sh + token] = l_tot == 0.f ? -INFINITY : __builtin_fmaf(fast_log2(l_tot), kLn2, m_ref[r] * a.scale);
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
@@ -563,10 +579,10 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
   for (int it = 0; it < 8; ++it) {
     const int r = (lane >> 4) + 4 * it, row = my_row0 + r;
-    if (row < row0 + rows && chunk * 8 < p.D) {
+    if (row < row0 + rows && chunk * 8 < a.D) {
       int of_group;
-      const int token = s.start + p.by_group.quotient(row, of_group);
-      *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + (hk * p.G + of_group) * p.o_sh + chunk * 8) =
+      const int token = s.start + a.by_group.quotient(row, of_group);
+      *reinterpret_cast<u32x4*>(a.out + b * a.o_sb + (int64_t)token * a.o_ss + (hk * a.G + of_group) * a.o_sh + chunk * 8) =
           *reinterpret_cast<const u32x4*>(os + r * (kOStride * 2) + chunk * 16);
     }
   }
