@@ -532,9 +532,10 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
     p.few_rows = 0x7fffffff;
     launch(p, dtype == MHIP_E4M3, rows, st);
   } else {
-    // Packed sequences may be of either kind: two pairs of launches, one after the other on the stream, share the workspace.
-    p.few_rows = starts ? kFewRows : -1;
-    if (starts) launch(p, dtype == MHIP_E4M3, rows, st);
+    // Packed sequences may be of either kind, such as generate a token at a time and such as take a chunk: two pairs of launches, one
+    // after the other on the stream, share the workspace.
+    p.few_rows = starts && p.G <= kFewRows ? 16 * row_blocks(p.G) : -1;
+    if (p.few_rows > 0) launch(p, dtype == MHIP_E4M3, p.few_rows, st);
     paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st);
   }
   return launch_status();

@@ -83,7 +83,7 @@ __device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane) {
   return cut;
 }
 // Pieces (and those of items in more than one) before each lane's run of sequences.
-struct Layout { int per; int64_t before, mine, slots_before; };
+struct Layout { int per; int64_t before, mine, slots_before, slots; };
 __device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, int lane) {
   Layout y;
   y.per = (p.g.B + 63) / 64;
@@ -104,6 +104,7 @@ __device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, 
   }
   y.before = sum - y.mine;
   y.slots_before = sum_slots - slots;
+  y.slots = __shfl((long long)sum_slots, 63);
   return y;
 }
 // piece i of a sequence: K/V heads fastest (eight of them: one to an XCD's L2), then the row tiles, the last (longest) first
@@ -189,44 +190,49 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const uint32_t lds_rows = lds_smem + wave * 2048;    // the wavefront's 8 rows of a stage
   const int* table = p.g.table + b * p.g.t_sb;
-  // The four quarters of a tile, 16 keys (of one page) each; the wavefront's rows are in quarter wave / 2.  A look-up reads their
-  // table entries (of keys past the last one the last one's), settle() uses them.
-  // gone: four bits of each of the last eight tiles, that its quarters are not here.
-  struct Entries { int page[4], slot; };               // slot: of the wavefront's own quarter
+  // A wavefront's 8 rows of a tile lie in one page.  A look-up reads its table entry (past the last key the last key's), settle() uses
+  // it.  Pages that are not here are rare: whether there are any among the piece's is found out once, and only then every tile's four
+  // quarters of 16 keys are looked up; gone holds four bits of each of the last eight tiles, that its quarters are not here.
+  struct Entry { int page, slot; };
   struct Rows { int64_t at; int page, slot, held, bytes; };      // at: from the first row of the head; bytes: of the rows there are
   uint32_t gone = 0;
-  const int last_entry = seen_last > 0 ? p.g.by_page.quotient(seen_last - 1) : 0;
+  bool any_gone = false;
+  if (ntiles > 0) {
+    int rest;
+    const int first = p.g.by_page.quotient(t0 * kBN, rest);
+    const int end = (t0 + ntiles) * kBN < seen_last ? (t0 + ntiles) * kBN : seen_last, last = p.g.by_page.quotient(end - 1, rest);
+    bool missing = false;
+    for (int e = first + lane; e <= last; e += 64) missing = missing || (uint32_t)table[e] >= (uint32_t)p.g.pages;
+    any_gone = __builtin_amdgcn_ballot_w64(missing) != 0;
+  }
   auto look_up = [&](int t) {
-    Entries e;
-    int slot, index = p.g.by_page.quotient((t0 + t) * kBN, slot);
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      e.page[h] = uniform_load(table, index < last_entry ? index : last_entry);
-      if (h == wave >> 1) e.slot = slot + 8 * (wave & 1);
-      slot += 16;
-      if (slot >= p.g.page) { slot = 0; ++index; }
-    }
+    const int key = (t0 + t) * kBN + 8 * wave;
+    Entry e;
+    e.page = uniform_load(table, p.g.by_page.quotient(key < seen_last ? key : seen_last - 1, e.slot));
     return e;
   };
   const int row_step = (int)p.c_ss16 * 16, row_tail = p.D * 2 - row_step;        // (bf16)
-  auto settle = [&](int t, Entries e) {
-    asm volatile("" : "+s"(e.page[0]), "+s"(e.page[1]), "+s"(e.page[2]), "+s"(e.page[3]));      // waited for here
-    uint32_t bits = 0;
-    Rows x{0, 0, e.slot, 0, 0};
+  auto settle = [&](int t, Entry e) {
+    asm volatile("" : "+s"(e.page));                   // waited for here
     const int left = seen_last - ((t0 + t) * kBN + 8 * wave), held = left < 8 ? left : 8;
-    const bool some = t < ntiles && left > 0;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const bool here = (uint32_t)e.page[h] < (uint32_t)p.g.pages;
-      bits |= here ? 0u : 1u << h;
-      if (h == wave >> 1 && here && some) {
-        x.page = e.page[h];
-        x.held = held;
-        x.bytes = held * row_step + row_tail;
-      }
+    Rows x{0, 0, e.slot, 0, 0};
+    if ((uint32_t)e.page < (uint32_t)p.g.pages && t < ntiles && left > 0) {
+      x.page = e.page;
+      x.held = held;
+      x.bytes = held * row_step + row_tail;
     }
     x.at = row_offset(p, x.page, x.slot);
-    gone = (gone & ~(15u << (4 * (t & 7)))) | bits << (4 * (t & 7));
+    if (any_gone) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int key = (t0 + t) * kBN + 16 * h;
+        int slot;
+        const int page = uniform_load(table, p.g.by_page.quotient(key < seen_last ? key : seen_last - 1, slot));
+        bits |= (uint32_t)page < (uint32_t)p.g.pages ? 0u : 1u << h;
+      }
+      gone = (gone & ~(15u << (4 * (t & 7)))) | bits << (4 * (t & 7));
+    }
     return x;
   };
   int voff[2];                                         // bf16: of copy instruction u, 4 rows each
@@ -246,7 +252,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const int row8 = lane >> 3, col16 = (lane & 7) * 16;
   struct Codes { u32x4 w; float scale; };
   auto request = [&](const uint8_t* head, const float* scales, const Rows& x) {
-    Codes k{u32x4{}, 0.f};
+    Codes k{u32x4{}, 1.f};
     if (row8 < x.held && col16 < p.D) {
       k.w = *reinterpret_cast<const u32x4*>(head + x.at + row8 * (int)p.c_ss16 * 16 + col16);
       k.scale = scales[x.page * p.s_sp + (int64_t)(x.slot + row8) * p.s_ss + hk * p.s_sh];
@@ -256,11 +262,22 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   typedef __attribute__((address_space(3))) u32x4* lds_u32x4;
   auto put = [&](const Codes& k, uint32_t to) {
     u32x4 lo, hi;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], false), z = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], true);
-      const uint32_t w0 = pack_bf16(x[0] * k.scale, x[1] * k.scale), w1 = pack_bf16(z[0] * k.scale, z[1] * k.scale);
+    auto keep = [&](int i, uint32_t w0, uint32_t w1) {
       if (i < 2) { lo[2 * i] = w0; lo[2 * i + 1] = w1; } else { hi[2 * i - 4] = w0; hi[2 * i - 3] = w1; }
+    };
+    // scales 2^-126 .. 2^127 go into the conversion; others, and NaN, through fp32 and one rounding
+    const uint32_t bits = __builtin_bit_cast(uint32_t, k.scale);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x807fffffu) != 0 || bits - 0x00800000u >= 0x7f000000u) == 0, 1)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        keep(i, __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k.w[i], k.scale, false)),
+             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k.w[i], k.scale, true)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], false), z = __builtin_amdgcn_cvt_pk_f32_fp8(k.w[i], true);
+        keep(i, pack_bf16(x[0] * k.scale, x[1] * k.scale), pack_bf16(z[0] * k.scale, z[1] * k.scale));
+      }
     }
     const int swz = lds_row_swizzle(8 * wave + row8), chunk = (lane & 7) * 2;
     *(lds_u32x4)(uintptr_t)(to + row8 * 256 + ((chunk ^ swz) << 4)) = lo;
@@ -355,7 +372,10 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       nmsc[r] = fminf(-m_ref[r] * scale_log2, kMost);
     }
   };
-  constexpr int kEarlyPairs = 2;
+  // Up to 96 columns the matrix phase is the shorter one: it takes the tile copies of the vector phase then, and on 64 columns more of
+  // the exponentials.
+  constexpr bool kShortMatrix = COLS < 128;
+  constexpr int kEarlyPairs = COLS == 64 ? 6 : 2;
   auto sm_tile = [&]() {
 #pragma unroll
     for (int idx = kEarlyPairs; idx < kPairs; ++idx) sm_pair(idx);
@@ -403,6 +423,12 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     for (int i = 0; i < kFragDepth; ++i) frag[i] = read_frag(i);
   };
   auto early_slot = [](int idx) { return kSlotsS + DB + idx * (kSlotsO - DB) / kEarlyPairs; };
+  Rows next_v{}, next_k{};                             // of the tiles whose copies go out (e4m3: whose codes are put into LDS) next
+  auto copies = [&](int t) {                           // K(t + 4), V(t + 3)
+    copy_rows(k_head, next_k, lds_rows + (t & 3) * kTileLds);
+    copy_rows(v_head, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
+    next_v = next_k;
+  };
   auto matrix_phase = [&](int t) __attribute__((always_inline)) {
     const int k_step = stage_step(t + 1), v_step = stage_step(t);
 #pragma unroll
@@ -416,6 +442,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
         for (int e = 0; e < DB; ++e)
           if (e % kFragDepth == i - (kSlotsS + kSlotsO - kFragDepth)) v_a[e] += v_step;
       }
+      if (!E4M3 && kShortMatrix && i == 1) copies(t);
       if (i == kSlotsS) sm_mask(t + 1);
 #pragma unroll
       for (int idx = 0; idx < kEarlyPairs; ++idx)
@@ -425,6 +452,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   };
   // the same where tile t cuts
   auto matrix_phase_cut = [&](int t) __attribute__((always_inline)) {
+    if (!E4M3 && kShortMatrix) copies(t);
     pv_cut();
 #pragma unroll
     for (int i = 0; i < kSlotsS; ++i) {
@@ -448,7 +476,6 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(qf[r][ks]));      // loaded before the first copy goes out
     // Tiles 0 .. 3 of K and 0 .. 2 of V; in the loop K(t + 4) and V(t + 3) follow, whose places tile t's matrix phase and the one
     // before it were the last to read.  Codes that pass through registers are requested one tile before they are put there.
-    Rows next_v, next_k;                               // bf16: V(t + 3); e4m3: whose codes are in registers
     Codes ck, cv;
     if constexpr (!E4M3) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -459,6 +486,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
         if (t < 3) copy_rows(v_head, x, lds_rows + kVRing + t * kTileLds);
         next_v = x;
       }
+      next_k = settle(4, look_up(4));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     } else {
       Codes k[4], v[3];
@@ -498,16 +526,14 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) asm volatile("" : "+v"(sc[0][r]), "+v"(sc[MB - 1][r]));   // keeps the exponentials behind the barrier
       if constexpr (!E4M3) {
-        const Entries e = look_up(t + 4);
+        const Entry e = look_up(t + 5);
         sm_tile();
-        const Rows x = settle(t + 4, e);
-        copy_rows(k_head, x, lds_rows + (t & 3) * kTileLds);
-        copy_rows(v_head, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
-        next_v = x;
+        if (!kShortMatrix) copies(t);
+        next_k = settle(t + 5, e);
         if (t + 2 < ntiles) first_frags();
         asm volatile("s_waitcnt vmcnt(4)" ::: "memory");          // the four copies of one tile ago are done
       } else {
-        const Entries e = look_up(t + 5);
+        const Entry e = look_up(t + 5);
         sm_tile();
         const Rows x = settle(t + 5, e);
         put(ck, lds_rows + (t & 3) * kTileLds);
@@ -597,6 +623,7 @@ __global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, 
   const Cut cut = cut_of(p, lane);
   if (cut.total == 0) return;
   const Layout y = layout_of(p, cut, lane);
+  if (uniform64(y.slots) == 0) return;
   for (int k = 0; k < kJoinRows; ++k) {
     RowOf x;
     if (id0 + k >= n_rows) return;
