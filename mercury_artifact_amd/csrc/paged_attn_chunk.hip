@@ -159,7 +159,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const int hk = piece.hk, row0 = piece.rt * kBM;
   const int rows = s.n * p.G - row0 < kBM ? s.n * p.G - row0 : kBM;
   auto sees = [&](int row) {                           // keys that a row sees
-    return p.causal ? clamped(s.len - s.n + p.by_group.quotient(row) + 1, 0, s.len) : s.len;
+    return __builtin_amdgcn_readfirstlane(p.causal ? clamped(s.len - s.n + p.by_group.quotient(row) + 1, 0, s.len) : s.len);
   };
   const int seen_last = sees(row0 + rows - 1);
   const int64_t steps = (seen_last + kBN - 1) / kBN;
@@ -326,15 +326,20 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   auto cuts = [&](int t) { return (t0 + t + 1) * kBN > seen_first; };      // some row of the wavefront does not see some key
   auto sm_mask = [&](int t) {
     const uint32_t bits = gone >> (4 * (t & 7)) & 15u;
-    if (cuts(t) || bits) {
+    if (__builtin_expect(cuts(t) || bits, 0)) {
+      asm volatile("");                                // (a branch: not 32 selections on every tile)
       const int kv0 = (t0 + t) * kBN;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+        for (int mb = 0; mb < MB; ++mb) {
+          const int left = bits >> mb & 1 ? 0 : lim[r] - (kv0 + mb * 16) - lg * 4;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (kv0 + mb * 16 + lg * 4 + j >= lim[r] || (bits >> mb & 1)) sc[mb][r][j] = -INFINITY;
+            if (j >= left) sc[mb][r][j] = -INFINITY;
+          // (one comparison at a time: their masks would take the scalar registers that the loop's addresses are in)
+          __builtin_amdgcn_sched_barrier(0);
+        }
     }
   };
   auto sm_pair = [&](int idx) {
