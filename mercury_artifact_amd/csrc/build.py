@@ -26,7 +26,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall",
 # registers) there are no copies between the two register files in its main loop.
 # attn_fwd_fp8.hip: the form with one wavefront per SIMD would get accumulation registers and copy every score out of them.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-EXTRA_FLAGS = {"attn_bwd.hip": VGPR_FORM, "attn_fwd_fp8.hip": VGPR_FORM}
+EXTRA_FLAGS = {"attn_bwd.hip": VGPR_FORM, "attn_fwd_fp8.hip": VGPR_FORM, "paged_attn.hip": VGPR_FORM}
 
 
 def _run(cmd):

@@ -39,6 +39,10 @@ struct Entry {
   decltype(&mhip_pack_reduce) pack = nullptr;
   decltype(&mhip_unpack) unpack = nullptr;
   decltype(&mhip_quantize_e4m3) quantize = nullptr;
+  decltype(&mhip_paged_cache_write) paged_write = nullptr;
+  decltype(&mhip_paged_cache_read) paged_read = nullptr;
+  decltype(&mhip_paged_attn_workspace_bytes) paged_bytes = nullptr;
+  decltype(&mhip_paged_attn_fwd) paged_attn = nullptr;
   decltype(&mhip_error_string) error_string = nullptr;
 } entry;
 bool bound = false;
@@ -719,6 +723,157 @@ PyObject* quantize_e4m3(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// A paged cache (2, pages, page_size, Hkv, D) with its table and lengths, and what of it the entry points take.
+struct Paged {
+  const Tensor *cache, *scales, *table, *lengths, *starts;
+  int64_t B, pages, page, Hkv, D;
+  int type;
+  const char *k, *v;
+  float *ks = nullptr, *vs = nullptr;
+  int64_t s_sp = 0, s_ss = 0, s_sh = 0;
+  bool take(PyObject* cache_, PyObject* table_, PyObject* lengths_, PyObject* scales_, PyObject* starts_) {
+    cache = plain(cache_);
+    if (!cache || cache->dim() != 5 || cache->size(0) != 2 || cache->stride(4) != 1) return false;
+    const Tensor& c = *cache;
+    if (!optional(table_, c, table) || !optional(lengths_, c, lengths) || !optional(scales_, c, scales) || !optional(starts_, c, starts) ||
+        !table || !lengths)
+      return false;
+    pages = c.size(1); page = c.size(2); Hkv = c.size(3); D = c.size(4);
+    if (c.scalar_type() == at::kBFloat16) type = MHIP_BF16;
+    else if (c.scalar_type() == at::kFloat8_e4m3fn) type = MHIP_E4M3;
+    else return false;
+    if ((type == MHIP_E4M3) != (scales != nullptr)) return false;
+    if (scales && (scales->scalar_type() != at::kFloat || scales->sizes() != c.sizes().slice(0, 4))) return false;
+    if (lengths->dim() != 1 || lengths->scalar_type() != at::kInt || !lengths->is_contiguous()) return false;
+    B = lengths->size(0);
+    if (table->dim() != 2 || table->size(0) != B || table->scalar_type() != at::kInt || (table->size(1) > 1 && table->stride(1) != 1)) return false;
+    if (starts && (starts->dim() != 1 || starts->size(0) != B + 1 || starts->scalar_type() != at::kInt || !starts->is_contiguous())) return false;
+    if (!fits({B, pages, page, Hkv, D, table->size(1)}) || c.numel() == 0) return false;
+    k = static_cast<const char*>(c.data_ptr());
+    v = k + c.stride(0) * c.element_size();
+    if (scales) {
+      ks = floats(scales);
+      vs = ks + scales->stride(0);
+      s_sp = scales->stride(1); s_ss = scales->stride(2); s_sh = scales->stride(3);
+    }
+    return true;
+  }
+  // New tokens (B, n, heads, D), packed (T, heads, D), in bf16; n and T of them.
+  bool tokens(const Tensor& t, int64_t heads, int64_t& n, int64_t& T) const {
+    const int64_t d = starts ? 3 : 4;
+    if (t.dim() != d || t.device() != cache->device() || t.scalar_type() != at::kBFloat16 || t.stride(d - 1) != 1 || t.size(d - 1) != D ||
+        t.size(d - 2) != heads || (!starts && t.size(0) != B))
+      return false;
+    n = starts ? 0 : t.size(1);
+    T = starts ? t.size(0) : B * n;
+    return fits({heads, n, T});
+  }
+  int64_t stride(const Tensor& t, int i) const { return starts ? (i == 0 ? 0 : t.stride(i - 1)) : t.stride(i); }
+};
+
+// (k, v, cache, page_table, lengths, scales, starts) -> True
+PyObject* paged_cache_write(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ENTER(7);
+  Paged g;
+  const Tensor *k = plain(a[0]), *v = plain(a[1]);
+  int64_t n, T;
+  if (!k || !v || !g.take(a[2], a[3], a[4], a[5], a[6]) || !g.tokens(*k, g.Hkv, n, T) || !g.tokens(*v, g.Hkv, n, T) || k->sizes() != v->sizes()) SLOW;
+  OnDevice on(*k);
+  if (!on.current) SLOW;
+  const int code = without_gil([&] {
+    return entry.paged_write(k->data_ptr(), v->data_ptr(), const_cast<char*>(g.k), const_cast<char*>(g.v), g.ks, g.vs,
+                             static_cast<const int*>(g.table->data_ptr()), static_cast<const int*>(g.lengths->data_ptr()),
+                             static_cast<const int*>(data(g.starts)), g.B, n, T, g.Hkv, g.D, g.pages, g.page, g.table->size(1),
+                             g.table->stride(0), g.stride(*k, 0), g.stride(*k, 1), g.stride(*k, 2), g.stride(*v, 0), g.stride(*v, 1),
+                             g.stride(*v, 2), g.cache->stride(1), g.cache->stride(2), g.cache->stride(3), g.s_sp, g.s_ss, g.s_sh, g.type,
+                             on.stream);
+  });
+  if (code != MHIP_OK) return refused(code, "mhip_paged_cache_write");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache, page_table, lengths, rows, begin, scales, out) -> out
+PyObject* paged_cache_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ENTER(7);
+  Paged g;
+  if (!g.take(a[0], a[1], a[2], a[5], Py_None)) SLOW;
+  const Tensor* given;
+  if (!PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[4]) || !optional(a[6], *g.cache, given)) SLOW;
+  const long rows = PyLong_AsLong(a[3]), begin = PyLong_AsLong(a[4]);
+  if ((rows == -1 || begin == -1) && PyErr_Occurred()) { PyErr_Clear(); SLOW; }
+  if (rows < 0 || begin < 0 || !fits({rows, begin})) SLOW;
+  if (given && (given->dim() != 5 || given->size(0) != 2 || given->size(1) != g.B || given->size(2) != rows || given->size(3) != g.Hkv ||
+                given->size(4) != g.D || given->scalar_type() != at::kBFloat16 || given->stride(4) != 1))
+    SLOW;
+  OnDevice on(*g.cache);
+  if (!on.current) SLOW;
+  Tensor out;
+  const int code = without_gil([&] {
+    out = given ? *given : at::empty({2, g.B, rows, g.Hkv, g.D}, g.cache->options().dtype(at::kBFloat16).requires_grad(false));
+    return entry.paged_read(g.k, g.v, g.ks, g.vs, static_cast<const int*>(g.table->data_ptr()), static_cast<const int*>(g.lengths->data_ptr()),
+                            out.data_ptr(), g.B, begin, rows, g.Hkv, g.D, g.pages, g.page, g.table->size(1), g.table->stride(0),
+                            g.cache->stride(1), g.cache->stride(2), g.cache->stride(3), g.s_sp, g.s_ss, g.s_sh, out.stride(0), out.stride(1),
+                            out.stride(2), out.stride(3), g.type, on.stream);
+  });
+  if (code != MHIP_OK) return refused(code, "mhip_paged_cache_read");
+  return give(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse) -> (out, lse)
+PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ENTER(11);
+  Paged g;
+  const Tensor* q = plain(a[0]);
+  if (!q || q->dim() < 3 || !g.take(a[1], a[2], a[3], a[6], a[7])) SLOW;
+  const int64_t Hq = q->size(q->dim() - 2);
+  int64_t n, T;
+  if (!g.tokens(*q, Hq, n, T) || Hq == 0 || g.Hkv == 0 || Hq % g.Hkv) SLOW;
+  const double scale = PyFloat_AsDouble(a[4]);
+  if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); SLOW; }
+  const int causal = PyObject_IsTrue(a[5]);
+  if (causal < 0) { PyErr_Clear(); SLOW; }
+  int64_t most = g.starts ? T : n;
+  if (g.starts && a[8] != Py_None) {
+    if (!PyLong_CheckExact(a[8])) SLOW;
+    const long given = PyLong_AsLong(a[8]);
+    if (given == -1 && PyErr_Occurred()) { PyErr_Clear(); SLOW; }
+    if (given < 0) SLOW;
+    if (given < most) most = given;
+  }
+  const Tensor *out_given, *lse_given;
+  if (!optional(a[9], *q, out_given) || !optional(a[10], *q, lse_given)) SLOW;
+  int64_t n2, T2;
+  if (out_given && (!g.tokens(*out_given, Hq, n2, T2) || out_given->sizes() != q->sizes())) SLOW;
+  if (lse_given && (lse_given->scalar_type() != at::kFloat || !lse_given->is_contiguous() ||
+                    !(g.starts ? lse_given->dim() == 2 && lse_given->size(0) == Hq && lse_given->size(1) == T : shape3(*lse_given, g.B, Hq, n))))
+    SLOW;
+  OnDevice on(*q);
+  if (!on.current) SLOW;
+  const int64_t bytes = entry.paged_bytes(most, Hq, g.Hkv, g.D);
+  if (bytes < 0) SLOW;
+  Tensor out, lse, workspace;
+  const int code = without_gil([&] {
+    const auto options = q->options().requires_grad(false);
+    out = out_given ? *out_given : at::empty(q->sizes(), options);
+    lse = lse_given ? *lse_given : g.starts ? at::empty({Hq, T}, options.dtype(at::kFloat)) : at::empty({g.B, Hq, n}, options.dtype(at::kFloat));
+    workspace = at::empty({bytes}, options.dtype(at::kByte));
+    return entry.paged_attn(q->data_ptr(), g.k, g.v, g.ks, g.vs, static_cast<const int*>(g.table->data_ptr()),
+                            static_cast<const int*>(g.lengths->data_ptr()), static_cast<const int*>(data(g.starts)), out.data_ptr(),
+                            floats(&lse), g.B, n, T, most, Hq, g.Hkv, g.D, g.pages, g.page, g.table->size(1), g.table->stride(0),
+                            g.stride(*q, 0), g.stride(*q, 1), g.stride(*q, 2), g.cache->stride(1), g.cache->stride(2), g.cache->stride(3),
+                            g.s_sp, g.s_ss, g.s_sh, g.stride(out, 0), g.stride(out, 1), g.stride(out, 2), (float)scale,
+                            causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, workspace.data_ptr(), on.stream);
+  });
+  if (code != MHIP_OK) return refused(code, "mhip_paged_attn_fwd");
+  return give2(out, lse);
+  END_HANDLE_TH_ERRORS
+}
+
 // ({name: address}) of the library's entry points
 PyObject* bind(PyObject*, PyObject* table) {
   auto get = [&](const char* name) -> void* {
@@ -734,7 +889,9 @@ PyObject* bind(PyObject*, PyObject* table) {
                   take(entry.bwd_many, "mhip_attn_bwd_chunks") && take(entry.bwd_take, "mhip_attn_bwd_take") &&
                   take(entry.merge, "mhip_lse_merge") && take(entry.many, "mhip_lse_merge_many") &&
                   take(entry.pack, "mhip_pack_reduce") && take(entry.unpack, "mhip_unpack") &&
-                  take(entry.quantize, "mhip_quantize_e4m3") && take(entry.error_string, "mhip_error_string");
+                  take(entry.quantize, "mhip_quantize_e4m3") &&
+                  take(entry.paged_write, "mhip_paged_cache_write") && take(entry.paged_read, "mhip_paged_cache_read") &&
+                  take(entry.paged_bytes, "mhip_paged_attn_workspace_bytes") && take(entry.paged_attn, "mhip_paged_attn_fwd") && take(entry.error_string, "mhip_error_string");
   if (PyErr_Occurred()) return nullptr;
   bound = ok;
   return PyBool_FromLong(ok);
@@ -744,6 +901,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 PyMethodDef methods[] = {
     FAST(undispatched), FAST(written), FAST(apart), FAST(rows_fit), FAST(fwd_block), FAST(fwd_group), FAST(fwd_chain), FAST(fwd_blocks), FAST(no_dropout), FAST(bwd_block),
     FAST(bwd_chunk), FAST(bwd_group), FAST(bwd_chunks), FAST(merge_into), FAST(merge_many), FAST(pack_block), FAST(unpack_into), FAST(quantize_e4m3),
+    FAST(paged_cache_write), FAST(paged_cache_read), FAST(paged_attn_fwd),
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mercury_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -23,25 +23,23 @@ namespace {
 
 typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i32x2;
 
-constexpr int kWaves = 4;
 constexpr int kKeys = 32;                  // keys of a tile, one wavefront's
-constexpr int kUnit = kWaves * kKeys;      // and of a unit of work
 constexpr int kRing = 32768;               // bytes of K and V tiles of a wavefront
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
-constexpr int kWorkgroups = 256;           // one per CU
+constexpr int kWavefronts = 1024;          // of the launch: four on a CU, in workgroups of four or two
 constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
 struct Item { int rts; int64_t steps; };   // row tiles of a sequence and K/V head, units of each
-template <int ROWS>
+template <int ROWS, int UNIT>
 __device__ __forceinline__ Item item_of(const PagedAttn& p, const PagedSeq& s) {
   Item it;
   it.rts = s.n * p.G <= p.few_rows ? (s.n * p.G + ROWS - 1) / ROWS : 0;
-  it.steps = s.len > kUnit ? (s.len + kUnit - 1) / kUnit : 1;
+  it.steps = s.len > UNIT ? (s.len + UNIT - 1) / UNIT : 1;
   return it;
 }
-template <int ROWS, bool UNIFORM>
+template <int ROWS, int UNIT, bool UNIFORM>
 __device__ __forceinline__ int64_t units_of(const PagedAttn& p, int b) {
-  const Item it = item_of<ROWS>(p, paged_seq<UNIFORM>(p.g, b));
+  const Item it = item_of<ROWS, UNIT>(p, paged_seq<UNIFORM>(p.g, b));
   return it.steps * it.rts * p.Hkv;
 }
 
@@ -50,13 +48,13 @@ struct Plan {
   int per;                   // sequences of a lane
   int64_t before, mine, total;
 };
-template <int ROWS>
+template <int ROWS, int UNIT>
 __device__ __forceinline__ Plan plan_of(const PagedAttn& p, int lane) {
   Plan plan;
   plan.per = (p.g.B + 63) / 64;
   plan.mine = 0;
   for (int j = 0; j < plan.per; ++j)
-    if (lane * plan.per + j < p.g.B) plan.mine += units_of<ROWS, false>(p, lane * plan.per + j);
+    if (lane * plan.per + j < p.g.B) plan.mine += units_of<ROWS, UNIT, false>(p, lane * plan.per + j);
   int64_t sum = plan.mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -72,9 +70,9 @@ __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks 
   return ROWB == 256 ? lds_row_swizzle_16(row) : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-template <bool E4M3, int COLS, int NR>
-__global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn p) {
-  constexpr int ROWS = 16 * NR;
+template <bool E4M3, int COLS, int NR, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn p) {
+  constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys;
   constexpr int kSize = E4M3 ? 1 : 2;
   constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
   constexpr int kChunks = ROWB / 16;
@@ -85,11 +83,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
   constexpr int kStage = 2 * kTileBytes + (E4M3 ? 256 : 0);      // K, V, 32 scales of each
   constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
   constexpr int KB = COLS / 32, DB = COLS / 16;
+  constexpr int kPair = NR < 2 ? NR : 2;               // blocks of rows that are worked on together
   constexpr int kRegion = kStages * kStage;
   static_assert(ROWS * COLS * 4 <= kRegion, "a wavefront's O takes the place of its ring");
   static_assert(kStages * (nK + nV) < 64, "copies in flight are counted in 6 bits");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[kWaves * kRegion];
-  __shared__ f32x2 stats[kWaves][ROWS];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[WAVES * kRegion];
+  __shared__ f32x2 stats[WAVES][ROWS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
@@ -97,7 +96,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
   // ---- this workgroup's share ------------------------------------------------------------------------------
   // (workgroups of one XCD take neighbouring shares)
   const int w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  const Plan plan = plan_of<ROWS>(p, lane);
+  const Plan plan = plan_of<ROWS, UNIT>(p, lane);
   const int64_t total = uniform64(plan.total);
   const int64_t shares = total < (int64_t)gridDim.x ? total : gridDim.x;
   if (w >= shares) return;
@@ -106,7 +105,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
   const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= plan.before && lo < plan.before + plan.mine));
   int b = owner * plan.per;
   int64_t pos = lo - uniform64(__shfl((long long)plan.before, owner));     // inside sequence b
-  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<ROWS, true>(p, b)); ++b) pos -= u;
+  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<ROWS, UNIT, true>(p, b)); ++b) pos -= u;
 
   // ---- what does not change from segment to segment -----------------------------------------------------------
   const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
@@ -158,7 +157,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
 
   for (;;) {
     const PagedSeq s = paged_seq<true>(p.g, b);
-    const Item it = item_of<ROWS>(p, s);
+    const Item it = item_of<ROWS, UNIT>(p, s);
     const int64_t item = pos / it.steps;
     const int first = (int)(pos - item * it.steps);
     const int64_t left = hi - lo;
@@ -185,12 +184,14 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
       }
     }
     // keys that all rows see, and that some row sees
-    const int seen_first = p.causal ? clamped(s.len - s.n + p.by_group.quotient(row0) + 1, 0, s.len) : s.len;
-    const int seen_last = p.causal ? clamped(s.len - s.n + p.by_group.quotient(row0 + rows - 1) + 1, 0, s.len) : s.len;
+    auto sees = [&](int row) {
+      return __builtin_amdgcn_readfirstlane(p.causal ? clamped(s.len - s.n + p.by_group.quotient(row) + 1, 0, s.len) : s.len);
+    };
+    const int seen_first = sees(row0), seen_last = sees(row0 + rows - 1);
 
     // ---- copies of tile t of this wavefront, 16 keys (of one page) at a time -----------------------------------------
     const int* table = p.g.table + b * p.g.t_sb;
-    auto key_of = [&](int t) { return ((first + t) * kWaves + wave) * kKeys; };
+    auto key_of = [&](int t) { return ((first + t) * WAVES + wave) * kKeys; };
     int page[2], slot[2], held[2];                     // of the tile whose copies go out next
     auto look_up = [&](int t) {
 #pragma unroll
@@ -239,6 +240,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db][r] = f32x4{};
     }
+    look_up(0);                                        // (on its way with Q)
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int t = 0; t < kStages; ++t) {
-      look_up(t);
+      if (t > 0) look_up(t);
       settle(t);
       copy_k(t);
       copy_v(t);
@@ -257,112 +259,123 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
       const int stage = t % kStages, at = stage * kStage, key0 = key_of(t);
       const uint32_t hidden = gone >> (2 * stage) & 3u;
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"(nV + (kStages - 1) * (nK + nV)) : "memory");     // K of tile t is there
-      f32x4 sc[2][NR];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < KR; ++i) {
-          const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
-#pragma unroll
-          for (int e = 0; e < KB / KR; ++e) {
-            const bf16x8 kf = E4M3 ? codes_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
-            const int ks = E4M3 ? 2 * i + e : i;
-#pragma unroll
-            for (int r = 0; r < NR; ++r) sc[kb][r] = mfma(kf, qf[r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
-          }
-        }
-      f32x4 k_scale[2], v_scale[2];
-      if constexpr (E4M3)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          k_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + kb * 64 + lg * 16);
-          v_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + 128 + kb * 64 + lg * 16);
-          asm volatile("" : "+v"(k_scale[kb]), "+v"(v_scale[kb]));
-        }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the tile has been read: its place can be filled
-      settle(stage);
-      copy_k(stage);
-
-      // ---- softmax --------------------------------------------------------------------------------------------
       const bool cut = key0 + kKeys > seen_first;                // some row does not see some key
-      u32x4 pw[NR];
-      bool moved = false;
-      float alpha[NR];
+      f32x4 k_scale[2], v_scale[2];
+      // Two blocks of rows at a time: with all four of 64 rows the registers run out.  The second time K and V are read from LDS again.
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
+      for (int r0 = 0; r0 < NR; r0 += kPair) {
+        f32x4 sc[2][kPair];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[kb][r][j] *= E4M3 ? p.scale_log2 * k_scale[kb][j] : p.scale_log2;
-        if (cut || hidden) {
+          for (int i = 0; i < KR; ++i) {
+            const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
+#pragma unroll
+            for (int e = 0; e < KB / KR; ++e) {
+              const bf16x8 kf = E4M3 ? codes_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
+              const int ks = E4M3 ? 2 * i + e : i;
+#pragma unroll
+              for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
+            }
+          }
+        if (E4M3 && r0 == 0)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            k_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + kb * 64 + lg * 16);
+            v_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + 128 + kb * 64 + lg * 16);
+            asm volatile("" : "+v"(k_scale[kb]), "+v"(v_scale[kb]));
+          }
+        if (r0 + kPair >= NR) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the tile has been read: its place can be filled
+          settle(stage);
+          copy_k(stage);
+        }
+
+        // ---- softmax --------------------------------------------------------------------------------------------
+        u32x4 pw[kPair];
+        bool moved = false;
+        float alpha[kPair];
+#pragma unroll
+        for (int r = 0; r < kPair; ++r) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (key0 + 16 * kb + 4 * lg + j >= lim[r] || (hidden >> kb & 1)) sc[kb][r][j] = -INFINITY;
+            for (int j = 0; j < 4; ++j) sc[kb][r][j] *= E4M3 ? p.scale_log2 * k_scale[kb][j] : p.scale_log2;
+          if (cut || hidden) {
+            asm volatile("");
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              const int left = hidden >> kb & 1 ? 0 : lim[r0 + r] - (key0 + 16 * kb) - 4 * lg;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j >= left) sc[kb][r][j] = -INFINITY;
+            }
+          }
+          float top = sc[0][r][0];
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[kb][r][j]);
+          top = fmaxf(quad_max(top), m[r0 + r]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          alpha[r] = fast_exp2(m[r0 + r] - ref);
+          moved = moved || !(m[r0 + r] == top);
+          m[r0 + r] = top;
+          float x[8], sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = fast_exp2(sc[i >> 2][r][i & 3] - ref);
+            sum += x[i];
+          }
+          l[r0 + r] = l[r0 + r] * alpha[r] + sum;
+          if constexpr (E4M3)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
         }
-        float top = sc[0][r][0];
+        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int r = 0; r < kPair; ++r)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[kb][r][j]);
-        top = fmaxf(quad_max(top), m[r]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        alpha[r] = fast_exp2(m[r] - ref);
-        moved = moved || !(m[r] == top);
-        m[r] = top;
-        float x[8], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = fast_exp2(sc[i >> 2][r][i & 3] - ref);
-          sum += x[i];
+            for (int db = 0; db < DB; ++db) o[db][r0 + r] *= alpha[r];
         }
-        l[r] = l[r] * alpha[r] + sum;
-        if constexpr (E4M3)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-      }
-      if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) o[db][r] *= alpha[r];
-      }
 
-      // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
-      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(nK + (kStages - 1) * (nK + nV)) : "memory");     // V of tile t is there
-      if (!(cut && seen_first < seen_last)) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const bf16x8 vf = read_v(db, at);
-#pragma unroll
-          for (int r = 0; r < NR; ++r) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
-        }
-      } else {
-        // (some rows do not see some of the keys: see finite_part)
-        uint32_t odd = 0;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, finite_part(__builtin_bit_cast(u32x4, read_v(db, at)), odd));
-#pragma unroll
-          for (int r = 0; r < NR; ++r) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+        // ---- O^T += V^T P^T ---------------------------------------------------------------------------------------
+        if (r0 == 0)                                             // V of tile t is there
+          asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NR <= kPair ? nK : 0) + (kStages - 1) * (nK + nV)) : "memory");
+        if (!(cut && seen_first < seen_last)) {
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, at))));
+            const bf16x8 vf = read_v(db, at);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              const f32x4 counts = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[r])), f32x4{});
+            for (int r = 0; r < kPair; ++r) o[db][r0 + r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r0 + r]);
+          }
+        } else {
+          // (some rows do not see some of the keys: see finite_part)
+          uint32_t odd = 0;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) o[db][r][j] = with_odd(o[db][r][j], counts[j]);
-            }
+          for (int db = 0; db < DB; ++db) {
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, finite_part(__builtin_bit_cast(u32x4, read_v(db, at)), odd));
+#pragma unroll
+            for (int r = 0; r < kPair; ++r) o[db][r0 + r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r0 + r]);
             __builtin_amdgcn_sched_barrier(0);
           }
+          if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, at))));
+#pragma unroll
+              for (int r = 0; r < kPair; ++r) {
+                const f32x4 counts = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[r])), f32x4{});
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[db][r0 + r][j] = with_odd(o[db][r0 + r][j], counts[j]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         }
+        if (NR > kPair) __builtin_amdgcn_sched_barrier(0);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       copy_v(stage);
@@ -384,21 +397,21 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
     const bool whole = count == it.steps;
     const int64_t slot_of = 2 * (int64_t)w + (first == 0 ? 1 : 0);
 #pragma unroll
-    for (int i = 0; i < ROWS * COLS / 4 / (kWaves * 64); ++i) {
-      const int unit = i * (kWaves * 64) + threadIdx.x;
+    for (int i = 0; i < ROWS * COLS / 4 / (WAVES * 64); ++i) {
+      const int unit = i * (WAVES * 64) + threadIdx.x;
       const int row = unit / (COLS / 4), c4 = unit % (COLS / 4);
       if (row >= rows) continue;
-      f32x2 st[kWaves];
+      f32x2 st[WAVES];
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
+      for (int v = 0; v < WAVES; ++v) {
         st[v] = stats[v][row];
         top = fmaxf(top, st[v][0]);
       }
       const float ref = top == -INFINITY ? 0.f : top;
       f32x4 acc{};
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
+      for (int v = 0; v < WAVES; ++v) {
         const float weight = fast_exp2(st[v][0] - ref);
         sum += st[v][1] * weight;
         acc += *reinterpret_cast<const f32x4*>(smem + v * kRegion + row * (COLS * 4) + ((c4 ^ (row & 15)) << 4)) * weight;
@@ -422,42 +435,60 @@ __global__ __launch_bounds__(kWaves * 64, 1) void paged_attn_few(const PagedAttn
     if (lo >= hi) break;
     if (pos >= it.steps * it.rts * p.Hkv) {
       pos = 0;
-      for (++b; b + 1 < p.g.B && units_of<ROWS, true>(p, b) == 0;) ++b;
+      for (++b; b + 1 < p.g.B && units_of<ROWS, UNIT, true>(p, b) == 0;) ++b;
     }
     __syncthreads();
   }
 }
 
-// The rows that several workgroups shared, a wavefront each.
-template <int COLS, int ROWS>
-__global__ __launch_bounds__(256) void paged_attn_few_join(const PagedAttn p, int64_t n_rows, int workgroups) {
+// The rows that several workgroups shared, a wavefront each; where there are many it does `each` of them, counting the units once.
+template <int COLS, int ROWS, int UNIT>
+__global__ __launch_bounds__(256) void paged_attn_few_join(const PagedAttn p, int64_t n_rows, int workgroups, int each) {
   const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  RowOf x;
-  if (id >= n_rows || !row_of(p, (int)id, lane, x) || x.s.n * p.G > p.few_rows) return;
-  const int rt = x.r / ROWS, row = x.r % ROWS;
-  const Plan plan = plan_of<ROWS>(p, lane);
-  const int64_t total = uniform64(plan.total);
-  int64_t before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
-  for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, true>(p, c);
-  const Item it = item_of<ROWS>(p, x.s);
-  const int64_t u0 = before + ((int64_t)x.hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
-  const int64_t shares = total < workgroups ? total : workgroups;
-  const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
-  if (w0 == w1) return;                                // one workgroup had all of it
-  join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.token, x.head);
+  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
+  const Plan plan = plan_of<ROWS, UNIT>(p, lane);
+  const int64_t total = uniform64(plan.total), shares = total < workgroups ? total : workgroups;
+  for (int k = 0; k < each; ++k) {
+    RowOf x;
+    if (id0 + k >= n_rows) return;
+    if (!row_of(p, (int)(id0 + k), lane, x) || x.s.n * p.G > p.few_rows) continue;
+    const int rt = x.r / ROWS, row = x.r % ROWS;
+    int64_t before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
+    for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, UNIT, true>(p, c);
+    const Item it = item_of<ROWS, UNIT>(p, x.s);
+    const int64_t u0 = before + ((int64_t)x.hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
+    const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
+    if (w0 == w1) continue;                            // one workgroup had all of it
+    join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.token, x.head);
+  }
 }
 
 // Tiles of 16, 32 or 64 rows: the least that holds the rows of a sequence with `most` new tokens.
 int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-int64_t few_bytes(int64_t rows, int D) { return 2 * kWorkgroups * 16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4; }
+// Workgroups of four wavefronts, one to a CU, or of two, two to a CU: the pair covers the one's pauses between items (Q, the first tiles,
+// the wavefronts' results) with the other's reading, and costs twice as many partial results.  Items to a workgroup decide; us, four / two:
+//   items   8: 1 x 131072 H32/8 102.3 / 104.6, 8 tokens at 32768 34.9 / 38.0       16: 8 x 8192 H16/2 D64 e4m3 24.4 / 25.3
+//          32: 4 x 131072 H32/8 e4m3 194.3 / 201.4    128: 16 x 211 .. 4099 H16/8 D80 36.5 / 30.3    256: 32 x 300 .. 16384 H32/8 203.8 / 203.8
+//         512: 64 x 100 .. 2048 H32/8 68.0 / 62.3, e4m3 66.5 / 55.6                 2048: 256 x 20 .. 512 H32/8 90.7 / 78.2
+constexpr int64_t kManyItems = 128;
 
-template <bool E4M3, int COLS, int NR>
+// One partial result at each end of a workgroup's share.
+int64_t few_bytes(int64_t rows, int D) { return kWavefronts * 16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4; }
+
+template <bool E4M3, int COLS, int NR, int WAVES>
 void launch_few(PagedAttn p, hipStream_t st) {
-  p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)kWorkgroups * 16 * NR * COLS);
-  hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR>), dim3(kWorkgroups), dim3(kWaves * 64), 0, st, p);
+  constexpr int workgroups = kWavefronts / WAVES;
+  p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)workgroups * 16 * NR * COLS);
+  hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR, WAVES>), dim3(workgroups), dim3(WAVES * 64), 0, st, p);
   const int64_t n_rows = (int64_t)p.g.T * p.Hq;
-  hipLaunchKernelGGL((paged_attn_few_join<COLS, 16 * NR>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p, n_rows, kWorkgroups);
+  const int each = join_rows(n_rows);
+  hipLaunchKernelGGL((paged_attn_few_join<COLS, 16 * NR, WAVES * kKeys>), dim3((unsigned)((n_rows + 4 * each - 1) / (4 * each))), dim3(256), 0,
+                     st, p, n_rows, workgroups, each);
+}
+template <bool E4M3, int COLS, int NR>
+void launch_few(const PagedAttn& p, hipStream_t st) {
+  if ((int64_t)p.g.B * p.Hkv >= kManyItems) launch_few<E4M3, COLS, NR, 2>(p, st);
+  else launch_few<E4M3, COLS, NR, 4>(p, st);
 }
 template <bool E4M3, int COLS>
 void launch_rows(const PagedAttn& p, int64_t rows, hipStream_t st) {

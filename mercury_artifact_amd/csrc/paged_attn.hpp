@@ -78,29 +78,43 @@ __device__ __forceinline__ int64_t row_offset(const PagedAttn& p, int page, int 
   return (int64_t)(((uint64_t)(uint32_t)page * p.c_sp16 + (uint64_t)((uint32_t)slot * p.c_ss16)) << 4);
 }
 
-// One row from its partial results, the slot of number k at at(k): a wavefront, two columns a lane.
+// One row from its partial results, the slot of number k at at(k): a wavefront, two columns a lane.  The weights are found by a
+// lane each, so that the rows' loads wait for nothing.
 template <int COLS, class At>
 __device__ __forceinline__ void join_row(const PagedAttn& p, int lane, int n_parts, At at, int b, int token, int head) {
   float top = -INFINITY;
-  for (int k = lane; k < n_parts; k += 64) top = fmaxf(top, p.part_ml[at(k)][0]);
+  f32x2 ml = {-INFINITY, 0.f};
+  for (int k = lane; k < n_parts; k += 64) {
+    ml = p.part_ml[at(k)];
+    top = fmaxf(top, ml[0]);
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   const float ref = top == -INFINITY ? 0.f : top;
-  const int col = lane * 2;
+  const int col = lane * 2 < COLS ? lane * 2 : 0;
   float sum = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < n_parts; ++k) {
-    const f32x2 ml = p.part_ml[at(k)];
+  for (int k0 = 0; k0 < n_parts; k0 += 64) {
+    if (n_parts > 64) ml = k0 + lane < n_parts ? p.part_ml[at(k0 + lane)] : f32x2{-INFINITY, 0.f};
     const float weight = fast_exp2(ml[0] - ref);
     sum += ml[1] * weight;
-    if (col < COLS) {
-      const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_o + at(k) * COLS + col);
-      a0 += x[0] * weight;
-      a1 += x[1] * weight;
+    const int here = n_parts - k0 < 64 ? n_parts - k0 : 64;
+    for (int k = 0; k < here; k += 8) {
+      f32x2 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        x[u] = *reinterpret_cast<const f32x2*>(p.part_o + at(k0 + (k + u < here ? k + u : here - 1)) * COLS + col);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k + u));
+        a0 += k + u < here ? x[u][0] * w : 0.f;        // (past the last part its row again, which may hold an infinity)
+        a1 += k + u < here ? x[u][1] * w : 0.f;
+      }
     }
   }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (col < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
+  if (lane * 2 < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
   if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
 }
 
@@ -123,6 +137,9 @@ __device__ __forceinline__ bool row_of(const PagedAttn& p, int id, int lane, Row
   x.token = x.s.start + i;
   return true;
 }
+
+// Rows of a wavefront of the last step: one while there are CUs without any, up to eight.
+inline int join_rows(int64_t n_rows) { return n_rows <= 8192 ? 1 : n_rows >= 65536 ? 8 : (int)(n_rows / 8192); }
 
 int64_t paged_attn_chunk_bytes(int D);
 void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);

@@ -619,17 +619,16 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   }
 }
 
-// The rows that several workgroups shared, a wavefront each; a wavefront does eight, so that it counts the pieces once for them.
-constexpr int kJoinRows = 8;
+// The rows that several workgroups shared, a wavefront each; where there are many it does `each` of them, counting the pieces once.
 template <int COLS>
-__global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows) {
+__global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows, int each) {
   const int lane = threadIdx.x & 63;
-  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kJoinRows;
+  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
   const Cut cut = cut_of(p, lane);
   if (cut.total == 0) return;
   const Layout y = layout_of(p, cut, lane);
   if (uniform64(y.slots) == 0) return;
-  for (int k = 0; k < kJoinRows; ++k) {
+  for (int k = 0; k < each; ++k) {
     RowOf x;
     if (id0 + k >= n_rows) return;
     if (!row_of(p, (int)(id0 + k), lane, x)) continue;
@@ -649,9 +648,10 @@ __global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, 
 template <bool E4M3, int COLS>
 void launch(const PagedAttn& p, hipStream_t st) {
   const int64_t n_rows = (int64_t)p.g.T * p.Hq, rows = (int64_t)p.g.T * p.G;
+  const int each = join_rows(n_rows);
   const int64_t items = p.Hkv * (p.g.starts ? rows / kBM + p.g.B : p.g.B * (((int64_t)p.g.n * p.G + kBM - 1) / kBM));
   hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)(items + kParts)), dim3(512), 0, st, p);
-  hipLaunchKernelGGL((paged_attn_chunk_join<COLS>), dim3((unsigned)((n_rows + 4 * kJoinRows - 1) / (4 * kJoinRows))), dim3(256), 0, st, p, n_rows);
+  hipLaunchKernelGGL((paged_attn_chunk_join<COLS>), dim3((unsigned)((n_rows + 4 * each - 1) / (4 * each))), dim3(256), 0, st, p, n_rows, each);
 }
 template <bool E4M3>
 void launch(const PagedAttn& p, hipStream_t st) {

@@ -94,6 +94,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, pag
     own, the least power of two that keeps its largest value within 448; a row with an infinity or a NaN gets the scale NaN
     and reads back as NaN.  Rows of pages that are not here are dropped.  No two new tokens of a call may lie in one row
     (sequences that share the page they write to)."""
+    if N.host.paged_cache_write(k, v, cache, page_table, lengths, scales, starts):
+        return
     B = _check_cache(cache, scales, page_table, lengths, starts)
     _, pages, page_size, Hkv, D = cache.shape
     n, T = _check_tokens("k", k, B, starts, Hkv, D, cache.device)
@@ -113,6 +115,9 @@ def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: tor
                      scales: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows ``begin`` up to ``begin + rows`` of every sequence as a chunk ``(2, B, rows, Hkv, D)`` in bfloat16, as the ring
     steps take it; zeros past a sequence's end and where a page is not here."""
+    done = N.host.paged_cache_read(cache, page_table, lengths, rows, begin, scales, out)
+    if done is not None:
+        return done
     B = _check_cache(cache, scales, page_table, lengths)
     _, pages, page_size, Hkv, D = cache.shape
     if out is None:
@@ -138,6 +143,9 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     (B, Hq, n) -- packed: (Hq, T) -- in float32.  ``causal``: new token i of n sees the keys up to ``lengths - n + i``, else all
     of them.  Rows that see no key get 0 and -inf.  ``most_new``: with ``starts``, about how many new tokens a sequence has at
     most (default: all of them in one); it chooses the form of the kernels, the result does not depend on it."""
+    done = N.host.paged_attn_fwd(q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse)
+    if done is not None:
+        return done
     B = _check_cache(cache, scales, page_table, lengths, starts)
     _, pages, page_size, Hkv, D = cache.shape
     Hq = q.shape[-2] if q.dim() >= 2 else 0
