@@ -448,18 +448,25 @@ __global__ __launch_bounds__(256) void paged_attn_few_join(const PagedAttn p, in
   const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
   const Plan plan = plan_of<ROWS, UNIT>(p, lane);
   const int64_t total = uniform64(plan.total), shares = total < workgroups ? total : workgroups;
-  for (int k = 0; k < each; ++k) {
-    RowOf x;
-    if (id0 + k >= n_rows) return;
-    if (!row_of(p, (int)(id0 + k), lane, x) || x.s.n * p.G > p.few_rows) continue;
-    const int rt = x.r / ROWS, row = x.r % ROWS;
-    int64_t before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
-    for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, UNIT, true>(p, c);
+  RowOf x;
+  bool real = false;
+  int64_t before = 0;
+  for (int k = 0, token = -1; k < each && id0 + k < n_rows; ++k) {
+    if (const int t = token_of(p, (int)(id0 + k), x); t != token) {
+      token = t;
+      real = seq_of(p, t, lane, x) && x.s.n * p.G <= p.few_rows;
+      if (!real) continue;
+      before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
+      for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, UNIT, true>(p, c);
+    }
+    if (!real) continue;
+    const int r = row_number(p, x), rt = r / ROWS, row = r % ROWS;
     const Item it = item_of<ROWS, UNIT>(p, x.s);
     const int64_t u0 = before + ((int64_t)x.hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
     const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
     if (w0 == w1) continue;                            // one workgroup had all of it
-    join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.token, x.head);
+    join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.s.start + x.i,
+                   x.head);
   }
 }
 

@@ -118,24 +118,28 @@ __device__ __forceinline__ void join_row(const PagedAttn& p, int lane, int n_par
   if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
 }
 
-// The row of q that number `id` of all T * Hq stands for: its sequence, and the row's number there.  False where there is none.
-struct RowOf { int b, head, hk, r, token; PagedSeq s; };
-__device__ __forceinline__ bool row_of(const PagedAttn& p, int id, int lane, RowOf& x) {
-  int i = 0;
+// Number `id` of all T * Hq rows of q, in two steps: the token (whose number is returned) and the head; the token's sequence and
+// its number there, false where there is none.  row_number: the row's number among those of the sequence and K/V head.
+struct RowOf { int b, i, head, hk; PagedSeq s; };
+__device__ __forceinline__ int token_of(const PagedAttn& p, int id, RowOf& x) {
   const int t = __builtin_amdgcn_readfirstlane(p.by_heads.quotient(id, x.head));
   x.head = __builtin_amdgcn_readfirstlane(x.head);
+  return t;
+}
+__device__ __forceinline__ bool seq_of(const PagedAttn& p, int t, int lane, RowOf& x) {
+  int i = 0;
   if (p.g.starts) x.b = paged_owner<64>(p.g, t, lane);
   else x.b = p.by_new.quotient(t, i);
   x.b = __builtin_amdgcn_readfirstlane(x.b);
   if (x.b >= p.g.B) return false;
   x.s = paged_seq<true>(p.g, x.b);
-  if (p.g.starts) i = t - x.s.start;
-  if (i < 0 || i >= x.s.n) return false;
+  x.i = p.g.starts ? t - x.s.start : i;
+  return x.i >= 0 && x.i < x.s.n;
+}
+__device__ __forceinline__ int row_number(const PagedAttn& p, RowOf& x) {
   int of_group;
   x.hk = p.by_group.quotient(x.head, of_group);
-  x.r = i * p.G + of_group;
-  x.token = x.s.start + i;
-  return true;
+  return x.i * p.G + of_group;
 }
 
 // Rows of a wavefront of the last step: one while there are CUs without any, up to eight.

@@ -53,18 +53,28 @@ __device__ __forceinline__ T wave_sum(T x) {
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
   return x;
 }
-__device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane) {
+// (A lane counts a run of sequences; the first one's numbers are loaded once for both counts.)
+__device__ __forceinline__ PagedSeq lane_seq(const PagedAttn& p, int lane) {
   const int per = (p.g.B + 63) / 64;
-  long long steps = 0, items = 0;
-  for (int j = 0; j < per; ++j)
+  return lane * per < p.g.B ? paged_seq<false>(p.g, lane * per) : PagedSeq{0, 0, 0};
+}
+__device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane, const PagedSeq& own) {
+  const int per = (p.g.B + 63) / 64;
+  long long steps, items;
+  {
+    const Pieces c = chunk_items(p, own);
+    items = c.rts;
+    steps = c.rts * c.steps;
+  }
+  for (int j = 1; j < per; ++j)
     if (lane * per + j < p.g.B) {
       const Pieces c = chunk_items(p, paged_seq<false>(p.g, lane * per + j));
       items += c.rts;
       steps += c.rts * c.steps;
     }
   Cut cut;
-  items = uniform64(wave_sum(items)) * p.Hkv;
-  cut.total = uniform64(wave_sum(steps)) * p.Hkv;
+  items = uniform64(p.g.B > 1 ? wave_sum(items) : items) * p.Hkv;
+  cut.total = uniform64(p.g.B > 1 ? wave_sum(steps) : steps) * p.Hkv;
   cut.want = items < kParts ? items : kParts;            // pieces of items in several: at most so many
   if (items > 0 && items < kParts) {
     // the number of pieces that takes the least rounds of 256 workgroups times their length; lane l tries so many to an item
@@ -84,23 +94,28 @@ __device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane) {
 }
 // Pieces (and those of items in more than one) before each lane's run of sequences.
 struct Layout { int per; int64_t before, mine, slots_before, slots; };
-__device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, int lane) {
+__device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, int lane, const PagedSeq& own) {
   Layout y;
   y.per = (p.g.B + 63) / 64;
   y.mine = 0;
   int64_t slots = 0;
   for (int j = 0; j < y.per; ++j)
     if (lane * y.per + j < p.g.B) {
-      const Pieces c = chunk_pieces(p, paged_seq<false>(p.g, lane * y.per + j), cut);
+      const Pieces c = chunk_pieces(p, j == 0 ? own : paged_seq<false>(p.g, lane * y.per + j), cut);
       const int64_t n = (int64_t)p.Hkv * c.rts * c.parts;
       y.mine += n;
       if (c.parts > 1) slots += n;
     }
   int64_t sum = y.mine, sum_slots = slots;
+  if (p.g.B > 1) {
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t a = __shfl_up((long long)sum, off), b = __shfl_up((long long)sum_slots, off);
-    if (lane >= off) { sum += a; sum_slots += b; }
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t a = __shfl_up((long long)sum, off), b = __shfl_up((long long)sum_slots, off);
+      if (lane >= off) { sum += a; sum_slots += b; }
+    }
+  } else {
+    sum = uniform64(sum);
+    sum_slots = uniform64(sum_slots);
   }
   y.before = sum - y.mine;
   y.slots_before = sum_slots - slots;
@@ -138,9 +153,10 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const bool group_b = wave >= 4;
 
   // ---- this workgroup's piece --------------------------------------------------------------------------------
-  const Cut cut = cut_of(p, lane);
+  const PagedSeq own = lane_seq(p, lane);
+  const Cut cut = cut_of(p, lane, own);
   if (cut.total == 0) return;
-  const Layout y = layout_of(p, cut, lane);
+  const Layout y = layout_of(p, cut, lane, own);
   const int64_t id = blockIdx.x;
   const uint64_t owners = __builtin_amdgcn_ballot_w64(id >= y.before && id < y.before + y.mine);
   if (owners == 0) return;                             // past the last piece
@@ -195,6 +211,19 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   // quarters of 16 keys are looked up; gone holds four bits of each of the last eight tiles, that its quarters are not here.
   struct Entry { int page, slot; };
   struct Rows { int64_t at; int page, slot, held, bytes; };      // at: from the first row of the head; bytes: of the rows there are
+  auto look_up = [&](int t) {
+    const int key = (t0 + t) * kBN + 8 * wave;
+    Entry e;
+    e.page = uniform_load(table, p.g.by_page.quotient(key < seen_last ? key : seen_last - 1, e.slot));
+    return e;
+  };
+  // (on their way together with Q: the entries of the first tiles, and all of the piece's)
+  constexpr int kAhead = 5;
+  Entry ahead[kAhead];
+  if (ntiles > 0) {
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) ahead[t] = look_up(t);
+  }
   uint32_t gone = 0;
   bool any_gone = false;
   if (ntiles > 0) {
@@ -205,12 +234,6 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     for (int e = first + lane; e <= last; e += 64) missing = missing || (uint32_t)table[e] >= (uint32_t)p.g.pages;
     any_gone = __builtin_amdgcn_ballot_w64(missing) != 0;
   }
-  auto look_up = [&](int t) {
-    const int key = (t0 + t) * kBN + 8 * wave;
-    Entry e;
-    e.page = uniform_load(table, p.g.by_page.quotient(key < seen_last ? key : seen_last - 1, e.slot));
-    return e;
-  };
   const int row_step = (int)p.c_ss16 * 16, row_tail = p.D * 2 - row_step;        // (bf16)
   auto settle = [&](int t, Entry e) {
     asm volatile("" : "+s"(e.page));                   // waited for here
@@ -482,48 +505,56 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     // Tiles 0 .. 3 of K and 0 .. 2 of V; in the loop K(t + 4) and V(t + 3) follow, whose places tile t's matrix phase and the one
     // before it were the last to read.  Codes that pass through registers are requested one tile before they are put there.
     Codes ck, cv;
+    auto first_tile = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < KB; ++ks) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) s_mfma(mb, ks, read_k(mb, ks));
+        k_a[ks] += kTileLds;
+      }
+      sm_mask(0);
+      sm_fix(true);
+      sm_exps();
+#pragma unroll
+      for (int r = 0; r < 2; ++r) l_run[r] = rs[r];
+    };
     if constexpr (!E4M3) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const Rows x = settle(t, look_up(t));
+        const Rows x = settle(t, ahead[t]);
         copy_rows(k_head, x, lds_rows + t * kTileLds);
         if (t < 3) copy_rows(v_head, x, lds_rows + kVRing + t * kTileLds);
         next_v = x;
       }
-      next_k = settle(4, look_up(4));
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      next_k = settle(4, ahead[4]);
+      asm volatile("s_waitcnt vmcnt(12)" ::: "memory");         // K(0)
+      __builtin_amdgcn_s_barrier();
+      first_tile();
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");          // V(0) and K(1); the loop waits for the others
+      __builtin_amdgcn_s_barrier();
     } else {
       Codes k[4], v[3];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const Rows x = settle(t, look_up(t));
+        const Rows x = settle(t, ahead[t]);
         k[t] = request(k_head, p.k_scales, x);
         if (t < 3) v[t] = request(v_head, p.v_scales, x);
         next_v = x;
       }
+      next_k = settle(4, ahead[4]);
+      put(k[0], lds_rows);
+      __syncthreads();
+      first_tile();
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        put(k[t], lds_rows + t * kTileLds);
+        if (t > 0) put(k[t], lds_rows + t * kTileLds);
         if (t < 3) put(v[t], lds_rows + kVRing + t * kTileLds);
       }
       cv = request(v_head, p.v_scales, next_v);
-      next_k = settle(4, look_up(4));
       ck = request(k_head, p.k_scales, next_k);
+      __syncthreads();
     }
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < KB; ++ks) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) s_mfma(mb, ks, read_k(mb, ks));
-      k_a[ks] += kTileLds;
-    }
-    sm_mask(0);
-    sm_fix(true);
-    sm_exps();
-#pragma unroll
-    for (int r = 0; r < 2; ++r) l_run[r] = rs[r];
-    __syncthreads();                                   // K(0) has been read by all
     if (ntiles > 1) first_frags();
     if (group_b) __builtin_amdgcn_s_barrier();
     // vector phase of tile t: softmax of tile t + 1 and the copies ahead
@@ -566,7 +597,11 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       vector_phase(t);
       __builtin_amdgcn_s_barrier();
     }
-    pv_cut();
+    if (cuts(ntiles - 1)) pv_cut();
+    else {
+#pragma unroll
+      for (int i = 0; i < kSlotsO; ++i) o_mfma(i % DB, i / DB, read_v(i % DB, i / DB));
+    }
     if (!group_b) __builtin_amdgcn_s_barrier();
   }
 
@@ -624,24 +659,34 @@ template <int COLS>
 __global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows, int each) {
   const int lane = threadIdx.x & 63;
   const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
-  const Cut cut = cut_of(p, lane);
+  const PagedSeq own = lane_seq(p, lane);
+  const Cut cut = cut_of(p, lane, own);
   if (cut.total == 0) return;
-  const Layout y = layout_of(p, cut, lane);
+  const Layout y = layout_of(p, cut, lane, own);
   if (uniform64(y.slots) == 0) return;
-  for (int k = 0; k < each; ++k) {
-    RowOf x;
-    if (id0 + k >= n_rows) return;
-    if (!row_of(p, (int)(id0 + k), lane, x)) continue;
-    const Pieces c = chunk_pieces(p, x.s, cut);
-    if (c.rts == 0 || c.parts == 1) continue;
-    int64_t before = uniform64(__shfl((long long)y.slots_before, x.b / y.per));
-    for (int e = x.b / y.per * y.per; e < x.b; ++e) {
-      const Pieces d = chunk_pieces(p, paged_seq<true>(p.g, e), cut);
-      if (d.parts > 1) before += (int64_t)p.Hkv * d.rts * d.parts;
+  RowOf x;
+  bool real = false;
+  Pieces c{};
+  int64_t before = 0;
+  for (int k = 0, token = -1; k < each && id0 + k < n_rows; ++k) {
+    if (const int t = token_of(p, (int)(id0 + k), x); t != token) {
+      token = t;
+      real = seq_of(p, t, lane, x);
+      if (!real) continue;
+      c = chunk_pieces(p, x.s, cut);
+      real = c.rts > 0 && c.parts > 1;
+      if (!real) continue;
+      before = uniform64(__shfl((long long)y.slots_before, x.b / y.per));
+      for (int e = x.b / y.per * y.per; e < x.b; ++e) {
+        const Pieces d = chunk_pieces(p, paged_seq<true>(p.g, e), cut);
+        if (d.parts > 1) before += (int64_t)p.Hkv * d.rts * d.parts;
+      }
     }
-    const int64_t first = before + piece_number(c, p.Hkv, 0, x.r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
-    const int row = x.r % kBM;
-    join_row<COLS>(p, lane, c.parts, [&](int part) { return (first + part * step) * kBM + row; }, x.b, x.token, x.head);
+    if (!real) continue;
+    const int r = row_number(p, x);
+    const int64_t first = before + piece_number(c, p.Hkv, 0, r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
+    const int row = r % kBM;
+    join_row<COLS>(p, lane, c.parts, [&](int part) { return (first + part * step) * kBM + row; }, x.b, x.s.start + x.i, x.head);
   }
 }
 
