@@ -379,9 +379,10 @@ int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float*
  * results over different pages of a sequence (other entries -1) merge as those of different chunks do.  A key a row does not see has
  * no part in its result, whatever the cache holds there.  most_new: with starts, about how many new tokens a sequence has at most;
  * it chooses the form of the kernels, results are right whatever it says.  `workspace`: 16-byte aligned,
- * mhip_paged_attn_workspace_bytes(most_new or n, Hq, Hkv, D) bytes of device memory; calls that overlap in time need one each.
+ * mhip_paged_attn_workspace_bytes(B, n, T, most_new, whether there are starts, Hq, Hkv, D) bytes of device memory; calls that overlap
+ * in time need one each.
  */
-int64_t mhip_paged_attn_workspace_bytes(int most_new, int Hq, int Hkv, int D);
+int64_t mhip_paged_attn_workspace_bytes(int B, int n, int T, int most_new, int packed, int Hq, int Hkv, int D);
 int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
                         const int* page_table, const int* lengths, const int* starts, void* out, float* lse,
                         int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,

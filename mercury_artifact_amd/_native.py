@@ -86,7 +86,7 @@ _SIGNATURES = {
     "mhip_quantize_e4m3": (c_int, [_P, _I, _L, _P, _P, _P, _P]),
     "mhip_paged_cache_write": (c_int, [_P] * 9 + [_I] * 8 + [_L] * 13 + [_I, _P]),
     "mhip_paged_cache_read": (c_int, [_P] * 7 + [_I] * 8 + [_L] * 11 + [_I, _P]),
-    "mhip_paged_attn_workspace_bytes": (c_int64, [_I] * 4),
+    "mhip_paged_attn_workspace_bytes": (c_int64, [_I] * 8),
     "mhip_paged_attn_fwd": (c_int, [_P] * 10 + [_I] * 10 + [_L] * 13 + [_F, _I, _I, _P, _P]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -854,7 +854,7 @@ PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     SLOW;
   OnDevice on(*q);
   if (!on.current) SLOW;
-  const int64_t bytes = entry.paged_bytes(most, Hq, g.Hkv, g.D);
+  const int64_t bytes = entry.paged_bytes(g.B, n, T, most, g.starts != nullptr, Hq, g.Hkv, g.D);
   if (bytes < 0) SLOW;
   Tensor out, lse, workspace;
   const int code = without_gil([&] {

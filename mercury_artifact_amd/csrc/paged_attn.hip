@@ -519,10 +519,11 @@ void launch(const PagedAttn& p, bool e4m3, int64_t rows, hipStream_t st) {
 
 using namespace mhip;
 
-extern "C" int64_t mhip_paged_attn_workspace_bytes(int most_new, int Hq, int Hkv, int D) {
-  if (most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
+extern "C" int64_t mhip_paged_attn_workspace_bytes(int B, int n, int T, int most_new, int packed, int Hq, int Hkv, int D) {
+  if (B < 0 || n < 0 || T < 0 || most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
   if (D <= 0 || D > 128) return MHIP_EHEADDIM;
-  const int64_t rows = (int64_t)most_new * (Hq / Hkv), few = few_bytes(rows, D), chunk = rows > kFewRows ? paged_attn_chunk_bytes(D) : 0;
+  const int64_t rows = (int64_t)(packed ? most_new : n) * (Hq / Hkv), few = few_bytes(rows, D);
+  const int64_t chunk = rows > kFewRows ? paged_attn_chunk_bytes(B, n, T, Hq / Hkv, Hkv, D, packed != 0) : 0;
   return few > chunk ? few : chunk;
 }
 
@@ -574,7 +575,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
     // after the other on the stream, share the workspace.
     p.few_rows = starts && p.G <= kFewRows ? 16 * row_blocks(p.G) : -1;
     if (p.few_rows > 0) launch(p, dtype == MHIP_E4M3, p.few_rows, st);
-    paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st);
+    if (int code = paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st)) return code;
   }
   return launch_status();
 }

@@ -7,6 +7,11 @@
 
 namespace mhip {
 
+// What the plan of a launch of long chunks leaves of a sequence (its first piece; the slot of its first partial result, where there
+// are several parts; parts of an item; row tiles), and of all (partial results).
+struct Record { int first, slot, parts, rts; };
+struct PlanOut { int slots; };
+
 struct PagedAttn {
   PagedGeom g;
   const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
@@ -20,6 +25,7 @@ struct PagedAttn {
   Divisor by_group, by_heads, by_new;
   int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
   float* part_o; f32x2* part_ml;           // partial results
+  PlanOut* plan; Record* records; int* pieces;
 };
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
@@ -145,7 +151,7 @@ __device__ __forceinline__ int row_number(const PagedAttn& p, RowOf& x) {
 // Rows of a wavefront of the last step: one while there are CUs without any, up to eight.
 inline int join_rows(int64_t n_rows) { return n_rows <= 8192 ? 1 : n_rows >= 65536 ? 8 : (int)(n_rows / 8192); }
 
-int64_t paged_attn_chunk_bytes(int D);
-void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
+int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed);
+int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
 
 }  // namespace mhip

@@ -25,12 +25,16 @@ constexpr int kTileLds = kBN * 256;        // a K or V tile in LDS, rows of 256 
 constexpr int kRingStages = 4;
 constexpr int kVRing = kRingStages * kTileLds;
 constexpr int kParts = 512;                // partial results there is room for
-constexpr float kPieceCost = 12.f;         // what a piece costs besides its tiles, in tiles
+constexpr float kPieceCost = 8.f;          // what a piece costs besides its steps, and joining costs, in steps
+constexpr float kJoinCost = 6.f;
 
-// How the items (sequence, K/V head, tile of rows) are cut into pieces of their keys, one workgroup each: all alike where the
-// sequences are, in proportion to their lengths where they are not, so that `want` pieces of equal length would do.
-struct Cut { int64_t want, total; };       // S of a sequence: steps * want / total, at least 1
-struct Pieces { int rts, parts; int64_t steps; };     // tiles of rows, pieces of each, 64-key steps
+// How the items (sequence, K/V head, tile of rows) are cut into pieces of their keys, one workgroup each: of so many steps of 64 keys at
+// most, an item's all alike.
+struct Pieces { int rts, parts, steps; };              // tiles of rows, pieces of each item, its steps
+__device__ __forceinline__ int parts_of(int steps, int longest) {
+  const int parts = (steps + longest - 1) / longest, most = steps / 4;         // (none shorter than four)
+  return parts < most ? parts : most > 1 ? most : 1;
+}
 __device__ __forceinline__ Pieces chunk_items(const PagedAttn& p, const PagedSeq& s) {
   Pieces c;
   c.rts = s.n * p.G > p.few_rows ? (s.n * p.G + kBM - 1) / kBM : 0;
@@ -38,93 +42,129 @@ __device__ __forceinline__ Pieces chunk_items(const PagedAttn& p, const PagedSeq
   c.parts = 1;
   return c;
 }
-__device__ __forceinline__ Pieces chunk_pieces(const PagedAttn& p, const PagedSeq& s, const Cut& cut) {
-  Pieces c = chunk_items(p, s);
-  if (c.rts > 0) {
-    const int64_t parts = c.steps * cut.want / cut.total, most = c.steps / 4;
-    c.parts = (int)(parts < most ? parts : most);
-    if (c.parts < 1) c.parts = 1;
+// ---- the plan ------------------------------------------------------------------------------------------------------------
+// One workgroup counts the items, cuts them into pieces and deals the pieces out, the longest first, since workgroups take them in order
+// as CUs come free.  It leaves for every piece its sequence (-1: none) and for every sequence its numbers.
+constexpr int kPlanWaves = 16, kStaged = 2048, kBuckets = 64;
+__global__ __launch_bounds__(kPlanWaves * 64) void paged_attn_chunk_plan(const PagedAttn p, int places) {
+  __shared__ int steps_of[kStaged], rts_of[kStaged];
+  __shared__ float sums[kPlanWaves][3][64];
+  __shared__ int extremes[2], longest, bucket[kBuckets], slots;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = kPlanWaves * 64;
+  if (tid == 0) { extremes[0] = 0; extremes[1] = 0x7fffffff; slots = 0; }
+  if (tid < kBuckets) bucket[tid] = 0;
+  for (int i = tid; i < places; i += threads) p.pieces[i] = -1;
+  __syncthreads();
+  for (int b = tid; b < p.g.B; b += threads) {
+    const Pieces c = chunk_items(p, paged_seq<false>(p.g, b));
+    if (b < kStaged) { steps_of[b] = c.steps; rts_of[b] = c.rts; }
+    if (c.rts > 0) {
+      atomicMax(&extremes[0], c.steps);
+      atomicMin(&extremes[1], c.steps);
+    }
   }
-  return c;
-}
-template <class T>
-__device__ __forceinline__ T wave_sum(T x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
-  return x;
-}
-// (A lane counts a run of sequences; the first one's numbers are loaded once for both counts.)
-__device__ __forceinline__ PagedSeq lane_seq(const PagedAttn& p, int lane) {
-  const int per = (p.g.B + 63) / 64;
-  return lane * per < p.g.B ? paged_seq<false>(p.g, lane * per) : PagedSeq{0, 0, 0};
-}
-__device__ __forceinline__ Cut cut_of(const PagedAttn& p, int lane, const PagedSeq& own) {
-  const int per = (p.g.B + 63) / 64;
-  long long steps, items;
+  __syncthreads();
+  const int most = extremes[0], least = extremes[1];
+  if (most == 0) {
+    if (tid == 0) p.plan[0] = PlanOut{0};
+    return;
+  }
+  // Each lane tries a length (the longest item in 1 .. 32, then up to 256 pieces) and estimates the launch's time: one round where
+  // there is a CU for each piece, whole rounds where all are alike, else the mean of the CUs and a third of the last piece.
   {
-    const Pieces c = chunk_items(p, own);
-    items = c.rts;
-    steps = c.rts * c.steps;
-  }
-  for (int j = 1; j < per; ++j)
-    if (lane * per + j < p.g.B) {
-      const Pieces c = chunk_items(p, paged_seq<false>(p.g, lane * per + j));
-      items += c.rts;
-      steps += c.rts * c.steps;
+    const int tries = lane < 32 ? lane + 1 : 32 + (lane - 31) * 7, bound = (most + tries - 1) / tries;
+    float pieces = 0.f, cut = 0.f, steps = 0.f;
+    int length = 0;
+    for (int b = wave; b < p.g.B; b += kPlanWaves) {
+      int rts, of;
+      if (b < kStaged) { rts = rts_of[b]; of = steps_of[b]; }
+      else { const Pieces c = chunk_items(p, paged_seq<true>(p.g, b)); rts = c.rts; of = c.steps; }
+      if (rts == 0) continue;
+      const int parts = parts_of(of, bound), here = (of + parts - 1) / parts;
+      const float n = (float)rts * parts;
+      pieces += n;
+      cut += parts > 1 ? n : 0.f;
+      steps += (float)rts * of;
+      length = here > length ? here : length;
     }
-  Cut cut;
-  items = uniform64(p.g.B > 1 ? wave_sum(items) : items) * p.Hkv;
-  cut.total = uniform64(p.g.B > 1 ? wave_sum(steps) : steps) * p.Hkv;
-  cut.want = items < kParts ? items : kParts;            // pieces of items in several: at most so many
-  if (items > 0 && items < kParts) {
-    // the number of pieces that takes the least rounds of 256 workgroups times their length; lane l tries so many to an item
-    const int unit = items < 4 ? 4 / (int)items : 1, parts = (lane + 1) * unit;
-    const float mean = (float)cut.total / (float)items;
-    const int rounds = (int)((items * parts + 255) / 256);
-    float time = rounds * (mean / parts + kPieceCost) + (parts > 1 ? kPieceCost : 0.f);
-    if (parts > 1 && items * parts > kParts) time = INFINITY;
-    if (lane == 0 && unit > 1) time = mean + kPieceCost;           // (stands for one piece)
-    float best = time;
+    // (the two counts are whole numbers far below 2^24 wherever they decide)
+    sums[wave][0][lane] = pieces;
+    sums[wave][1][lane] = cut;
+    sums[wave][2][lane] = steps;
+    __shared__ int lengths[kPlanWaves][64];
+    lengths[wave][lane] = length;
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kPlanWaves; ++w) {
+        pieces += sums[w][0][lane];
+        cut += sums[w][1][lane];
+        steps += sums[w][2][lane];
+        length = lengths[w][lane] > length ? lengths[w][lane] : length;
+      }
+      pieces *= p.Hkv;
+      cut *= p.Hkv;
+      steps *= p.Hkv;
+      const float one = length + kPieceCost;
+      float time = pieces <= 256.f ? one : least == most ? __builtin_ceilf(pieces / 256.f) * one : (steps + pieces * kPieceCost) / 256.f + one / 3.f;
+      if (time < one) time = one;
+      if (cut > 0.f) time += kJoinCost;
+      if (cut > kParts) time = INFINITY;
+      float best = time;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) best = fminf(best, __shfl_xor(best, off));
-    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(time == best));
-    cut.want = items * (at == 0 ? 1 : (at + 1) * unit);
-  }
-  return cut;
-}
-// Pieces (and those of items in more than one) before each lane's run of sequences.
-struct Layout { int per; int64_t before, mine, slots_before, slots; };
-__device__ __forceinline__ Layout layout_of(const PagedAttn& p, const Cut& cut, int lane, const PagedSeq& own) {
-  Layout y;
-  y.per = (p.g.B + 63) / 64;
-  y.mine = 0;
-  int64_t slots = 0;
-  for (int j = 0; j < y.per; ++j)
-    if (lane * y.per + j < p.g.B) {
-      const Pieces c = chunk_pieces(p, j == 0 ? own : paged_seq<false>(p.g, lane * y.per + j), cut);
-      const int64_t n = (int64_t)p.Hkv * c.rts * c.parts;
-      y.mine += n;
-      if (c.parts > 1) slots += n;
+      for (int off = 32; off > 0; off >>= 1) best = fminf(best, __shfl_xor(best, off));
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(time == best));
+      if (lane == at) longest = bound;
     }
-  int64_t sum = y.mine, sum_slots = slots;
-  if (p.g.B > 1) {
+    __syncthreads();
+  }
+  // pieces by length, in 64 buckets, the longest first
+  auto seq = [&](int b) {
+    Pieces c;
+    if (b < kStaged) { c.rts = rts_of[b]; c.steps = steps_of[b]; c.parts = 1; }
+    else c = chunk_items(p, paged_seq<false>(p.g, b));
+    if (c.rts > 0) c.parts = parts_of(c.steps, longest);
+    return c;
+  };
+  auto bucket_of = [&](const Pieces& c) { return kBuckets - 1 - (int)((int64_t)((c.steps + c.parts - 1) / c.parts) * (kBuckets - 1) / most); };
+  for (int b = tid; b < p.g.B; b += threads) {
+    const Pieces c = seq(b);
+    if (c.rts > 0) atomicAdd(&bucket[bucket_of(c)], p.Hkv * c.rts * c.parts);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int sum = bucket[lane];
+    const int own = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int64_t a = __shfl_up((long long)sum, off), b = __shfl_up((long long)sum_slots, off);
-      if (lane >= off) { sum += a; sum_slots += b; }
+      const int below = __shfl_up(sum, off);
+      if (lane >= off) sum += below;
     }
-  } else {
-    sum = uniform64(sum);
-    sum_slots = uniform64(sum_slots);
+    bucket[lane] = sum - own;
   }
-  y.before = sum - y.mine;
-  y.slots_before = sum_slots - slots;
-  y.slots = __shfl((long long)sum_slots, 63);
-  return y;
+  __syncthreads();
+  for (int b = tid; b < p.g.B; b += threads) {
+    const Pieces c = seq(b);
+    if (c.rts == 0) continue;
+    const int n = p.Hkv * c.rts * c.parts;
+    p.records[b] = Record{atomicAdd(&bucket[bucket_of(c)], n), c.parts > 1 ? atomicAdd(&slots, n) : 0, c.parts, c.rts};
+  }
+  __syncthreads();
+  if (tid == 0) p.plan[0] = PlanOut{slots};
+  for (int b = wave; b < p.g.B; b += kPlanWaves) {
+    const Pieces c = seq(b);
+    if (c.rts == 0) continue;
+    const int first = p.records[b].first, n = p.Hkv * c.rts * c.parts;
+    for (int i = lane; i < n; i += 64)
+      if (first + i < places) p.pieces[first + i] = b;
+  }
+}
+__device__ __forceinline__ Record record_of(const PagedAttn& p, int b) {
+  const int* r = reinterpret_cast<const int*>(p.records + b);
+  return Record{uniform_load(r, 0), uniform_load(r, 1), uniform_load(r, 2), uniform_load(r, 3)};
 }
 // piece i of a sequence: K/V heads fastest (eight of them: one to an XCD's L2), then the row tiles, the last (longest) first
 struct Piece { int part, rt, hk; };
-__device__ __forceinline__ Piece piece_of(const Pieces& c, int Hkv, int64_t i) {
+__device__ __forceinline__ Piece piece_of(const Record& c, int Hkv, int64_t i) {
   Piece x;
   const int64_t of_part = (int64_t)c.rts * Hkv;
   x.part = (int)(i / of_part);
@@ -133,7 +173,7 @@ __device__ __forceinline__ Piece piece_of(const Pieces& c, int Hkv, int64_t i) {
   x.hk = rest % Hkv;
   return x;
 }
-__device__ __forceinline__ int64_t piece_number(const Pieces& c, int Hkv, int part, int rt, int hk) {
+__device__ __forceinline__ int64_t piece_number(const Record& c, int Hkv, int part, int rt, int hk) {
   return ((int64_t)part * c.rts + (c.rts - 1 - rt)) * Hkv + hk;
 }
 
@@ -153,24 +193,11 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const bool group_b = wave >= 4;
 
   // ---- this workgroup's piece --------------------------------------------------------------------------------
-  const PagedSeq own = lane_seq(p, lane);
-  const Cut cut = cut_of(p, lane, own);
-  if (cut.total == 0) return;
-  const Layout y = layout_of(p, cut, lane, own);
-  const int64_t id = blockIdx.x;
-  const uint64_t owners = __builtin_amdgcn_ballot_w64(id >= y.before && id < y.before + y.mine);
-  if (owners == 0) return;                             // past the last piece
-  const int owner = __builtin_ctzll(owners);
-  int b = owner * y.per;
-  int64_t pos = id - uniform64(__shfl((long long)y.before, owner)), slot0 = uniform64(__shfl((long long)y.slots_before, owner));
-  PagedSeq s = paged_seq<true>(p.g, b);
-  Pieces c = chunk_pieces(p, s, cut);
-  for (int64_t n; b + 1 < p.g.B && pos >= (n = (int64_t)p.Hkv * c.rts * c.parts);) {
-    pos -= n;
-    if (c.parts > 1) slot0 += n;
-    s = paged_seq<true>(p.g, ++b);
-    c = chunk_pieces(p, s, cut);
-  }
+  const int b = uniform_load(p.pieces, blockIdx.x);
+  if (b < 0) return;                                   // past the last piece
+  const PagedSeq s = paged_seq<true>(p.g, b);
+  const Record c = record_of(p, b);
+  const int pos = (int)blockIdx.x - c.first;
   const Piece piece = piece_of(c, p.Hkv, pos);
   const int hk = piece.hk, row0 = piece.rt * kBM;
   const int rows = s.n * p.G - row0 < kBM ? s.n * p.G - row0 : kBM;
@@ -610,7 +637,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   const PagedAttn a = arguments_again();
   __syncthreads();                                     // every wavefront is done with K and V
   if (c.parts > 1) {
-    const int64_t at = (slot0 + pos) * kBM + wave * 32;
+    const int64_t at = ((int64_t)c.slot + pos) * kBM + wave * 32;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float l_tot = quad_sum(l_run[r]);
@@ -659,60 +686,66 @@ template <int COLS>
 __global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows, int each) {
   const int lane = threadIdx.x & 63;
   const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
-  const PagedSeq own = lane_seq(p, lane);
-  const Cut cut = cut_of(p, lane, own);
-  if (cut.total == 0) return;
-  const Layout y = layout_of(p, cut, lane, own);
-  if (uniform64(y.slots) == 0) return;
+  if (uniform_load(&p.plan->slots, 0) == 0) return;
   RowOf x;
   bool real = false;
-  Pieces c{};
-  int64_t before = 0;
+  Record c{};
   for (int k = 0, token = -1; k < each && id0 + k < n_rows; ++k) {
     if (const int t = token_of(p, (int)(id0 + k), x); t != token) {
       token = t;
-      real = seq_of(p, t, lane, x);
+      real = seq_of(p, t, lane, x) && x.s.n * p.G > p.few_rows;
       if (!real) continue;
-      c = chunk_pieces(p, x.s, cut);
-      real = c.rts > 0 && c.parts > 1;
-      if (!real) continue;
-      before = uniform64(__shfl((long long)y.slots_before, x.b / y.per));
-      for (int e = x.b / y.per * y.per; e < x.b; ++e) {
-        const Pieces d = chunk_pieces(p, paged_seq<true>(p.g, e), cut);
-        if (d.parts > 1) before += (int64_t)p.Hkv * d.rts * d.parts;
-      }
+      c = record_of(p, x.b);
+      real = c.parts > 1;
     }
     if (!real) continue;
     const int r = row_number(p, x);
-    const int64_t first = before + piece_number(c, p.Hkv, 0, r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
+    const int64_t first = c.slot + piece_number(c, p.Hkv, 0, r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
     const int row = r % kBM;
     join_row<COLS>(p, lane, c.parts, [&](int part) { return (first + part * step) * kBM + row; }, x.b, x.s.start + x.i, x.head);
   }
 }
 
+int64_t places_of(int64_t B, int64_t T, int64_t n, int G, int Hkv, bool packed) {
+  return Hkv * (packed ? T * G / kBM + B : B * ((n * G + kBM - 1) / kBM)) + kParts;
+}
+int columns_of(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+int64_t up16(int64_t x) { return (x + 15) & ~int64_t(15); }
+
 template <bool E4M3, int COLS>
-void launch(const PagedAttn& p, hipStream_t st) {
-  const int64_t n_rows = (int64_t)p.g.T * p.Hq, rows = (int64_t)p.g.T * p.G;
+void launch(const PagedAttn& p, int places, hipStream_t st) {
+  const int64_t n_rows = (int64_t)p.g.T * p.Hq;
   const int each = join_rows(n_rows);
-  const int64_t items = p.Hkv * (p.g.starts ? rows / kBM + p.g.B : p.g.B * (((int64_t)p.g.n * p.G + kBM - 1) / kBM));
-  hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)(items + kParts)), dim3(512), 0, st, p);
+  hipLaunchKernelGGL(paged_attn_chunk_plan, dim3(1), dim3(kPlanWaves * 64), 0, st, p, places);
+  hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)places), dim3(512), 0, st, p);
   hipLaunchKernelGGL((paged_attn_chunk_join<COLS>), dim3((unsigned)((n_rows + 4 * each - 1) / (4 * each))), dim3(256), 0, st, p, n_rows, each);
 }
 template <bool E4M3>
-void launch(const PagedAttn& p, hipStream_t st) {
-  if (p.D <= 64) launch<E4M3, 64>(p, st);
-  else if (p.D <= 96) launch<E4M3, 96>(p, st);
-  else launch<E4M3, 128>(p, st);
+void launch(const PagedAttn& p, int places, hipStream_t st) {
+  if (p.D <= 64) launch<E4M3, 64>(p, places, st);
+  else if (p.D <= 96) launch<E4M3, 96>(p, places, st);
+  else launch<E4M3, 128>(p, places, st);
 }
 
 }  // namespace
 
-int64_t paged_attn_chunk_bytes(int D) { return (int64_t)kParts * kBM * ((D <= 64 ? 64 : D <= 96 ? 96 : 128) + 2) * 4; }
-void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
+// The workspace: partial results, their maxima and sums, the plan's count, its records, its pieces.
+int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed) {
+  return (int64_t)kParts * kBM * (columns_of(D) + 2) * 4 + 16 + 16 * B + up16(4 * places_of(B, T, n, G, Hkv, packed));
+}
+int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
+  const int64_t places = places_of(p.g.B, p.g.T, p.g.n, p.G, p.Hkv, p.g.starts != nullptr);
+  if (places >= int64_t(1) << 31) return MHIP_EUNSUPPORTED;
   PagedAttn q = p;
-  q.part_ml = reinterpret_cast<f32x2*>(q.part_o + (int64_t)kParts * kBM * (p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128));
-  if (e4m3) launch<true>(q, stream);
-  else launch<false>(q, stream);
+  char* at = reinterpret_cast<char*>(q.part_o) + (int64_t)kParts * kBM * columns_of(p.D) * 4;
+  q.part_ml = reinterpret_cast<f32x2*>(at);
+  at += (int64_t)kParts * kBM * 8;
+  q.plan = reinterpret_cast<PlanOut*>(at);
+  q.records = reinterpret_cast<Record*>(at + 16);
+  q.pieces = reinterpret_cast<int*>(at + 16 + 16 * (int64_t)p.g.B);
+  if (e4m3) launch<true>(q, (int)places, stream);
+  else launch<false>(q, (int)places, stream);
+  return MHIP_OK;
 }
 
 }  // namespace mhip

@@ -166,7 +166,7 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
         if lse.shape != shape or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != cache.device:
             raise RuntimeError(f"lse must be a contiguous float32 {shape} tensor on the cache's device")
     most = n if starts is None else T if most_new is None else min(most_new, T)
-    size = N.lib().mhip_paged_attn_workspace_bytes(most, Hq, Hkv, D)
+    size = N.lib().mhip_paged_attn_workspace_bytes(B, n, T, most, int(starts is not None), Hq, Hkv, D)
     if size < 0:
         N.check(int(size), "mhip_paged_attn_workspace_bytes")
     workspace = torch.empty((int(size),), dtype=torch.uint8, device=q.device)

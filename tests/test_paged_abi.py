@@ -104,10 +104,10 @@ def test_attention_refuses(lib):
     assert _attn(lib, tokens=(384, 132, 64)) == EALIGN
     assert _attn(lib, starts=P, T=1 << 29) == EUNSUPPORTED
     assert _attn(lib, n=0) == OK
-    assert lib.mhip_paged_attn_workspace_bytes(1, 5, 2, 64) == EINVAL
-    assert lib.mhip_paged_attn_workspace_bytes(-1, 4, 2, 64) == EINVAL
-    assert lib.mhip_paged_attn_workspace_bytes(1, 4, 2, 136) == EHEADDIM
-    assert lib.mhip_paged_attn_workspace_bytes(1, 4, 2, 64) > 0
+    assert lib.mhip_paged_attn_workspace_bytes(2, 1, 2, 1, 0, 5, 2, 64) == EINVAL
+    assert lib.mhip_paged_attn_workspace_bytes(2, 1, 2, -1, 1, 4, 2, 64) == EINVAL
+    assert lib.mhip_paged_attn_workspace_bytes(2, 1, 2, 1, 0, 4, 2, 136) == EHEADDIM
+    assert lib.mhip_paged_attn_workspace_bytes(2, 1, 2, 1, 0, 4, 2, 64) > 0
 
 
 def test_no_cpu_fallback():
