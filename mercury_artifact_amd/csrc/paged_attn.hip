@@ -99,7 +99,11 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
   const Plan plan = plan_of<ROWS, UNIT>(p, lane);
   const int64_t total = uniform64(plan.total);
   const int64_t shares = total < (int64_t)gridDim.x ? total : gridDim.x;
-  if (w >= shares) return;
+  if (w >= shares) {
+    if (threadIdx.x == 0 && !p.by_item) p.shared[w].rows = 0;
+    return;
+  }
+  bool leaves = false;                                 // an item that begins here and ends elsewhere
   int64_t lo = total * w / shares;
   const int64_t hi = total * (w + 1) / shares;
   const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= plan.before && lo < plan.before + plan.mine));
@@ -396,6 +400,14 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
     __syncthreads();
     const bool whole = count == it.steps;
     const int64_t slot_of = 2 * (int64_t)w + (first == 0 ? 1 : 0);
+    if (first == 0) {
+      leaves = leaves || !whole;
+      if (threadIdx.x == 0 && (p.by_item || !whole)) {
+        const int last = (int)(((lo + it.steps) * shares - 1) / total);        // the workgroup with its last unit
+        const int64_t at = p.by_item ? (int64_t)b * it.rts * p.Hkv + item : w;
+        p.shared[at] = Shared{b, hk, row0, whole ? 0 : rows, last - w + 1, 2 * w + 1, 2 * (w + 1), 2};
+      }
+    }
 #pragma unroll
     for (int i = 0; i < ROWS * COLS / 4 / (WAVES * 64); ++i) {
       const int unit = i * (WAVES * 64) + threadIdx.x;
@@ -439,35 +451,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
     }
     __syncthreads();
   }
-}
-
-// The rows that several workgroups shared, a wavefront each; where there are many it does `each` of them, counting the units once.
-template <int COLS, int ROWS, int UNIT>
-__global__ __launch_bounds__(256) void paged_attn_few_join(const PagedAttn p, int64_t n_rows, int workgroups, int each) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
-  const Plan plan = plan_of<ROWS, UNIT>(p, lane);
-  const int64_t total = uniform64(plan.total), shares = total < workgroups ? total : workgroups;
-  RowOf x;
-  bool real = false;
-  int64_t before = 0;
-  for (int k = 0, token = -1; k < each && id0 + k < n_rows; ++k) {
-    if (const int t = token_of(p, (int)(id0 + k), x); t != token) {
-      token = t;
-      real = seq_of(p, t, lane, x) && x.s.n * p.G <= p.few_rows;
-      if (!real) continue;
-      before = uniform64(__shfl((long long)plan.before, x.b / plan.per));
-      for (int c = x.b / plan.per * plan.per; c < x.b; ++c) before += units_of<ROWS, UNIT, true>(p, c);
-    }
-    if (!real) continue;
-    const int r = row_number(p, x), rt = r / ROWS, row = r % ROWS;
-    const Item it = item_of<ROWS, UNIT>(p, x.s);
-    const int64_t u0 = before + ((int64_t)x.hk * it.rts + rt) * it.steps, u1 = u0 + it.steps;
-    const int w0 = (int)(((u0 + 1) * shares - 1) / total), w1 = (int)((u1 * shares - 1) / total);
-    if (w0 == w1) continue;                            // one workgroup had all of it
-    join_row<COLS>(p, lane, w1 - w0 + 1, [&](int k) { return (2 * (int64_t)(w0 + k) + (k == 0 ? 1 : 0)) * ROWS + row; }, x.b, x.s.start + x.i,
-                   x.head);
-  }
+  if (!leaves && threadIdx.x == 0 && !p.by_item) p.shared[w].rows = 0;
 }
 
 // Tiles of 16, 32 or 64 rows: the least that holds the rows of a sequence with `most` new tokens.
@@ -480,29 +464,32 @@ int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 constexpr int64_t kManyItems = 128;
 
 // One partial result at each end of a workgroup's share.
-int64_t few_bytes(int64_t rows, int D) { return kWavefronts * 16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4; }
+int64_t few_bytes(int64_t rows, int D) { return kWavefronts * (16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4 + 16); }
 
 template <bool E4M3, int COLS, int NR, int WAVES>
-void launch_few(PagedAttn p, hipStream_t st) {
+void launch_few(PagedAttn p, int64_t rows, hipStream_t st) {
   constexpr int workgroups = kWavefronts / WAVES;
   p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)workgroups * 16 * NR * COLS);
+  p.shared = reinterpret_cast<Shared*>(p.part_ml + 2 * (int64_t)workgroups * 16 * NR);
+  // Where the items are known and not more than the workgroups, the last step has one row of workgroups for each of them, not for
+  // each workgroup that one might begin in (8 items of 32 rows: 34.1 us instead of 39.7, of which launching 2048 workgroups was 5).
+  const int64_t items = (int64_t)p.g.B * p.Hkv * ((rows + 16 * NR - 1) / (16 * NR));
+  p.by_item = !p.g.starts && items <= workgroups;
+  const int blocks = !p.g.starts && rows < 16 * NR ? (int)((rows + 3) / 4) : 4 * NR;       // (packed, `rows` is a hint)
   hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR, WAVES>), dim3(workgroups), dim3(WAVES * 64), 0, st, p);
-  const int64_t n_rows = (int64_t)p.g.T * p.Hq;
-  const int each = join_rows(n_rows);
-  hipLaunchKernelGGL((paged_attn_few_join<COLS, 16 * NR, WAVES * kKeys>), dim3((unsigned)((n_rows + 4 * each - 1) / (4 * each))), dim3(256), 0,
-                     st, p, n_rows, workgroups, each);
+  hipLaunchKernelGGL((paged_attn_join<COLS, 16 * NR, 1, 4>), dim3(blocks, p.by_item ? (int)items : workgroups), dim3(256), 0, st, p);
 }
 template <bool E4M3, int COLS, int NR>
-void launch_few(const PagedAttn& p, hipStream_t st) {
-  if ((int64_t)p.g.B * p.Hkv >= kManyItems) launch_few<E4M3, COLS, NR, 2>(p, st);
-  else launch_few<E4M3, COLS, NR, 4>(p, st);
+void launch_few(const PagedAttn& p, int64_t rows, hipStream_t st) {
+  if ((int64_t)p.g.B * p.Hkv >= kManyItems) launch_few<E4M3, COLS, NR, 2>(p, rows, st);
+  else launch_few<E4M3, COLS, NR, 4>(p, rows, st);
 }
 template <bool E4M3, int COLS>
 void launch_rows(const PagedAttn& p, int64_t rows, hipStream_t st) {
   const int blocks = row_blocks(rows);
-  if (blocks == 1) launch_few<E4M3, COLS, 1>(p, st);
-  else if (blocks == 2) launch_few<E4M3, COLS, 2>(p, st);
-  else launch_few<E4M3, COLS, 4>(p, st);
+  if (blocks == 1) launch_few<E4M3, COLS, 1>(p, rows, st);
+  else if (blocks == 2) launch_few<E4M3, COLS, 2>(p, rows, st);
+  else launch_few<E4M3, COLS, 4>(p, rows, st);
 }
 void launch(const PagedAttn& p, bool e4m3, int64_t rows, hipStream_t st) {
   if (e4m3) {

@@ -7,10 +7,12 @@
 
 namespace mhip {
 
-// What the plan of a launch of long chunks leaves of a sequence (its first piece; the slot of its first partial result, where there
-// are several parts; parts of an item; row tiles), and of all (partial results).
+// What the plan of a launch of long chunks leaves of a sequence: its first piece; the slot of its first partial result, where there
+// are several parts; parts of an item; row tiles.
 struct Record { int first, slot, parts, rts; };
-struct PlanOut { int slots; };
+// Rows (of sequence b and K/V head hk, from number row0 on; none: no item) that several workgroups shared: their partial results are in
+// the slots first, second, second + step, ...
+struct Shared { int b, hk, row0, rows, parts, first, second, step; };
 
 struct PagedAttn {
   PagedGeom g;
@@ -23,9 +25,10 @@ struct PagedAttn {
   int Hq, Hkv, G, D, causal;
   float scale, scale_log2;
   Divisor by_group, by_heads, by_new;
+  int by_item;                             // paged_attn_few: shared items by their number, not by the workgroup they begin in
   int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
   float* part_o; f32x2* part_ml;           // partial results
-  PlanOut* plan; Record* records; int* pieces;
+  Shared* shared; Record* records; int* pieces;
 };
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
@@ -84,72 +87,84 @@ __device__ __forceinline__ int64_t row_offset(const PagedAttn& p, int page, int 
   return (int64_t)(((uint64_t)(uint32_t)page * p.c_sp16 + (uint64_t)((uint32_t)slot * p.c_ss16)) << 4);
 }
 
-// One row from its partial results, the slot of number k at at(k): a wavefront, two columns a lane.  The weights are found by a
-// lane each, so that the rows' loads wait for nothing.
-template <int COLS, class At>
-__device__ __forceinline__ void join_row(const PagedAttn& p, int lane, int n_parts, At at, int b, int token, int head) {
-  float top = -INFINITY;
-  f32x2 ml = {-INFINITY, 0.f};
-  for (int k = lane; k < n_parts; k += 64) {
-    ml = p.part_ml[at(k)];
-    top = fmaxf(top, ml[0]);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float ref = top == -INFINITY ? 0.f : top;
+// The last step of items that several workgroups shared: their partial results with the weights that their maxima and sums give.  A
+// wavefront does R rows at a time, two columns a lane; the weights are found by a lane each, so that the rows' loads wait for nothing.
+// (The rows of an item are neighbouring workgroups, on all XCDs; the few items' own numbers are often all of one.)
+template <int COLS, int ROWS, int R, int BLOCK>
+__global__ __launch_bounds__(256) void paged_attn_join(const PagedAttn p) {
+  static_assert(BLOCK % (4 * R) == 0, "rows of a workgroup");
+  const int* record = reinterpret_cast<const int*>(p.shared + blockIdx.y);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = uniform_load(record, 3), begin = blockIdx.x * BLOCK;
+  if (begin >= rows) return;
+  const int b = uniform_load(record, 0), hk = uniform_load(record, 1), row0 = uniform_load(record, 2), n_parts = uniform_load(record, 4);
+  const int first = uniform_load(record, 5), second = uniform_load(record, 6), step = uniform_load(record, 7);
+  const PagedSeq s = paged_seq<true>(p.g, b);
   const int col = lane * 2 < COLS ? lane * 2 : 0;
-  float sum = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int k0 = 0; k0 < n_parts; k0 += 64) {
-    if (n_parts > 64) ml = k0 + lane < n_parts ? p.part_ml[at(k0 + lane)] : f32x2{-INFINITY, 0.f};
-    const float weight = fast_exp2(ml[0] - ref);
-    sum += ml[1] * weight;
-    const int here = n_parts - k0 < 64 ? n_parts - k0 : 64;
-    for (int k = 0; k < here; k += 8) {
-      f32x2 x[8];
+  for (int row = begin + wave * R; row < begin + BLOCK && row < rows; row += 4 * R) {
+    auto at = [&](int k, int r) {
+      const int here = row + r < rows ? row + r : rows - 1;
+      return (int64_t)(k == 0 ? first : second + (k - 1) * step) * ROWS + here;
+    };
+    f32x2 ml[R];
+    float top[R], ref[R], sum[R], a0[R], a1[R];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        x[u] = *reinterpret_cast<const f32x2*>(p.part_o + at(k0 + (k + u < here ? k + u : here - 1)) * COLS + col);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k + u));
-        a0 += k + u < here ? x[u][0] * w : 0.f;        // (past the last part its row again, which may hold an infinity)
-        a1 += k + u < here ? x[u][1] * w : 0.f;
+    for (int r = 0; r < R; ++r) {
+      ml[r] = f32x2{-INFINITY, 0.f};
+      top[r] = -INFINITY;
+      sum[r] = a0[r] = a1[r] = 0.f;
+      for (int k = lane; k < n_parts; k += 64) {
+        ml[r] = p.part_ml[at(k, r)];
+        top[r] = fmaxf(top[r], ml[r][0]);
       }
     }
-  }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (lane * 2 < p.D) *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0 * inv, a1 * inv);
-  if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) top[r] = fmaxf(top[r], __shfl_xor(top[r], off));
+      ref[r] = top[r] == -INFINITY ? 0.f : top[r];
+    }
+    for (int k0 = 0; k0 < n_parts; k0 += 64) {
+      float weight[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (n_parts > 64) ml[r] = k0 + lane < n_parts ? p.part_ml[at(k0 + lane, r)] : f32x2{-INFINITY, 0.f};
+        weight[r] = fast_exp2(ml[r][0] - ref[r]);
+        sum[r] += ml[r][1] * weight[r];
+      }
+      const int here = n_parts - k0 < 64 ? n_parts - k0 : 64;
+      constexpr int kDeep = 8 / R;
+      for (int k = 0; k < here; k += kDeep) {
+        f32x2 x[kDeep][R];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            x[u][r] = *reinterpret_cast<const f32x2*>(p.part_o + at(k0 + (k + u < here ? k + u : here - 1), r) * COLS + col);
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight[r]), k + u));
+            a0[r] += k + u < here ? x[u][r][0] * w : 0.f;        // (past the last part its row again, which may hold an infinity)
+            a1[r] += k + u < here ? x[u][r][1] * w : 0.f;
+          }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) sum[r] += __shfl_xor(sum[r], off);
+      if (row + r >= rows) continue;
+      int of_group;
+      const int token = s.start + p.by_group.quotient(row0 + row + r, of_group), head = hk * p.G + of_group;
+      const float inv = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+      if (lane * 2 < p.D)
+        *reinterpret_cast<uint32_t*>(p.out + b * p.o_sb + (int64_t)token * p.o_ss + head * p.o_sh + col) = pack_bf16(a0[r] * inv, a1[r] * inv);
+      if (lane == 0) p.lse[b * p.l_sb + head * p.l_sh + token] = sum[r] == 0.f ? -INFINITY : (top[r] + fast_log2(sum[r])) * kLn2;
+    }
+  }
 }
-
-// Number `id` of all T * Hq rows of q, in two steps: the token (whose number is returned) and the head; the token's sequence and
-// its number there, false where there is none.  row_number: the row's number among those of the sequence and K/V head.
-struct RowOf { int b, i, head, hk; PagedSeq s; };
-__device__ __forceinline__ int token_of(const PagedAttn& p, int id, RowOf& x) {
-  const int t = __builtin_amdgcn_readfirstlane(p.by_heads.quotient(id, x.head));
-  x.head = __builtin_amdgcn_readfirstlane(x.head);
-  return t;
-}
-__device__ __forceinline__ bool seq_of(const PagedAttn& p, int t, int lane, RowOf& x) {
-  int i = 0;
-  if (p.g.starts) x.b = paged_owner<64>(p.g, t, lane);
-  else x.b = p.by_new.quotient(t, i);
-  x.b = __builtin_amdgcn_readfirstlane(x.b);
-  if (x.b >= p.g.B) return false;
-  x.s = paged_seq<true>(p.g, x.b);
-  x.i = p.g.starts ? t - x.s.start : i;
-  return x.i >= 0 && x.i < x.s.n;
-}
-__device__ __forceinline__ int row_number(const PagedAttn& p, RowOf& x) {
-  int of_group;
-  x.hk = p.by_group.quotient(x.head, of_group);
-  return x.i * p.G + of_group;
-}
-
-// Rows of a wavefront of the last step: one while there are CUs without any, up to eight.
-inline int join_rows(int64_t n_rows) { return n_rows <= 8192 ? 1 : n_rows >= 65536 ? 8 : (int)(n_rows / 8192); }
 
 int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed);
 int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);

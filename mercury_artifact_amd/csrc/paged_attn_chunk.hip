@@ -42,18 +42,31 @@ __device__ __forceinline__ Pieces chunk_items(const PagedAttn& p, const PagedSeq
   c.parts = 1;
   return c;
 }
+// piece i of a sequence: K/V heads fastest (eight of them: one to an XCD's L2), then the row tiles, the last (longest) first
+struct Piece { int part, rt, hk; };
+__device__ __forceinline__ Piece piece_of(const Record& c, int Hkv, int64_t i) {
+  Piece x;
+  const int64_t of_part = (int64_t)c.rts * Hkv;
+  x.part = (int)(i / of_part);
+  const int rest = (int)(i - x.part * of_part);
+  x.rt = c.rts - 1 - rest / Hkv;
+  x.hk = rest % Hkv;
+  return x;
+}
+
 // ---- the plan ------------------------------------------------------------------------------------------------------------
 // One workgroup counts the items, cuts them into pieces and deals the pieces out, the longest first, since workgroups take them in order
-// as CUs come free.  It leaves for every piece its sequence (-1: none) and for every sequence its numbers.
+// as CUs come free.  It leaves for every piece its sequence (-1: none), for every sequence its numbers, and the items in several pieces.
 constexpr int kPlanWaves = 16, kStaged = 2048, kBuckets = 64;
 __global__ __launch_bounds__(kPlanWaves * 64) void paged_attn_chunk_plan(const PagedAttn p, int places) {
   __shared__ int steps_of[kStaged], rts_of[kStaged];
   __shared__ float sums[kPlanWaves][3][64];
-  __shared__ int extremes[2], longest, bucket[kBuckets], slots;
+  __shared__ int extremes[2], longest, bucket[kBuckets], slots, items;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = kPlanWaves * 64;
-  if (tid == 0) { extremes[0] = 0; extremes[1] = 0x7fffffff; slots = 0; }
+  if (tid == 0) { extremes[0] = 0; extremes[1] = 0x7fffffff; slots = items = 0; }
   if (tid < kBuckets) bucket[tid] = 0;
   for (int i = tid; i < places; i += threads) p.pieces[i] = -1;
+  for (int i = tid; i < kParts / 2; i += threads) p.shared[i].rows = 0;
   __syncthreads();
   for (int b = tid; b < p.g.B; b += threads) {
     const Pieces c = chunk_items(p, paged_seq<false>(p.g, b));
@@ -65,10 +78,7 @@ __global__ __launch_bounds__(kPlanWaves * 64) void paged_attn_chunk_plan(const P
   }
   __syncthreads();
   const int most = extremes[0], least = extremes[1];
-  if (most == 0) {
-    if (tid == 0) p.plan[0] = PlanOut{0};
-    return;
-  }
+  if (most == 0) return;
   // Each lane tries a length (the longest item in 1 .. 32, then up to 256 pieces) and estimates the launch's time: one round where
   // there is a CU for each piece, whole rounds where all are alike, else the mean of the CUs and a third of the last piece.
   {
@@ -149,34 +159,30 @@ __global__ __launch_bounds__(kPlanWaves * 64) void paged_attn_chunk_plan(const P
     p.records[b] = Record{atomicAdd(&bucket[bucket_of(c)], n), c.parts > 1 ? atomicAdd(&slots, n) : 0, c.parts, c.rts};
   }
   __syncthreads();
-  if (tid == 0) p.plan[0] = PlanOut{slots};
   for (int b = wave; b < p.g.B; b += kPlanWaves) {
     const Pieces c = seq(b);
     if (c.rts == 0) continue;
-    const int first = p.records[b].first, n = p.Hkv * c.rts * c.parts;
+    const Record r = p.records[b];
+    const int n = p.Hkv * c.rts * c.parts, in_part = p.Hkv * c.rts;
     for (int i = lane; i < n; i += 64)
-      if (first + i < places) p.pieces[first + i] = b;
+      if (r.first + i < places) p.pieces[r.first + i] = b;
+    if (c.parts == 1) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&items, in_part);
+    at = __builtin_amdgcn_readfirstlane(at);
+    const int rows = paged_seq<true>(p.g, b).n * p.G;
+    for (int i = lane; i < in_part; i += 64) {           // (as many as partial results / parts, so that there is room)
+      const Piece x = piece_of(r, p.Hkv, i);
+      const int left = rows - x.rt * kBM;
+      if (at + i < kParts / 2)
+        p.shared[at + i] = Shared{b, x.hk, x.rt * kBM, left < kBM ? left : kBM, c.parts, r.slot + i, r.slot + in_part + i, in_part};
+    }
   }
 }
 __device__ __forceinline__ Record record_of(const PagedAttn& p, int b) {
   const int* r = reinterpret_cast<const int*>(p.records + b);
   return Record{uniform_load(r, 0), uniform_load(r, 1), uniform_load(r, 2), uniform_load(r, 3)};
 }
-// piece i of a sequence: K/V heads fastest (eight of them: one to an XCD's L2), then the row tiles, the last (longest) first
-struct Piece { int part, rt, hk; };
-__device__ __forceinline__ Piece piece_of(const Record& c, int Hkv, int64_t i) {
-  Piece x;
-  const int64_t of_part = (int64_t)c.rts * Hkv;
-  x.part = (int)(i / of_part);
-  const int rest = (int)(i - x.part * of_part);
-  x.rt = c.rts - 1 - rest / Hkv;
-  x.hk = rest % Hkv;
-  return x;
-}
-__device__ __forceinline__ int64_t piece_number(const Record& c, int Hkv, int part, int rt, int hk) {
-  return ((int64_t)part * c.rts + (c.rts - 1 - rt)) * Hkv + hk;
-}
-
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
 constexpr int kFragDepth = 4;              // LDS operand reads in flight ahead of the MFMAs
 constexpr int kOStride = 136;              // epilogue staging of O, bf16 elements per row
@@ -681,31 +687,6 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   }
 }
 
-// The rows that several workgroups shared, a wavefront each; where there are many it does `each` of them, counting the pieces once.
-template <int COLS>
-__global__ __launch_bounds__(256) void paged_attn_chunk_join(const PagedAttn p, int64_t n_rows, int each) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each;
-  if (uniform_load(&p.plan->slots, 0) == 0) return;
-  RowOf x;
-  bool real = false;
-  Record c{};
-  for (int k = 0, token = -1; k < each && id0 + k < n_rows; ++k) {
-    if (const int t = token_of(p, (int)(id0 + k), x); t != token) {
-      token = t;
-      real = seq_of(p, t, lane, x) && x.s.n * p.G > p.few_rows;
-      if (!real) continue;
-      c = record_of(p, x.b);
-      real = c.parts > 1;
-    }
-    if (!real) continue;
-    const int r = row_number(p, x);
-    const int64_t first = c.slot + piece_number(c, p.Hkv, 0, r / kBM, x.hk), step = (int64_t)c.rts * p.Hkv;
-    const int row = r % kBM;
-    join_row<COLS>(p, lane, c.parts, [&](int part) { return (first + part * step) * kBM + row; }, x.b, x.s.start + x.i, x.head);
-  }
-}
-
 int64_t places_of(int64_t B, int64_t T, int64_t n, int G, int Hkv, bool packed) {
   return Hkv * (packed ? T * G / kBM + B : B * ((n * G + kBM - 1) / kBM)) + kParts;
 }
@@ -714,11 +695,10 @@ int64_t up16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
 template <bool E4M3, int COLS>
 void launch(const PagedAttn& p, int places, hipStream_t st) {
-  const int64_t n_rows = (int64_t)p.g.T * p.Hq;
-  const int each = join_rows(n_rows);
   hipLaunchKernelGGL(paged_attn_chunk_plan, dim3(1), dim3(kPlanWaves * 64), 0, st, p, places);
   hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)places), dim3(512), 0, st, p);
-  hipLaunchKernelGGL((paged_attn_chunk_join<COLS>), dim3((unsigned)((n_rows + 4 * each - 1) / (4 * each))), dim3(256), 0, st, p, n_rows, each);
+  constexpr int rows = 8;                              // of a workgroup: 4 / 8 / 16 / 32 take 57.0 / 58.6 / 65.2 / 76.4 us with 64 tokens at 32768
+  hipLaunchKernelGGL((paged_attn_join<COLS, kBM, 2, rows>), dim3(kBM / rows, kParts / 2), dim3(256), 0, st, p);
 }
 template <bool E4M3>
 void launch(const PagedAttn& p, int places, hipStream_t st) {
@@ -729,9 +709,9 @@ void launch(const PagedAttn& p, int places, hipStream_t st) {
 
 }  // namespace
 
-// The workspace: partial results, their maxima and sums, the plan's count, its records, its pieces.
+// The workspace: partial results, their maxima and sums, the items that are shared, the sequences' records, the pieces.
 int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed) {
-  return (int64_t)kParts * kBM * (columns_of(D) + 2) * 4 + 16 + 16 * B + up16(4 * places_of(B, T, n, G, Hkv, packed));
+  return (int64_t)kParts * kBM * (columns_of(D) + 2) * 4 + kParts / 2 * 32 + 16 * B + up16(4 * places_of(B, T, n, G, Hkv, packed));
 }
 int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
   const int64_t places = places_of(p.g.B, p.g.T, p.g.n, p.G, p.Hkv, p.g.starts != nullptr);
@@ -740,9 +720,10 @@ int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
   char* at = reinterpret_cast<char*>(q.part_o) + (int64_t)kParts * kBM * columns_of(p.D) * 4;
   q.part_ml = reinterpret_cast<f32x2*>(at);
   at += (int64_t)kParts * kBM * 8;
-  q.plan = reinterpret_cast<PlanOut*>(at);
-  q.records = reinterpret_cast<Record*>(at + 16);
-  q.pieces = reinterpret_cast<int*>(at + 16 + 16 * (int64_t)p.g.B);
+  q.shared = reinterpret_cast<Shared*>(at);
+  at += kParts / 2 * 32;
+  q.records = reinterpret_cast<Record*>(at);
+  q.pieces = reinterpret_cast<int*>(at + 16 * (int64_t)p.g.B);
   if (e4m3) launch<true>(q, (int)places, stream);
   else launch<false>(q, (int)places, stream);
   return MHIP_OK;
