@@ -29,18 +29,26 @@ constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descrip
 constexpr int kWavefronts = 1024;          // of the launch: four on a CU, in workgroups of four or two
 constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
-struct Item { int rts; int64_t steps; };   // row tiles of a sequence and K/V head, units of each
+// Row tiles of a sequence and K/V head, units of each, and what an item counts for: its units behind `pause` more, the time in which a
+// workgroup that enters it does not read.  Without it a workgroup with many short items ends last; where there are fewer items than
+// workgroups it would only spoil even shares.  us, 0 / 1 / 2 / 3 units: 64 x 20 .. 1024 H32/8 48.6 / 35.5 / 31.6 / 32.0, 64 x 100 .. 2048
+// 63.1 / 55.8 / 55.2 / 54.0 (e4m3 56.2 / 49.8 / 43.7 / 42.0), 256 x 20 .. 512 72.1 / 62.4 / 54.8 / 53.4, 32 x 300 .. 16384 203.0 / 202.6 /
+// 203.9 / 207.1; 8 tokens at 32768 34.4 / 35.8 / 35.7 / 35.8.
+struct Item { int rts, steps, weight; };
+template <int UNIT>
+constexpr int kPauseOf = UNIT == 2 * kKeys ? 2 : 0;
 template <int ROWS, int UNIT>
 __device__ __forceinline__ Item item_of(const PagedAttn& p, const PagedSeq& s) {
   Item it;
   it.rts = s.n * p.G <= p.few_rows ? (s.n * p.G + ROWS - 1) / ROWS : 0;
   it.steps = s.len > UNIT ? (s.len + UNIT - 1) / UNIT : 1;
+  it.weight = it.steps + kPauseOf<UNIT>;
   return it;
 }
 template <int ROWS, int UNIT, bool UNIFORM>
 __device__ __forceinline__ int64_t units_of(const PagedAttn& p, int b) {
   const Item it = item_of<ROWS, UNIT>(p, paged_seq<UNIFORM>(p.g, b));
-  return it.steps * it.rts * p.Hkv;
+  return (int64_t)it.weight * it.rts * p.Hkv;
 }
 
 // The units before each lane's run of sequences, and of all of them.
@@ -72,7 +80,7 @@ __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks 
 
 template <bool E4M3, int COLS, int NR, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn p) {
-  constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys;
+  constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys, kPause = kPauseOf<UNIT>;
   constexpr int kSize = E4M3 ? 1 : 2;
   constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
   constexpr int kChunks = ROWB / 16;
@@ -162,10 +170,14 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
   for (;;) {
     const PagedSeq s = paged_seq<true>(p.g, b);
     const Item it = item_of<ROWS, UNIT>(p, s);
-    const int64_t item = pos / it.steps;
-    const int first = (int)(pos - item * it.steps);
-    const int64_t left = hi - lo;
-    const int count = (int)(it.steps - first < left ? it.steps - first : left);
+    const int64_t item = pos / it.weight;
+    const int from = (int)(pos - item * it.weight);
+    const int take = (int)(it.weight - from < hi - lo ? it.weight - from : hi - lo);
+    const int first = from > kPause ? from - kPause : 0, count = from + take > kPause ? from + take - kPause - first : 0;
+    const int64_t start = lo - from;                   // of the item
+    lo += take;
+    pos += take;
+    if (count > 0) {
     const int hk = (int)(item / it.rts), rt = (int)(item - (int64_t)hk * it.rts);
     const int row0 = rt * ROWS;
     const int rows = s.n * p.G - row0 < ROWS ? s.n * p.G - row0 : ROWS;
@@ -403,7 +415,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
     if (first == 0) {
       leaves = leaves || !whole;
       if (threadIdx.x == 0 && (p.by_item || !whole)) {
-        const int last = (int)(((lo + it.steps) * shares - 1) / total);        // the workgroup with its last unit
+        const int last = (int)(((start + it.weight) * shares - 1) / total);        // the workgroup with its last unit
         const int64_t at = p.by_item ? (int64_t)b * it.rts * p.Hkv + item : w;
         p.shared[at] = Shared{b, hk, row0, whole ? 0 : rows, last - w + 1, 2 * w + 1, 2 * (w + 1), 2};
       }
@@ -442,14 +454,13 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
       }
     }
 
-    lo += count;
-    pos += count;
+    if (lo < hi) __syncthreads();
+    }
     if (lo >= hi) break;
-    if (pos >= it.steps * it.rts * p.Hkv) {
+    if (pos >= (int64_t)it.weight * it.rts * p.Hkv) {
       pos = 0;
       for (++b; b + 1 < p.g.B && units_of<ROWS, UNIT, true>(p, b) == 0;) ++b;
     }
-    __syncthreads();
   }
   if (!leaves && threadIdx.x == 0 && !p.by_item) p.shared[w].rows = 0;
 }
