@@ -341,7 +341,7 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
  * tokens' among them, which are the last ones.  An entry outside [0, pages) is a page that is not here (freed, not yet given,
  * or another rank's): nobody sees its keys, rows written to it are dropped, rows read from it are zeros.  New tokens lie in
  * tensors (B, n, heads, D), or, with `starts` (B + 1 whole numbers that do not fall), packed as (T, heads, D): rows starts[b] up
- * to starts[b + 1] are sequence b's, rows outside of all of them are neither read nor written.  Without starts T is B * n.
+ * to starts[b + 1] are sequence b's, rows outside of all of them take no part and stay as they are.  Without starts T is B * n.
  * page_table, lengths and starts are DEVICE arrays of int32, read when the kernels run (a captured graph follows them); a length
  * counts as one from 0 to table_pages * page_size, a start as one from 0 to T.
  * page_size: a multiple of 16, table_pages * page_size < 2^31, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
