@@ -125,6 +125,12 @@ __device__ __forceinline__ void copy16_to_lds(u32x4 rsrc, uint32_t lds_addr, int
                :: "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voffset), "s"(rsrc),
                   "s"(__builtin_amdgcn_readfirstlane(soffset)) : "memory");
 }
+// The same of data that nobody reads again soon: it takes no place in the caches from what is.
+__device__ __forceinline__ void copy16_once_to_lds(u32x4 rsrc, uint32_t lds_addr, int voffset, int soffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voffset), "s"(rsrc),
+                  "s"(__builtin_amdgcn_readfirstlane(soffset)) : "memory");
+}
 __device__ __forceinline__ void copy4_to_lds(u32x4 rsrc, uint32_t lds_addr, int voffset, int soffset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voffset), "s"(rsrc),

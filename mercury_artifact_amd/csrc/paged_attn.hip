@@ -234,7 +234,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
         const uint8_t* from = base + (held[h] > 0 ? row_offset(p, page[h], slot[h]) + hk * p.c_sh : 0);
         const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * (int)p.c_ss16 * 16 + p.D * kSize) : 0u);
 #pragma unroll
-        for (int u = 0; u < kCopies; ++u) copy16_to_lds(rs, ring + at + h * 16 * ROWB + u * 1024, voff[u], 0);
+        for (int u = 0; u < kCopies; ++u) copy16_once_to_lds(rs, ring + at + h * 16 * ROWB + u * 1024, voff[u], 0);
       }
     };
     auto copy_k = [&](int stage) {

@@ -121,7 +121,11 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const RowsParams p) {
 
 constexpr int kReadRows = 2;       // pairs of rows of a group of lanes, so that their loads are in flight together
 
-template <bool E4M3, int LANES>
+// ONCE: a chunk that does not fit the last-level cache (256 MB) passes it by, and so do the rows: 537 MB of e4m3 rows as bf16 take 154 us
+// so and 167 otherwise, 46 MB 13.5 and 11.1.
+constexpr int64_t kLastLevel = int64_t(256) << 20;
+
+template <bool E4M3, int LANES, bool ONCE>
 __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
   constexpr int kGroups = 256 / LANES;
   const int col = (threadIdx.x % LANES) * 8;
@@ -157,10 +161,12 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
       for (int half = 0; half < 2; ++half) {
         const uint8_t* src = (half ? p.v_cache : p.k_cache) + at;
         if constexpr (E4M3) {
-          codes[u][half] = *reinterpret_cast<const u32x2*>(src + col);
+          const u32x2* from = reinterpret_cast<const u32x2*>(src + col);
+          codes[u][half] = ONCE ? __builtin_nontemporal_load(from) : *from;
           scale[u][half] = (half ? p.v_scales : p.k_scales)[s];
         } else {
-          w[u][half] = *reinterpret_cast<const u32x4*>(src + col * 2);
+          const u32x4* from = reinterpret_cast<const u32x4*>(src + col * 2);
+          w[u][half] = ONCE ? __builtin_nontemporal_load(from) : *from;
         }
       }
     }
@@ -179,7 +185,9 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
           w[u][half][2 * h + 1] = pack_bf16(hi[0] * scale[u][half], hi[1] * scale[u][half]);
         }
       }
-      *reinterpret_cast<u32x4*>(p.out + half * p.o_half + b[u] * p.o_sb + i[u] * p.o_ss + head[u] * p.o_sh + col) = w[u][half];
+      u32x4* to = reinterpret_cast<u32x4*>(p.out + half * p.o_half + b[u] * p.o_sb + i[u] * p.o_ss + head[u] * p.o_sh + col);
+      if (ONCE) __builtin_nontemporal_store(w[u][half], to);
+      else *to = w[u][half];
     }
   }
 }
@@ -292,12 +300,17 @@ extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, c
   const bool wide = D > 64;
   const int groups = (wide ? 16 : 32) * kReadRows;
   const dim3 grid((unsigned)((p.total + groups - 1) / groups)), block(256);
-  if (dtype == MHIP_E4M3) {
-    if (wide) hipLaunchKernelGGL((paged_read_kernel<true, 16>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((paged_read_kernel<true, 8>), grid, block, 0, st, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((paged_read_kernel<false, 16>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((paged_read_kernel<false, 8>), grid, block, 0, st, p);
-  }
+  const bool once = (int64_t)p.total * D * 4 > kLastLevel;
+  auto launch = [&](auto lanes, auto past) {
+    constexpr int L = decltype(lanes)::value;
+    constexpr bool O = decltype(past)::value;
+    if (dtype == MHIP_E4M3) hipLaunchKernelGGL((paged_read_kernel<true, L, O>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_read_kernel<false, L, O>), grid, block, 0, st, p);
+  };
+  using std::integral_constant;
+  if (wide && once) launch(integral_constant<int, 16>{}, std::true_type{});
+  else if (wide) launch(integral_constant<int, 16>{}, std::false_type{});
+  else if (once) launch(integral_constant<int, 8>{}, std::true_type{});
+  else launch(integral_constant<int, 8>{}, std::false_type{});
   return launch_status();
 }
