@@ -484,3 +484,98 @@ def test_refusals_say_why():
     ]:
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+@pytest.mark.parametrize("Hq,new", [(80, 1), (128, 1), (80, 2), (65, 1), (64, 1), (33, 2)])
+def test_many_query_heads_on_one_key_head(Hq, new):
+    """More rows of one token than the kernel for few rows takes, padded and packed."""
+    s = Setting([200, 1, 77], 1, 64, 16, True, seed=Hq)
+    q = torch.randn(3, new, Hq, 64, generator=s.g).bfloat16()
+    out, lse = _attend(s, q, 0.125)
+    _check(s, q, out, lse, 0.125)
+    starts = [0, new, 2 * new, 3 * new]
+    packed = q.reshape(3 * new, Hq, 64)
+    for most in (None, new):
+        out, lse = _attend(s, packed, 0.125, starts=starts, most_new=most)
+        _check(s, packed, out, lse, 0.125, starts=starts)
+
+
+@pytest.mark.parametrize("new,Hq", [(1, 2), (40, 2)])
+def test_thousands_of_sequences(new, Hq):
+    """More sequences than the plan of a launch keeps on chip; some of them against the restatement."""
+    B = 2500
+    s = Setting([(7 * b) % 45 for b in range(B)], 1, 16, 16, False, seed=B)
+    q = torch.randn(B, new, Hq, 16, generator=s.g).bfloat16()
+    out, lse = _attend(s, q, 0.25)
+    for b in (0, 1, 63, 64, 65, 1000, 2047, 2048, 2049, 2499):
+        one = Setting.__new__(Setting)
+        one.cache, one.scales, one.lengths, one.table = s.cache, None, [s.lengths[b]], [s.table[b]]
+        _check(one, q[b:b + 1], out[b:b + 1], lse[b:b + 1], 0.25)
+
+
+def test_scales_that_are_no_powers_of_two():
+    """Such as max|x| / 448: few rows take them exactly, long chunks count the rows as rounded to bf16."""
+    for new in (1, 90):
+        s = Setting([300], 1, 64, 16, True, seed=17)
+        s.scales = s.scales * 0.77
+        s.dev_scales = s.scales.transpose(2, 3).contiguous().cuda().transpose(2, 3)
+        q = torch.randn(1, new, 2, 64, generator=s.g).bfloat16()
+        out, lse = _attend(s, q, 0.125)
+        if new > 1:
+            s.cache, s.scales = (s.cache * s.scales.double()[..., None]).bfloat16(), None
+        _check(s, q, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_no_new_tokens_and_outputs_over_q(e4m3):
+    s = Setting([40, 9], 2, 64, 16, e4m3, seed=1)
+    out, lse = _attend(s, torch.zeros(2, 0, 4, 64, dtype=torch.bfloat16), 0.1)
+    assert out.shape == (2, 0, 4, 64) and lse.shape == (2, 4, 0)
+    out, lse = _attend(s, torch.zeros(0, 4, 64, dtype=torch.bfloat16), 0.1, starts=[0, 0, 0])
+    assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    for new in (1, 100):
+        q = torch.randn(2, new, 4, 64, generator=s.g).bfloat16()
+        want = _attend(s, q, 0.1)
+        dev = q.cuda()
+        table, lengths = s.tables()
+        got, _ = M.paged_attn_fwd(dev, s.dev, table, lengths, 0.1, scales=s.dev_scales, out=dev)
+        assert got.data_ptr() == dev.data_ptr() and torch.equal(got.cpu(), want[0])
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_the_interpreters_path_gives_the_same(monkeypatch, new):
+    """A call that the compiled host module leaves to Python."""
+    s = Setting([140, 95], 2, 64, 16, True, seed=3)
+    q = torch.randn(2, new, 4, 64, generator=s.g).bfloat16()
+    k = torch.randn(2, 3, 2, 64, generator=s.g).bfloat16().cuda()
+    table, lengths = s.tables()
+    M.paged_cache_write(k, k, s.dev, table, lengths, scales=s.dev_scales)
+    want, want_read = _attend(s, q, 0.1), M.paged_cache_read(s.dev, table, lengths, 150, scales=s.dev_scales)
+    codes = s.dev.view(torch.uint8).clone()
+
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    monkeypatch.setattr(N, "host", Declines())
+    M.paged_cache_write(k, k, s.dev, table, lengths, scales=s.dev_scales)
+    assert torch.equal(s.dev.view(torch.uint8), codes)
+    got, got_read = _attend(s, q, 0.1), M.paged_cache_read(s.dev, table, lengths, 150, scales=s.dev_scales)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got_read, want_read)
+
+
+def test_a_captured_packed_step_follows_its_starts():
+    """Long chunks and single tokens in one captured call, replayed with other shares of the same packed rows."""
+    s = Setting([150, 260, 90], 1, 64, 16, False, seed=23)
+    table, lengths = s.tables()
+    T, starts = 140, torch.zeros(4, dtype=torch.int32).cuda()
+    q = torch.randn(T, 4, 64, generator=s.g).bfloat16()
+    dev, out, lse = q.cuda(), torch.zeros(T, 4, 64, dtype=torch.bfloat16).cuda(), torch.zeros(4, T).cuda()
+    graphed = M.GraphedStep(lambda: M.paged_attn_fwd(dev, s.dev, table, lengths, 0.1, starts=starts, out=out, lse=lse))
+    for new in ([130, 1, 9], [1, 130, 2], [50, 0, 90], [0, 0, 0], [1, 1, 1], [140, 0, 0]):
+        out.fill_(7.0)
+        starts.copy_(torch.tensor(_starts(new), dtype=torch.int32))
+        graphed.replay()
+        torch.cuda.synchronize()
+        _check(s, q, out.cpu(), lse.cpu(), 0.1, starts=_starts(new))
+        assert (out[sum(new):] == 7).all()
