@@ -4,18 +4,19 @@
 // once for all of them: rows r = token * G + head of the group.
 //
 // paged_attn_few: bound by memory (each byte of the cache feeds as many multiply-adds as there are rows).
-//   work       : a unit is 128 keys of one (sequence, K/V head, tile of rows).  The units of all sequences, counted by every
+//   work       : a unit is 128 (or 64) keys of one (sequence, K/V head, tile of rows).  The units of all sequences, counted by every
 //                workgroup from the lengths in device memory, are dealt out evenly and in order to one workgroup per CU: a
 //                long sequence beside short ones, or alone, keeps all CUs reading, without the host knowing a length.  A
 //                workgroup whose share ends inside an item leaves a partial result, and paged_attn_join adds those up.
-//   wavefront  : every fourth tile of 32 keys is its own, in a ring of 32 KB of LDS filled by copies that do not pass through
-//                registers (buffer_load ... lds): no barrier in the loop, and 64 to 128 KB in flight on a CU, where 25 bytes
-//                a nanosecond times the latency of a microsecond asks for 25 KB.
+//   wavefront  : every fourth (second) tile of 32 keys is its own, in a ring of LDS filled by copies that do not pass through
+//                registers (buffer_load ... lds) nor stay in the caches (a key is read once): no barrier in the loop, and 64
+//                to 128 KB in flight on a CU, where 25 bytes a nanosecond times the latency of a microsecond asks for 25 KB.
 //   S^T = K Q^T: v_mfma_f32_16x16x32_bf16 with A = K rows from LDS and B = Q rows in registers: lane (ln, lg) then holds
 //                keys 4 lg .. +3 of both halves of a tile for row ln, softmax is lane-local but for two exchanges.
 //   O^T = V^T P^T: the same lane's P is the B operand, and the transposing LDS reads fetch V^T in its key order.
 //   e4m3       : codes are exact in bf16 (v_cvt_scalef32_pk_bf16_fp8); a key's scale multiplies its score, a value's scale
-//                its weight, in fp32.  Rounding P to bf16 (2^-9 of each weight at most) is the only rounding before the last.
+//                its weight, in fp32.  The weights go to the product as bf16 (off by 2^-8 of each at most), up to 16 rows as
+//                two bf16 numbers (2^-16); there is no other rounding below 32 bits before the last.
 #include "paged_attn.hpp"
 
 namespace mhip {
@@ -24,9 +25,13 @@ namespace {
 typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i32x2;
 
 constexpr int kKeys = 32;                  // keys of a tile, one wavefront's
-constexpr int kRing = 32768;               // bytes of K and V tiles of a wavefront
+// Bytes of K and V tiles of a wavefront, of which a CU has 128 KB: four wavefronts of them, or eight of half as much.  Eight where each has
+// conversions to do beside its copies and registers for two on a SIMD: e4m3 with up to 16 rows (four / eight wavefronts: 64 x 100 .. 2048
+// H32/8 43.4 / 35.9 us, 32 x 300 .. 16384 111.1 / 102.3, 16 x 5 tokens behind 211 .. 4099 D80 29.1 / 24.4, 4 x 131072 180.6 / 181.2).
+template <bool E4M3, int NR>
+constexpr int kRingOf = E4M3 && NR == 1 ? 16384 : 32768;
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
-constexpr int kWavefronts = 1024;          // of the launch: four on a CU, in workgroups of four or two
+constexpr int kWavefronts = 1024;          // of a launch with rings of 32 KB: four on a CU, in workgroups of four or two
 constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
 // Row tiles of a sequence and K/V head, units of each, and what an item counts for: its units behind `pause` more, the time in which a
@@ -79,7 +84,7 @@ __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks 
 }
 
 template <bool E4M3, int COLS, int NR, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn p) {
+__global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged_attn_few(const PagedAttn p) {
   constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys, kPause = kPauseOf<UNIT>;
   constexpr int kSize = E4M3 ? 1 : 2;
   constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
@@ -87,11 +92,14 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
   constexpr int kCopyRows = 1024 / ROWB;               // rows of one copy instruction
   constexpr int kCopies = 16 / kCopyRows;              // and instructions of half a tile
   constexpr int kTileBytes = kKeys * ROWB;
-  constexpr int kStages = kRing / (2 * kTileBytes);
+  constexpr int kStages = kRingOf<E4M3, NR> / (2 * kTileBytes);
   constexpr int kStage = 2 * kTileBytes + (E4M3 ? 256 : 0);      // K, V, 32 scales of each
   constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
   constexpr int KB = COLS / 32, DB = COLS / 16;
   constexpr int kPair = NR < 2 ? NR : 2;               // blocks of rows that are worked on together
+  // Weights to 16 bits of their mantissa, in two products, where that costs next to nothing: up to 16 rows (32 sequences of 300 .. 16384
+  // bf16 177.8 us and 177.8, e4m3 102.3 and 103.3).  With more rows the matrix instructions show, and weights are rounded to bf16 once.
+  constexpr bool kTwice = NR == 1;
   constexpr int kRegion = kStages * kStage;
   static_assert(ROWS * COLS * 4 <= kRegion, "a wavefront's O takes the place of its ring");
   static_assert(kStages * (nK + nV) < 64, "copies in flight are counted in 6 bits");
@@ -271,6 +279,10 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
     }
     look_up(kStages);
 
+    auto weigh = [&](int db, int r, const bf16x8& vf, const u32x4& high, const u32x4& low) __attribute__((always_inline)) {
+      o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, high), o[db][r]);
+      if (kTwice) o[db][r] = mfma(vf, __builtin_bit_cast(bf16x8, low), o[db][r]);
+    };
     for (int t = 0; t < count; ++t) {
       const int stage = t % kStages, at = stage * kStage, key0 = key_of(t);
       const uint32_t hidden = gone >> (2 * stage) & 3u;
@@ -308,7 +320,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
         }
 
         // ---- softmax --------------------------------------------------------------------------------------------
-        u32x4 pw[kPair];
+        u32x4 pw[kPair], pl[kPair];                              // weights in bf16, and what rounding left of them
         bool moved = false;
         float alpha[kPair];
 #pragma unroll
@@ -348,7 +360,10 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+          for (int i = 0; i < 4; ++i) {
+            pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            if (kTwice) pl[r][i] = pack_bf16(x[2 * i] - bf16_lo(pw[r][i]), x[2 * i + 1] - bf16_hi(pw[r][i]));
+          }
         }
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
@@ -365,7 +380,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
           for (int db = 0; db < DB; ++db) {
             const bf16x8 vf = read_v(db, at);
 #pragma unroll
-            for (int r = 0; r < kPair; ++r) o[db][r0 + r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r0 + r]);
+            for (int r = 0; r < kPair; ++r) weigh(db, r0 + r, vf, pw[r], pl[r]);
           }
         } else {
           // (some rows do not see some of the keys: see finite_part)
@@ -374,7 +389,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void paged_attn_few(const PagedAttn 
           for (int db = 0; db < DB; ++db) {
             const bf16x8 vf = __builtin_bit_cast(bf16x8, finite_part(__builtin_bit_cast(u32x4, read_v(db, at)), odd));
 #pragma unroll
-            for (int r = 0; r < kPair; ++r) o[db][r0 + r] = mfma(vf, __builtin_bit_cast(bf16x8, pw[r]), o[db][r0 + r]);
+            for (int r = 0; r < kPair; ++r) weigh(db, r0 + r, vf, pw[r], pl[r]);
             __builtin_amdgcn_sched_barrier(0);
           }
           if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
@@ -475,11 +490,11 @@ int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 constexpr int64_t kManyItems = 128;
 
 // One partial result at each end of a workgroup's share.
-int64_t few_bytes(int64_t rows, int D) { return kWavefronts * (16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4 + 16); }
+int64_t few_bytes(int64_t rows, int D) { return 2 * kWavefronts * (16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4 + 16); }
 
 template <bool E4M3, int COLS, int NR, int WAVES>
 void launch_few(PagedAttn p, int64_t rows, hipStream_t st) {
-  constexpr int workgroups = kWavefronts / WAVES;
+  constexpr int workgroups = kWavefronts * (32768 / kRingOf<E4M3, NR>) / WAVES;
   p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)workgroups * 16 * NR * COLS);
   p.shared = reinterpret_cast<Shared*>(p.part_ml + 2 * (int64_t)workgroups * 16 * NR);
   // Where the items are known and not more than the workgroups, the last step has one row of workgroups for each of them, not for
