@@ -344,7 +344,7 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
  * to starts[b + 1] are sequence b's, rows outside of all of them take no part and stay as they are.  Without starts T is B * n.
  * page_table, lengths and starts are DEVICE arrays of int32, read when the kernels run (a captured graph follows them); a length
  * counts as one from 0 to table_pages * page_size, a start as one from 0 to T.
- * page_size: a multiple of 16, table_pages * page_size < 2^31, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
+ * page_size: a multiple of 16, table_pages * page_size <= 2^31 - 2^16, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
  * multiple of 8 (MHIP_E4M3: of 16) up to 128.  Bases and rows on 16 bytes.
  */
 

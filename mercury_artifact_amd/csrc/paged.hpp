@@ -16,7 +16,7 @@ struct PagedGeom {
   const int* table; const int* lengths; const int* starts;     // starts: NULL where every sequence has n new tokens
   int64_t t_sb;                    // entries from one sequence's table row to the next one's
   int B, n, T;                     // sequences, new tokens of each, new tokens of all
-  int pages, page, width;          // pages of the cache, their rows, entries of a table row (width * page < 2^31)
+  int pages, page, width;          // pages of the cache, their rows, entries of a table row (width * page <= 2^31 - 2^16)
   Divisor by_page;
 };
 

@@ -16,7 +16,7 @@
 //   O^T = V^T P^T: the same lane's P is the B operand, and the transposing LDS reads fetch V^T in its key order.
 //   e4m3       : codes are exact in bf16 (v_cvt_scalef32_pk_bf16_fp8); a key's scale multiplies its score, a value's scale
 //                its weight, in fp32.  The weights go to the product as bf16 (off by 2^-8 of each at most), up to 16 rows as
-//                two bf16 numbers (2^-16); there is no other rounding below 32 bits before the last.
+//                two bf16 numbers (2^-14); there is no other rounding below 32 bits before the last.
 #include "paged_attn.hpp"
 
 namespace mhip {
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
   constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
   constexpr int KB = COLS / 32, DB = COLS / 16;
   constexpr int kPair = NR < 2 ? NR : 2;               // blocks of rows that are worked on together
-  // Weights to 16 bits of their mantissa, in two products, where that costs next to nothing: up to 16 rows (32 sequences of 300 .. 16384
+  // Weights to 14 bits and more of their mantissa, in two products, where that costs next to nothing: up to 16 rows (32 sequences of 300 .. 16384
   // bf16 177.8 us and 177.8, e4m3 102.3 and 103.3).  With more rows the matrix instructions show, and weights are rounded to bf16 once.
   constexpr bool kTwice = NR == 1;
   constexpr int kRegion = kStages * kStage;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
         }
 
         // ---- softmax --------------------------------------------------------------------------------------------
-        u32x4 pw[kPair], pl[kPair];                              // weights in bf16, and what rounding left of them
+        u32x4 pw[kPair], pl[kPair];                              // weights in bf16, and what that leaves of them
         bool moved = false;
         float alpha[kPair];
 #pragma unroll
@@ -361,8 +361,15 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
             for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-            if (kTwice) pl[r][i] = pack_bf16(x[2 * i] - bf16_lo(pw[r][i]), x[2 * i + 1] - bf16_hi(pw[r][i]));
+            if constexpr (kTwice) {
+              // (cut off, not rounded, and the rest a little large: both have the weight's sign and are zero only with it, so that
+              // infinite values stay what they are)
+              pw[r][i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
+              pl[r][i] = pack_bf16(__builtin_fmaf(x[2 * i], 0x1.00004p0f, -bf16_lo(pw[r][i])),
+                                   __builtin_fmaf(x[2 * i + 1], 0x1.00004p0f, -bf16_hi(pw[r][i])));
+            } else {
+              pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            }
           }
         }
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {

@@ -12,8 +12,8 @@
 //                at the start of a vector phase and used at its end, when nothing else waits on that counter
 //   e4m3       : a wavefront's 8 rows of codes come through registers, requested one tile ahead, and go into LDS as bf16 rows
 //                times their scale, exact for a power of two: converted once by one wavefront, not by all eight
-//   pieces     : where the items are few, or one is long, several workgroups share an item's keys (cut_of) and a second kernel
-//                joins their partial results
+//   pieces     : where the items are few, or one is long, several workgroups share an item's keys: paged_attn_chunk_plan cuts
+//                them and deals them out, paged_attn_join adds the partial results up
 #include "paged_attn.hpp"
 
 namespace mhip {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kPlanWaves * 64) void paged_attn_chunk_plan(const P
     const Record r = p.records[b];
     const int n = p.Hkv * c.rts * c.parts, in_part = p.Hkv * c.rts;
     for (int i = lane; i < n; i += 64)
-      if (r.first + i < places) p.pieces[r.first + i] = b;
+      if ((uint32_t)(r.first + i) < (uint32_t)places) p.pieces[r.first + i] = b;       // (starts that fall may count more than there are)
     if (c.parts == 1) continue;
     int at = 0;
     if (lane == 0) at = atomicAdd(&items, in_part);

@@ -222,7 +222,7 @@ int paged_cache_fits(const void* kc, const void* vc, const float* ks, const floa
 int paged_geometry(PagedGeom& g, const int* table, const int* lengths, const int* starts, int64_t t_sb, int B, int n, int T, int pages,
                    int page, int width) {
   if (B < 0 || n < 0 || T < 0 || pages < 0 || width < 0 || page <= 0) return MHIP_EINVAL;
-  if (page % 16 != 0 || (int64_t)width * page >= (int64_t(1) << 31)) return MHIP_EUNSUPPORTED;
+  if (page % 16 != 0 || (int64_t)width * page > 0x7fff0000) return MHIP_EUNSUPPORTED;      // (positions a few tiles past the last key are ints)
   if (B > 0 && (!lengths || (width > 0 && !table))) return MHIP_EINVAL;
   if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(starts)) & 3u) return MHIP_EALIGN;
   g.table = table; g.lengths = lengths; g.starts = starts;

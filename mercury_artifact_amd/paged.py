@@ -11,10 +11,11 @@ different chunks do (``merge_many``, ``update_out_and_lse``).
 New tokens come as ``(B, n, heads, D)``, or packed as ``(T, heads, D)`` with ``starts`` ``(B + 1,)``: rows ``starts[b]`` up to
 ``starts[b + 1]`` belong to sequence b, rows outside of all are left alone.  They are the last ones of their sequence:
 ``lengths`` counts them.  Nothing here waits for the GPU or looks at the values of tables, lengths and starts on the host.
-The reference has no counterpart; an operator that is asked for something it does not do raises ``RuntimeError``.
+They compute no gradients.  The reference has no counterpart; an operator that is asked for something it does not do raises ``RuntimeError``.
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -54,6 +55,8 @@ def _check_cache(cache, scales, page_table, lengths, starts=None):
         raise RuntimeError("page_table must be an int32 (B, pages of a sequence) tensor with contiguous rows")
     if starts is not None and (starts.shape != (B + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous()):
         raise RuntimeError("starts must be a contiguous int32 (B + 1,) tensor")
+    _whole("the number of pages", cache.shape[1])
+    _whole("the number of entries of page_table", page_table.shape[1])
     for t in (scales, page_table, lengths, starts):
         if t is not None and t.device != cache.device:
             raise RuntimeError("cache, scales, page_table, lengths and starts must be on one device")
@@ -67,7 +70,18 @@ def _check_tokens(name, t, B, starts, heads, head_dim, device):
         raise RuntimeError(f"{name} must be (B, new tokens, heads, head_dim), or (all new tokens, heads, head_dim) with starts")
     if t.shape[-2] != heads or t.shape[-1] != head_dim or t.stride(-1) != 1 or t.dtype != torch.bfloat16 or t.device != device:
         raise RuntimeError(f"{name} must be bfloat16 with {heads} heads of {head_dim}, a contiguous last dimension, on the cache's device")
-    return (t.shape[1], t.shape[0] * t.shape[1]) if starts is None else (0, t.shape[0])
+    return (t.shape[1], _whole("the number of new tokens", t.shape[0] * t.shape[1])) if starts is None else (0, t.shape[0])
+
+
+def _whole(name, x, bits=31):
+    """x as a number that a C int (or one of as many bits) holds."""
+    try:
+        whole = operator.index(x)
+    except TypeError:
+        whole = -1
+    if not 0 <= whole < 2 ** bits:
+        raise RuntimeError(f"invalid {name}: {x!r} is no whole number from 0 to 2^{bits} - 1")
+    return whole
 
 
 def _token_strides(t):
@@ -120,9 +134,8 @@ def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: tor
         return done
     B = _check_cache(cache, scales, page_table, lengths)
     _, pages, page_size, Hkv, D = cache.shape
+    rows, begin = _whole("rows", rows), _whole("begin", begin)
     if out is None:
-        if rows < 0:
-            raise RuntimeError("rows must not be negative")
         out = torch.empty((2, B, rows, Hkv, D), dtype=torch.bfloat16, device=cache.device)
     elif out.shape != (2, B, rows, Hkv, D) or out.dtype != torch.bfloat16 or out.stride(-1) != 1 or out.device != cache.device:
         raise RuntimeError("out must be (2, B, rows, kv_heads, head_dim) bfloat16 with a contiguous last dimension, on the cache's device")
@@ -165,7 +178,7 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
         N.require_cuda(lse)
         if lse.shape != shape or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != cache.device:
             raise RuntimeError(f"lse must be a contiguous float32 {shape} tensor on the cache's device")
-    most = n if starts is None else T if most_new is None else min(most_new, T)
+    most = n if starts is None else T if most_new is None else min(_whole("most_new", most_new, 63), T)
     size = N.lib().mhip_paged_attn_workspace_bytes(B, n, T, most, int(starts is not None), Hq, Hkv, D)
     if size < 0:
         N.check(int(size), "mhip_paged_attn_workspace_bytes")

@@ -579,3 +579,34 @@ def test_a_captured_packed_step_follows_its_starts():
         torch.cuda.synchronize()
         _check(s, q, out.cpu(), lse.cpu(), 0.1, starts=_starts(new))
         assert (out[sum(new):] == 7).all()
+
+
+@pytest.mark.parametrize("new,Hq", [(1, 4), (16, 1), (12, 2), (20, 2), (130, 1)])
+def test_infinite_values_that_every_row_sees(new, Hq):
+    """Weights are all above 2^-60 here: a value of infinity is one in every row's result, whatever sign, and no NaN."""
+    s = Setting([200], 1, 64, 16, False, seed=new)
+    q = torch.randn(1, new, Hq, 64, generator=s.g).bfloat16()
+    for key, column, what in ((3, 5, math.inf), (70, 6, -math.inf), (199, 7, math.inf)):
+        page, slot = s.table[0][key // 16], key % 16
+        s.cache[1, page, slot, 0, column] = what
+        s.dev[1, page, slot, 0, column] = what
+    out, lse = _attend(s, q, 0.125, causal=False)
+    _check(s, q, out, lse, 0.125, causal=False)
+    for column, what in ((5, math.inf), (6, -math.inf), (7, math.inf)):
+        assert (out[0, :, :, column] == what).all()
+
+
+def test_numbers_that_no_c_int_holds():
+    s = Setting([40], 1, 64, 16, False)
+    table, lengths = s.tables()
+    for rows, begin in ((5, 2 ** 32), (2 ** 32 + 5, 0), (5, 1.5), (None, 0)):
+        with pytest.raises(RuntimeError, match="invalid"):
+            M.paged_cache_read(s.dev, table, lengths, rows, begin)
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16).cuda()
+    starts = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    for most in (2 ** 63, -1, "1"):
+        with pytest.raises(RuntimeError, match="invalid"):
+            M.paged_attn_fwd(q, s.dev, table, lengths, 0.1, starts=starts, most_new=most)
+    assert (M.paged_cache_read(s.dev, table, lengths, 3, 2 ** 31 - 4) == 0).all()
+    for most in (2 ** 32 + 1, 1):
+        M.paged_attn_fwd(q, s.dev, table, lengths, 0.1, starts=starts, most_new=most)

@@ -124,3 +124,9 @@ def test_no_cpu_fallback():
             call()
     with pytest.raises(RuntimeError, match="bfloat16 or float8"):
         M.paged_cache(2, 16, 2, 64, dtype=torch.float16, device="cpu")
+
+
+def test_positions_stay_below_the_last_ints(lib):
+    for call in (_write, _read, _attn):
+        assert call(lib, width=(1 << 27) - (1 << 12) + 1) == EUNSUPPORTED
+    assert _attn(lib, B=0, width=(1 << 27) - (1 << 12)) == OK
