@@ -25,6 +25,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall",
 # unit: with MFMA results in arithmetic registers (and only the stationary operands in accumulation
 # registers) there are no copies between the two register files in its main loop.
 # attn_fwd_fp8.hip: the form with one wavefront per SIMD would get accumulation registers and copy every score out of them.
+# paged_attn.hip: one or two wavefronts per SIMD, whose rescaled O would move between the two register files with every new maximum.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 EXTRA_FLAGS = {"attn_bwd.hip": VGPR_FORM, "attn_fwd_fp8.hip": VGPR_FORM, "paged_attn.hip": VGPR_FORM}
 

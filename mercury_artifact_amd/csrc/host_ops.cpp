@@ -891,7 +891,8 @@ PyObject* bind(PyObject*, PyObject* table) {
                   take(entry.pack, "mhip_pack_reduce") && take(entry.unpack, "mhip_unpack") &&
                   take(entry.quantize, "mhip_quantize_e4m3") &&
                   take(entry.paged_write, "mhip_paged_cache_write") && take(entry.paged_read, "mhip_paged_cache_read") &&
-                  take(entry.paged_bytes, "mhip_paged_attn_workspace_bytes") && take(entry.paged_attn, "mhip_paged_attn_fwd") && take(entry.error_string, "mhip_error_string");
+                  take(entry.paged_bytes, "mhip_paged_attn_workspace_bytes") && take(entry.paged_attn, "mhip_paged_attn_fwd") &&
+                  take(entry.error_string, "mhip_error_string");
   if (PyErr_Occurred()) return nullptr;
   bound = ok;
   return PyBool_FromLong(ok);

@@ -155,7 +155,8 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     """Attention of the new tokens over their sequences' keys, their own among them: ``out`` like q in bfloat16 and ``lse``
     (B, Hq, n) -- packed: (Hq, T) -- in float32.  ``causal``: new token i of n sees the keys up to ``lengths - n + i``, else all
     of them.  Rows that see no key get 0 and -inf.  ``most_new``: with ``starts``, about how many new tokens a sequence has at
-    most (default: all of them in one); it chooses the form of the kernels, the result does not depend on it."""
+    most (default: all of them in one); it chooses the form of the kernels, the result does not depend on it.  ``out`` may be
+    q itself."""
     done = N.host.paged_attn_fwd(q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse)
     if done is not None:
         return done

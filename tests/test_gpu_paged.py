@@ -610,3 +610,20 @@ def test_numbers_that_no_c_int_holds():
     assert (M.paged_cache_read(s.dev, table, lengths, 3, 2 ** 31 - 4) == 0).all()
     for most in (2 ** 32 + 1, 1):
         M.paged_attn_fwd(q, s.dev, table, lengths, 0.1, starts=starts, most_new=most)
+
+
+@pytest.mark.parametrize("new,Hq", [(1, 4), (12, 4), (20, 8), (300, 2)])
+def test_out_may_take_the_place_of_q(new, Hq):
+    s = Setting([1500, 320, 700], 2, 128, 16, True, seed=new)
+    q = torch.randn(3, new, Hq, 128, generator=s.g).bfloat16()
+    want = _attend(s, q, 0.1)
+    table, lengths = s.tables()
+    mine = q.cuda()
+    out, lse = M.paged_attn_fwd(mine, s.dev, table, lengths, 0.1, scales=s.dev_scales, out=mine)
+    assert out.data_ptr() == mine.data_ptr()
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(lse.cpu(), want[1])
+    starts = torch.tensor([0, new, 2 * new, 3 * new], dtype=torch.int32).cuda()
+    mine = q.reshape(3 * new, Hq, 128).cuda()
+    packed, lse = M.paged_attn_fwd(mine.clone(), s.dev, table, lengths, 0.1, scales=s.dev_scales, starts=starts)
+    M.paged_attn_fwd(mine, s.dev, table, lengths, 0.1, scales=s.dev_scales, starts=starts, out=mine)
+    assert torch.equal(mine, packed)
