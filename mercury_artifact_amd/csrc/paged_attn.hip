@@ -50,24 +50,29 @@ __device__ __forceinline__ Item item_of(const PagedAttn& p, const PagedSeq& s) {
   it.weight = it.steps + kPauseOf<UNIT>;
   return it;
 }
-template <int ROWS, int UNIT, bool UNIFORM>
-__device__ __forceinline__ int64_t units_of(const PagedAttn& p, int b) {
-  const Item it = item_of<ROWS, UNIT>(p, paged_seq<UNIFORM>(p.g, b));
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int64_t units_of(const PagedAttn& p, const PagedSeq& s) {
+  const Item it = item_of<ROWS, UNIT>(p, s);
   return (int64_t)it.weight * it.rts * p.Hkv;
 }
 
 // The units before each lane's run of sequences, and of all of them.
 struct Plan {
   int per;                   // sequences of a lane
+  PagedSeq last;             // and the last of them
   int64_t before, mine, total;
 };
 template <int ROWS, int UNIT>
 __device__ __forceinline__ Plan plan_of(const PagedAttn& p, int lane) {
   Plan plan;
   plan.per = (p.g.B + 63) / 64;
+  plan.last = PagedSeq{};
   plan.mine = 0;
   for (int j = 0; j < plan.per; ++j)
-    if (lane * plan.per + j < p.g.B) plan.mine += units_of<ROWS, UNIT, false>(p, lane * plan.per + j);
+    if (lane * plan.per + j < p.g.B) {
+      plan.last = paged_seq<false>(p.g, lane * plan.per + j);
+      plan.mine += units_of<ROWS, UNIT>(p, plan.last);
+    }
   int64_t sum = plan.mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -125,7 +130,13 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
   const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= plan.before && lo < plan.before + plan.mine));
   int b = owner * plan.per;
   int64_t pos = lo - uniform64(__shfl((long long)plan.before, owner));     // inside sequence b
-  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<ROWS, UNIT, true>(p, b)); ++b) pos -= u;
+  // (up to 64 sequences are a lane's each, which need not be read once more)
+  PagedSeq s{__builtin_amdgcn_readlane(plan.last.start, owner), __builtin_amdgcn_readlane(plan.last.n, owner),
+             __builtin_amdgcn_readlane(plan.last.len, owner)};
+  if (plan.per > 1) {
+    for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<ROWS, UNIT>(p, paged_seq<true>(p.g, b))); ++b) pos -= u;
+    s = paged_seq<true>(p.g, b);
+  }
 
   // ---- what does not change from segment to segment -----------------------------------------------------------
   const uint32_t lds_smem = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
@@ -176,7 +187,6 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
   auto mfma = [](const bf16x8& x, const bf16x8& y, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); };
 
   for (;;) {
-    const PagedSeq s = paged_seq<true>(p.g, b);
     const Item it = item_of<ROWS, UNIT>(p, s);
     const int64_t item = pos / it.weight;
     const int from = (int)(pos - item * it.weight);
@@ -481,7 +491,8 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
     if (lo >= hi) break;
     if (pos >= (int64_t)it.weight * it.rts * p.Hkv) {
       pos = 0;
-      for (++b; b + 1 < p.g.B && units_of<ROWS, UNIT, true>(p, b) == 0;) ++b;
+      for (++b; b + 1 < p.g.B && units_of<ROWS, UNIT>(p, paged_seq<true>(p.g, b)) == 0;) ++b;
+      s = paged_seq<true>(p.g, b);
     }
   }
   if (!leaves && threadIdx.x == 0 && !p.by_item) p.shared[w].rows = 0;
