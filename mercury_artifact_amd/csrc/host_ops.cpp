@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/record_function.h>
+#include <c10/core/Allocator.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -856,18 +857,18 @@ PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (!on.current) SLOW;
   const int64_t bytes = entry.paged_bytes(g.B, n, T, most, g.starts != nullptr, Hq, g.Hkv, g.D);
   if (bytes < 0) SLOW;
-  Tensor out, lse, workspace;
+  Tensor out, lse;
   const int code = without_gil([&] {
     const auto options = q->options().requires_grad(false);
     out = out_given ? *out_given : at::empty(q->sizes(), options);
     lse = lse_given ? *lse_given : g.starts ? at::empty({Hq, T}, options.dtype(at::kFloat)) : at::empty({g.B, Hq, n}, options.dtype(at::kFloat));
-    workspace = at::empty({bytes}, options.dtype(at::kByte));
+    const c10::DataPtr workspace = c10::GetAllocator(c10::kCUDA)->allocate(bytes);       // (memory of the current stream: no tensor needed)
     return entry.paged_attn(q->data_ptr(), g.k, g.v, g.ks, g.vs, static_cast<const int*>(g.table->data_ptr()),
                             static_cast<const int*>(g.lengths->data_ptr()), static_cast<const int*>(data(g.starts)), out.data_ptr(),
                             floats(&lse), g.B, n, T, most, Hq, g.Hkv, g.D, g.pages, g.page, g.table->size(1), g.table->stride(0),
                             g.stride(*q, 0), g.stride(*q, 1), g.stride(*q, 2), g.cache->stride(1), g.cache->stride(2), g.cache->stride(3),
                             g.s_sp, g.s_ss, g.s_sh, g.stride(out, 0), g.stride(out, 1), g.stride(out, 2), (float)scale,
-                            causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, workspace.data_ptr(), on.stream);
+                            causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, workspace.get(), on.stream);
   });
   if (code != MHIP_OK) return refused(code, "mhip_paged_attn_fwd");
   return give2(out, lse);
