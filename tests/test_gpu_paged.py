@@ -627,3 +627,19 @@ def test_out_may_take_the_place_of_q(new, Hq):
     packed, lse = M.paged_attn_fwd(mine.clone(), s.dev, table, lengths, 0.1, scales=s.dev_scales, starts=starts)
     M.paged_attn_fwd(mine, s.dev, table, lengths, 0.1, scales=s.dev_scales, starts=starts, out=mine)
     assert torch.equal(mine, packed)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [1, 3, 130])
+def test_a_rank_that_holds_no_page(e4m3, new):
+    """Sequences with tokens, all of whose pages are elsewhere: no row sees a key, in a cache of no pages too."""
+    for pages in (0, 3):
+        cache, scales = M.paged_cache(pages, 16, 2, 64, E4M3 if e4m3 else torch.bfloat16)
+        table = torch.full((2, 20), pages, dtype=torch.int32).cuda()
+        table[1] = -1
+        lengths = torch.tensor([300, 150], dtype=torch.int32).cuda()
+        q = torch.ones(2, new, 4, 64, dtype=torch.bfloat16).cuda()
+        M.paged_cache_write(q[:, :, :2], q[:, :, :2], cache, table, lengths, scales=scales)
+        out, lse = M.paged_attn_fwd(q, cache, table, lengths, 0.1, scales=scales)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        assert (M.paged_cache_read(cache, table, lengths, 310, scales=scales) == 0).all()
