@@ -377,11 +377,11 @@ int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float*
  * out = softmax(scale * q k^T) v, lse fp32 (B, Hq, n) contiguous, packed (Hq, T), natural logarithm.  MHIP_MASK_CAUSAL: new token i
  * of n sees keys j <= lengths[b] - n + i; MHIP_MASK_NONE: all of them.  Rows that see no key get out = 0, lse = -inf, so
  * results over different pages of a sequence (other entries -1) merge as those of different chunks do.  A key a row does not see has
- * no part in its result, whatever the cache holds there.  Scales of an e4m3 cache that are no powers of two are allowed; sequences
- * with many new tokens then see each value code * scale rounded to bf16.  out may be q itself, and overlap nothing else.  most_new: with starts, about how many new tokens a sequence has at most;
- * it chooses the form of the kernels, results are right whatever it says.  `workspace`: 16-byte aligned,
- * mhip_paged_attn_workspace_bytes(B, n, T, most_new, whether there are starts, Hq, Hkv, D) bytes of device memory; calls that overlap
- * in time need one each.
+ * no part in its result, whatever the cache holds there.  Scales of an e4m3 cache that are no powers of two are allowed;
+ * sequences with many new tokens then see each code * scale rounded to bf16.  out may be q itself, and overlap nothing else.
+ * most_new: with starts, about how many new tokens a sequence has at most; it chooses the form of the kernels, results are
+ * right whatever it says.  `workspace`: 16-byte aligned, mhip_paged_attn_workspace_bytes(B, n, T, most_new, whether there are
+ * starts, Hq, Hkv, D) bytes of device memory; calls that overlap in time need one each.
  */
 int64_t mhip_paged_attn_workspace_bytes(int B, int n, int T, int most_new, int packed, int Hq, int Hkv, int D);
 int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,

@@ -36,7 +36,7 @@ constexpr int kFewRows = 64;               // rows of a sequence and K/V head th
 
 // Row tiles of a sequence and K/V head, units of each, and what an item counts for: its units behind `pause` more, the time in which a
 // workgroup that enters it does not read.  Without it a workgroup with many short items ends last; where there are fewer items than
-// workgroups it would only spoil even shares.  us, 0 / 1 / 2 / 3 units: 64 x 20 .. 1024 H32/8 48.6 / 35.5 / 31.6 / 32.0, 64 x 100 .. 2048
+// workgroups it would only spoil even shares.  us, 0 / 1 / 2 / 3 units (e4m3 with four wavefronts on a CU): 64 x 20 .. 1024 H32/8 48.6 / 35.5 / 31.6 / 32.0, 64 x 100 .. 2048
 // 63.1 / 55.8 / 55.2 / 54.0 (e4m3 56.2 / 49.8 / 43.7 / 42.0), 256 x 20 .. 512 72.1 / 62.4 / 54.8 / 53.4, 32 x 300 .. 16384 203.0 / 202.6 /
 // 203.9 / 207.1; 8 tokens at 32768 34.4 / 35.8 / 35.7 / 35.8.
 struct Item { int rts, steps, weight; };
@@ -502,9 +502,11 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
 int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 // Workgroups of four wavefronts, one to a CU, or of two, two to a CU: the pair covers the one's pauses between items (Q, the first tiles,
 // the wavefronts' results) with the other's reading, and costs twice as many partial results.  Items to a workgroup decide; us, four / two:
-//   items   8: 1 x 131072 H32/8 102.3 / 104.6, 8 tokens at 32768 34.9 / 38.0       16: 8 x 8192 H16/2 D64 e4m3 24.4 / 25.3
-//          32: 4 x 131072 H32/8 e4m3 194.3 / 201.4    128: 16 x 211 .. 4099 H16/8 D80 36.5 / 30.3    256: 32 x 300 .. 16384 H32/8 203.8 / 203.8
-//         512: 64 x 100 .. 2048 H32/8 68.0 / 62.3, e4m3 66.5 / 55.6                 2048: 256 x 20 .. 512 H32/8 90.7 / 78.2
+//   items   8: 1 x 131072 H32/8 88.0 / 89.4, e4m3 57.5 / 61.2, 8 tokens at 32768 33.1 / 37.8    16: 8 x 8192 H16/2 D64 e4m3 16.9 / 20.8
+//          32: 4 x 131072 H32/8 e4m3 180.7 / 182.7    128: 16 x 5 tokens at 211 .. 4099 H16/8 D80 36.4 / 27.1, e4m3 26.4 / 24.4
+//         256: 32 x 300 .. 16384 H32/8 177.9 / 177.5    512: 64 x 100 .. 2048 H32/8 64.8 / 54.1, e4m3 49.7 / 35.3
+//        2048: 256 x 20 .. 512 H32/8 84.1 / 55.5, e4m3 63.9 / 40.7
+// (e4m3 with up to 16 rows: twice as many of either, see kRingOf)
 constexpr int64_t kManyItems = 128;
 
 // One partial result at each end of a workgroup's share.

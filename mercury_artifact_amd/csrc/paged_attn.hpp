@@ -109,7 +109,8 @@ __global__ __launch_bounds__(256) void paged_attn_join(const PagedAttn p) {
     f32x2 ml[R];
     float top[R], ref[R], sum[R], a0[R], a1[R];
     constexpr int kDeep = 8 / R;
-    f32x2 next[kDeep][R];                                  // the parts that are added next, on their way beside the weights (64 tokens at 32768: 57.9 us to 56.1)
+    // The parts that are added next, on their way while the weights are found (64 tokens at 32768: 57.9 us to 56.1).
+    f32x2 next[kDeep][R];
     auto request = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < kDeep; ++u)

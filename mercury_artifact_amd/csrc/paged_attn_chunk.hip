@@ -697,7 +697,8 @@ template <bool E4M3, int COLS>
 void launch(const PagedAttn& p, int places, hipStream_t st) {
   hipLaunchKernelGGL(paged_attn_chunk_plan, dim3(1), dim3(kPlanWaves * 64), 0, st, p, places);
   hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)places), dim3(512), 0, st, p);
-  constexpr int rows = 8;                              // of a workgroup: 4 / 8 / 16 / 32 took 57.0 / 58.6 / 65.2 / 76.4 us with 64 tokens at 32768 (8 now 56.1)
+  // rows of a workgroup: 4 / 8 / 16 / 32 took 57.0 / 58.6 / 65.2 / 76.4 us with 64 tokens at 32768 (8 now 56.1)
+  constexpr int rows = 8;
   hipLaunchKernelGGL((paged_attn_join<COLS, kBM, 2, rows>), dim3(kBM / rows, kParts / 2), dim3(256), 0, st, p);
 }
 template <bool E4M3>
