@@ -25,20 +25,22 @@ namespace {
 typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i32x2;
 
 constexpr int kKeys = 32;                  // keys of a tile, one wavefront's
-// Bytes of K and V tiles of a wavefront, of which a CU has 128 KB: four wavefronts of them, or eight of half as much.  Eight where each has
-// conversions to do beside its copies and registers for two on a SIMD: e4m3 with up to 16 rows (four / eight wavefronts: 64 x 100 .. 2048
-// H32/8 43.4 / 35.9 us, 32 x 300 .. 16384 111.1 / 102.3, 16 x 5 tokens behind 211 .. 4099 D80 29.1 / 24.4, 4 x 131072 180.6 / 181.2).
-template <bool E4M3, int NR>
-constexpr int kRingOf = E4M3 && NR == 1 ? 16384 : 32768;
+// Bytes of K and V tiles of a wavefront, of which a CU has 128 KB: four wavefronts of them, or eight of half as much.  Eight where there are
+// registers for two on a SIMD and half as much still holds two tiles: up to 16 rows, of up to 128 bytes.  us, four / eight wavefronts:
+// e4m3 64 x 100 .. 2048 H32/8 43.4 / 35.9, 32 x 300 .. 16384 111.1 / 102.3, 16 x 5 tokens at 211 .. 4099 H16/8 D80 29.1 / 24.4, 4 x 131072
+// 180.6 / 181.2; bf16 D64 64 x 100 .. 2048 35.5 / 31.5, 32 x 300 .. 16384 96.5 / 94.4, 16 x 5 23.4 / 21.7, 8 x 8192 H16/2 15.3 / 15.6.
+template <bool E4M3, int COLS, int NR>
+constexpr int kRingOf = NR == 1 && COLS * (E4M3 ? 1 : 2) <= 128 ? 16384 : 32768;
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
 constexpr int kWavefronts = 1024;          // of a launch with rings of 32 KB: four on a CU, in workgroups of four or two
 constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
 // Row tiles of a sequence and K/V head, units of each, and what an item counts for: its units behind `pause` more, the time in which a
 // workgroup that enters it does not read.  Without it a workgroup with many short items ends last; where there are fewer items than
-// workgroups it would only spoil even shares.  us, 0 / 1 / 2 / 3 units (e4m3 with four wavefronts on a CU): 64 x 20 .. 1024 H32/8 48.6 / 35.5 / 31.6 / 32.0, 64 x 100 .. 2048
-// 63.1 / 55.8 / 55.2 / 54.0 (e4m3 56.2 / 49.8 / 43.7 / 42.0), 256 x 20 .. 512 72.1 / 62.4 / 54.8 / 53.4, 32 x 300 .. 16384 203.0 / 202.6 /
-// 203.9 / 207.1; 8 tokens at 32768 34.4 / 35.8 / 35.7 / 35.8.
+// workgroups it would only spoil even shares.  us, 0 / 1 / 2 / 3 units (e4m3 with four wavefronts on a CU): 64 x 20 .. 1024 H32/8 48.6 / 35.5
+// / 31.6 / 32.0, 64 x 100 .. 2048 63.1 / 55.8 / 55.2 / 54.0 (e4m3 56.2 / 49.8 / 43.7 / 42.0), 256 x 20 .. 512 72.1 / 62.4 / 54.8 / 53.4,
+// 32 x 300 .. 16384 203.0 / 202.6 / 203.9 / 207.1; 8 tokens at 32768 34.4 / 35.8 / 35.7 / 35.8.  With eight wavefronts, 1 / 2 / 3 units: e4m3
+// 256 x 20 .. 512 44.5 / 40.9 / 42.1, 64 x 100 .. 2048 37.2 / 36.2 / 36.3.
 struct Item { int rts, steps, weight; };
 template <int UNIT>
 constexpr int kPauseOf = UNIT == 2 * kKeys ? 2 : 0;
@@ -89,7 +91,7 @@ __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks 
 }
 
 template <bool E4M3, int COLS, int NR, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged_attn_few(const PagedAttn p) {
+__global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void paged_attn_few(const PagedAttn p) {
   constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys, kPause = kPauseOf<UNIT>;
   constexpr int kSize = E4M3 ? 1 : 2;
   constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, NR>)) void paged
   constexpr int kCopyRows = 1024 / ROWB;               // rows of one copy instruction
   constexpr int kCopies = 16 / kCopyRows;              // and instructions of half a tile
   constexpr int kTileBytes = kKeys * ROWB;
-  constexpr int kStages = kRingOf<E4M3, NR> / (2 * kTileBytes);
+  constexpr int kStages = kRingOf<E4M3, COLS, NR> / (2 * kTileBytes);
   constexpr int kStage = 2 * kTileBytes + (E4M3 ? 256 : 0);      // K, V, 32 scales of each
   constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
   constexpr int KB = COLS / 32, DB = COLS / 16;
@@ -506,7 +508,7 @@ int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 //          32: 4 x 131072 H32/8 e4m3 180.7 / 182.7    128: 16 x 5 tokens at 211 .. 4099 H16/8 D80 36.4 / 27.1, e4m3 26.4 / 24.4
 //         256: 32 x 300 .. 16384 H32/8 177.9 / 177.5    512: 64 x 100 .. 2048 H32/8 64.8 / 54.1, e4m3 49.7 / 35.3
 //        2048: 256 x 20 .. 512 H32/8 84.1 / 55.5, e4m3 63.9 / 40.7
-// (e4m3 with up to 16 rows: twice as many of either, see kRingOf)
+// (twice as many of either where kRingOf halves the rings)
 constexpr int64_t kManyItems = 128;
 
 // One partial result at each end of a workgroup's share.
@@ -514,7 +516,7 @@ int64_t few_bytes(int64_t rows, int D) { return 2 * kWavefronts * (16 * (int64_t
 
 template <bool E4M3, int COLS, int NR, int WAVES>
 void launch_few(PagedAttn p, int64_t rows, hipStream_t st) {
-  constexpr int workgroups = kWavefronts * (32768 / kRingOf<E4M3, NR>) / WAVES;
+  constexpr int workgroups = kWavefronts * (32768 / kRingOf<E4M3, COLS, NR>) / WAVES;
   p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)workgroups * 16 * NR * COLS);
   p.shared = reinterpret_cast<Shared*>(p.part_ml + 2 * (int64_t)workgroups * 16 * NR);
   // Where the items are known and not more than the workgroups, the last step has one row of workgroups for each of them, not for
