@@ -564,7 +564,10 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       asm volatile("s_waitcnt vmcnt(12)" ::: "memory");         // K(0)
       __builtin_amdgcn_s_barrier();
       first_tile();
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");          // V(0) and K(1); the loop waits for the others
+      // V(0), K(1), V(1) and K(2) are read before their copiers' next wait: the first group reads K(2) in its vector phase of tile 0 and
+      // V(1) in the phase after, beside the other group's vector phase of tile 0.  V(2) and K(3) may be on their way, every wavefront waits
+      // for them in that phase; from there on the vector phase of tile t waits for K(t + 3) and V(t + 2), read from the next one on.
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       __builtin_amdgcn_s_barrier();
     } else {
       Codes k[4], v[3];
