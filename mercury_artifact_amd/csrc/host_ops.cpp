@@ -724,6 +724,11 @@ PyObject* quantize_e4m3(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether autograd would want a derivative through t.
+bool differentiated(const Tensor& t) {
+  return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+}
+
 // A paged cache (2, pages, page_size, Hkv, D) with its table and lengths, and what of it the entry points take.
 struct Paged {
   const Tensor *cache, *scales, *table, *lengths, *starts;
@@ -743,7 +748,7 @@ struct Paged {
     if (c.scalar_type() == at::kBFloat16) type = MHIP_BF16;
     else if (c.scalar_type() == at::kFloat8_e4m3fn) type = MHIP_E4M3;
     else return false;
-    if ((type == MHIP_E4M3) != (scales != nullptr)) return false;
+    if ((type == MHIP_E4M3) != (scales != nullptr) || differentiated(c) || (scales && differentiated(*scales))) return false;
     if (scales && (scales->scalar_type() != at::kFloat || scales->sizes() != c.sizes().slice(0, 4))) return false;
     if (lengths->dim() != 1 || lengths->scalar_type() != at::kInt || !lengths->is_contiguous()) return false;
     B = lengths->size(0);
@@ -763,7 +768,7 @@ struct Paged {
   bool tokens(const Tensor& t, int64_t heads, int64_t& n, int64_t& T) const {
     const int64_t d = starts ? 3 : 4;
     if (t.dim() != d || t.device() != cache->device() || t.scalar_type() != at::kBFloat16 || t.stride(d - 1) != 1 || t.size(d - 1) != D ||
-        t.size(d - 2) != heads || (!starts && t.size(0) != B))
+        t.size(d - 2) != heads || (!starts && t.size(0) != B) || differentiated(t))
       return false;
     n = starts ? 0 : t.size(1);
     T = starts ? t.size(0) : B * n;
@@ -807,7 +812,7 @@ PyObject* paged_cache_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if ((rows == -1 || begin == -1) && PyErr_Occurred()) { PyErr_Clear(); SLOW; }
   if (rows < 0 || begin < 0 || !fits({rows, begin})) SLOW;
   if (given && (given->dim() != 5 || given->size(0) != 2 || given->size(1) != g.B || given->size(2) != rows || given->size(3) != g.Hkv ||
-                given->size(4) != g.D || given->scalar_type() != at::kBFloat16 || given->stride(4) != 1))
+                given->size(4) != g.D || given->scalar_type() != at::kBFloat16 || given->stride(4) != 1 || differentiated(*given)))
     SLOW;
   OnDevice on(*g.cache);
   if (!on.current) SLOW;
@@ -850,7 +855,7 @@ PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (!optional(a[9], *q, out_given) || !optional(a[10], *q, lse_given)) SLOW;
   int64_t n2, T2;
   if (out_given && (!g.tokens(*out_given, Hq, n2, T2) || out_given->sizes() != q->sizes())) SLOW;
-  if (lse_given && (lse_given->scalar_type() != at::kFloat || !lse_given->is_contiguous() ||
+  if (lse_given && (lse_given->scalar_type() != at::kFloat || !lse_given->is_contiguous() || differentiated(*lse_given) ||
                     !(g.starts ? lse_given->dim() == 2 && lse_given->size(0) == Hq && lse_given->size(1) == T : shape3(*lse_given, g.B, Hq, n))))
     SLOW;
   OnDevice on(*q);

@@ -1,0 +1,65 @@
+"""What the operators over a paged cache do with tensors that autograd looks after (no GPU needed: they say so before anything else)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import mercury_artifact_amd as M
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _data(device="cpu"):
+    cache, scales = M.paged_cache(2, 16, 2, 64, E4M3, device=device)
+    table = torch.tensor([[1]], dtype=torch.int32, device=device)
+    lengths = torch.tensor([5], dtype=torch.int32, device=device)
+    return cache, scales, table, lengths, torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device=device)
+
+
+def _calls(asks, device="cpu"):
+    """Name of the tensor that asks for a gradient, call."""
+    cache, scales, table, lengths, x = _data(device)
+    lse, chunk = torch.zeros(1, 2, 1, device=device), torch.zeros(2, 1, 3, 2, 64, dtype=torch.bfloat16, device=device)
+    return [
+        ("q", lambda: M.paged_attn_fwd(asks(x), cache, table, lengths, 0.1, scales=scales)),
+        ("scales", lambda: M.paged_attn_fwd(x, cache, table, lengths, 0.1, scales=asks(scales))),
+        ("out", lambda: M.paged_attn_fwd(x, cache, table, lengths, 0.1, scales=scales, out=asks(x))),
+        ("lse", lambda: M.paged_attn_fwd(x, cache, table, lengths, 0.1, scales=scales, lse=asks(lse))),
+        ("cache", lambda: M.paged_attn_fwd(x, asks(x.new_zeros(2, 2, 16, 2, 64)), table, lengths, 0.1)),
+        ("k", lambda: M.paged_cache_write(asks(x), x, cache, table, lengths, scales=scales)),
+        ("v", lambda: M.paged_cache_write(x, asks(x), cache, table, lengths, scales=scales)),
+        ("scales", lambda: M.paged_cache_write(x, x, cache, table, lengths, scales=asks(scales))),
+        ("cache", lambda: M.paged_cache_write(x, x, asks(x.new_zeros(2, 2, 16, 2, 64)), table, lengths)),
+        ("cache", lambda: M.paged_cache_read(asks(x.new_zeros(2, 2, 16, 2, 64)), table, lengths, 3)),
+        ("scales", lambda: M.paged_cache_read(cache, table, lengths, 3, scales=asks(scales))),
+        ("out", lambda: M.paged_cache_read(cache, table, lengths, 3, scales=scales, out=asks(chunk))),
+    ]
+
+
+def _refused(device):
+    for name, call in _calls(lambda t: t.detach().requires_grad_(), device):
+        with pytest.raises(RuntimeError, match=f"no gradients, which {name} asks for"):
+            call()
+    with forward_ad.dual_level():
+        for name, call in _calls(lambda t: forward_ad.make_dual(t.detach(), torch.ones_like(t)), device):
+            with pytest.raises(RuntimeError, match=f"no gradients, which {name} asks for"):
+                call()
+
+
+def test_a_gradient_that_is_asked_for_is_refused():
+    _refused("cpu")
+
+
+def test_without_gradients_the_call_goes_on():
+    with torch.no_grad():
+        for _, call in _calls(lambda t: t.detach().requires_grad_()):
+            with pytest.raises(RuntimeError, match="GPU only"):
+                call()
+
+
+@pytest.mark.gpu
+def test_a_gradient_that_is_asked_for_is_refused_on_the_gpu():
+    _refused("cuda")
+    with torch.no_grad():
+        for _, call in _calls(lambda t: t.detach().requires_grad_(), "cuda"):
+            call()
+    torch.cuda.synchronize()
