@@ -170,13 +170,13 @@ PyObject* undispatched(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 
 // Says that the tensors have been written to, as an operator does for the arguments it mutates: autograd compares the
 // count with what it saved.
+void count_write(const Tensor* t) {
+  if (t && t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 PyObject* written(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  for (Py_ssize_t i = 0; i < nargs; ++i) {
-    if (!THPVariable_Check(a[i])) continue;
-    const Tensor& t = THPVariable_Unpack(a[i]);
-    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
+  for (Py_ssize_t i = 0; i < nargs; ++i)
+    if (THPVariable_Check(a[i])) count_write(&THPVariable_Unpack(a[i]));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -796,6 +796,8 @@ PyObject* paged_cache_write(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                              on.stream);
   });
   if (code != MHIP_OK) return refused(code, "mhip_paged_cache_write");
+  count_write(g.cache);
+  count_write(g.scales);
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -825,6 +827,7 @@ PyObject* paged_cache_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                             out.stride(2), out.stride(3), g.type, on.stream);
   });
   if (code != MHIP_OK) return refused(code, "mhip_paged_cache_read");
+  count_write(given);
   return give(out);
   END_HANDLE_TH_ERRORS
 }
@@ -876,6 +879,8 @@ PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                             causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, workspace.get(), on.stream);
   });
   if (code != MHIP_OK) return refused(code, "mhip_paged_attn_fwd");
+  count_write(out_given);
+  count_write(lse_given);
   return give2(out, lse);
   END_HANDLE_TH_ERRORS
 }

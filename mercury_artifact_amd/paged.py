@@ -132,6 +132,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, pag
             B, n, T, Hkv, D, pages, page_size, page_table.shape[1], page_table.stride(0),
             *_token_strides(k), *_token_strides(v), *strides, _dtype(cache), N.stream_of(cache))
     N.check(code, "mhip_paged_cache_write")
+    N.host.written(cache, scales)
 
 
 def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, rows: int, begin: int = 0,
@@ -155,6 +156,7 @@ def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: tor
             *pointers, N.ptr(page_table), N.ptr(lengths), N.ptr(out), B, begin, rows, Hkv, D, pages, page_size,
             page_table.shape[1], page_table.stride(0), *strides, *out.stride()[:4], _dtype(cache), N.stream_of(cache))
     N.check(code, "mhip_paged_cache_read")
+    N.host.written(out)
     return out
 
 
@@ -203,4 +205,5 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
             *_token_strides(q), *strides, *_token_strides(out), float(softmax_scale),
             N.MASK_CAUSAL if causal else N.MASK_NONE, _dtype(cache), N.ptr(workspace), N.stream_of(cache))
     N.check(code, "mhip_paged_attn_fwd")
+    N.host.written(out, lse)
     return out, lse
