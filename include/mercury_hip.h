@@ -345,7 +345,10 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
  * page_table, lengths and starts are DEVICE arrays of int32, read when the kernels run (a captured graph follows them); a length
  * counts as one from 0 to table_pages * page_size, a start as one from 0 to T.
  * page_size: a multiple of 16, table_pages * page_size <= 2^31 - 2^16, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
- * multiple of 8 (MHIP_E4M3: of 16) up to 128.  Bases and rows on 16 bytes.
+ * multiple of 8 (MHIP_E4M3: of 16) up to 128.  Bases and rows on 16 bytes.  A launch has fewer than 2^32 threads, so a call takes
+ * T * Hkv rows to write up to 2^28 - 128 and B * rows * Hkv to read up to 2^29 - 256, twice as many of 64 columns or fewer; attention T * Hq
+ * rows below 2^31 - 256 and, where most_new * Hq / Hkv passes 64, B * Hkv + T * Hq / 256 below 2^23 - 512.  More is refused before anything
+ * is launched (MHIP_EUNSUPPORTED).
  */
 
 /*

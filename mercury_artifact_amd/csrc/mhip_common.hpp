@@ -214,6 +214,9 @@ __device__ __forceinline__ constexpr int lds_half_row_swizzle(int row) { return 
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether one dimension of a launch takes so many workgroups: HIP counts its threads in 32 bits.
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups <= 0xffffffffll / threads; }
+
 inline int launch_status() {
   return hipGetLastError() == hipSuccess ? MHIP_OK : MHIP_ELAUNCH;
 }

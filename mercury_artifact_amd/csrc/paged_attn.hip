@@ -582,7 +582,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3u)) return MHIP_EALIGN;
   for (int64_t s : {q_sb, q_ss, q_sh, o_sb, o_ss, o_sh})
     if (s % 8 != 0) return MHIP_EALIGN;
-  if ((int64_t)T * Hq >= (int64_t(1) << 31) - 64) return MHIP_EUNSUPPORTED;
+  if ((int64_t)T * Hq >= (int64_t(1) << 31) - 256) return MHIP_EUNSUPPORTED;       // (rows, up to a whole tile of them, are ints)
   const int size = dtype == MHIP_E4M3 ? 1 : 2;
   // places are counted in 16 bytes: 32 bits for a page, and for the rows of one
   if (c_sp < 0 || c_sp * size / 16 > 0xffffffffll || c_ss * size / 16 * page_size > 0xffffffffll) return MHIP_EUNSUPPORTED;
@@ -601,6 +601,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   p.by_group = Divisor(p.G); p.by_heads = Divisor(Hq); p.by_new = Divisor(n);
   p.part_o = static_cast<float*>(workspace);
   const int64_t rows = (int64_t)most_new * p.G;
+  if (rows > kFewRows && !paged_attn_chunk_fits(B, n, T, p.G, Hkv, starts != nullptr)) return MHIP_EUNSUPPORTED;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows <= kFewRows) {                  // (a sequence with more rows all the same is several tiles of them)
     p.few_rows = 0x7fffffff;
@@ -610,7 +611,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
     // after the other on the stream, share the workspace.
     p.few_rows = starts && p.G <= kFewRows ? 16 * row_blocks(p.G) : -1;
     if (p.few_rows > 0) launch(p, dtype == MHIP_E4M3, p.few_rows, st);
-    if (int code = paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st)) return code;
+    paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st);
   }
   return launch_status();
 }

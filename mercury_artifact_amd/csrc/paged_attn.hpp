@@ -178,6 +178,7 @@ __global__ __launch_bounds__(256) void paged_attn_join(const PagedAttn p) {
 }
 
 int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed);
-int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
+bool paged_attn_chunk_fits(int64_t B, int64_t n, int64_t T, int G, int Hkv, bool packed);       // into a launch
+void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
 
 }  // namespace mhip

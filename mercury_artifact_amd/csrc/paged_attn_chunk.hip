@@ -717,9 +717,11 @@ void launch(const PagedAttn& p, int places, hipStream_t st) {
 int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed) {
   return (int64_t)kParts * kBM * (columns_of(D) + 2) * 4 + kParts / 2 * 32 + 16 * B + up16(4 * places_of(B, T, n, G, Hkv, packed));
 }
-int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
-  const int64_t places = places_of(p.g.B, p.g.T, p.g.n, p.G, p.Hkv, p.g.starts != nullptr);
-  if (places >= int64_t(1) << 31) return MHIP_EUNSUPPORTED;
+bool paged_attn_chunk_fits(int64_t B, int64_t n, int64_t T, int G, int Hkv, bool packed) {
+  return grid_fits(places_of(B, T, n, G, Hkv, packed), 512);
+}
+void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
+  const int places = (int)places_of(p.g.B, p.g.T, p.g.n, p.G, p.Hkv, p.g.starts != nullptr);
   PagedAttn q = p;
   char* at = reinterpret_cast<char*>(q.part_o) + (int64_t)kParts * kBM * columns_of(p.D) * 4;
   q.part_ml = reinterpret_cast<f32x2*>(at);
@@ -728,9 +730,8 @@ int paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
   at += kParts / 2 * 32;
   q.records = reinterpret_cast<Record*>(at);
   q.pieces = reinterpret_cast<int*>(at + 16 * (int64_t)p.g.B);
-  if (e4m3) launch<true>(q, (int)places, stream);
-  else launch<false>(q, (int)places, stream);
-  return MHIP_OK;
+  if (e4m3) launch<true>(q, places, stream);
+  else launch<false>(q, places, stream);
 }
 
 }  // namespace mhip

@@ -30,7 +30,7 @@ struct RowsParams {
 // (32768 rows read back 153.9 us to 150.8, 16403 tokens written 27.4 to 25.7; bf16 rows as they come, 46 MB read back in 11.2 us and 11.6).
 template <bool E4M3>
 __device__ __forceinline__ int block_here() { return E4M3 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x; }
-dim3 blocks_of(int total, int each) { return dim3(((unsigned)((total + each - 1) / each) + 7) & ~7u); }
+int64_t blocks_of(int64_t total, int each) { return ((total + each - 1) / each + 7) & ~int64_t(7); }
 
 // Largest of the lane's group of 16 or 8, in all of its lanes.
 template <int LANES>
@@ -260,7 +260,10 @@ extern "C" int mhip_paged_cache_write(const void* k, const void* v, void* k_cach
   if (!aligned16(k) || !aligned16(v)) return MHIP_EALIGN;
   for (int64_t s : {k_sb, k_ss, k_sh, v_sb, v_ss, v_sh})
     if (!mult(s, 8)) return MHIP_EALIGN;
-  if ((int64_t)T * 2 * Hkv >= (int64_t(1) << 31) - 64) return MHIP_EUNSUPPORTED;
+  const bool wide = D > 64;
+  const int groups = wide ? 16 : 32;
+  const int64_t blocks = blocks_of((int64_t)T * Hkv, groups);
+  if (!grid_fits(blocks, 256)) return MHIP_EUNSUPPORTED;       // (so T * Hkv is an int)
   take_cache(p, k_cache, v_cache, k_scales, v_scales, c_sp, c_ss, c_sh, s_sp, s_ss, s_sh, D, dtype);
   p.k = static_cast<const uint16_t*>(k); p.v = static_cast<const uint16_t*>(v);
   p.k_sb = k_sb; p.k_ss = k_ss; p.k_sh = k_sh;
@@ -268,9 +271,7 @@ extern "C" int mhip_paged_cache_write(const void* k, const void* v, void* k_cach
   p.total = T * Hkv;
   p.by_head = Divisor(Hkv); p.by_new = Divisor(n);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool wide = D > 64;
-  const int groups = wide ? 16 : 32;
-  const dim3 grid = blocks_of(p.total, groups), block(256);
+  const dim3 grid((unsigned)blocks), block(256);
   if (dtype == MHIP_E4M3) {
     if (wide) hipLaunchKernelGGL((paged_write_kernel<true, 16>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((paged_write_kernel<true, 8>), grid, block, 0, st, p);
@@ -296,6 +297,10 @@ extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, c
   for (int64_t s : {o_half, o_sb, o_ss, o_sh})
     if (!mult(s, 8)) return MHIP_EALIGN;
   if ((double)B * rows * 2 * Hkv >= 2147483648.0 - 256) return MHIP_EUNSUPPORTED;
+  const bool wide = D > 64;
+  const int groups = (wide ? 16 : 32) * kReadRows;
+  const int64_t blocks = blocks_of((int64_t)B * rows * Hkv, groups);
+  if (!grid_fits(blocks, 256)) return MHIP_EUNSUPPORTED;
   take_cache(p, k_cache, v_cache, k_scales, v_scales, c_sp, c_ss, c_sh, s_sp, s_ss, s_sh, D, dtype);
   p.out = static_cast<uint16_t*>(out);
   p.o_half = o_half; p.o_sb = o_sb; p.o_ss = o_ss; p.o_sh = o_sh;
@@ -303,9 +308,7 @@ extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, c
   p.begin = begin;
   p.by_head = Divisor(Hkv); p.by_rows = Divisor(rows);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool wide = D > 64;
-  const int groups = (wide ? 16 : 32) * kReadRows;
-  const dim3 grid = blocks_of(p.total, groups), block(256);
+  const dim3 grid((unsigned)blocks), block(256);
   const bool once = (int64_t)p.total * D * 4 > kLastLevel;
   auto launch = [&](auto lanes, auto past) {
     constexpr int L = decltype(lanes)::value;

@@ -130,3 +130,26 @@ def test_positions_stay_below_the_last_ints(lib):
     for call in (_write, _read, _attn):
         assert call(lib, width=(1 << 27) - (1 << 12) + 1) == EUNSUPPORTED
     assert _attn(lib, B=0, width=(1 << 27) - (1 << 12)) == OK
+
+
+def test_a_call_that_no_launch_takes_is_refused(lib):
+    """A launch counts its threads in 32 bits; none of these may come as far as launching."""
+    for starts in (None, P):
+        many = dict(starts=starts, B=1, n=0 if starts else 1 << 28, T=1 << 28 if starts else 0, Hkv=1, tokens=(0, 128, 128))
+        assert _write(lib, D=128, **many) == EUNSUPPORTED
+        many["n"], many["T"] = many["n"] * 2, many["T"] * 2
+        for dtype in (0, 1):
+            assert _write(lib, D=64, dtype=dtype, **many) == EUNSUPPORTED
+    for dtype in (0, 1):
+        assert _read(lib, B=1, rows=1 << 29, Hkv=1, D=128, dtype=dtype) == EUNSUPPORTED
+        assert _read(lib, B=1, rows=(1 << 30) - 129, Hkv=1, D=64, dtype=dtype) == EUNSUPPORTED
+        # items of 256 rows: as many sequences
+        assert _attn(lib, B=1 << 23, n=65, Hq=1, Hkv=1, dtype=dtype) == EUNSUPPORTED
+        assert _attn(lib, starts=P, B=1 << 23, n=0, T=4, most=65, Hq=1, Hkv=1, tokens=(0, 64, 64), dtype=dtype) == EUNSUPPORTED
+        assert _attn(lib, starts=P, B=1 << 20, n=0, T=4, most=65, Hq=8, Hkv=8, tokens=(0, 512, 64), dtype=dtype) == EUNSUPPORTED
+
+
+def test_rows_of_a_sequence_and_a_tile_are_ints(lib):
+    for T in (2 ** 31 - 65, 2 ** 31 - 256):
+        assert _attn(lib, starts=P, B=1, n=0, T=T, most=1, Hq=1, Hkv=1, tokens=(0, 64, 64)) == EUNSUPPORTED
+        assert _attn(lib, B=1, n=T, Hq=1, Hkv=1, tokens=(0, 64, 64)) == EUNSUPPORTED
