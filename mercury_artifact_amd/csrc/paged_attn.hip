@@ -366,11 +366,10 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
           for (int i = 0; i < 8; ++i) {
             x[i] = fast_exp2(sc[i >> 2][r][i & 3] - ref);
             sum += x[i];
+            // (a masked key's scale may be anything; a NaN of one that the row sees counts however small its weight is)
+            if constexpr (E4M3) x[i] = sc[i >> 2][r][i & 3] == -INFINITY ? 0.f : x[i] * v_scale[i >> 2][i & 3];
           }
           l[r0 + r] = l[r0 + r] * alpha[r] + sum;
-          if constexpr (E4M3)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] == 0.f ? 0.f : x[i] * v_scale[i >> 2][i & 3];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if constexpr (kTwice) {
@@ -417,7 +416,10 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
               const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, at))));
 #pragma unroll
               for (int r = 0; r < kPair; ++r) {
-                const f32x4 counts = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[r])), f32x4{});
+                int left[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) left[kb] = hidden >> kb & 1 ? 0 : lim[r0 + r] - (key0 + 16 * kb) - 4 * lg;
+                const f32x4 counts = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(left[0], left[1])), f32x4{});
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[db][r0 + r][j] = with_odd(o[db][r0 + r][j], counts[j]);
               }

@@ -60,10 +60,15 @@ __device__ __forceinline__ u32x4 odd_marks(const u32x4& v) {
   }
   return marks;
 }
-__device__ __forceinline__ u32x4 seen_marks(const u32x4& p) {
+// Of a lane's keys, four and four, of which its row sees the first left0 and left1: ones in bf16.  (By place and not by weight: a weight may
+// be zero for being small.)
+__device__ __forceinline__ u32x4 seen_marks(int left0, int left1) {
   u32x4 marks;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) marks[i] = (p[i] & 0x7fffu ? 0x3f80u : 0u) | (p[i] & 0x7fff0000u ? 0x3f800000u : 0u);
+  for (int i = 0; i < 4; ++i) {
+    const int left = i < 2 ? left0 : left1, j = 2 * (i & 1);
+    marks[i] = (j < left ? 0x3f80u : 0u) | (j + 1 < left ? 0x3f800000u : 0u);
+  }
   return marks;
 }
 __device__ __forceinline__ float with_odd(float o, float counts) {

@@ -448,7 +448,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     for (int r = 0; r < 2; ++r) l_run[r] += rs[r];
   };
   // O^T of a tile that cuts (see finite_part).
-  auto pv_cut = [&]() __attribute__((always_inline)) {
+  auto pv_cut = [&](int tile) __attribute__((always_inline)) {
     uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < kSlotsO; ++i) {
@@ -463,7 +463,13 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       for (int t = 0; t < kSteps; ++t) {
         const bf16x8 marks = __builtin_bit_cast(bf16x8, odd_marks(__builtin_bit_cast(u32x4, read_v(db, t))));
 #pragma unroll
-        for (int r = 0; r < 2; ++r) counts[r] = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(pw[t][r])), counts[r]);
+        for (int r = 0; r < 2; ++r) {
+          int left[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            left[h] = gone >> (4 * (tile & 7) + 2 * t + h) & 1u ? 0 : lim[r] - ((t0 + tile) * kBN + (2 * t + h) * 16) - lg * 4;
+          counts[r] = mfma(marks, __builtin_bit_cast(bf16x8, seen_marks(left[0], left[1])), counts[r]);
+        }
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r)
@@ -514,7 +520,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   // the same where tile t cuts
   auto matrix_phase_cut = [&](int t) __attribute__((always_inline)) {
     if (!E4M3 && kShortMatrix) copies(t);
-    pv_cut();
+    pv_cut(t);
 #pragma unroll
     for (int i = 0; i < kSlotsS; ++i) {
       s_mfma(i % MB, i / MB, read_k(i % MB, i / MB));
@@ -633,7 +639,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
       vector_phase(t);
       __builtin_amdgcn_s_barrier();
     }
-    if (cuts(ntiles - 1)) pv_cut();
+    if (cuts(ntiles - 1)) pv_cut(ntiles - 1);
     else {
 #pragma unroll
       for (int i = 0; i < kSlotsO; ++i) o_mfma(i % DB, i / DB, read_v(i % DB, i / DB));
