@@ -11,7 +11,7 @@ different chunks do (``merge_many``, ``update_out_and_lse``).
 New tokens come as ``(B, n, heads, D)``, or packed as ``(T, heads, D)`` with ``starts`` ``(B + 1,)``: rows ``starts[b]`` up to
 ``starts[b + 1]`` belong to sequence b, rows outside of all are left alone.  They are the last ones of their sequence:
 ``lengths`` counts them.  Nothing here waits for the GPU or looks at the values of tables, lengths and starts on the host.
-They compute no gradients, and refuse tensors that require one unless ``torch.no_grad()`` is on.  The reference has no counterpart;
+They compute no gradients, and refuse tensors that require one unless ``torch.no_grad()`` is on; nor do they take fake tensors.  The reference has no counterpart;
 an operator that is asked for something it does not do raises ``RuntimeError``.
 """
 from __future__ import annotations
@@ -20,6 +20,7 @@ import operator
 from typing import Optional, Tuple
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _native as N
 
@@ -38,8 +39,11 @@ def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype:
     return cache, torch.empty((2, pages, kv_heads, page_size), dtype=torch.float32, device=device).transpose(2, 3)
 
 
-def _no_gradients(**tensors):
+def _check_plain(**tensors):
+    """Nothing that only a registered operator could do: a derivative, or shapes without data."""
     for name, t in tensors.items():
+        if isinstance(t, FakeTensor):
+            raise RuntimeError(f"the operators over a paged cache have no fake form, and {name} is a fake tensor: keep them out of traced programs")
         if t is not None and ((torch.is_grad_enabled() and t.requires_grad) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
             raise RuntimeError(f"the operators over a paged cache compute no gradients, which {name} asks for: "
                                "call them under torch.no_grad(), or with detached tensors")
@@ -118,7 +122,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, pag
     (sequences that share the page they write to)."""
     if N.host.paged_cache_write(k, v, cache, page_table, lengths, scales, starts):
         return
-    _no_gradients(k=k, v=v, cache=cache, scales=scales)
+    _check_plain(k=k, v=v, cache=cache, scales=scales)
     B = _check_cache(cache, scales, page_table, lengths, starts)
     _, pages, page_size, Hkv, D = cache.shape
     n, T = _check_tokens("k", k, B, starts, Hkv, D, cache.device)
@@ -142,7 +146,7 @@ def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: tor
     done = N.host.paged_cache_read(cache, page_table, lengths, rows, begin, scales, out)
     if done is not None:
         return done
-    _no_gradients(cache=cache, scales=scales, out=out)
+    _check_plain(cache=cache, scales=scales, out=out)
     B = _check_cache(cache, scales, page_table, lengths)
     _, pages, page_size, Hkv, D = cache.shape
     rows, begin = _whole("rows", rows), _whole("begin", begin)
@@ -172,7 +176,7 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     done = N.host.paged_attn_fwd(q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse)
     if done is not None:
         return done
-    _no_gradients(q=q, cache=cache, scales=scales, out=out, lse=lse)
+    _check_plain(q=q, cache=cache, scales=scales, out=out, lse=lse)
     B = _check_cache(cache, scales, page_table, lengths, starts)
     _, pages, page_size, Hkv, D = cache.shape
     Hq = q.shape[-2] if q.dim() >= 2 else 0

@@ -1,6 +1,7 @@
-"""What the operators over a paged cache do with tensors that autograd looks after (no GPU needed: they say so before anything else)."""
+"""What the operators over a paged cache do with tensors that autograd or a trace looks after (no GPU needed: they say so before anything else)."""
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
 import mercury_artifact_amd as M
@@ -54,6 +55,14 @@ def test_without_gradients_the_call_goes_on():
     with torch.no_grad():
         for _, call in _calls(lambda t: t.detach().requires_grad_()):
             with pytest.raises(RuntimeError, match="GPU only"):
+                call()
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_fake_tensors_are_refused(device):
+    with FakeTensorMode():
+        for _, call in _calls(lambda t: t, device):
+            with pytest.raises(RuntimeError, match="no fake form"):
                 call()
 
 
