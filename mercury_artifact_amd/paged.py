@@ -171,8 +171,10 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     """Attention of the new tokens over their sequences' keys, their own among them: ``out`` like q in bfloat16 and ``lse``
     (B, Hq, n) -- packed: (Hq, T) -- in float32.  ``causal``: new token i of n sees the keys up to ``lengths - n + i``, else all
     of them.  Rows that see no key get 0 and -inf.  ``most_new``: with ``starts``, about how many new tokens a sequence has at
-    most (default: all of them in one); it chooses the form of the kernels, the result does not depend on it.  ``out`` may be
-    q itself."""
+    most (default: all of them in one).  Results are right whatever it says; it chooses the form of the kernels, and those round
+    differently.  With up to 16 rows (new tokens times query heads of a K/V head) the values' weights are carried as two bfloat16
+    numbers, with more they are rounded to bfloat16 once; with up to 64 rows the scales of a cache are applied in float32, with more
+    a row times its scale is rounded to bfloat16, which is exact for powers of two.  ``out`` may be q itself."""
     done = N.host.paged_attn_fwd(q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse)
     if done is not None:
         return done
