@@ -596,11 +596,11 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   p.q_sb = starts ? 0 : q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
   p.o_sb = starts ? 0 : o_sb; p.o_ss = o_ss; p.o_sh = o_sh;
   p.l_sb = starts ? 0 : (int64_t)Hq * n; p.l_sh = starts ? T : n;
-  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D;
+  p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D;
   p.causal = mask == MHIP_MASK_CAUSAL;
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * kLog2e;
-  p.by_group = Divisor(p.G); p.by_heads = Divisor(Hq); p.by_new = Divisor(n);
+  p.by_group = Divisor(p.G);
   p.part_o = static_cast<float*>(workspace);
   const int64_t rows = (int64_t)most_new * p.G;
   if (rows > kFewRows && !paged_attn_chunk_fits(B, n, T, p.G, Hkv, starts != nullptr)) return MHIP_EUNSUPPORTED;

@@ -14,6 +14,7 @@ struct Record { int first, slot, parts, rts; };
 // the slots first, second, second + step, ...
 struct Shared { int b, hk, row0, rows, parts, first, second, step; };
 
+// (Arguments are read by lines of 64 bytes: with the numbers behind the pointers a call of one token takes 9.8 us, in other orders up to 10.2.)
 struct PagedAttn {
   PagedGeom g;
   const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
@@ -22,13 +23,13 @@ struct PagedAttn {
   int64_t s_sp, s_ss, s_sh;                // of the scales, elements
   const uint16_t* q; uint16_t* out; float* lse;
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, l_sb, l_sh;
-  int Hq, Hkv, G, D, causal;
-  float scale, scale_log2;
-  Divisor by_group, by_heads, by_new;
-  int by_item;                             // paged_attn_few: shared items by their number, not by the workgroup they begin in
-  int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
   float* part_o; f32x2* part_ml;           // partial results
   Shared* shared; Record* records; int* pieces;
+  int Hkv, G, D, causal;
+  float scale, scale_log2;
+  Divisor by_group;
+  int by_item;                             // paged_attn_few: shared items by their number, not by the workgroup they begin in
+  int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
 };
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {

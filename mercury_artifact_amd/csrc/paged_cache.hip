@@ -22,7 +22,7 @@ struct RowsParams {
   int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
   uint16_t* out;                                           // read: the chunk
   int64_t o_half, o_sb, o_ss, o_sh;
-  int total, begin, rows, D;       // total: pairs of rows to move
+  int total, begin, D;             // total: pairs of rows to move
   Divisor by_rows, by_head, by_new;
 };
 
