@@ -67,7 +67,9 @@ def _check_cache(cache, scales, page_table, lengths, starts=None):
         raise RuntimeError("page_table must be an int32 (B, pages of a sequence) tensor with contiguous rows")
     if starts is not None and (starts.shape != (B + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous()):
         raise RuntimeError("starts must be a contiguous int32 (B + 1,) tensor")
-    _whole("the number of pages", cache.shape[1])
+    for name, size in zip(("pages", "rows of a page", "K/V heads", "columns"), cache.shape[1:]):
+        _whole(f"the number of {name}", size)
+    _whole("the number of sequences", B)
     _whole("the number of entries of page_table", page_table.shape[1])
     for t in (scales, page_table, lengths, starts):
         if t is not None and t.device != cache.device:
@@ -82,7 +84,9 @@ def _check_tokens(name, t, B, starts, heads, head_dim, device):
         raise RuntimeError(f"{name} must be (B, new tokens, heads, head_dim), or (all new tokens, heads, head_dim) with starts")
     if t.shape[-2] != heads or t.shape[-1] != head_dim or t.stride(-1) != 1 or t.dtype != torch.bfloat16 or t.device != device:
         raise RuntimeError(f"{name} must be bfloat16 with {heads} heads of {head_dim}, a contiguous last dimension, on the cache's device")
-    return (t.shape[1], _whole("the number of new tokens", t.shape[0] * t.shape[1])) if starts is None else (0, t.shape[0])
+    _whole("the number of heads", heads)
+    n = 0 if starts is not None else _whole("the number of new tokens of a sequence", t.shape[1])
+    return n, _whole("the number of new tokens", t.shape[0] if starts is not None else t.shape[0] * n)
 
 
 def _whole(name, x, bits=31):
