@@ -40,6 +40,7 @@ extern "C" {
 #define MHIP_BF16  0
 #define MHIP_E4M3  1   /* OCP float8 e4m3fn */
 #define MHIP_F32   2   /* input type of mhip_quantize_e4m3 only */
+#define MHIP_E2M1  3   /* OCP float4 e2m1, two to a byte; a paged cache only */
 
 /* ---- mask classes of one (Q shard, KV chunk) block -------------------------------- */
 #define MHIP_MASK_NONE    0
@@ -54,8 +55,9 @@ extern "C" {
  * 8: mhip_attn_fwd_blocks takes the number of chunks of a result; mhip_attn_fwd_chain.
  * 9: mhip_attn_bwd_take.
  * 10: mhip_attn_fwd_tile, mhip_attn_bwd_chunks_plan.
- * 11: mhip_paged_cache_write, mhip_paged_cache_read, mhip_paged_attn_workspace_bytes, mhip_paged_attn_fwd. */
-#define MHIP_ABI_VERSION 11
+ * 11: mhip_paged_cache_write, mhip_paged_cache_read, mhip_paged_attn_workspace_bytes, mhip_paged_attn_fwd.
+ * 12: a paged cache may be MHIP_E2M1, and its scales are passed as void*. */
+#define MHIP_ABI_VERSION 12
 int         mhip_abi_version(void);   /* the MHIP_ABI_VERSION the library was built with */
 int         mhip_version(void);
 /* Optional: per-device set-up the entry points otherwise do on their first call on a device (today: the address
@@ -337,6 +339,10 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
  * length in pages of page_size rows.  k_cache and v_cache are (pages, page_size, Hkv, D) with the element strides c_sp, c_ss,
  * c_sh (the same for both, D contiguous, c_ss >= D), MHIP_BF16 or MHIP_E4M3; e4m3 rows have one fp32 scale each, k_scales and
  * v_scales (pages, page_size, Hkv) with the strides s_sp, s_ss, s_sh, and stand for code * scale (NULL for MHIP_BF16).
+ * MHIP_E2M1: a row is D / 2 bytes, column 2 i in the low four bits of byte i and column 2 i + 1 in the high ones (strides of the cache
+ * count bytes, c_ss >= D / 2), codes 0 .. 7 stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6 and 8 .. 15 for their negatives.  Its scales are four
+ * bytes for each row (4-byte aligned, strides count rows of four): byte c stands for 2^(byte - 127) and belongs to columns 32 c ..
+ * 32 c + 31 (255: NaN; 0 may count as zero; bytes past the last column are neither read nor written).
  * Key j of sequence b is row j % page_size of page page_table[b * t_sb + j / page_size]; lengths[b] counts its keys, the new
  * tokens' among them, which are the last ones.  An entry outside [0, pages) is a page that is not here (freed, not yet given,
  * or another rank's): nobody sees its keys, rows written to it are dropped, rows read from it are zeros.  New tokens lie in
@@ -345,7 +351,7 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
  * page_table, lengths and starts are DEVICE arrays of int32, read when the kernels run (a captured graph follows them); a length
  * counts as one from 0 to table_pages * page_size, a start as one from 0 to T.
  * page_size: a multiple of 16, table_pages * page_size <= 2^31 - 2^16, 16 rows of the cache within 2^30 bytes (MHIP_EUNSUPPORTED).  D: a
- * multiple of 8 (MHIP_E4M3: of 16) up to 128.  Bases and rows on 16 bytes.  A launch has fewer than 2^32 threads, so a call takes
+ * multiple of 8 (MHIP_E4M3: of 16, MHIP_E2M1: of 32) up to 128.  Bases and rows on 16 bytes.  A launch has fewer than 2^32 threads, so a call takes
  * T * Hkv rows to write up to 2^28 - 128 and B * rows * Hkv to read up to 2^29 - 256, twice as many of 64 columns or fewer; attention T * Hq
  * rows below 2^31 - 256 and, where most_new * Hq / Hkv passes 64, B * Hkv + T * Hq / 256 below 2^23 - 512.  More is refused before anything
  * is launched (MHIP_EUNSUPPORTED).
@@ -354,10 +360,11 @@ int mhip_grad_accumulate(const float* acc, const void* block, float* dst, int64_
 /*
  * The new tokens' keys and values (bf16) into their rows of the cache.  MHIP_E4M3: a row x gets the scale s = 2^e, the least
  * power of two from 2^-126 on with max|x| <= 448 s (1 if all of x is zero), and the codes round-to-nearest-even e4m3fn(x / s); a
- * row with an infinity or a NaN gets the scale NaN.  Two new tokens of a call must not lie in one row of the cache
+ * row with an infinity or a NaN gets the scale NaN.  MHIP_E2M1: the same for each 32 columns of a row, with the least power of two
+ * from 2^-126 to 2^125 that keeps them within 6 (larger values count as 6 * 2^125).  Two new tokens of a call must not lie in one row of the cache
  * (sequences that share the page they write to): which of them stays is not defined.
  */
-int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, void* k_scales, void* v_scales,
                            const int* page_table, const int* lengths, const int* starts,
                            int B, int n, int T, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
                            int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t v_sb, int64_t v_ss, int64_t v_sh,
@@ -367,9 +374,9 @@ int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_
 /*
  * Rows begin .. begin + rows - 1 of every sequence as a dense bf16 chunk: out (2, B, rows, Hkv, D), keys and values, element
  * strides o_half, o_sb, o_ss, o_sh.  Rows past a sequence's end are zeros.  e4m3 rows are rounded once, and what
- * mhip_paged_cache_write wrote comes back exactly (down to the least numbers of bf16).
+ * mhip_paged_cache_write wrote comes back exactly (down to the least numbers of bf16), e2m1 rows whatever their scales.
  */
-int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
                           const int* page_table, const int* lengths, void* out,
                           int B, int begin, int rows, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
                           int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
@@ -387,7 +394,7 @@ int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float*
  * starts, Hq, Hkv, D) bytes of device memory; calls that overlap in time need one each.
  */
 int64_t mhip_paged_attn_workspace_bytes(int B, int n, int T, int most_new, int packed, int Hq, int Hkv, int D);
-int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
                         const int* page_table, const int* lengths, const int* starts, void* out, float* lse,
                         int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
                         int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,

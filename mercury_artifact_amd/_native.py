@@ -19,7 +19,7 @@ import torch
 # MERCURY_HIP_LIB is a deployment option: the path of the built library when it is not kept next to the package.
 _BUILT = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("MERCURY_HIP_LIB") or os.path.join(_BUILT, "libmercury_hip.so")
-ABI_VERSION = 11     # MHIP_ABI_VERSION of include/mercury_hip.h the signatures below were written against
+ABI_VERSION = 12     # MHIP_ABI_VERSION of include/mercury_hip.h the signatures below were written against
 
 
 class _NoHost:
@@ -50,7 +50,7 @@ def _load_host():
 
 host = _load_host()
 
-MHIP_BF16, MHIP_E4M3, MHIP_F32 = 0, 1, 2
+MHIP_BF16, MHIP_E4M3, MHIP_F32, MHIP_E2M1 = 0, 1, 2, 3
 MASK_NONE, MASK_CAUSAL = 0, 1
 
 _lib = None

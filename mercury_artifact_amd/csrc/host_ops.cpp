@@ -735,7 +735,7 @@ struct Paged {
   int64_t B, pages, page, Hkv, D;
   int type;
   const char *k, *v;
-  float *ks = nullptr, *vs = nullptr;
+  char *ks = nullptr, *vs = nullptr;
   int64_t s_sp = 0, s_ss = 0, s_sh = 0;
   bool take(PyObject* cache_, PyObject* table_, PyObject* lengths_, PyObject* scales_, PyObject* starts_) {
     cache = plain(cache_);
@@ -747,9 +747,17 @@ struct Paged {
     pages = c.size(1); page = c.size(2); Hkv = c.size(3); D = c.size(4);
     if (c.scalar_type() == at::kBFloat16) type = MHIP_BF16;
     else if (c.scalar_type() == at::kFloat8_e4m3fn) type = MHIP_E4M3;
+    else if (c.scalar_type() == at::kFloat4_e2m1fn_x2) type = MHIP_E2M1;
     else return false;
-    if ((type == MHIP_E4M3) != (scales != nullptr) || differentiated(c) || (scales && differentiated(*scales))) return false;
-    if (scales && (scales->scalar_type() != at::kFloat || scales->sizes() != c.sizes().slice(0, 4))) return false;
+    if (type == MHIP_E2M1 && D > INT32_MAX / 2) return false;
+    if (type == MHIP_E2M1) D *= 2;
+    if ((type != MHIP_BF16) != (scales != nullptr) || differentiated(c) || (scales && differentiated(*scales))) return false;
+    if (scales && (scales->dim() != (type == MHIP_E2M1 ? 5 : 4) || scales->sizes().slice(0, 4) != c.sizes().slice(0, 4) ||
+                   scales->scalar_type() != (type == MHIP_E2M1 ? at::kFloat8_e8m0fnu : at::kFloat)))
+      return false;
+    if (type == MHIP_E2M1 && (scales->size(4) != 4 || scales->stride(4) != 1 ||
+                              (scales->stride(0) | scales->stride(1) | scales->stride(2) | scales->stride(3)) & 3))
+      return false;
     if (lengths->dim() != 1 || lengths->scalar_type() != at::kInt || !lengths->is_contiguous()) return false;
     B = lengths->size(0);
     if (table->dim() != 2 || table->size(0) != B || table->scalar_type() != at::kInt || (table->size(1) > 1 && table->stride(1) != 1)) return false;
@@ -758,9 +766,10 @@ struct Paged {
     k = static_cast<const char*>(c.data_ptr());
     v = k + c.stride(0) * c.element_size();
     if (scales) {
-      ks = floats(scales);
-      vs = ks + scales->stride(0);
-      s_sp = scales->stride(1); s_ss = scales->stride(2); s_sh = scales->stride(3);
+      const int64_t each = type == MHIP_E2M1 ? 4 : 1;      // (strides of four bytes: a float, or a row of four)
+      ks = static_cast<char*>(scales->data_ptr());
+      vs = ks + scales->stride(0) * scales->element_size();
+      s_sp = scales->stride(1) / each; s_ss = scales->stride(2) / each; s_sh = scales->stride(3) / each;
     }
     return true;
   }

@@ -58,10 +58,23 @@ __device__ __forceinline__ int paged_owner(const PagedGeom& g, int t, int lane) 
   return b;
 }
 
+// Bytes of a row of the cache, and four fp4 scales of a row, a byte each: that of 32 columns as an fp32 power of two, exact from 2^-126 on.
+constexpr int row_bytes(int type, int D) { return type == MHIP_BF16 ? 2 * D : type == MHIP_E4M3 ? D : D / 2; }
+__device__ __forceinline__ float e8m0(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Eight e2m1 codes of a dword, times a scale that is a power of two, as bf16: exact while they are normal numbers there; a scale with
+// the exponent 255 makes them NaN, and one with the exponent 0 counts as 2^-127.
+__device__ __forceinline__ u32x4 e2m1_to_bf16(uint32_t codes, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
 // What the entry points ask of tables, lengths and starts, and of the cache: MHIP_OK, or the code to return.
 int paged_geometry(PagedGeom& g, const int* table, const int* lengths, const int* starts, int64_t t_sb, int B, int n, int T, int pages,
                    int page, int width);
-int paged_cache_fits(const void* kc, const void* vc, const float* ks, const float* vs, int pages, int Hkv, int D,
+int paged_cache_fits(const void* kc, const void* vc, const void* ks, const void* vs, int pages, int Hkv, int D,
                      int64_t c_sp, int64_t c_ss, int64_t c_sh, int dtype);
 
 }  // namespace mhip

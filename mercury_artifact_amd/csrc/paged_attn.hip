@@ -17,6 +17,8 @@
 //   e4m3       : codes are exact in bf16 (v_cvt_scalef32_pk_bf16_fp8); a key's scale multiplies its score, a value's scale
 //                its weight, in fp32.  The weights go to the product as bf16 (off by 2^-8 of each at most), up to 16 rows as
 //                two bf16 numbers (2^-14); there is no other rounding below 32 bits before the last.
+//   e2m1       : a key's codes times their scales are exact in bf16.  A value's scale is of 32 columns, so each 32 columns have weights of
+//                their own, the keys' weights times the scales in fp32, rounded to bf16 once.
 #include "paged_attn.hpp"
 
 namespace mhip {
@@ -29,8 +31,8 @@ constexpr int kKeys = 32;                  // keys of a tile, one wavefront's
 // registers for two on a SIMD and half as much still holds two tiles: up to 16 rows, of up to 128 bytes.  us, four / eight wavefronts:
 // e4m3 64 x 100 .. 2048 H32/8 43.4 / 35.9, 32 x 300 .. 16384 111.1 / 102.3, 16 x 5 tokens at 211 .. 4099 H16/8 D80 29.1 / 24.4, 4 x 131072
 // 180.6 / 181.2; bf16 D64 64 x 100 .. 2048 35.5 / 31.5, 32 x 300 .. 16384 96.5 / 94.4, 16 x 5 23.4 / 21.7, 8 x 8192 H16/2 15.3 / 15.6.
-template <bool E4M3, int COLS, int NR>
-constexpr int kRingOf = NR == 1 && COLS * (E4M3 ? 1 : 2) <= 128 ? 16384 : 32768;
+template <int TYPE, int COLS, int NR>
+constexpr int kRingOf = NR == 1 && row_bytes(TYPE, COLS) <= 128 ? 16384 : 32768;
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
 constexpr int kWavefronts = 1024;          // of a launch with rings of 32 KB: four on a CU, in workgroups of four or two
 constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
@@ -90,23 +92,24 @@ __device__ __forceinline__ int swizzle(int row) {      // of the 16-byte chunks 
   return ROWB == 256 ? lds_row_swizzle_16(row) : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-template <bool E4M3, int COLS, int NR, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void paged_attn_few(const PagedAttn p) {
+template <int TYPE, int COLS, int NR, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void paged_attn_few(const PagedAttn p) {
   constexpr int ROWS = 16 * NR, UNIT = WAVES * kKeys, kPause = kPauseOf<UNIT>;
-  constexpr int kSize = E4M3 ? 1 : 2;
-  constexpr int ROWB = COLS * kSize;                   // bytes of a row in LDS
+  constexpr bool E4M3 = TYPE == MHIP_E4M3, E2M1 = TYPE == MHIP_E2M1, SCALED = E4M3 || E2M1;
+  constexpr int ROWB = E2M1 ? 64 : row_bytes(TYPE, COLS);        // bytes of a row in LDS (e2m1: a copy takes 16 rows, with chunks of zeros up to 64 columns)
   constexpr int kChunks = ROWB / 16;
   constexpr int kCopyRows = 1024 / ROWB;               // rows of one copy instruction
   constexpr int kCopies = 16 / kCopyRows;              // and instructions of half a tile
   constexpr int kTileBytes = kKeys * ROWB;
-  constexpr int kStages = kRingOf<E4M3, COLS, NR> / (2 * kTileBytes);
-  constexpr int kStage = 2 * kTileBytes + (E4M3 ? 256 : 0);      // K, V, 32 scales of each
-  constexpr int nK = 2 * kCopies + (E4M3 ? 1 : 0), nV = 2 * kCopies;
+  constexpr int kStages = kRingOf<TYPE, COLS, NR> / (2 * kTileBytes);
+  constexpr int kStage = 2 * kTileBytes + (SCALED ? 256 : 0);    // K, V, 32 scales (e2m1: rows of four) of each
+  constexpr int nK = 2 * kCopies + (SCALED ? 1 : 0), nV = 2 * kCopies;
   constexpr int KB = COLS / 32, DB = COLS / 16;
   constexpr int kPair = NR < 2 ? NR : 2;               // blocks of rows that are worked on together
   // Weights to 14 bits and more of their mantissa, in two products, where that costs next to nothing: up to 16 rows (32 sequences of 300 .. 16384
   // bf16 177.8 us and 177.8, e4m3 102.3 and 103.3).  With more rows the matrix instructions show, and weights are rounded to bf16 once.
-  constexpr bool kTwice = NR == 1;
+  // (nor in e2m1, where each block of columns has weights of its own, times its scale, and two of them would be 32 instructions more)
+  constexpr bool kTwice = NR == 1 && !E2M1;
   constexpr int kRegion = kStages * kStage;
   static_assert(ROWS * COLS * 4 <= kRegion, "a wavefront's O takes the place of its ring");
   static_assert(kStages * (nK + nV) < 64, "copies in flight are counted in 6 bits");
@@ -147,19 +150,29 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
 #pragma unroll
   for (int u = 0; u < kCopies; ++u) {
     const int row = u * kCopyRows + lane / kChunks, chunk = (lane % kChunks) ^ swizzle<ROWB>(row);
-    voff[u] = chunk * 16 < p.D * kSize ? row * (int)p.c_ss16 * 16 + chunk * 16 : kNoColumn;
+    voff[u] = chunk * 16 < row_bytes(TYPE, p.D) ? row * (int)p.c_ss16 * 16 + chunk * 16 : kNoColumn;
   }
-  // K operand: 16 bytes of row ln; in e4m3 they serve two k-steps of 32 columns
-  constexpr int KR = E4M3 ? KB / 2 : KB;               // 16-byte reads of a K row
+  // K operand: 16 bytes of row ln; in e4m3 they serve two k-steps of 32 columns; in e2m1 all four of 128 columns, and 8 bytes both of 64, and they
+  // are of one block of 32 columns
+  constexpr int KR = E2M1 ? 1 : E4M3 ? KB / 2 : KB;    // reads of a K row
+  const int k_block = COLS == 128 ? lg : lg >> 1;      // (e2m1)
   int k_a[KR];
+  if constexpr (E2M1) k_a[0] = (int)ring + ln * ROWB + ((k_block ^ swizzle<ROWB>(ln)) << 4) + (COLS == 128 ? 0 : (lg & 1) * 8);
+  else {
 #pragma unroll
-  for (int i = 0; i < KR; ++i) k_a[i] = (int)ring + ln * ROWB + (((4 * i + lg) ^ swizzle<ROWB>(ln)) << 4);
+    for (int i = 0; i < KR; ++i) k_a[i] = (int)ring + ln * ROWB + (((4 * i + lg) ^ swizzle<ROWB>(ln)) << 4);
+  }
   // V^T operand: keys 4 lg .. +3 of both halves of the tile, one column of a strip of 16 per lane.  bf16: within 16 lanes lane s
-  // supplies the address of columns 4 (s % 4) .. +3 of row s / 4 and receives column s; e4m3: of columns 8 (s % 2) .. +7 of row s / 2.
-  int v_a[DB];
+  // supplies the address of columns 4 (s % 4) .. +3 of row s / 4 and receives column s; e4m3: of columns 8 (s % 2) .. +7 of row s / 2; e2m1: of a strip's 16
+  // columns of row s % 8, for two strips at once, those of a block of 32 columns.
+  constexpr int VR = E2M1 ? DB / 2 : DB;
+  int v_a[VR];
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    if (E4M3) {
+  for (int db = 0; db < VR; ++db) {
+    if (E2M1) {
+      const int row = (ln & 3) + 4 * lg + 4 * (ln & 4);
+      v_a[db] = (int)ring + kTileBytes + row * ROWB + ((db ^ swizzle<ROWB>(row & 15)) << 4) + (ln >> 3) * 8;
+    } else if (E4M3) {
       const int r8 = ln >> 1, row = (r8 & 3) + 4 * lg + 16 * (r8 >> 2);
       v_a[db] = (int)ring + kTileBytes + row * ROWB + ((db ^ swizzle<ROWB>(row & 15)) << 4) + (ln & 1) * 8;
     } else {
@@ -170,6 +183,8 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
   typedef __attribute__((address_space(3))) bf16x4* lds_bf16x4;
   typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
   typedef __attribute__((address_space(3))) const u32x4* lds_u32x4;
+  typedef __attribute__((address_space(3))) const u32x2* lds_u32x2;
+  typedef __attribute__((address_space(3))) const uint8_t* lds_byte;
   typedef __attribute__((address_space(3))) const f32x4* lds_f32x4;
   auto codes_to_bf16 = [](uint32_t a, uint32_t c) -> bf16x8 {
     const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
@@ -214,7 +229,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
       lim[r] = p.causal ? clamped(s.len - s.n + token + 1, 0, s.len) : s.len;
 #pragma unroll
       for (int ks = 0; ks < KB; ++ks) {
-        const int col = E4M3 ? (ks >> 1) * 64 + lg * 16 + (ks & 1) * 8 : ks * 32 + lg * 8;
+        const int col = E2M1 ? (lg * KB + ks) * 8 : E4M3 ? (ks >> 1) * 64 + lg * 16 + (ks & 1) * 8 : ks * 32 + lg * 8;
         qf[r][ks] = bf16x8{};
         if (row < rows && col < p.D) qf[r][ks] = *reinterpret_cast<const bf16x8*>(src + col);
       }
@@ -252,13 +267,13 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint8_t* from = base + (held[h] > 0 ? row_offset(p, page[h], slot[h]) + hk * p.c_sh : 0);
-        const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * (int)p.c_ss16 * 16 + p.D * kSize) : 0u);
+        const u32x4 rs = rsrc_words(from, held[h] > 0 ? (uint32_t)((held[h] - 1) * (int)p.c_ss16 * 16 + row_bytes(TYPE, p.D)) : 0u);
 #pragma unroll
         for (int u = 0; u < kCopies; ++u) copy16_once_to_lds(rs, ring + at + h * 16 * ROWB + u * 1024, voff[u], 0);
       }
     };
     auto copy_k = [&](int stage) {
-      if constexpr (E4M3) {
+      if constexpr (SCALED) {
         const int h = (lane >> 4) & 1, row = ln < held[h] ? ln : held[h] - 1;
         const float* at = (lane >> 5 ? p.v_scales : p.k_scales) + (page[h] * p.s_sp + (slot[h] + row) * p.s_ss + hk * p.s_sh);
         copy4_to_lds(held[h] > 0 ? static_cast<const void*>(at) : p.q, ring + stage * kStage + 2 * kTileBytes);
@@ -300,13 +315,30 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
       const uint32_t hidden = gone >> (2 * stage) & 3u;
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"(nV + (kStages - 1) * (nK + nV)) : "memory");     // K of tile t is there
       const bool cut = key0 + kKeys > seen_first;                // some row does not see some key
-      f32x4 k_scale[2], v_scale[2];
+      f32x4 k_scale[2], v_scale[2];                              // (e2m1: the values' scales are rows of four bytes)
       // Two blocks of rows at a time: with all four of 64 rows the registers run out.  The second time K and V are read from LDS again.
 #pragma unroll
       for (int r0 = 0; r0 < NR; r0 += kPair) {
         f32x4 sc[2][kPair];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
+          if constexpr (E2M1) {
+            u32x4 w{};
+            if constexpr (COLS == 128) w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[0] + at + kb * 16 * ROWB);
+            else {
+              const u32x2 x = *(lds_u32x2)(uintptr_t)(uint32_t)(k_a[0] + at + kb * 16 * ROWB);
+              w[0] = x[0];
+              w[1] = x[1];
+            }
+            const uint32_t byte = *(lds_byte)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + (kb * 16 + ln) * 4 + k_block);
+            const float scale = k_block * 32 < p.D ? e8m0(byte) : 1.f;         // (past the last column there may be anything)
+#pragma unroll
+            for (int ks = 0; ks < KB; ++ks) {
+              const bf16x8 kf = __builtin_bit_cast(bf16x8, e2m1_to_bf16(w[ks], scale));
+#pragma unroll
+              for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
+            }
+          } else
 #pragma unroll
           for (int i = 0; i < KR; ++i) {
             const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
@@ -318,7 +350,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
               for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
             }
           }
-        if (E4M3 && r0 == 0)
+        if (SCALED && r0 == 0)
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             k_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + kb * 64 + lg * 16);
@@ -333,6 +365,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
 
         // ---- softmax --------------------------------------------------------------------------------------------
         u32x4 pw[kPair], pl[kPair];                              // weights in bf16, and what that leaves of them
+        float wide[kPair][8];                                    // (e2m1: in fp32, for each block of columns to scale)
         bool moved = false;
         float alpha[kPair];
 #pragma unroll
@@ -367,12 +400,14 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
             x[i] = fast_exp2(sc[i >> 2][r][i & 3] - ref);
             sum += x[i];
             // (a masked key's scale may be anything; a NaN of one that the row sees counts however small its weight is)
+            if constexpr (E2M1) wide[r][i] = x[i];
             if constexpr (E4M3) x[i] = sc[i >> 2][r][i & 3] == -INFINITY ? 0.f : x[i] * v_scale[i >> 2][i & 3];
           }
           l[r0 + r] = l[r0 + r] * alpha[r] + sum;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (kTwice) {
+            if constexpr (E2M1) {
+            } else if constexpr (kTwice) {
               // (cut off, not rounded, and the rest a little large: both have the weight's sign and are zero only with it, so that
               // infinite values stay what they are)
               pw[r][i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
@@ -393,7 +428,42 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<E4M3, COLS, NR>)) void
         // ---- O^T += V^T P^T ---------------------------------------------------------------------------------------
         if (r0 == 0)                                             // V of tile t is there
           asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NR <= kPair ? nK : 0) + (kStages - 1) * (nK + nV)) : "memory");
-        if (!(cut && seen_first < seen_last)) {
+        if constexpr (E2M1) {
+          // (a masked key's scales may be anything, and its weight is 0: its scales count as 0, too.  The last bit set is 2^-23 of a scale,
+          // and makes the exponent 255 a NaN.)
+          u32x4 quads[kPair][2];
+#pragma unroll
+          for (int r = 0; r < kPair; ++r)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              quads[r][kb] = __builtin_bit_cast(u32x4, v_scale[kb]);
+              if (cut || hidden) {
+                asm volatile("");
+                const int left = hidden >> kb & 1 ? 0 : lim[r0 + r] - (key0 + 16 * kb) - 4 * lg;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) quads[r][kb][j] = j < left ? quads[r][kb][j] : 0u;
+              }
+            }
+#pragma unroll
+          for (int c = 0; c < VR; ++c) {
+#pragma unroll
+            for (int r = 0; r < kPair; ++r) {
+              float x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                x[i] = wide[r][i] * __builtin_bit_cast(float, ((quads[r][i >> 2][i & 3] >> (8 * c) & 0xffu) << 23) | 1u);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            }
+            const i32x2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2)(uintptr_t)(uint32_t)(v_a[c] + at));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, e2m1_to_bf16((uint32_t)codes[e], 1.f));
+#pragma unroll
+              for (int r = 0; r < kPair; ++r) weigh(2 * c + e, r0 + r, vf, pw[r], pl[r]);
+            }
+          }
+        } else if (!(cut && seen_first < seen_last)) {
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
             const bf16x8 vf = read_v(db, at);
@@ -516,9 +586,9 @@ constexpr int64_t kManyItems = 128;
 // One partial result at each end of a workgroup's share.
 int64_t few_bytes(int64_t rows, int D) { return 2 * kWavefronts * (16 * (int64_t)row_blocks(rows) * ((D <= 64 ? 64 : 128) + 2) * 4 + 16); }
 
-template <bool E4M3, int COLS, int NR, int WAVES>
+template <int TYPE, int COLS, int NR, int WAVES>
 void launch_few(PagedAttn p, int64_t rows, hipStream_t st) {
-  constexpr int workgroups = kWavefronts * (32768 / kRingOf<E4M3, COLS, NR>) / WAVES;
+  constexpr int workgroups = kWavefronts * (32768 / kRingOf<TYPE, COLS, NR>) / WAVES;
   p.part_ml = reinterpret_cast<f32x2*>(p.part_o + 2 * (int64_t)workgroups * 16 * NR * COLS);
   p.shared = reinterpret_cast<Shared*>(p.part_ml + 2 * (int64_t)workgroups * 16 * NR);
   // Where the items are known and not more than the workgroups, the last step has one row of workgroups for each of them, not for
@@ -526,29 +596,30 @@ void launch_few(PagedAttn p, int64_t rows, hipStream_t st) {
   const int64_t items = (int64_t)p.g.B * p.Hkv * ((rows + 16 * NR - 1) / (16 * NR));
   p.by_item = !p.g.starts && items <= workgroups;
   const int blocks = !p.g.starts && rows < 16 * NR ? (int)((rows + 3) / 4) : 4 * NR;       // (packed, `rows` is a hint)
-  hipLaunchKernelGGL((paged_attn_few<E4M3, COLS, NR, WAVES>), dim3(workgroups), dim3(WAVES * 64), 0, st, p);
+  hipLaunchKernelGGL((paged_attn_few<TYPE, COLS, NR, WAVES>), dim3(workgroups), dim3(WAVES * 64), 0, st, p);
   hipLaunchKernelGGL((paged_attn_join<COLS, 16 * NR, 1, 4>), dim3(blocks, p.by_item ? (int)items : workgroups), dim3(256), 0, st, p);
 }
-template <bool E4M3, int COLS, int NR>
+template <int TYPE, int COLS, int NR>
 void launch_few(const PagedAttn& p, int64_t rows, hipStream_t st) {
-  if ((int64_t)p.g.B * p.Hkv >= kManyItems) launch_few<E4M3, COLS, NR, 2>(p, rows, st);
-  else launch_few<E4M3, COLS, NR, 4>(p, rows, st);
+  if ((int64_t)p.g.B * p.Hkv >= kManyItems) launch_few<TYPE, COLS, NR, 2>(p, rows, st);
+  else launch_few<TYPE, COLS, NR, 4>(p, rows, st);
 }
-template <bool E4M3, int COLS>
+template <int TYPE, int COLS>
 void launch_rows(const PagedAttn& p, int64_t rows, hipStream_t st) {
   const int blocks = row_blocks(rows);
-  if (blocks == 1) launch_few<E4M3, COLS, 1>(p, rows, st);
-  else if (blocks == 2) launch_few<E4M3, COLS, 2>(p, rows, st);
-  else launch_few<E4M3, COLS, 4>(p, rows, st);
+  if (blocks == 1) launch_few<TYPE, COLS, 1>(p, rows, st);
+  else if (blocks == 2) launch_few<TYPE, COLS, 2>(p, rows, st);
+  else launch_few<TYPE, COLS, 4>(p, rows, st);
 }
-void launch(const PagedAttn& p, bool e4m3, int64_t rows, hipStream_t st) {
-  if (e4m3) {
-    if (p.D <= 64) launch_rows<true, 64>(p, rows, st);
-    else launch_rows<true, 128>(p, rows, st);
-  } else {
-    if (p.D <= 64) launch_rows<false, 64>(p, rows, st);
-    else launch_rows<false, 128>(p, rows, st);
-  }
+template <int TYPE>
+void launch(const PagedAttn& p, int64_t rows, hipStream_t st) {
+  if (p.D <= 64) launch_rows<TYPE, 64>(p, rows, st);
+  else launch_rows<TYPE, 128>(p, rows, st);
+}
+void launch(const PagedAttn& p, int type, int64_t rows, hipStream_t st) {
+  if (type == MHIP_E2M1) launch<MHIP_E2M1>(p, rows, st);
+  else if (type == MHIP_E4M3) launch<MHIP_E4M3>(p, rows, st);
+  else launch<MHIP_BF16>(p, rows, st);
 }
 
 }  // namespace
@@ -564,7 +635,7 @@ extern "C" int64_t mhip_paged_attn_workspace_bytes(int B, int n, int T, int most
   return few > chunk ? few : chunk;
 }
 
-extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
                                    const int* page_table, const int* lengths, const int* starts, void* out, float* lse,
                                    int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
                                    int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
@@ -585,11 +656,11 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   for (int64_t s : {q_sb, q_ss, q_sh, o_sb, o_ss, o_sh})
     if (s % 8 != 0) return MHIP_EALIGN;
   if ((int64_t)T * Hq >= (int64_t(1) << 31) - 256) return MHIP_EUNSUPPORTED;       // (rows, up to a whole tile of them, are ints)
-  const int size = dtype == MHIP_E4M3 ? 1 : 2;
+  const int size = dtype == MHIP_BF16 ? 2 : 1;
   // places are counted in 16 bytes: 32 bits for a page, and for the rows of one
   if (c_sp < 0 || c_sp * size / 16 > 0xffffffffll || c_ss * size / 16 * page_size > 0xffffffffll) return MHIP_EUNSUPPORTED;
   p.k = static_cast<const uint8_t*>(k_cache); p.v = static_cast<const uint8_t*>(v_cache);
-  p.k_scales = k_scales; p.v_scales = v_scales;
+  p.k_scales = static_cast<const float*>(k_scales); p.v_scales = static_cast<const float*>(v_scales);
   p.c_sp16 = (uint32_t)(c_sp * size / 16); p.c_ss16 = (uint32_t)(c_ss * size / 16); p.c_sh = c_sh * size;
   p.s_sp = s_sp; p.s_ss = s_ss; p.s_sh = s_sh;
   p.q = static_cast<const uint16_t*>(q); p.out = static_cast<uint16_t*>(out); p.lse = lse;
@@ -607,13 +678,13 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows <= kFewRows) {                  // (a sequence with more rows all the same is several tiles of them)
     p.few_rows = 0x7fffffff;
-    launch(p, dtype == MHIP_E4M3, rows, st);
+    launch(p, dtype, rows, st);
   } else {
     // Packed sequences may be of either kind, such as generate a token at a time and such as take a chunk: two pairs of launches, one
     // after the other on the stream, share the workspace.
     p.few_rows = starts && p.G <= kFewRows ? 16 * row_blocks(p.G) : -1;
-    if (p.few_rows > 0) launch(p, dtype == MHIP_E4M3, p.few_rows, st);
-    paged_attn_chunk_launch(p, dtype == MHIP_E4M3, st);
+    if (p.few_rows > 0) launch(p, dtype, p.few_rows, st);
+    paged_attn_chunk_launch(p, dtype, st);
   }
   return launch_status();
 }

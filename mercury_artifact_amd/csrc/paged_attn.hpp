@@ -17,7 +17,7 @@ struct Shared { int b, hk, row0, rows, parts, first, second, step; };
 // (Arguments are read by lines of 64 bytes: with the numbers behind the pointers a call of one token takes 9.8 us, in other orders up to 10.2.)
 struct PagedAttn {
   PagedGeom g;
-  const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;
+  const uint8_t* k; const uint8_t* v; const float* k_scales; const float* v_scales;      // (e2m1: four bytes of scales in a float's place)
   uint32_t c_sp16, c_ss16;                 // strides of the cache from page to page and slot to slot, in 16 bytes,
   int64_t c_sh;                            // and from head to head, bytes
   int64_t s_sp, s_ss, s_sh;                // of the scales, elements
@@ -185,6 +185,6 @@ __global__ __launch_bounds__(256) void paged_attn_join(const PagedAttn p) {
 
 int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, int D, bool packed);
 bool paged_attn_chunk_fits(int64_t B, int64_t n, int64_t T, int G, int Hkv, bool packed);       // into a launch
-void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream);
+void paged_attn_chunk_launch(const PagedAttn& p, int type, hipStream_t stream);
 
 }  // namespace mhip

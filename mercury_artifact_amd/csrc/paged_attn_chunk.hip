@@ -10,7 +10,7 @@
 // and what the pages change:
 //   copies     : a wavefront copies 8 rows of each tile, which lie in one page; the table's entries are read through the scalar cache
 //                at the start of a vector phase and used at its end, when nothing else waits on that counter
-//   e4m3       : a wavefront's 8 rows of codes come through registers, requested one tile ahead, and go into LDS as bf16 rows
+//   e4m3, e2m1 : a wavefront's 8 rows of codes come through registers, requested one tile ahead, and go into LDS as bf16 rows
 //                times their scale, exact for a power of two: converted once by one wavefront, not by all eight
 //   pieces     : where the items are few, or one is long, several workgroups share an item's keys: paged_attn_chunk_plan cuts
 //                them and deals them out, paged_attn_join adds the partial results up
@@ -187,8 +187,9 @@ constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descrip
 constexpr int kFragDepth = 4;              // LDS operand reads in flight ahead of the MFMAs
 constexpr int kOStride = 136;              // epilogue staging of O, bf16 elements per row
 
-template <bool E4M3, int COLS>
+template <int TYPE, int COLS>
 __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
+  constexpr bool E2M1 = TYPE == MHIP_E2M1, CODES = TYPE != MHIP_BF16;
   constexpr int KB = COLS / 32, DB = COLS / 16;        // k-steps of S^T, blocks of O^T
   constexpr int MB = kBN / 16, kSteps = kBN / 32;      // key blocks of S^T, k-steps of O^T
   constexpr int kSlotsS = MB * KB, kSlotsO = kSteps * DB;
@@ -304,14 +305,23 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) copy16_to_lds(rs, to + u * 1024, voff[u], 0);
   };
-  // e4m3: lane l takes codes 16 (l % 8) .. +15 of row l / 8
+  // e4m3 and e2m1: lane l takes codes 16 (l % 8) .. +15 of row l / 8, which have one scale
   const int row8 = lane >> 3, col16 = (lane & 7) * 16;
   struct Codes { u32x4 w; float scale; };
   auto request = [&](const uint8_t* head, const float* scales, const Rows& x) {
-    Codes k{u32x4{}, 1.f};
+    Codes k{u32x4{}, E2M1 ? 0.f : 1.f};
     if (row8 < x.held && col16 < p.D) {
-      k.w = *reinterpret_cast<const u32x4*>(head + x.at + row8 * (int)p.c_ss16 * 16 + col16);
-      k.scale = scales[x.page * p.s_sp + (int64_t)(x.slot + row8) * p.s_ss + hk * p.s_sh];
+      const uint8_t* at = head + x.at + row8 * (int)p.c_ss16 * 16 + (E2M1 ? col16 / 2 : col16);
+      const float* scale = scales + (x.page * p.s_sp + (int64_t)(x.slot + row8) * p.s_ss + hk * p.s_sh);
+      if constexpr (E2M1) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+        k.w[0] = w[0];
+        k.w[1] = w[1];
+        k.scale = __builtin_bit_cast(float, (uint32_t)reinterpret_cast<const uint8_t*>(scale)[col16 >> 5]);      // (the byte: nothing waits for it here)
+      } else {
+        k.w = *reinterpret_cast<const u32x4*>(at);
+        k.scale = *scale;
+      }
     }
     return k;
   };
@@ -323,7 +333,10 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     };
     // scales 2^-126 .. 2^127 go into the conversion; others, and NaN, through fp32 and one rounding
     const uint32_t bits = __builtin_bit_cast(uint32_t, k.scale);
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x807fffffu) != 0 || bits - 0x00800000u >= 0x7f000000u) == 0, 1)) {
+    if constexpr (E2M1) {
+      lo = e2m1_to_bf16(k.w[0], e8m0(bits));
+      hi = e2m1_to_bf16(k.w[1], e8m0(bits));
+    } else if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x807fffffu) != 0 || bits - 0x00800000u >= 0x7f000000u) == 0, 1)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         keep(i, __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k.w[i], k.scale, false)),
@@ -490,7 +503,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     for (int i = 0; i < kFragDepth; ++i) frag[i] = read_frag(i);
   };
   auto early_slot = [](int idx) { return kSlotsS + DB + idx * (kSlotsO - DB) / kEarlyPairs; };
-  Rows next_v{}, next_k{};                             // of the tiles whose copies go out (e4m3: whose codes are put into LDS) next
+  Rows next_v{}, next_k{};                             // of the tiles whose copies go out (of codes: which are put into LDS) next
   auto copies = [&](int t) {                           // K(t + 4), V(t + 3)
     copy_rows(k_head, next_k, lds_rows + (t & 3) * kTileLds);
     copy_rows(v_head, next_v, lds_rows + kVRing + ((t + 3) & 3) * kTileLds);
@@ -509,7 +522,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
         for (int e = 0; e < DB; ++e)
           if (e % kFragDepth == i - (kSlotsS + kSlotsO - kFragDepth)) v_a[e] += v_step;
       }
-      if (!E4M3 && kShortMatrix && i == 1) copies(t);
+      if (!CODES && kShortMatrix && i == 1) copies(t);
       if (i == kSlotsS) sm_mask(t + 1);
 #pragma unroll
       for (int idx = 0; idx < kEarlyPairs; ++idx)
@@ -519,7 +532,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
   };
   // the same where tile t cuts
   auto matrix_phase_cut = [&](int t) __attribute__((always_inline)) {
-    if (!E4M3 && kShortMatrix) copies(t);
+    if (!CODES && kShortMatrix) copies(t);
     pv_cut(t);
 #pragma unroll
     for (int i = 0; i < kSlotsS; ++i) {
@@ -557,7 +570,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) l_run[r] = rs[r];
     };
-    if constexpr (!E4M3) {
+    if constexpr (!CODES) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -603,7 +616,7 @@ __global__ __launch_bounds__(512, 2) void paged_attn_chunk(const PagedAttn p) {
     auto vector_phase = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) asm volatile("" : "+v"(sc[0][r]), "+v"(sc[MB - 1][r]));   // keeps the exponentials behind the barrier
-      if constexpr (!E4M3) {
+      if constexpr (!CODES) {
         const Entry e = look_up(t + 5);
         sm_tile();
         if (!kShortMatrix) copies(t);
@@ -702,19 +715,19 @@ int64_t places_of(int64_t B, int64_t T, int64_t n, int G, int Hkv, bool packed) 
 int columns_of(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 int64_t up16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
-template <bool E4M3, int COLS>
+template <int TYPE, int COLS>
 void launch(const PagedAttn& p, int places, hipStream_t st) {
   hipLaunchKernelGGL(paged_attn_chunk_plan, dim3(1), dim3(kPlanWaves * 64), 0, st, p, places);
-  hipLaunchKernelGGL((paged_attn_chunk<E4M3, COLS>), dim3((unsigned)places), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((paged_attn_chunk<TYPE, COLS>), dim3((unsigned)places), dim3(512), 0, st, p);
   // rows of a workgroup: 4 / 8 / 16 / 32 took 57.0 / 58.6 / 65.2 / 76.4 us with 64 tokens at 32768 (8 now 56.1)
   constexpr int rows = 8;
   hipLaunchKernelGGL((paged_attn_join<COLS, kBM, 2, rows>), dim3(kBM / rows, kParts / 2), dim3(256), 0, st, p);
 }
-template <bool E4M3>
+template <int TYPE>
 void launch(const PagedAttn& p, int places, hipStream_t st) {
-  if (p.D <= 64) launch<E4M3, 64>(p, places, st);
-  else if (p.D <= 96) launch<E4M3, 96>(p, places, st);
-  else launch<E4M3, 128>(p, places, st);
+  if (p.D <= 64) launch<TYPE, 64>(p, places, st);
+  else if (p.D <= 96) launch<TYPE, 96>(p, places, st);
+  else launch<TYPE, 128>(p, places, st);
 }
 
 }  // namespace
@@ -726,7 +739,7 @@ int64_t paged_attn_chunk_bytes(int64_t B, int64_t n, int64_t T, int G, int Hkv, 
 bool paged_attn_chunk_fits(int64_t B, int64_t n, int64_t T, int G, int Hkv, bool packed) {
   return grid_fits(places_of(B, T, n, G, Hkv, packed), 512);
 }
-void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) {
+void paged_attn_chunk_launch(const PagedAttn& p, int type, hipStream_t stream) {
   const int places = (int)places_of(p.g.B, p.g.T, p.g.n, p.G, p.Hkv, p.g.starts != nullptr);
   PagedAttn q = p;
   char* at = reinterpret_cast<char*>(q.part_o) + (int64_t)kParts * kBM * columns_of(p.D) * 4;
@@ -736,8 +749,9 @@ void paged_attn_chunk_launch(const PagedAttn& p, bool e4m3, hipStream_t stream) 
   at += kParts / 2 * 32;
   q.records = reinterpret_cast<Record*>(at);
   q.pieces = reinterpret_cast<int*>(at + 16 * (int64_t)p.g.B);
-  if (e4m3) launch<true>(q, places, stream);
-  else launch<false>(q, places, stream);
+  if (type == MHIP_E2M1) launch<MHIP_E2M1>(q, places, stream);
+  else if (type == MHIP_E4M3) launch<MHIP_E4M3>(q, places, stream);
+  else launch<MHIP_BF16>(q, places, stream);
 }
 
 }  // namespace mhip

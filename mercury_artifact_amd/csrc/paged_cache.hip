@@ -8,6 +8,9 @@
 // code * s are exact (s times four bits fits bf16), and the codes' relative step of 2^-4 is the same as with max|x| / 448;
 // what it costs is at most one of the 18 binades below the largest value.  A row that holds an infinity or a NaN gets
 // the scale NaN and codes of 0: it reads back as NaN, and attention sees that in the rows that see the key.
+//
+// An e2m1 row is the same 32 columns at a time: codes of four bits, rounded to nearest even by v_cvt_scalef32_pk_fp4_f32, and a byte
+// for the least power of two from 2^-126 to 2^125 with max|x| <= 6 s; beyond, 6 * 2^125 is the largest that stays finite when it is read back.
 #include "paged.hpp"
 
 namespace mhip {
@@ -28,11 +31,11 @@ struct RowsParams {
 
 // Workgroup i runs on XCD i % 8.  The scales of neighbouring keys share a line, so with them each XCD gets a run of neighbouring rows
 // (32768 rows read back 153.9 us to 150.8, 16403 tokens written 27.4 to 25.7; bf16 rows as they come, 46 MB read back in 11.2 us and 11.6).
-template <bool E4M3>
-__device__ __forceinline__ int block_here() { return E4M3 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x; }
+template <int TYPE>
+__device__ __forceinline__ int block_here() { return TYPE != MHIP_BF16 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x; }
 int64_t blocks_of(int64_t total, int each) { return ((total + each - 1) / each + 7) & ~int64_t(7); }
 
-// Largest of the lane's group of 16 or 8, in all of its lanes.
+// Largest of the lane's group of 16, 8 or 4, in all of its lanes.
 template <int LANES>
 __device__ __forceinline__ uint32_t group_max(uint32_t x) {
   auto with = [](uint32_t v, auto ctrl) {
@@ -41,17 +44,17 @@ __device__ __forceinline__ uint32_t group_max(uint32_t x) {
   };
   x = with(x, std::integral_constant<int, 0xb1>{});      // the other of a pair
   x = with(x, std::integral_constant<int, 0x4e>{});      // the other pair of four
-  x = with(x, std::integral_constant<int, 0x141>{});     // the other four of eight, mirrored
+  if (LANES >= 8) x = with(x, std::integral_constant<int, 0x141>{});     // the other four of eight, mirrored
   if (LANES == 16) x = with(x, std::integral_constant<int, 0x128>{});          // the other eight of sixteen
   return x;
 }
 
 // LANES = 16, or 8 where a row has 64 columns or fewer.  The key and the value of a token and head lie in the same slot, so a group of
 // lanes moves both with one look-up, and asks for them before it looks up (16403 tokens H8 D128: 36.9 us to 26.3).
-template <bool E4M3, int LANES>
+template <int TYPE, int LANES>
 __global__ __launch_bounds__(256) void paged_write_kernel(const RowsParams p) {
   const int lane = threadIdx.x & 63, col = (threadIdx.x % LANES) * 8;
-  const int id = block_here<E4M3>() * (256 / LANES) + threadIdx.x / LANES;
+  const int id = block_here<TYPE>() * (256 / LANES) + threadIdx.x / LANES;
   // pairs of rows in the order (token, head); lanes past the last one repeat it and store nothing
   int head, i = 0, b;
   const int token = p.by_head.quotient(id < p.total ? id : p.total - 1, head);
@@ -86,7 +89,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const RowsParams p) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     uint8_t* dst = (half ? p.v_cache : p.k_cache) + at;
-    if constexpr (!E4M3) {
+    if constexpr (TYPE == MHIP_BF16) {
       if (real) *reinterpret_cast<u32x4*>(dst + col * 2) = w[half];
       continue;
     }
@@ -96,6 +99,27 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const RowsParams p) {
     for (int j = 0; j < 4; ++j) {
       const uint32_t lo = w[half][j] << 16 & 0x7fffffffu, hi = w[half][j] & 0x7fff0000u, m = lo > hi ? lo : hi;
       top = m > top ? m : top;
+    }
+    const int64_t s_at = (int64_t)page * p.s_sp + (int64_t)slot * p.s_ss + (int64_t)head * p.s_sh;
+    if constexpr (TYPE == MHIP_E2M1) {
+      // (four lanes share 32 columns) 6 = 1.5 * 2^2: the least e is t - 2, one more if 1.f > 1.5
+      top = group_max<4>(top);
+      int power = (int)((top + 0x3fffffu) >> 23) - 2;
+      power = top == 0 ? 127 : power < 1 ? 1 : power > 252 ? 252 : power;
+      const bool finite = top < 0x7f800000u;
+      uint32_t codes = 0;
+      if (finite) {
+        const float scale = e8m0((uint32_t)power);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, bf16_lo(w[half][0]), bf16_hi(w[half][0]), scale, 0);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, bf16_lo(w[half][1]), bf16_hi(w[half][1]), scale, 1);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, bf16_lo(w[half][2]), bf16_hi(w[half][2]), scale, 2);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, bf16_lo(w[half][3]), bf16_hi(w[half][3]), scale, 3);
+      }
+      if (real) {
+        *reinterpret_cast<uint32_t*>(dst + col / 2) = codes;
+        if (col % 32 == 0) reinterpret_cast<uint8_t*>((half ? p.v_scales : p.k_scales) + s_at)[col / 32] = (uint8_t)(finite ? power : 255);
+      }
+      continue;
     }
     top = group_max<LANES>(top);
     // top = 1.f * 2^t with 1 <= 1.f < 2, and 448 = 1.75 * 2^8: the least e is t - 8, one more if 1.f > 1.75
@@ -120,7 +144,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const RowsParams p) {
     if (real) {
       *reinterpret_cast<u32x2*>(dst + col) = codes;
       if (col == 0)
-        (half ? p.v_scales : p.k_scales)[(int64_t)page * p.s_sp + (int64_t)slot * p.s_ss + (int64_t)head * p.s_sh] = scale;
+        (half ? p.v_scales : p.k_scales)[s_at] = scale;
     }
   }
 }
@@ -131,12 +155,12 @@ constexpr int kReadRows = 2;       // pairs of rows of a group of lanes, so that
 // so and 167 otherwise, 46 MB 13.5 and 11.1.
 constexpr int64_t kLastLevel = int64_t(256) << 20;
 
-template <bool E4M3, int LANES, bool ONCE>
+template <int TYPE, int LANES, bool ONCE>
 __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
   constexpr int kGroups = 256 / LANES;
   const int col = (threadIdx.x % LANES) * 8;
   if (col >= p.D) return;
-  const int first = block_here<E4M3>() * (kGroups * kReadRows) + threadIdx.x / LANES;
+  const int first = block_here<TYPE>() * (kGroups * kReadRows) + threadIdx.x / LANES;
   // keys and values of (sequence, row, head), in the chunk's order
   int b[kReadRows], i[kReadRows], head[kReadRows], page[kReadRows], slot[kReadRows];
 #pragma unroll
@@ -166,7 +190,11 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint8_t* src = (half ? p.v_cache : p.k_cache) + at;
-        if constexpr (E4M3) {
+        if constexpr (TYPE == MHIP_E2M1) {
+          const uint32_t* from = reinterpret_cast<const uint32_t*>(src + col / 2);
+          codes[u][half][0] = ONCE ? __builtin_nontemporal_load(from) : *from;
+          scale[u][half] = e8m0(reinterpret_cast<const uint8_t*>((half ? p.v_scales : p.k_scales) + s)[col / 32]);
+        } else if constexpr (TYPE == MHIP_E4M3) {
           const u32x2* from = reinterpret_cast<const u32x2*>(src + col);
           codes[u][half] = ONCE ? __builtin_nontemporal_load(from) : *from;
           scale[u][half] = (half ? p.v_scales : p.k_scales)[s];
@@ -182,7 +210,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
     if (first + kGroups * u >= p.total) break;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      if constexpr (E4M3) {
+      if constexpr (TYPE == MHIP_E2M1) w[u][half] = e2m1_to_bf16(codes[u][half][0], scale[u][half]);
+      if constexpr (TYPE == MHIP_E4M3) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t c = codes[u][half][h];
@@ -200,11 +229,11 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const RowsParams p) {
 
 bool mult(int64_t x, int m) { return x % m == 0; }
 
-void take_cache(RowsParams& p, const void* kc, const void* vc, const float* ks, const float* vs, int64_t c_sp, int64_t c_ss, int64_t c_sh,
+void take_cache(RowsParams& p, const void* kc, const void* vc, const void* ks, const void* vs, int64_t c_sp, int64_t c_ss, int64_t c_sh,
                 int64_t s_sp, int64_t s_ss, int64_t s_sh, int D, int dtype) {
-  const int size = dtype == MHIP_E4M3 ? 1 : 2;
+  const int size = dtype == MHIP_BF16 ? 2 : 1;
   p.k_cache = static_cast<uint8_t*>(const_cast<void*>(kc)); p.v_cache = static_cast<uint8_t*>(const_cast<void*>(vc));
-  p.k_scales = const_cast<float*>(ks); p.v_scales = const_cast<float*>(vs);
+  p.k_scales = static_cast<float*>(const_cast<void*>(ks)); p.v_scales = static_cast<float*>(const_cast<void*>(vs));
   p.c_sp = c_sp * size; p.c_ss = c_ss * size; p.c_sh = c_sh * size;
   p.s_sp = s_sp; p.s_ss = s_ss; p.s_sh = s_sh;
   p.D = D;
@@ -212,16 +241,17 @@ void take_cache(RowsParams& p, const void* kc, const void* vc, const float* ks, 
 
 }  // namespace
 
-int paged_cache_fits(const void* kc, const void* vc, const float* ks, const float* vs, int pages, int Hkv, int D,
+int paged_cache_fits(const void* kc, const void* vc, const void* ks, const void* vs, int pages, int Hkv, int D,
                      int64_t c_sp, int64_t c_ss, int64_t c_sh, int dtype) {
-  if (dtype != MHIP_BF16 && dtype != MHIP_E4M3) return MHIP_EDTYPE;
+  if (dtype != MHIP_BF16 && dtype != MHIP_E4M3 && dtype != MHIP_E2M1) return MHIP_EDTYPE;
   if (Hkv <= 0) return MHIP_EINVAL;
-  const int step = dtype == MHIP_E4M3 ? 16 : 8;
-  if (D <= 0 || D > 128 || D % step) return MHIP_EHEADDIM;
-  if (pages > 0 && (!kc || !vc || (dtype == MHIP_E4M3 && (!ks || !vs)))) return MHIP_EINVAL;
-  if (c_ss < D || c_ss * 16 * (dtype == MHIP_E4M3 ? 1 : 2) >= (int64_t(1) << 30)) return MHIP_EUNSUPPORTED;
+  if (D <= 0 || D > 128 || row_bytes(dtype, D) % 16 || (dtype == MHIP_E2M1 && D % 32)) return MHIP_EHEADDIM;
+  const bool scaled = dtype != MHIP_BF16;
+  const int size = scaled ? 1 : 2, step = 16 / size;
+  if (pages > 0 && (!kc || !vc || (scaled && (!ks || !vs)))) return MHIP_EINVAL;
+  if (c_ss < row_bytes(dtype, D) / size || c_ss >= (int64_t(1) << 30) / 16 / size) return MHIP_EUNSUPPORTED;
   if (!aligned16(kc) || !aligned16(vc) || !mult(c_sp, step) || !mult(c_ss, step) || !mult(c_sh, step)) return MHIP_EALIGN;
-  if (dtype == MHIP_E4M3 && ((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & 3u)) return MHIP_EALIGN;
+  if (scaled && ((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & 3u)) return MHIP_EALIGN;
   return MHIP_OK;
 }
 
@@ -243,7 +273,7 @@ int paged_geometry(PagedGeom& g, const int* table, const int* lengths, const int
 
 using namespace mhip;
 
-extern "C" int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+extern "C" int mhip_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_cache, void* k_scales, void* v_scales,
                                       const int* page_table, const int* lengths, const int* starts,
                                       int B, int n, int T, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
                                       int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t v_sb, int64_t v_ss, int64_t v_sh,
@@ -272,17 +302,18 @@ extern "C" int mhip_paged_cache_write(const void* k, const void* v, void* k_cach
   p.by_head = Divisor(Hkv); p.by_new = Divisor(n);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks), block(256);
-  if (dtype == MHIP_E4M3) {
-    if (wide) hipLaunchKernelGGL((paged_write_kernel<true, 16>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((paged_write_kernel<true, 8>), grid, block, 0, st, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((paged_write_kernel<false, 16>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((paged_write_kernel<false, 8>), grid, block, 0, st, p);
-  }
+  auto launch = [&](auto type) {
+    constexpr int T = decltype(type)::value;
+    if (wide) hipLaunchKernelGGL((paged_write_kernel<T, 16>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_write_kernel<T, 8>), grid, block, 0, st, p);
+  };
+  if (dtype == MHIP_E2M1) launch(std::integral_constant<int, MHIP_E2M1>{});
+  else if (dtype == MHIP_E4M3) launch(std::integral_constant<int, MHIP_E4M3>{});
+  else launch(std::integral_constant<int, MHIP_BF16>{});
   return launch_status();
 }
 
-extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
                                      const int* page_table, const int* lengths, void* out,
                                      int B, int begin, int rows, int Hkv, int D, int pages, int page_size, int table_pages, int64_t t_sb,
                                      int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
@@ -313,8 +344,9 @@ extern "C" int mhip_paged_cache_read(const void* k_cache, const void* v_cache, c
   auto launch = [&](auto lanes, auto past) {
     constexpr int L = decltype(lanes)::value;
     constexpr bool O = decltype(past)::value;
-    if (dtype == MHIP_E4M3) hipLaunchKernelGGL((paged_read_kernel<true, L, O>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((paged_read_kernel<false, L, O>), grid, block, 0, st, p);
+    if (dtype == MHIP_E2M1) hipLaunchKernelGGL((paged_read_kernel<MHIP_E2M1, L, O>), grid, block, 0, st, p);
+    else if (dtype == MHIP_E4M3) hipLaunchKernelGGL((paged_read_kernel<MHIP_E4M3, L, O>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_read_kernel<MHIP_BF16, L, O>), grid, block, 0, st, p);
   };
   using std::integral_constant;
   if (wide && once) launch(integral_constant<int, 16>{}, std::true_type{});

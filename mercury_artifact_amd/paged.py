@@ -3,7 +3,9 @@
 The ring steps take a rank's K/V as dense ``(2, B, S, Hkv, D)`` chunks, every sequence of one length.  Sequences that grow
 token by token, each at its own length, lie in pages instead: ``cache`` is ``(2, pages, page_size, Hkv, D)`` -- keys and
 values, as in a chunk -- in bfloat16, or in float8_e4m3fn with one float32 scale for each row, ``scales``
-``(2, pages, page_size, Hkv)``; ``page_table`` ``(B, pages of a sequence)`` and ``lengths`` ``(B,)`` (int32, on the GPU) say
+``(2, pages, page_size, Hkv)``, or in float4_e2m1fn_x2, two columns to an element (the even one in its low half), so that the last
+dimension is D / 2, with a float8_e8m0fnu scale for each 32 columns, ``scales`` ``(2, pages, page_size, Hkv, 4)`` whatever D is;
+``page_table`` ``(B, pages of a sequence)`` and ``lengths`` ``(B,)`` (int32, on the GPU) say
 where a sequence's tokens lie and how many there are.  An entry outside ``[0, pages)`` is a page that is not here.  A rank
 that holds some pages of a sequence attends over those alone, and the ranks' ``(out, lse)`` merge as the results of
 different chunks do (``merge_many``, ``update_out_and_lse``).
@@ -29,13 +31,19 @@ __all__ = ["paged_cache", "paged_cache_write", "paged_cache_read", "paged_attn_f
 
 def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
                 device="cuda") -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """An empty cache ``(2, pages, page_size, kv_heads, head_dim)`` and, for float8_e4m3fn, its scales.  In memory the rows
-    of one head of a page lie together, which is how attention reads them; the operators take any other order too."""
-    if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
-        raise RuntimeError("a paged cache is bfloat16 or float8_e4m3fn")
-    cache = torch.empty((2, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device).transpose(2, 3)
+    """An empty cache ``(2, pages, page_size, kv_heads, head_dim)`` (float4_e2m1fn_x2: head_dim / 2) and, in 8 or 4 bits, its
+    scales.  In memory the rows of one head of a page lie together, which is how attention reads them; the operators take any
+    other order too."""
+    if dtype not in (torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+        raise RuntimeError("a paged cache is bfloat16 or float8_e4m3fn or float4_e2m1fn_x2")
+    four = dtype == torch.float4_e2m1fn_x2
+    if four and head_dim % 32:
+        raise RuntimeError(f"a float4_e2m1fn_x2 cache has a multiple of 32 columns, not {head_dim}")
+    cache = torch.empty((2, pages, kv_heads, page_size, head_dim // 2 if four else head_dim), dtype=dtype, device=device).transpose(2, 3)
     if dtype == torch.bfloat16:
         return cache, None
+    if four:
+        return cache, torch.empty((2, pages, kv_heads, page_size, 4), dtype=torch.float8_e8m0fnu, device=device).transpose(2, 3)
     return cache, torch.empty((2, pages, kv_heads, page_size), dtype=torch.float32, device=device).transpose(2, 3)
 
 
@@ -56,8 +64,13 @@ def _check_cache(cache, scales, page_table, lengths, starts=None):
     if cache.dtype == torch.float8_e4m3fn:
         if scales is None or scales.shape != cache.shape[:-1] or scales.dtype != torch.float32:
             raise RuntimeError(f"a float8_e4m3fn cache needs float32 scales {tuple(cache.shape[:-1])}")
+    elif cache.dtype == torch.float4_e2m1fn_x2:
+        if scales is None or scales.shape != (*cache.shape[:-1], 4) or scales.dtype != torch.float8_e8m0fnu:
+            raise RuntimeError(f"a float4_e2m1fn_x2 cache needs float8_e8m0fnu scales {(*cache.shape[:-1], 4)}")
+        if scales.stride(-1) != 1 or any(x % 4 for x in scales.stride()[:4]):
+            raise RuntimeError("the four scales of a row must lie together, on 4 bytes")
     elif cache.dtype != torch.bfloat16:
-        raise RuntimeError(f"unsupported cache dtype {cache.dtype}: bfloat16 or float8_e4m3fn")
+        raise RuntimeError(f"unsupported cache dtype {cache.dtype}: bfloat16 or float8_e4m3fn or float4_e2m1fn_x2")
     elif scales is not None:
         raise RuntimeError("a bfloat16 cache has no scales")
     B = lengths.shape[0] if lengths.dim() == 1 else -1
@@ -75,6 +88,12 @@ def _check_cache(cache, scales, page_table, lengths, starts=None):
         if t is not None and t.device != cache.device:
             raise RuntimeError("cache, scales, page_table, lengths and starts must be on one device")
     return B
+
+
+def _sizes(cache):
+    """Pages, rows of a page, K/V heads, columns."""
+    _, pages, page_size, Hkv, D = cache.shape
+    return pages, page_size, Hkv, 2 * D if cache.dtype == torch.float4_e2m1fn_x2 else D
 
 
 def _check_tokens(name, t, B, starts, heads, head_dim, device):
@@ -110,25 +129,27 @@ def _cache_args(cache, scales):
     k, v = cache.data_ptr(), cache.data_ptr() + cache.stride(0) * size if cache.numel() else cache.data_ptr()
     if scales is None:
         return (k, v, None, None), (*cache.stride()[1:4], 0, 0, 0)
-    ks = scales.data_ptr()
-    return (k, v, ks, ks + scales.stride(0) * 4 if scales.numel() else ks), (*cache.stride()[1:4], *scales.stride()[1:])
+    ks, each = scales.data_ptr(), 4 // scales.element_size()             # (strides of four bytes: a float, or a row of four)
+    strides = [x // each for x in scales.stride()[:4]]
+    return (k, v, ks, ks + strides[0] * 4 if scales.numel() else ks), (*cache.stride()[1:4], *strides[1:])
 
 
 def _dtype(cache):
-    return N.MHIP_BF16 if cache.dtype == torch.bfloat16 else N.MHIP_E4M3
+    return {torch.bfloat16: N.MHIP_BF16, torch.float8_e4m3fn: N.MHIP_E4M3, torch.float4_e2m1fn_x2: N.MHIP_E2M1}[cache.dtype]
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                       scales: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None) -> None:
     """The keys and values of the new tokens (bfloat16) into their rows of the cache.  In e4m3 each row gets a scale of its
     own, the least power of two that keeps its largest value within 448; a row with an infinity or a NaN gets the scale NaN
-    and reads back as NaN.  Rows of pages that are not here are dropped.  No two new tokens of a call may lie in one row
+    and reads back as NaN.  In e2m1 the same goes for each 32 columns, whose largest value is kept within 6 (values past 6 * 2^125
+    count as that).  Rows of pages that are not here are dropped.  No two new tokens of a call may lie in one row
     (sequences that share the page they write to)."""
     if N.host.paged_cache_write(k, v, cache, page_table, lengths, scales, starts):
         return
     _check_plain(k=k, v=v, cache=cache, scales=scales)
     B = _check_cache(cache, scales, page_table, lengths, starts)
-    _, pages, page_size, Hkv, D = cache.shape
+    pages, page_size, Hkv, D = _sizes(cache)
     n, T = _check_tokens("k", k, B, starts, Hkv, D, cache.device)
     _check_tokens("v", v, B, starts, Hkv, D, cache.device)
     if k.shape != v.shape:
@@ -152,7 +173,7 @@ def paged_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: tor
         return done
     _check_plain(cache=cache, scales=scales, out=out)
     B = _check_cache(cache, scales, page_table, lengths)
-    _, pages, page_size, Hkv, D = cache.shape
+    pages, page_size, Hkv, D = _sizes(cache)
     rows, begin = _whole("rows", rows), _whole("begin", begin)
     if out is None:
         out = torch.empty((2, B, rows, Hkv, D), dtype=torch.bfloat16, device=cache.device)
@@ -177,14 +198,14 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     of them.  Rows that see no key get 0 and -inf.  ``most_new``: with ``starts``, about how many new tokens a sequence has at
     most (default: all of them in one).  Results are right whatever it says; it chooses the form of the kernels, and those round
     differently.  With up to 16 rows (new tokens times query heads of a K/V head) the values' weights are carried as two bfloat16
-    numbers, with more they are rounded to bfloat16 once; with up to 64 rows the scales of a cache are applied in float32, with more
+    numbers (not over a cache in e2m1), with more they are rounded to bfloat16 once; with up to 64 rows the scales of a cache are applied in float32, with more
     a row times its scale is rounded to bfloat16, which is exact for powers of two.  ``out`` may be q itself."""
     done = N.host.paged_attn_fwd(q, cache, page_table, lengths, softmax_scale, causal, scales, starts, most_new, out, lse)
     if done is not None:
         return done
     _check_plain(q=q, cache=cache, scales=scales, out=out, lse=lse)
     B = _check_cache(cache, scales, page_table, lengths, starts)
-    _, pages, page_size, Hkv, D = cache.shape
+    pages, page_size, Hkv, D = _sizes(cache)
     Hq = q.shape[-2] if q.dim() >= 2 else 0
     n, T = _check_tokens("q", q, B, starts, Hq, D, cache.device)
     if Hkv == 0 or Hq == 0 or Hq % Hkv != 0:

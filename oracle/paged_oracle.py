@@ -99,3 +99,59 @@ def paged_attention(q, cache, table, lengths, scale, causal=True, scales=None, s
                 lse_off[h, i] = delta + sums + abs(lse[h, i].item()) * 2.0 ** -22
         got.append((out, lse, out_off, lse_off))
     return got
+
+
+# The columns of a row in e2m1, 32 at a time: code c stands for E2M1[c % 8], negative from 8 on, times 2^(byte - 127).
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def quantise_block(x: torch.Tensor):
+    """(codes, byte of the scale) of 32 columns: the least power of two from 2^-126 to 2^125 with max|x| <= 6 s."""
+    x = x.double()
+    if not torch.isfinite(x).all():
+        return [0] * x.numel(), 255
+    top, e = x.abs().max().item(), 0
+    if top > 0:
+        e = -126
+        while top > 6 * 2.0 ** e and e < 125:
+            e += 1
+    codes = []
+    for v in x.tolist():
+        y = abs(v) / 2.0 ** e
+        # the nearest, of two equally near the even code, and nothing beyond 6
+        best = min(range(8), key=lambda c: (abs(E2M1[c] - y), c % 2))
+        codes.append(best + (8 if math.copysign(1.0, v) < 0 else 0))
+    return codes, e + 127
+
+
+def quantise_e2m1(x: torch.Tensor):
+    """A row of D columns as D / 2 bytes of two codes and D / 32 bytes of scales."""
+    codes, scales = [], []
+    for block in x.view(-1, 32):
+        c, s = quantise_block(block)
+        codes += c
+        scales.append(s)
+    return torch.tensor([lo + 16 * hi for lo, hi in zip(codes[::2], codes[1::2])], dtype=torch.uint8), torch.tensor(scales, dtype=torch.uint8)
+
+
+def e2m1_values(codes: torch.Tensor, scales: torch.Tensor):
+    """What bytes (..., D / 2) and scales (..., 4) stand for, (..., D) in 64 bits."""
+    table = torch.tensor([*E2M1, *(-v for v in E2M1)], dtype=torch.float64)
+    x = torch.stack([table[(codes % 16).long()], table[(codes // 16).long()]], -1).flatten(-2)
+    power = torch.where(scales == 255, math.nan, torch.exp2(scales.double() - 127))
+    return x * power.repeat_interleave(32, -1)[..., :x.shape[-1]]
+
+
+def paged_write_e2m1(k, v, codes, scales, table, lengths, starts=None):
+    """In place, on CPU tensors of bytes (2, pages, page, Hkv, D / 2) and (2, pages, page, Hkv, 4)."""
+    pages, page = codes.shape[1:3]
+    for b, length in enumerate(lengths):
+        for half, x in ((0, tokens_of(b, k, starts)), (1, tokens_of(b, v, starts))):
+            for i in range(x.shape[0]):
+                j = length - x.shape[0] + i
+                if j < 0 or not 0 <= table[b][j // page] < pages:
+                    continue
+                for h in range(x.shape[1]):
+                    row, scale = quantise_e2m1(x[i, h])
+                    codes[half, table[b][j // page], j % page, h] = row
+                    scales[half, table[b][j // page], j % page, h, :scale.numel()] = scale
