@@ -56,7 +56,7 @@ extern "C" {
  * 9: mhip_attn_bwd_take.
  * 10: mhip_attn_fwd_tile, mhip_attn_bwd_chunks_plan.
  * 11: mhip_paged_cache_write, mhip_paged_cache_read, mhip_paged_attn_workspace_bytes, mhip_paged_attn_fwd.
- * 12: a paged cache may be MHIP_E2M1, and its scales are passed as void*. */
+ * 12: a paged cache may be MHIP_E2M1, and its scales are passed as void*; mhip_paged_attn_weights, mhip_paged_cache_evict. */
 #define MHIP_ABI_VERSION 12
 int         mhip_abi_version(void);   /* the MHIP_ABI_VERSION the library was built with */
 int         mhip_version(void);
@@ -401,6 +401,40 @@ int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache,
                         int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
                         int64_t o_sb, int64_t o_ss, int64_t o_sh,
                         float softmax_scale, int mask, int dtype, void* workspace, void* stream);
+
+/*
+ * What attention each key has had.  weights and out: (pages, page_size, Hkv) fp32 with the element strides w_sp, w_ss, w_sh and o_sp,
+ * o_ss, o_sh; they may be one tensor, and else overlap nothing.  For every key j of a sequence whose page is here
+ *   out = decay * weights (0 for the keys of the call's new tokens) + sum of exp(softmax_scale * q k - lse)
+ * over the new tokens that see it (mask as for mhip_paged_attn_fwd) and the query heads of its K/V head; q and lse as they went into
+ * and came out of mhip_paged_attn_fwd, or an lse merged over the parts of a sequence.  Rows with lse = -inf weigh nothing.  A
+ * sequence without new tokens keeps its weights.  decay: 0 (weights are not read then) or a finite positive number.  Entries that belong
+ * to no key stay as they are.  most_new as for mhip_paged_attn_fwd.
+ */
+int mhip_paged_attn_weights(const void* q, const void* k_cache, const void* k_scales, const int* page_table, const int* lengths,
+                            const int* starts, const float* lse, const float* weights, float* out,
+                            int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
+                            int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                            int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                            int64_t w_sp, int64_t w_ss, int64_t w_sh, int64_t o_sp, int64_t o_ss, int64_t o_sh,
+                            float softmax_scale, float decay, int mask, int dtype, void* stream);
+
+/*
+ * Sequences of more than `limit` tokens cut to `keep` (0 <= recent <= keep <= limit): each K/V head keeps the keys of the `recent` last
+ * tokens and, of the others, the keep - recent with the largest weights (NaN above all, of equal ones the first), in their order, in
+ * rows 0 .. keep - 1 of the sequence; its values, scales and weights go with them.  kept (B, Hkv, limit) gets their
+ * old positions and -1 behind them, left (B) the numbers of tokens; lengths is not written.  Shorter sequences keep all tokens, and a
+ * sequence of which some page is not here stays as it is (left its length, kept -1).  out_table NULL: in the sequences' own pages,
+ * which no two sequences may share.  Else out_table (B, out_pages), stride ot_sb, names the pages that all kept rows go to, also those
+ * of sequences that are not cut; out_pages * page_size >= limit, none of them may be in page_table up to a sequence's length,
+ * and rows of entries outside [0, pages) are dropped.  weights as for mhip_paged_attn_weights.
+ */
+int mhip_paged_cache_evict(void* k_cache, void* v_cache, void* k_scales, void* v_scales, const int* page_table, const int* out_table,
+                           const int* lengths, float* weights, int* kept, int* left,
+                           int B, int Hkv, int D, int pages, int page_size, int table_pages, int out_pages,
+                           int64_t t_sb, int64_t ot_sb, int keep, int recent, int limit,
+                           int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
+                           int64_t w_sp, int64_t w_ss, int64_t w_sh, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

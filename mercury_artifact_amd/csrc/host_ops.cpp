@@ -44,6 +44,8 @@ struct Entry {
   decltype(&mhip_paged_cache_read) paged_read = nullptr;
   decltype(&mhip_paged_attn_workspace_bytes) paged_bytes = nullptr;
   decltype(&mhip_paged_attn_fwd) paged_attn = nullptr;
+  decltype(&mhip_paged_attn_weights) paged_weights = nullptr;
+  decltype(&mhip_paged_cache_evict) paged_evict = nullptr;
   decltype(&mhip_error_string) error_string = nullptr;
 } entry;
 bool bound = false;
@@ -894,6 +896,101 @@ PyObject* paged_attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// A number that a Python int or float holds; false for anything else.
+bool number(PyObject* o, double& x) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  x = PyFloat_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return true;
+}
+// A whole number from 0 on that a C int holds.
+bool whole(PyObject* o, int64_t& x) {
+  if (!PyLong_CheckExact(o)) return false;
+  x = PyLong_AsLong(o);
+  if (x == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return x >= 0 && x <= INT32_MAX;
+}
+// What attention keys have had: (pages, page_size, Hkv) in fp32.
+bool weights_of(const Tensor* t, const Paged& g) {
+  return t && t->device() == g.cache->device() && t->scalar_type() == at::kFloat && shape3(*t, g.pages, g.page, g.Hkv) && !differentiated(*t);
+}
+
+// (q, cache, page_table, lengths, softmax_scale, lse, weights, causal, scales, starts, most_new, decay, out) -> out
+PyObject* paged_attn_weights(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ENTER(13);
+  Paged g;
+  const Tensor* q = plain(a[0]);
+  if (!q || q->dim() < 3 || !g.take(a[1], a[2], a[3], a[8], a[9])) SLOW;
+  const int64_t Hq = q->size(q->dim() - 2);
+  int64_t n, T;
+  if (!g.tokens(*q, Hq, n, T) || Hq == 0 || g.Hkv == 0 || Hq % g.Hkv) SLOW;
+  double scale, decay;
+  const int causal = PyObject_IsTrue(a[7]);
+  if (causal < 0) { PyErr_Clear(); SLOW; }
+  if (!number(a[4], scale) || !number(a[11], decay)) SLOW;
+  int64_t most = g.starts ? T : n, given;
+  if (g.starts && a[10] != Py_None) {
+    if (!whole(a[10], given)) SLOW;
+    if (given < most) most = given;
+  }
+  const Tensor *lse = plain(a[5]), *weights = plain(a[6]), *out = weights;
+  if (!lse || lse->device() != q->device() || lse->scalar_type() != at::kFloat || !lse->is_contiguous() || differentiated(*lse) ||
+      !(g.starts ? lse->dim() == 2 && lse->size(0) == Hq && lse->size(1) == T : shape3(*lse, g.B, Hq, n)))
+    SLOW;
+  if (a[12] != Py_None) out = plain(a[12]);
+  if (!weights_of(weights, g) || !weights_of(out, g)) SLOW;
+  OnDevice on(*q);
+  if (!on.current) SLOW;
+  const int code = without_gil([&] {
+    return entry.paged_weights(q->data_ptr(), g.k, g.ks, static_cast<const int*>(g.table->data_ptr()), static_cast<const int*>(g.lengths->data_ptr()),
+                               static_cast<const int*>(data(g.starts)), floats(lse), floats(weights), floats(out), g.B, n, T, most, Hq, g.Hkv,
+                               g.D, g.pages, g.page, g.table->size(1), g.table->stride(0), g.stride(*q, 0), g.stride(*q, 1), g.stride(*q, 2),
+                               g.cache->stride(1), g.cache->stride(2), g.cache->stride(3), g.s_sp, g.s_ss, g.s_sh, weights->stride(0),
+                               weights->stride(1), weights->stride(2), out->stride(0), out->stride(1), out->stride(2), (float)scale,
+                               (float)decay, causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, on.stream);
+  });
+  if (code != MHIP_OK) return refused(code, "mhip_paged_attn_weights");
+  count_write(out);
+  return give(*out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache, page_table, lengths, weights, keep, recent, limit, scales, out_table) -> (kept, left)
+PyObject* paged_cache_evict(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ENTER(9);
+  Paged g;
+  if (!g.take(a[0], a[1], a[2], a[7], Py_None)) SLOW;
+  const Tensor *weights = plain(a[3]), *out_table;
+  int64_t keep, recent, limit;
+  if (!weights_of(weights, g) || !whole(a[4], keep) || !whole(a[5], recent) || !whole(a[6], limit) || recent > keep || keep > limit) SLOW;
+  if (!optional(a[8], *g.cache, out_table)) SLOW;
+  if (out_table && (out_table->dim() != 2 || out_table->size(0) != g.B || out_table->scalar_type() != at::kInt || !fits({out_table->size(1)}) ||
+                    (out_table->size(1) > 1 && out_table->stride(1) != 1) || out_table->size(1) * g.page < limit))
+    SLOW;
+  OnDevice on(*g.cache);
+  if (!on.current) SLOW;
+  Tensor kept, left;
+  const int code = without_gil([&] {
+    const auto options = g.lengths->options();
+    kept = at::empty({g.B, g.Hkv, limit}, options);
+    left = at::empty({g.B}, options);
+    return entry.paged_evict(const_cast<char*>(g.k), const_cast<char*>(g.v), g.ks, g.vs, static_cast<const int*>(g.table->data_ptr()),
+                             static_cast<const int*>(data(out_table)), static_cast<const int*>(g.lengths->data_ptr()), floats(weights),
+                             static_cast<int*>(kept.data_ptr()), static_cast<int*>(left.data_ptr()), g.B, g.Hkv, g.D, g.pages, g.page,
+                             g.table->size(1), out_table ? out_table->size(1) : 0, g.table->stride(0), out_table ? out_table->stride(0) : 0,
+                             keep, recent, limit, g.cache->stride(1), g.cache->stride(2), g.cache->stride(3), g.s_sp, g.s_ss, g.s_sh,
+                             weights->stride(0), weights->stride(1), weights->stride(2), g.type, on.stream);
+  });
+  if (code != MHIP_OK) return refused(code, "mhip_paged_cache_evict");
+  count_write(g.cache);
+  count_write(g.scales);
+  count_write(weights);
+  return give2(kept, left);
+  END_HANDLE_TH_ERRORS
+}
+
 // ({name: address}) of the library's entry points
 PyObject* bind(PyObject*, PyObject* table) {
   auto get = [&](const char* name) -> void* {
@@ -912,6 +1009,7 @@ PyObject* bind(PyObject*, PyObject* table) {
                   take(entry.quantize, "mhip_quantize_e4m3") &&
                   take(entry.paged_write, "mhip_paged_cache_write") && take(entry.paged_read, "mhip_paged_cache_read") &&
                   take(entry.paged_bytes, "mhip_paged_attn_workspace_bytes") && take(entry.paged_attn, "mhip_paged_attn_fwd") &&
+                  take(entry.paged_weights, "mhip_paged_attn_weights") && take(entry.paged_evict, "mhip_paged_cache_evict") &&
                   take(entry.error_string, "mhip_error_string");
   if (PyErr_Occurred()) return nullptr;
   bound = ok;
@@ -922,7 +1020,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 PyMethodDef methods[] = {
     FAST(undispatched), FAST(written), FAST(apart), FAST(rows_fit), FAST(fwd_block), FAST(fwd_group), FAST(fwd_chain), FAST(fwd_blocks), FAST(no_dropout), FAST(bwd_block),
     FAST(bwd_chunk), FAST(bwd_group), FAST(bwd_chunks), FAST(merge_into), FAST(merge_many), FAST(pack_block), FAST(unpack_into), FAST(quantize_e4m3),
-    FAST(paged_cache_write), FAST(paged_cache_read), FAST(paged_attn_fwd),
+    FAST(paged_cache_write), FAST(paged_cache_read), FAST(paged_attn_fwd), FAST(paged_attn_weights), FAST(paged_cache_evict),
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mercury_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -28,6 +28,10 @@ struct PagedSeq { int start, n, len; };
 __device__ __forceinline__ int uniform_load(const int* p, int64_t i) {
   return ((__attribute__((address_space(4))) const int*)(uintptr_t)p)[i];
 }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
 __device__ __forceinline__ int clamped(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
 
 template <bool UNIFORM>
@@ -61,6 +65,13 @@ __device__ __forceinline__ int paged_owner(const PagedGeom& g, int t, int lane) 
 // Bytes of a row of the cache, and four fp4 scales of a row, a byte each: that of 32 columns as an fp32 power of two, exact from 2^-126 on.
 constexpr int row_bytes(int type, int D) { return type == MHIP_BF16 ? 2 * D : type == MHIP_E4M3 ? D : D / 2; }
 __device__ __forceinline__ float e8m0(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Eight e4m3 codes as bf16, exact.
+__device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t a, uint32_t c) {
+  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
+  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true);
+  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
 
 // Eight e2m1 codes of a dword, times a scale that is a power of two, as bf16: exact while they are normal numbers there; a scale with
 // the exponent 255 makes them NaN, and one with the exponent 0 counts as 2^-127.

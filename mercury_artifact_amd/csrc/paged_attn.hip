@@ -186,15 +186,10 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
   typedef __attribute__((address_space(3))) const u32x2* lds_u32x2;
   typedef __attribute__((address_space(3))) const uint8_t* lds_byte;
   typedef __attribute__((address_space(3))) const f32x4* lds_f32x4;
-  auto codes_to_bf16 = [](uint32_t a, uint32_t c) -> bf16x8 {
-    const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
-    const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true);
-    return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-  };
   auto read_v = [&](int db, int stage_at) -> bf16x8 {
     if constexpr (E4M3) {
       const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(uintptr_t)(uint32_t)(v_a[db] + stage_at));
-      return codes_to_bf16((uint32_t)c[0], (uint32_t)c[1]);
+      return e4m3_to_bf16((uint32_t)c[0], (uint32_t)c[1]);
     } else {
       const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + stage_at));
       const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4)(uintptr_t)(uint32_t)(v_a[db] + stage_at + 16 * ROWB));
@@ -344,7 +339,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
             const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
 #pragma unroll
             for (int e = 0; e < KB / KR; ++e) {
-              const bf16x8 kf = E4M3 ? codes_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
+              const bf16x8 kf = E4M3 ? e4m3_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
               const int ks = E4M3 ? 2 * i + e : i;
 #pragma unroll
               for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);

@@ -32,11 +32,6 @@ struct PagedAttn {
   int few_rows;                            // sequences of up to so many rows are paged_attn_few's, the others paged_attn_chunk's
 };
 
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
-}
-
 // Values that are no numbers, in a tile of which some rows do not see some keys: 0 * NaN would reach rows that do not see the key.
 // They are zeros in the product with P then, and a product of odd_marks with seen_marks counts for every row and column how many
 // it sees of each kind: +inf in ones, -inf in 128s, NaN in 16384s (at most 64 keys; all of it exact).

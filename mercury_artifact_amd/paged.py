@@ -1,4 +1,5 @@
-"""A paged K/V cache: new tokens written into it, rows of it read back as a chunk, attention of new tokens over it.
+"""A paged K/V cache: new tokens written into it, rows of it read back as a chunk, attention of new tokens over it, and the keys
+that had least of it evicted.
 
 The ring steps take a rank's K/V as dense ``(2, B, S, Hkv, D)`` chunks, every sequence of one length.  Sequences that grow
 token by token, each at its own length, lie in pages instead: ``cache`` is ``(2, pages, page_size, Hkv, D)`` -- keys and
@@ -13,6 +14,7 @@ different chunks do (``merge_many``, ``update_out_and_lse``).
 New tokens come as ``(B, n, heads, D)``, or packed as ``(T, heads, D)`` with ``starts`` ``(B + 1,)``: rows ``starts[b]`` up to
 ``starts[b + 1]`` belong to sequence b, rows outside of all are left alone.  They are the last ones of their sequence:
 ``lengths`` counts them.  Nothing here waits for the GPU or looks at the values of tables, lengths and starts on the host.
+A step of generation within a budget: ``paged_cache_write``, ``paged_attn_fwd``, ``paged_attn_weights``, ``paged_cache_evict``.
 They compute no gradients, and refuse tensors that require one unless ``torch.no_grad()`` is on; nor do they take fake tensors.  The reference has no counterpart;
 an operator that is asked for something it does not do raises ``RuntimeError``.
 """
@@ -26,7 +28,7 @@ from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _native as N
 
-__all__ = ["paged_cache", "paged_cache_write", "paged_cache_read", "paged_attn_fwd"]
+__all__ = ["paged_cache", "paged_weights", "paged_cache_write", "paged_cache_read", "paged_attn_fwd", "paged_attn_weights", "paged_cache_evict"]
 
 
 def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -45,6 +47,11 @@ def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype:
     if four:
         return cache, torch.empty((2, pages, kv_heads, page_size, 4), dtype=torch.float8_e8m0fnu, device=device).transpose(2, 3)
     return cache, torch.empty((2, pages, kv_heads, page_size), dtype=torch.float32, device=device).transpose(2, 3)
+
+
+def paged_weights(pages: int, page_size: int, kv_heads: int, device="cuda") -> torch.Tensor:
+    """What attention the keys of a cache have had, ``(pages, page_size, kv_heads)`` in float32: nothing yet."""
+    return torch.zeros((pages, kv_heads, page_size), dtype=torch.float32, device=device).transpose(1, 2)
 
 
 def _check_plain(**tensors):
@@ -238,3 +245,91 @@ def paged_attn_fwd(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     N.check(code, "mhip_paged_attn_fwd")
     N.host.written(out, lse)
     return out, lse
+
+
+def _check_weights(name, t, cache):
+    N.require_cuda(t)
+    if t.shape != cache.shape[1:4] or t.dtype != torch.float32 or t.device != cache.device:
+        raise RuntimeError(f"{name} must be float32 {tuple(cache.shape[1:4])}, on the cache's device")
+
+
+def paged_attn_weights(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, softmax_scale: float,
+                       lse: torch.Tensor, weights: torch.Tensor, causal: bool = True, scales: Optional[torch.Tensor] = None,
+                       starts: Optional[torch.Tensor] = None, most_new: Optional[int] = None, decay: float = 1.0,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What attention each key has had: ``weights`` ``(pages, page_size, Hkv)`` in float32 become ``decay`` times what they were --
+    nothing for the keys of the new tokens -- plus the key's weight in the attention of every new token that sees it, summed over the
+    query heads of its K/V head.  ``q``, ``lse`` and the other arguments are those of ``paged_attn_fwd``; ``lse`` may be merged over the
+    ranks that hold parts of a sequence.  Rows whose ``lse`` is -inf weigh nothing, sequences without new tokens keep their weights, and
+    entries that belong to no key are left as they are.  ``out``: takes the results in place of ``weights`` (and is returned)."""
+    done = N.host.paged_attn_weights(q, cache, page_table, lengths, softmax_scale, lse, weights, causal, scales, starts, most_new, decay, out)
+    if done is not None:
+        return done
+    _check_plain(q=q, cache=cache, scales=scales, lse=lse, weights=weights, out=out)
+    B = _check_cache(cache, scales, page_table, lengths, starts)
+    pages, page_size, Hkv, D = _sizes(cache)
+    Hq = q.shape[-2] if q.dim() >= 2 else 0
+    n, T = _check_tokens("q", q, B, starts, Hq, D, cache.device)
+    if Hkv == 0 or Hq == 0 or Hq % Hkv != 0:
+        raise RuntimeError("number of query heads must be a multiple of the number of KV heads")
+    shape = (B, Hq, n) if starts is None else (Hq, T)
+    N.require_cuda(lse)
+    if lse.shape != shape or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != cache.device:
+        raise RuntimeError(f"lse must be a contiguous float32 {shape} tensor on the cache's device")
+    _check_weights("weights", weights, cache)
+    if out is None:
+        out = weights
+    else:
+        _check_weights("out", out, cache)
+    most = n if starts is None else T if most_new is None else min(_whole("most_new", most_new, 63), T)
+    (k, _, ks, _), strides = _cache_args(cache, scales)
+    with torch.cuda.device(cache.device):
+        code = N.lib().mhip_paged_attn_weights(
+            N.ptr(q), k, ks, N.ptr(page_table), N.ptr(lengths), N.ptr(starts), N.ptr(lse), N.ptr(weights), N.ptr(out),
+            B, n, T, most, Hq, Hkv, D, pages, page_size, page_table.shape[1], page_table.stride(0), *_token_strides(q), *strides,
+            *weights.stride(), *out.stride(), float(softmax_scale), float(decay), N.MASK_CAUSAL if causal else N.MASK_NONE, _dtype(cache),
+            N.stream_of(cache))
+    N.check(code, "mhip_paged_attn_weights")
+    N.host.written(out)
+    return out
+
+
+def paged_cache_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0,
+                      limit: Optional[int] = None, scales: Optional[torch.Tensor] = None, out_table: Optional[torch.Tensor] = None,
+                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Sequences of more than ``limit`` (default: ``keep``) tokens are cut to ``keep``: each K/V head keeps the keys of the ``recent``
+    last tokens and, of the others, those with the largest ``weights`` (NaN above all, of equal ones the first).  They move, in their
+    order, with values, scales and weights, to the first rows of the sequence -- in its own pages, which no two sequences may share, or
+    in those of ``out_table`` ``(B, at least limit / page_size)``, where the rows of sequences that are not cut go too; no page of it
+    may hold a sequence's rows.  Returns their old positions, ``kept`` ``(B, Hkv, limit)`` in int32 with -1 behind them, and the new
+    lengths, ``left`` ``(B,)``; ``lengths`` itself is not written.  A sequence of which a page is not here is left as it is, with -1
+    in all of ``kept``."""
+    limit = keep if limit is None else limit
+    done = N.host.paged_cache_evict(cache, page_table, lengths, weights, keep, recent, limit, scales, out_table)
+    if done is not None:
+        return done
+    _check_plain(cache=cache, scales=scales, weights=weights)
+    B = _check_cache(cache, scales, page_table, lengths)
+    pages, page_size, Hkv, D = _sizes(cache)
+    _check_weights("weights", weights, cache)
+    keep, recent, limit = _whole("keep", keep), _whole("recent", recent), _whole("limit", limit)
+    if not recent <= keep <= limit:
+        raise RuntimeError(f"keep ({keep}) must be from recent ({recent}) to limit ({limit})")
+    if out_table is not None:
+        N.require_cuda(out_table)
+        if out_table.dim() != 2 or out_table.shape[0] != B or out_table.dtype != torch.int32 or (out_table.shape[1] > 1 and out_table.stride(1) != 1) or out_table.device != cache.device:
+            raise RuntimeError("out_table must be an int32 (B, pages of a sequence) tensor with contiguous rows, on the cache's device")
+        if _whole("the number of entries of out_table", out_table.shape[1]) * page_size < limit:
+            raise RuntimeError(f"out_table must have pages for {limit} rows of a sequence")
+    kept = torch.empty((B, Hkv, limit), dtype=torch.int32, device=cache.device)
+    left = torch.empty((B,), dtype=torch.int32, device=cache.device)
+    pointers, strides = _cache_args(cache, scales)
+    with torch.cuda.device(cache.device):
+        code = N.lib().mhip_paged_cache_evict(
+            *pointers, N.ptr(page_table), N.ptr(out_table), N.ptr(lengths), N.ptr(weights), N.ptr(kept), N.ptr(left),
+            B, Hkv, D, pages, page_size, page_table.shape[1], 0 if out_table is None else out_table.shape[1],
+            page_table.stride(0), 0 if out_table is None else out_table.stride(0), keep, recent, limit, *strides, *weights.stride(),
+            _dtype(cache), N.stream_of(cache))
+    N.check(code, "mhip_paged_cache_evict")
+    N.host.written(cache, scales, weights)
+    return kept, left

@@ -155,3 +155,63 @@ def paged_write_e2m1(k, v, codes, scales, table, lengths, starts=None):
                     row, scale = quantise_e2m1(x[i, h])
                     codes[half, table[b][j // page], j % page, h] = row
                     scales[half, table[b][j // page], j % page, h, :scale.numel()] = scale
+
+
+def paged_weights(q, cache, table, lengths, scale, lse, weights, causal=True, starts=None, decay=1.0):
+    """What attention each key has had, (pages, page, Hkv) in 64 bits, and how far a kernel may be off.
+
+    The bound: with scores off by delta as in paged_attention, a weight exp(s - lse) that is formed in fp32 as 2^(s c - lse c) is
+    off by delta + 2^-22 (|s| + |lse|) + 2^-21 relatively, a sum of N weights by N 2^-23 more, and decay times the old one by 2^-23."""
+    out, off = weights.double().clone(), torch.zeros(weights.shape, dtype=torch.float64)
+    pages, page = cache.shape[1:3]
+    for b, length in enumerate(lengths):
+        x, here = rows_of(cache, None, table, length, b)
+        qs = tokens_of(b, q, starts).double()
+        n, Hq, D = qs.shape
+        if n == 0:
+            continue
+        G = Hq // cache.shape[3]
+        for h in range(cache.shape[3]):
+            total, wrong = torch.zeros(length, dtype=torch.float64), torch.zeros(length, dtype=torch.float64)
+            for i in range(n):
+                sees = max(length - n + i + 1, 0) if causal else length
+                for g in range(G):
+                    row = h * G + g
+                    l = (lse[b, row, i] if starts is None else lse[row, starts[b] + i]).double().item()
+                    if l == -math.inf:
+                        continue
+                    score = x[0, :sees, h] @ qs[i, row] * scale
+                    weight = torch.exp(score - l)
+                    delta = x[0, :sees, h].abs() @ qs[i, row].abs() * scale * (D + 4) * 2.0 ** -24
+                    total[:sees] += weight
+                    wrong[:sees] += weight * (delta + 2.0 ** -22 * (score.abs() + abs(l)) + 2.0 ** -21)
+            wrong += total * n * G * 2.0 ** -23
+            for j in range(length):
+                if here[j]:
+                    at = table[b][j // page], j % page, h
+                    old = decay * weights[at].double().item() if j < length - n and decay else 0.0
+                    out[at], off[at] = old + total[j], wrong[j] + 2.0 ** -23 * abs(old + total[j].item())
+    return out, off
+
+
+def evicted(weights, table, lengths, pages, keep, recent=0, limit=None):
+    """kept[b][h], the positions that stay (None where a page is not here), and left[b]."""
+    limit = keep if limit is None else limit
+    page, Hkv = weights.shape[1:]
+    kept, left = [], []
+    for b, length in enumerate(lengths):
+        if any(not 0 <= table[b][j] < pages for j in range(-(-length // page))):
+            kept.append(None)
+            left.append(length)
+            continue
+        left.append(keep if length > limit else length)
+        kept.append([])
+        for h in range(Hkv):
+            stay = list(range(length))
+            if length > limit:
+                others = list(range(length - recent))
+                value = [weights[table[b][j // page], j % page, h].item() for j in others]
+                rank = sorted(others, key=lambda j: (0 if math.isnan(value[j]) else 1, 0.0 if math.isnan(value[j]) else -value[j], j))
+                stay = sorted(rank[:keep - recent]) + list(range(length - recent, length))
+            kept[b].append(stay)
+    return kept, left
