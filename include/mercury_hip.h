@@ -56,7 +56,8 @@ extern "C" {
  * 9: mhip_attn_bwd_take.
  * 10: mhip_attn_fwd_tile, mhip_attn_bwd_chunks_plan.
  * 11: mhip_paged_cache_write, mhip_paged_cache_read, mhip_paged_attn_workspace_bytes, mhip_paged_attn_fwd.
- * 12: a paged cache may be MHIP_E2M1, and its scales are passed as void*; mhip_paged_attn_weights, mhip_paged_cache_evict. */
+ * 12: a paged cache may be MHIP_E2M1, and its scales are passed as void*; mhip_paged_attn_weights,
+ *     mhip_paged_attn_weights_workspace_bytes, mhip_paged_cache_evict. */
 #define MHIP_ABI_VERSION 12
 int         mhip_abi_version(void);   /* the MHIP_ABI_VERSION the library was built with */
 int         mhip_version(void);
@@ -409,15 +410,18 @@ int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache,
  * over the new tokens that see it (mask as for mhip_paged_attn_fwd) and the query heads of its K/V head; q and lse as they went into
  * and came out of mhip_paged_attn_fwd, or an lse merged over the parts of a sequence.  Rows with lse = -inf weigh nothing.  A
  * sequence without new tokens keeps its weights.  decay: 0 (weights are not read then) or a finite positive number.  Entries that belong
- * to no key stay as they are.  most_new as for mhip_paged_attn_fwd.
+ * to no key stay as they are.  most_new as for mhip_paged_attn_fwd.  `workspace`: 16-byte aligned,
+ * mhip_paged_attn_weights_workspace_bytes(n, T, most_new, whether there are starts, Hq, Hkv) bytes of device memory (may be NULL where
+ * that is 0); calls that overlap in time need one each.
  */
+int64_t mhip_paged_attn_weights_workspace_bytes(int n, int T, int most_new, int packed, int Hq, int Hkv);
 int mhip_paged_attn_weights(const void* q, const void* k_cache, const void* k_scales, const int* page_table, const int* lengths,
                             const int* starts, const float* lse, const float* weights, float* out,
                             int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
                             int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                             int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
                             int64_t w_sp, int64_t w_ss, int64_t w_sh, int64_t o_sp, int64_t o_ss, int64_t o_sh,
-                            float softmax_scale, float decay, int mask, int dtype, void* stream);
+                            float softmax_scale, float decay, int mask, int dtype, void* workspace, void* stream);
 
 /*
  * Sequences of more than `limit` tokens cut to `keep` (0 <= recent <= keep <= limit): each K/V head keeps the keys of the `recent` last

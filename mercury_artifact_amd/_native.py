@@ -88,7 +88,8 @@ _SIGNATURES = {
     "mhip_paged_cache_read": (c_int, [_P] * 7 + [_I] * 8 + [_L] * 11 + [_I, _P]),
     "mhip_paged_attn_workspace_bytes": (c_int64, [_I] * 8),
     "mhip_paged_attn_fwd": (c_int, [_P] * 10 + [_I] * 10 + [_L] * 13 + [_F, _I, _I, _P, _P]),
-    "mhip_paged_attn_weights": (c_int, [_P] * 9 + [_I] * 10 + [_L] * 16 + [_F, _F, _I, _I, _P]),
+    "mhip_paged_attn_weights": (c_int, [_P] * 9 + [_I] * 10 + [_L] * 16 + [_F, _F, _I, _I, _P, _P]),
+    "mhip_paged_attn_weights_workspace_bytes": (c_int64, [_I] * 6),
     "mhip_paged_cache_evict": (c_int, [_P] * 10 + [_I] * 7 + [_L] * 2 + [_I] * 3 + [_L] * 9 + [_I, _P]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -45,6 +45,7 @@ struct Entry {
   decltype(&mhip_paged_attn_workspace_bytes) paged_bytes = nullptr;
   decltype(&mhip_paged_attn_fwd) paged_attn = nullptr;
   decltype(&mhip_paged_attn_weights) paged_weights = nullptr;
+  decltype(&mhip_paged_attn_weights_workspace_bytes) paged_weights_bytes = nullptr;
   decltype(&mhip_paged_cache_evict) paged_evict = nullptr;
   decltype(&mhip_error_string) error_string = nullptr;
 } entry;
@@ -942,13 +943,16 @@ PyObject* paged_attn_weights(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (!weights_of(weights, g) || !weights_of(out, g)) SLOW;
   OnDevice on(*q);
   if (!on.current) SLOW;
+  const int64_t bytes = entry.paged_weights_bytes(n, T, most, g.starts != nullptr, Hq, g.Hkv);
+  if (bytes < 0) SLOW;
   const int code = without_gil([&] {
+    const c10::DataPtr workspace = bytes > 0 ? c10::GetAllocator(c10::kCUDA)->allocate(bytes) : c10::DataPtr();
     return entry.paged_weights(q->data_ptr(), g.k, g.ks, static_cast<const int*>(g.table->data_ptr()), static_cast<const int*>(g.lengths->data_ptr()),
                                static_cast<const int*>(data(g.starts)), floats(lse), floats(weights), floats(out), g.B, n, T, most, Hq, g.Hkv,
                                g.D, g.pages, g.page, g.table->size(1), g.table->stride(0), g.stride(*q, 0), g.stride(*q, 1), g.stride(*q, 2),
                                g.cache->stride(1), g.cache->stride(2), g.cache->stride(3), g.s_sp, g.s_ss, g.s_sh, weights->stride(0),
                                weights->stride(1), weights->stride(2), out->stride(0), out->stride(1), out->stride(2), (float)scale,
-                               (float)decay, causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, on.stream);
+                               (float)decay, causal ? MHIP_MASK_CAUSAL : MHIP_MASK_NONE, g.type, workspace.get(), on.stream);
   });
   if (code != MHIP_OK) return refused(code, "mhip_paged_attn_weights");
   count_write(out);
@@ -1009,7 +1013,8 @@ PyObject* bind(PyObject*, PyObject* table) {
                   take(entry.quantize, "mhip_quantize_e4m3") &&
                   take(entry.paged_write, "mhip_paged_cache_write") && take(entry.paged_read, "mhip_paged_cache_read") &&
                   take(entry.paged_bytes, "mhip_paged_attn_workspace_bytes") && take(entry.paged_attn, "mhip_paged_attn_fwd") &&
-                  take(entry.paged_weights, "mhip_paged_attn_weights") && take(entry.paged_evict, "mhip_paged_cache_evict") &&
+                  take(entry.paged_weights, "mhip_paged_attn_weights") &&
+                  take(entry.paged_weights_bytes, "mhip_paged_attn_weights_workspace_bytes") && take(entry.paged_evict, "mhip_paged_cache_evict") &&
                   take(entry.error_string, "mhip_error_string");
   if (PyErr_Occurred()) return nullptr;
   bound = ok;

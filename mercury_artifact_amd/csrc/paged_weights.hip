@@ -5,8 +5,16 @@
 // paged_weights_few: bound by memory, a key's row is read once.  No softmax is left to do, so keys are independent of one another: a
 // wavefront takes a run of units of 32 (bf16) or 64 keys, whose rows go from memory into registers as the B operand of S = Q K^T
 // (v_mfma_f32_16x16x32_bf16) while the queries (A) stay in registers for the run.  Lane (ln, lg) then holds rows 4 lg .. +3 of key ln: their
-// exponentials are added in the lane and over the four lane groups.  The units of all sequences are dealt out evenly to 16 wavefronts on
-// every CU, whose loads are in flight together; no LDS, no barrier, no atomics, so that results are the same in every run.
+// exponentials are added in the lane and over the four lane groups.  The units of all sequences are dealt out evenly to 16 (8 with
+// more than 16 rows) wavefronts on every CU, whose loads are in flight together; no LDS, no barrier, no atomics, so that results are the same in every run.
+//
+// paged_weights_many: for prompts, bound by the vector unit (an exponential, a multiply-add and an add for each 2 D operations of the matrix
+// unit).  Here the keys stay: a workgroup of four wavefronts holds 256 of a (sequence, K/V head), 64 to a wavefront, as the A operand of
+// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 32 queries of a head come through a ring in LDS, copied there without passing through
+// registers.  Lane (ln, lg) holds query ln, its keys' weights are added in registers, and over the lanes once in 64 tiles (which keeps
+// the sums short: 64 in a row, then 32 as a tree).  The tiles that see a key differ with the mask, so the tiles of all items are counted
+// in closed form and dealt out evenly, in order; a workgroup whose share ends inside an item leaves partial sums, and
+// paged_weights_join adds those up in their order.
 #include "paged.hpp"
 
 #include <math.h>
@@ -26,9 +34,12 @@ struct Gather {
   int Hkv, G, D, causal;
   float scale_log2, decay;
   Divisor by_group;
+  float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
 };
 
-constexpr int kWorkers = 4096;                   // wavefronts of a launch: 16 on a CU
+// Wavefronts on a SIMD: four where there are registers for them.
+template <int NR>
+constexpr int kFewWaves = NR == 1 ? 4 : 2;
 
 template <int TYPE>
 constexpr int kBlocksOf = TYPE == MHIP_BF16 ? 2 : 4;       // 16-key blocks of a unit
@@ -37,7 +48,7 @@ template <int UNIT>
 __device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) { return (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv; }
 
 template <int TYPE, int COLS, int NR>
-__global__ __launch_bounds__(256, 4) void paged_weights_few(const Gather p) {
+__global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Gather p) {
   constexpr int kBlocks = kBlocksOf<TYPE>, UNIT = 16 * kBlocks, ROWS = 16 * NR;
   constexpr bool E4M3 = TYPE == MHIP_E4M3, E2M1 = TYPE == MHIP_E2M1;
   constexpr int KB = COLS / 32, KR = E2M1 ? 1 : E4M3 ? KB / 2 : KB;      // k-steps of 32 columns, loads of a key's row
@@ -204,18 +215,294 @@ __global__ __launch_bounds__(256, 4) void paged_weights_few(const Gather p) {
   }
 }
 
+// ---- prompts -------------------------------------------------------------------------------------------------------------------
+constexpr int kKeys = 256, kQueries = 32;        // of a workgroup's item, of a step
+constexpr int kManyWorkers = 512;                // workgroups: two on a CU
+constexpr int kManyStages = 4;
+constexpr int kQueryTile = kQueries * 256, kStageBytes = kQueryTile + 4 * 256;      // rows of 256 bytes; each wavefront's copy of the rows' lse
+constexpr int kPause = 4;                        // what entering an item costs, in steps
+constexpr int kFlush = 64;                       // steps whose weights are added up in a register
+
+// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 8 k + z) on (all, without a mask),
+// so its steps are G times the rest, behind kPause.
+struct Steps {
+  int tiles, queries, G, flat, z;                // key tiles, query tiles, heads; key tiles that all query tiles see
+  int64_t all;                                   // of all key tiles
+  __device__ __forceinline__ Steps(const Gather& p, const PagedSeq& s) {
+    tiles = (s.len + kKeys - 1) / kKeys;
+    queries = (s.n + kQueries - 1) / kQueries;
+    G = p.G;
+    z = p.causal ? (s.n - s.len) >> 5 : 0;       // (floor)
+    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 3) + 1;
+    flat = flat < tiles ? flat : tiles;
+    all = before(tiles);
+  }
+  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 8 * k + z; }
+  __device__ __forceinline__ int of(int k) const { return queries > 0 ? (queries - first(k)) * G : 0; }
+  __device__ __forceinline__ int64_t before(int k) const {       // what the key tiles before k count for
+    int64_t sum = (int64_t)k * queries;
+    if (k > flat) sum -= 4 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)z * (k - flat);
+    return (queries > 0 ? sum * G : 0) + (int64_t)k * kPause;
+  }
+};
+
+// Sums over the 32 lanes of a half-wavefront of 32 registers each, lane ln with that of register ln: 31 exchanges instead of 160.
+__device__ __forceinline__ float sums_of_lanes(float (&x)[32], int ln) {
+#pragma unroll
+  for (int half = 16; half > 0; half >>= 1) {
+    const bool upper = ln & half;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float keep = upper ? x[i + half] : x[i], give = upper ? x[i] : x[i + half];
+      x[i] = keep + __shfl_xor(give, half);
+    }
+  }
+  return x[0];
+}
+
+// Where the weight of a key lies, if its page is here.
+struct Place { int page, slot; };
+__device__ __forceinline__ Place place_of(const Gather& p, int b, int key, int len) {
+  Place at{-1, 0};
+  if (key < len) at.page = p.g.table[b * p.g.t_sb + p.g.by_page.quotient(key, at.slot)];
+  if ((uint32_t)at.page >= (uint32_t)p.g.pages) at.page = -1;
+  return at;
+}
+__device__ __forceinline__ void leave(const Gather& p, const PagedSeq& s, const Place& at, int hk, int key, float sum) {
+  if (at.page < 0) return;
+  if ((s.n == 0 || p.decay != 0.f) && key < (s.n == 0 ? s.len : s.len - s.n)) {
+    const float old = p.old[(int64_t)at.page * p.w_sp + (int64_t)at.slot * p.w_ss + (int64_t)hk * p.w_sh];
+    sum += s.n == 0 ? old : p.decay * old;
+  }
+  p.out[(int64_t)at.page * p.o_sp + (int64_t)at.slot * p.o_ss + (int64_t)hk * p.o_sh] = sum;
+}
+
+template <int TYPE, int COLS>
+__global__ __launch_bounds__(256, 2) void paged_weights_many(const Gather p) {
+  constexpr int KB = COLS / 16;                  // k-steps of 16 columns
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kManyStages * kStageBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, lg = lane >> 5;
+
+  // ---- this workgroup's share ------------------------------------------------------------------------------------------------
+  const int w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int per = (p.g.B + 63) / 64;
+  int64_t mine = 0;
+  for (int j = 0; j < per; ++j)
+    if (lane * per + j < p.g.B) mine += Steps(p, paged_seq<false>(p.g, lane * per + j)).all * p.Hkv;
+  int64_t before = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t below = __shfl_up((long long)before, off);
+    if (lane >= off) before += below;
+  }
+  const int64_t total = uniform64(__shfl((long long)before, 63)), shares = total < (int64_t)gridDim.x ? total : gridDim.x;
+  before -= mine;
+  if (threadIdx.x == 0) p.shared[w * 4] = 0;
+  if (w >= shares) return;
+  int64_t lo = total * w / shares;
+  const int64_t hi = total * (w + 1) / shares;
+  const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= before && lo < before + mine));
+  int b = owner * per;
+  int64_t pos = lo - uniform64(__shfl((long long)before, owner));        // inside sequence b
+
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  int q_a[KB];                                   // Q operand (B): lane (ln, lg) reads chunk 2 ks + lg of row ln
+#pragma unroll
+  for (int ks = 0; ks < KB; ++ks) q_a[ks] = (int)lds + ln * 256 + (((2 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
+  typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8;
+  typedef __attribute__((address_space(3))) const float* lds_float;
+  float scale_log2 = p.scale_log2;
+  asm volatile("" : "+s"(scale_log2));
+
+  while (lo < hi) {
+    const PagedSeq s = paged_seq<true>(p.g, b);
+    const Steps st(p, s);
+    if (pos >= st.all * p.Hkv) {
+      pos -= st.all * p.Hkv;
+      ++b;
+      continue;
+    }
+    const int hk = (int)(pos / st.all);
+    const int64_t in_head = pos - hk * st.all;
+    int kt = 0;                                  // the last key tile that begins at or before in_head
+    for (int span = st.tiles; span > 1;) {
+      const int half = span / 2;
+      if (st.before(kt + half) <= in_head) { kt += half; span -= half; }
+      else span = half;
+    }
+    const int steps = st.of(kt), weight = steps + kPause, from = (int)(in_head - st.before(kt));
+    const int take = (int)(weight - from < hi - lo ? weight - from : hi - lo);
+    const int first = from > kPause ? from - kPause : 0, count = from + take > kPause ? from + take - kPause - first : 0;
+    const int64_t start = lo - from;             // of the item
+    lo += take;
+    pos += take;
+    const int key_at = kt * kKeys + wave * 64;   // the wavefront's first key
+    if (count == 0 && (steps > 0 || from > 0)) continue;
+
+    float total_sum = 0.f;
+    if (count > 0) {
+      // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of keys ln and 32 + ln, scaled -----------------------
+      bf16x8 kf[2][KB];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int key = key_at + kb * 32 + ln;
+        const Place at = place_of(p, b, key, s.len);
+        const uint8_t* row = p.k + ((int64_t)at.page * p.c_sp + (int64_t)at.slot * p.c_ss + (int64_t)hk * p.c_sh);
+        const float* scale = p.k_scales + ((int64_t)at.page * p.s_sp + (int64_t)at.slot * p.s_ss + (int64_t)hk * p.s_sh);
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks) {
+          const int col = ks * 16 + lg * 8;
+          kf[kb][ks] = bf16x8{};
+          if (at.page >= 0 && col < p.D) {
+            if constexpr (TYPE == MHIP_E2M1) {
+              const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + col / 2);
+              kf[kb][ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
+            } else if constexpr (TYPE == MHIP_E4M3) {
+              // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
+              const u32x2 codes = *reinterpret_cast<const u32x2*>(row + col);
+              u32x4 x;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], true);
+                x[2 * h] = pack_bf16(a[0] * *scale, a[1] * *scale);
+                x[2 * h + 1] = pack_bf16(c[0] * *scale, c[1] * *scale);
+              }
+              kf[kb][ks] = __builtin_bit_cast(bf16x8, x);
+            } else {
+              kf[kb][ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[kb][ks]));       // loaded before the first copy goes out
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();              // (the item before is through with the ring)
+
+      // ---- query tiles: step i is tile qt of head h, tiles fastest ---------------------------------------------------------------
+      const int qt0 = st.first(kt), of_head = st.queries - qt0;
+      int copy_h = first / of_head, copy_qt = first - copy_h * of_head, left = count;      // of the next copies, those that are left
+      auto copy = [&](int stage) {
+        const int head = hk * p.G + copy_h, row0 = (qt0 + copy_qt) * kQueries;
+        const uint16_t* base = p.q + b * p.q_sb + (int64_t)head * p.q_sh;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {            // (rows past the last repeat it, columns past the last are those of zeros in K)
+          const int r = wave * 8 + u * 4 + (lane >> 4), row = row0 + r < s.n ? row0 + r : s.n - 1, chunk = (lane & 15) ^ lds_row_swizzle(r);
+          copy16_to_lds(base + (int64_t)(s.start + row) * p.q_ss + (chunk * 8 < p.D ? chunk * 8 : 0), lds + stage * kStageBytes + (wave * 2 + u) * 1024);
+        }
+        const int row = row0 + ln < s.n ? row0 + ln : s.n - 1;
+        copy4_to_lds(p.lse + b * p.l_sb + (int64_t)head * p.l_sh + s.start + row, lds + stage * kStageBytes + kQueryTile + wave * 256);
+        if (left > 1) {                          // (past the share's last tile that one again)
+          --left;
+          if (++copy_qt == of_head) { copy_qt = 0; ++copy_h; }
+        }
+      };
+      int qt = qt0 + copy_qt;
+      copy(0);
+      copy(1);
+      copy(2);
+      float sum[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum[i] = 0.f;
+      const int old_keys = s.len - s.n;
+      for (int i = 0; i < count; ++i) {
+        // the copies of step i are done, by this wavefront and then by all; the stage of step i - 1 has been read by all
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        copy((i + 3) & 3);
+        const int at = (i & 3) * kStageBytes;
+        const float lse = *(lds_float)(uintptr_t)(uint32_t)(lds + at + kQueryTile + wave * 256 + ln * 4);
+        f32x16 sc[2];
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks) {
+          const bf16x8 qf = *(lds_bf16x8)(uintptr_t)(uint32_t)(q_a[ks] + at);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][ks], qf, ks == 0 ? f32x16{} : sc[kb], 0, 0, 0);
+        }
+        const int row = qt * kQueries + ln;
+        const bool counts = row < s.n && lse != -INFINITY;         // (a row that saw no key weighs nothing)
+        const float nlse = counts ? -lse * kLog2e : 0.f;
+        if ((p.causal && key_at + 63 > old_keys + qt * kQueries) || __builtin_amdgcn_ballot_w64(!counts) != 0) {
+          asm volatile("");
+          const int seen = counts ? (p.causal ? old_keys + row + 1 : s.len) - key_at - 4 * lg : 0x80000000;      // from the wavefront's first key
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (kb * 32 + 8 * (j >> 2) + (j & 3) >= seen) sc[kb][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[kb * 16 + j] += fast_exp2(__builtin_fmaf(sc[kb][j], scale_log2, nlse));
+        if (++qt == st.queries) qt = qt0;
+        if ((i & (kFlush - 1)) == kFlush - 1) {
+          total_sum += sums_of_lanes(sum, ln);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sum[e] = 0.f;
+        }
+      }
+      total_sum += sums_of_lanes(sum, ln);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // copies past the last step
+    }
+    // lane (ln, lg) has the sum of register ln: key 32 (ln / 16) + 8 (ln % 16 / 4) + 4 lg + ln % 4
+    const int own = (ln >> 4) * 32 + ((ln >> 2) & 3) * 8 + lg * 4 + (ln & 3);
+    if (count == steps) {
+      leave(p, s, place_of(p, b, key_at + own, s.len), hk, key_at + own, total_sum);
+      continue;
+    }
+    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 64 + own] = total_sum;
+    if (first == 0 && threadIdx.x == 0) {
+      const int last = (int)(((start + weight) * shares - 1) / total);           // the workgroup with its last unit
+      p.shared[w * 4 + 1] = b;
+      p.shared[w * 4 + 2] = hk;
+      p.shared[w * 4 + 3] = kt;
+      p.shared[w * 4] = last - w + 1;
+    }
+  }
+}
+
+// Items that several workgroups shared: their partial sums in order.  A workgroup for each that one may begin in, a thread for each key.
+__global__ __launch_bounds__(kKeys) void paged_weights_join(const Gather p) {
+  const int w = blockIdx.x, parts = uniform_load(p.shared, w * 4);
+  if (parts == 0) return;
+  const int b = uniform_load(p.shared, w * 4 + 1), hk = uniform_load(p.shared, w * 4 + 2), key = uniform_load(p.shared, w * 4 + 3) * kKeys + threadIdx.x;
+  const PagedSeq s = paged_seq<true>(p.g, b);
+  const Place at = place_of(p, b, key, s.len);
+  float sum = p.parts[(2 * (int64_t)w + 1) * kKeys + threadIdx.x];
+#pragma unroll 8
+  for (int i = 1; i < parts; ++i) sum += p.parts[2 * (int64_t)(w + i) * kKeys + threadIdx.x];
+  leave(p, s, at, hk, key, sum);
+}
+
+template <int TYPE>
+void launch_many(const Gather& p, hipStream_t st) {
+  if (p.D <= 64) hipLaunchKernelGGL((paged_weights_many<TYPE, 64>), dim3(kManyWorkers), dim3(256), 0, st, p);
+  else if (p.D <= 96) hipLaunchKernelGGL((paged_weights_many<TYPE, 96>), dim3(kManyWorkers), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((paged_weights_many<TYPE, 128>), dim3(kManyWorkers), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(paged_weights_join, dim3(kManyWorkers), dim3(kKeys), 0, st, p);
+}
+
+constexpr int kFewRows = 64;                     // rows of a sequence and K/V head that paged_weights_few takes
+constexpr int64_t kManyBytes = (int64_t)kManyWorkers * (2 * kKeys * 4 + 16);
+
 template <int TYPE, int COLS, int NR>
 void launch_few(const Gather& p, hipStream_t st) {
-  hipLaunchKernelGGL((paged_weights_few<TYPE, COLS, NR>), dim3(kWorkers / 4), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_weights_few<TYPE, COLS, NR>), dim3(256 * kFewWaves<NR>), dim3(256), 0, st, p);
 }
 template <int TYPE, int COLS>
 void launch_rows(const Gather& p, int64_t rows, hipStream_t st) {
   if (rows <= 16) launch_few<TYPE, COLS, 1>(p, st);
-  else launch_few<TYPE, COLS, 2>(p, st);
+  else if (rows <= 32) launch_few<TYPE, COLS, 2>(p, st);
+  else launch_few<TYPE, COLS, 4>(p, st);
 }
 template <int TYPE>
 void launch(const Gather& p, int64_t rows, hipStream_t st) {
-  if (p.D <= 64) launch_rows<TYPE, 64>(p, rows, st);
+  if (rows > kFewRows) launch_many<TYPE>(p, st);
+  else if (p.D <= 64) launch_rows<TYPE, 64>(p, rows, st);
   else launch_rows<TYPE, 128>(p, rows, st);
 }
 
@@ -224,13 +511,18 @@ void launch(const Gather& p, int64_t rows, hipStream_t st) {
 
 using namespace mhip;
 
+extern "C" int64_t mhip_paged_attn_weights_workspace_bytes(int n, int T, int most_new, int packed, int Hq, int Hkv) {
+  if (n < 0 || T < 0 || most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
+  return (int64_t)(packed ? most_new : n) * (Hq / Hkv) > kFewRows ? kManyBytes : 0;
+}
+
 extern "C" int mhip_paged_attn_weights(const void* q, const void* k_cache, const void* k_scales, const int* page_table, const int* lengths,
                                        const int* starts, const float* lse, const float* weights, float* out,
                                        int B, int n, int T, int most_new, int Hq, int Hkv, int D, int pages, int page_size, int table_pages,
                                        int64_t t_sb, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                                        int64_t c_sp, int64_t c_ss, int64_t c_sh, int64_t s_sp, int64_t s_ss, int64_t s_sh,
                                        int64_t w_sp, int64_t w_ss, int64_t w_sh, int64_t o_sp, int64_t o_ss, int64_t o_sh,
-                                       float softmax_scale, float decay, int mask, int dtype, void* stream) {
+                                       float softmax_scale, float decay, int mask, int dtype, void* workspace, void* stream) {
   Gather p{};
   if (B < 0 || n < 0 || T < 0 || most_new < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return MHIP_EINVAL;
   if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) return MHIP_EINVAL;
@@ -262,6 +554,12 @@ extern "C" int mhip_paged_attn_weights(const void* q, const void* k_cache, const
   p.decay = decay;
   p.by_group = Divisor(p.G);
   const int64_t rows = (int64_t)most_new * p.G;
+  if (rows > kFewRows) {
+    if (!workspace) return MHIP_EINVAL;
+    if (!aligned16(workspace)) return MHIP_EALIGN;
+    p.parts = static_cast<float*>(workspace);
+    p.shared = reinterpret_cast<int*>(p.parts + (int64_t)kManyWorkers * 2 * kKeys);
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == MHIP_E2M1) launch<MHIP_E2M1>(p, rows, st);
   else if (dtype == MHIP_E4M3) launch<MHIP_E4M3>(p, rows, st);

@@ -282,13 +282,17 @@ def paged_attn_weights(q: torch.Tensor, cache: torch.Tensor, page_table: torch.T
     else:
         _check_weights("out", out, cache)
     most = n if starts is None else T if most_new is None else min(_whole("most_new", most_new, 63), T)
+    size = N.lib().mhip_paged_attn_weights_workspace_bytes(n, T, most, int(starts is not None), Hq, Hkv)
+    if size < 0:
+        N.check(int(size), "mhip_paged_attn_weights_workspace_bytes")
+    workspace = torch.empty((int(size),), dtype=torch.uint8, device=q.device)
     (k, _, ks, _), strides = _cache_args(cache, scales)
     with torch.cuda.device(cache.device):
         code = N.lib().mhip_paged_attn_weights(
             N.ptr(q), k, ks, N.ptr(page_table), N.ptr(lengths), N.ptr(starts), N.ptr(lse), N.ptr(weights), N.ptr(out),
             B, n, T, most, Hq, Hkv, D, pages, page_size, page_table.shape[1], page_table.stride(0), *_token_strides(q), *strides,
             *weights.stride(), *out.stride(), float(softmax_scale), float(decay), N.MASK_CAUSAL if causal else N.MASK_NONE, _dtype(cache),
-            N.stream_of(cache))
+            N.ptr(workspace), N.stream_of(cache))
     N.check(code, "mhip_paged_attn_weights")
     N.host.written(out)
     return out

@@ -22,11 +22,12 @@ def _cache(Hkv, D, page):
 
 
 def _weigh(lib, q=P, kc=P, ks=P, table=P, lengths=P, starts=None, lse=P, w=P, out=P, B=2, n=3, T=0, most=3, Hq=4, Hkv=2, D=64, pages=9, page=16,
-           width=4, tokens=None, cache=None, scale=0.1, decay=1.0, mask=1, dtype=0):
+           width=4, tokens=None, cache=None, scale=0.1, decay=1.0, mask=1, dtype=0,
+           ws=P):
     tokens = (n * Hq * D, Hq * D, D) if tokens is None else tokens
     at = (Hkv * page, 1, page)
     return lib.mhip_paged_attn_weights(q, kc, ks, table, lengths, starts, lse, w, out, B, n, T, most, Hq, Hkv, D, pages, page, width, width,
-                                       *tokens, *(_cache(max(Hkv, 1), D, page) if cache is None else cache), *at, *at, scale, decay, mask, dtype, None)
+                                       *tokens, *(_cache(max(Hkv, 1), D, page) if cache is None else cache), *at, *at, scale, decay, mask, dtype, ws, None)
 
 
 def _evict(lib, kc=P, vc=P, ks=P, vs=P, table=P, out_table=None, lengths=P, w=P, kept=P, left=P, B=2, Hkv=2, D=64, pages=9, page=16, width=4,
@@ -81,6 +82,12 @@ def test_weights_refuse(lib):
     assert _weigh(lib, starts=P, T=1 << 29) == EUNSUPPORTED
     assert _weigh(lib, B=1 << 16, n=1 << 16) == EUNSUPPORTED
     assert _weigh(lib, width=0, table=None) == OK
+    many = dict(n=40, tokens=(40 * 4 * 64, 256, 64))
+    assert _weigh(lib, ws=None, **many) == EINVAL
+    assert _weigh(lib, ws=P + 8, **many) == EALIGN
+    size = lib.mhip_paged_attn_weights_workspace_bytes
+    assert size(1, 2, 1, 0, 4, 2) == 0 and size(40, 80, 40, 0, 4, 2) > 0 and size(0, 80, 40, 1, 4, 2) > 0 and size(0, 80, 1, 1, 4, 2) == 0
+    assert size(1, 2, 1, 0, 5, 2) == EINVAL and size(1, 2, -1, 1, 4, 2) == EINVAL
 
 
 def test_eviction_refuses(lib):
