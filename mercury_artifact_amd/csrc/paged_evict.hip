@@ -1,9 +1,9 @@
 // A paged K/V cache that stays within a budget.  A sequence of more than `limit` tokens is cut to `keep`: each K/V head keeps the keys
 // of its `recent` last tokens and, of the others, the keep - recent with the largest weights (of equal ones the first), in their order.
 //
-// paged_evict_choose: one workgroup for each (sequence, K/V head).  The weights are looked at as whole numbers that order like them: the
-//   number that the last kept one has is found eight bits at a time, by counting (the largest first), and a pass in order then
-//   leaves the positions that stay, each at its place in the result.
+// paged_evict_choose: one workgroup for each (sequence, K/V head).  The weights are looked at as whole numbers that order like them, read
+//   once and held in registers: the number that the last kept one has is found eleven bits at a time behind those that all have in
+//   common, by counting (the largest first), and a pass in order then leaves the positions that stay, each at its place in the result.
 // paged_evict_move: rows that stay, with scales and weights, to their new places.  In its own pages a row moves down or not at all, so a
 //   workgroup that reads a tile of rows whole, and then writes it, has read whatever it writes over, and rows of later tiles
 //   lie behind everything that it writes: one workgroup walks each (sequence, K/V head, half) from the first row on.  Into other
@@ -35,11 +35,181 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+constexpr int kDigits = 2048, kListed = 24576;
+struct ChooserLds {
+  uint32_t count[kDigits];
+  uint32_t waves[2][kChooserWaves];
+  uint32_t found[3];                             // the digit, how many of it are kept, and of how many
+  uint32_t listed;
+  uint32_t list[kListed];
+};
+
+// The keep - recent with the largest weights of the first `others` positions into kept, in order.  A wavefront has 64 HELD positions in a
+// row in registers.  HELD = 0: as many as there are, read anew each time, three times if all goes well: to count the first digits; to put
+// those with the digit of the last one kept into a list, their other bits and which wavefront's they are; and to leave the positions.
+// (4 x 131072 tokens to 100000, 2 heads: 237 us when every digit was counted over all, 149 so.)
+template <int HELD>
+__device__ __forceinline__ void choose(const Evict& p, ChooserLds& lds, const int* table, int hk, int others, int* kept) {
+  constexpr int kAtOnce = HELD > 0 ? HELD : 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int each = HELD > 0 ? HELD : (others + kChoosers * kAtOnce - 1) / (kChoosers * kAtOnce) * kAtOnce;
+  const int first = wave * each * 64 + lane;
+  uint32_t x[kAtOnce];
+  auto read = [&](int u0) {
+    int slot[kAtOnce], page[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int at = first + (u0 + u) * 64;
+      page[u] = table[p.g.by_page.quotient(at < others ? at : others - 1, slot[u])];
+    }
+    float w[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      w[u] = p.weights[(int64_t)page[u] * p.w_sp + (int64_t)slot[u] * p.w_ss + (int64_t)hk * p.w_sh];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) x[u] = order_of(w[u]);
+  };
+  auto all = [&](auto&& f) __attribute__((always_inline)) {              // f(position, its number, whether it is one)
+    for (int u0 = 0; u0 < each; u0 += kAtOnce) {
+      if (HELD == 0) read(u0);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) f(first + (u0 + u) * 64, x[u], first + (u0 + u) * 64 < others);
+    }
+  };
+  if (HELD > 0) read(0);
+
+  // ---- the bits that all have in common (of many they are not looked for) -----------------------------------------------------
+  uint32_t last = 0, need = p.keep - p.recent;
+  int bits = 32;                                 // that differ
+  if (HELD > 0) {
+    uint32_t high = 0, low = 0xffffffffu;
+    all([&](int, uint32_t v, bool real) {
+      high = real && v > high ? v : high;
+      low = real && v < low ? v : low;
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const uint32_t h = __shfl_xor(high, off), l = __shfl_xor(low, off);
+      high = h > high ? h : high;
+      low = l < low ? l : low;
+    }
+    if (lane == 0) {
+      lds.waves[0][wave] = high;
+      lds.waves[1][wave] = low;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kChooserWaves; ++v) {
+      high = lds.waves[0][v] > high ? lds.waves[0][v] : high;
+      low = lds.waves[1][v] < low ? lds.waves[1][v] : low;
+    }
+    bits = high == low ? 0 : 32 - __builtin_clz(high ^ low);
+    last = bits == 32 ? 0u : high >> bits << bits;
+  }
+
+  // ---- the number of the last one kept, and how many of that number are (or the number below the least kept, and none) ------------
+  bool listed = false;
+  uint32_t above = 0, equal = 0;                 // of this wavefront; listed: above the list's numbers
+  while (bits > 0) {
+    const int shift = bits > 11 ? bits - 11 : 0;
+    const uint32_t digits = (1u << (bits - shift)) - 1;
+    lds.count[tid] = lds.count[tid + kChoosers] = 0;
+    __syncthreads();
+    if (listed) {
+      for (uint32_t i = tid; i < lds.listed; i += kChoosers) {
+        const uint32_t v = lds.list[i];
+        if (((v ^ last) & 0x1fffffu) >> bits == 0) atomicAdd(&lds.count[v >> shift & digits], 1u);
+      }
+    } else {
+      all([&](int, uint32_t v, bool real) {
+        if (real && (bits == 32 || (v ^ last) >> bits == 0)) atomicAdd(&lds.count[v >> shift & digits], 1u);
+      });
+    }
+    __syncthreads();
+    // thread t has the digits 2047 - 2 t and 2046 - 2 t: how many are above them, and in which of them the last one kept is
+    const uint32_t c0 = lds.count[kDigits - 1 - 2 * tid], c1 = lds.count[kDigits - 2 - 2 * tid];
+    uint32_t higher = c0 + c1;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t v = __shfl_up(higher, off);
+      if (lane >= off) higher += v;
+    }
+    if (lane == 63) lds.waves[0][wave] = higher;
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) higher += lds.waves[0][v];
+    higher -= c0 + c1;
+    if (higher < need && need <= higher + c0 + c1) {
+      const bool upper = need <= higher + c0;
+      lds.found[0] = kDigits - 1 - 2 * tid - (upper ? 0 : 1);
+      lds.found[1] = need - higher - (upper ? 0 : c0);
+      lds.found[2] = upper ? c0 : c1;
+    }
+    if (tid == 0 && !listed) lds.listed = 0;
+    __syncthreads();
+    last |= lds.found[0] << shift;
+    need = lds.found[1];
+    bits = shift;
+    const uint32_t of = lds.found[2];
+    if (HELD > 0 && need == of && last > 0) {    // all with these digits are kept
+      --last;
+      need = 0;
+      break;
+    }
+    if (HELD == 0 && bits == 21 && of <= kListed) {
+      listed = true;
+      all([&](int, uint32_t v, bool real) {
+        const uint64_t in = __builtin_amdgcn_ballot_w64(real && v >> 21 == last >> 21);
+        above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(real && v >> 21 > last >> 21));
+        if (in == 0) return;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&lds.listed, (uint32_t)__builtin_popcountll(in));
+        at = __builtin_amdgcn_readfirstlane(at) + __builtin_popcountll(in & ((1ull << lane) - 1));
+        if (in >> lane & 1) lds.list[at] = (v & 0x1fffffu) | (uint32_t)wave << 28;
+      });
+    }
+    __syncthreads();
+  }
+
+  // ---- the positions in order: those above, and of those equal the first `need` ------------------------------------------------
+  if (listed) {
+    if (tid < kChooserWaves) lds.waves[1][tid] = 0;
+    if (lane == 0) lds.waves[0][wave] = above;
+    __syncthreads();
+    for (uint32_t i = tid; i < lds.listed; i += kChoosers) {
+      const uint32_t v = lds.list[i] & 0x1fffffu, whose = lds.list[i] >> 28;
+      if (v > (last & 0x1fffffu)) atomicAdd(&lds.waves[0][whose], 1u);
+      if (v == (last & 0x1fffffu)) atomicAdd(&lds.waves[1][whose], 1u);
+    }
+  } else {
+    all([&](int, uint32_t v, bool real) {
+      above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(real && v > last));
+      equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(real && v == last));
+    });
+    __syncthreads();
+    if (lane == 0) {
+      lds.waves[0][wave] = above;
+      lds.waves[1][wave] = equal;
+    }
+  }
+  __syncthreads();
+  above = equal = 0;
+  for (int v = 0; v < wave; ++v) {
+    above += lds.waves[0][v];
+    equal += lds.waves[1][v];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  all([&](int at, uint32_t v, bool real) {
+    const uint64_t mask_above = __builtin_amdgcn_ballot_w64(real && v > last), mask_equal = __builtin_amdgcn_ballot_w64(real && v == last);
+    const uint32_t here = above + __builtin_popcountll(mask_above & below), ties = equal + __builtin_popcountll(mask_equal & below);
+    if (real && (v > last || (v == last && ties < need))) kept[here + (ties < need ? ties : need)] = at;
+    above += __builtin_popcountll(mask_above);
+    equal += __builtin_popcountll(mask_equal);
+  });
+}
+
 __global__ __launch_bounds__(kChoosers) void paged_evict_choose(const Evict p) {
-  __shared__ uint32_t count[kChooserWaves][256];
-  __shared__ uint32_t found[2];                  // the digit, and how many of it are kept
-  __shared__ int waves[2][kChooserWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ ChooserLds lds;
+  const int tid = threadIdx.x;
   int hk;
   const int b = p.by_heads.quotient(blockIdx.x, hk);
   const int len = clamped(uniform_load(p.g.lengths, b), 0, p.g.width * p.g.page);
@@ -57,96 +227,20 @@ __global__ __launch_bounds__(kChoosers) void paged_evict_choose(const Evict p) {
     for (int i = tid; i < p.limit; i += kChoosers) kept[i] = whole && i < len ? i : -1;
     return;
   }
-  auto order_at = [&](int at) {
-    int slot;
-    const int page = table[p.g.by_page.quotient(at, slot)];
-    return order_of(p.weights[(int64_t)page * p.w_sp + (int64_t)slot * p.w_ss + (int64_t)hk * p.w_sh]);
-  };
-
-  // ---- the number of the last one kept, and how many of that number are ------------------------------------------------------
-  const int others = len - p.recent;             // (recent <= keep <= limit < len)
-  uint32_t need = p.keep - p.recent, last = 0;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < kChooserWaves * 256; i += kChoosers) (&count[0][0])[i] = 0;
-      __syncthreads();
-      for (int at = tid; at < others; at += kChoosers) {
-        const uint32_t x = order_at(at);
-        if (shift == 24 || (x ^ last) >> (shift + 8) == 0) atomicAdd(&count[wave][x >> shift & 255u], 1u);
-      }
-      __syncthreads();
-      if (tid < 256) {
-        uint32_t sum = 0;
-        for (int v = 0; v < kChooserWaves; ++v) sum += count[v][tid];
-        count[0][tid] = sum;
-      }
-      __syncthreads();
-      if (wave == 0) {
-        // lane l has the digits 255 - 4 l .. 252 - 4 l: how many are above them, and in which of them the last one kept is
-        uint32_t c[4], sum = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += c[e] = count[0][255 - 4 * lane - e];
-        uint32_t above = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const uint32_t x = __shfl_up(above, off);
-          if (lane >= off) above += x;
-        }
-        above -= sum;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (above < need && need <= above + c[e]) {
-            found[0] = 255 - 4 * lane - e;
-            found[1] = need - above;
-          }
-          above += c[e];
-        }
-      }
-      __syncthreads();
-      last |= found[0] << shift;
-      need = found[1];
-      __syncthreads();
-    }
-  }
-
-  // ---- the positions in order: those above, and of those equal the first `need` ------------------------------------------------
-  int above = 0, equal = 0;
-  if (p.keep > p.recent) {
-    for (int at0 = 0; at0 < others; at0 += kChoosers) {
-      const int at = at0 + tid;
-      const uint32_t x = at < others ? order_at(at) : 0;
-      const bool is_above = at < others && x > last, is_equal = at < others && x == last;
-      const uint64_t mask_above = __builtin_amdgcn_ballot_w64(is_above), mask_equal = __builtin_amdgcn_ballot_w64(is_equal);
-      if (lane == 0) {
-        waves[0][wave] = __builtin_popcountll(mask_above);
-        waves[1][wave] = __builtin_popcountll(mask_equal);
-      }
-      __syncthreads();
-      int here_above = above, here_equal = equal;
-      for (int v = 0; v < kChooserWaves; ++v) {
-        if (v < wave) {
-          here_above += waves[0][v];
-          here_equal += waves[1][v];
-        }
-        above += waves[0][v];
-        equal += waves[1][v];
-      }
-      const uint64_t below = (1ull << lane) - 1;
-      here_above += __builtin_popcountll(mask_above & below);
-      here_equal += __builtin_popcountll(mask_equal & below);
-      if (is_above || (is_equal && here_equal < (int)need)) kept[here_above + (here_equal < (int)need ? here_equal : (int)need)] = at;
-      __syncthreads();
-    }
-  }
-  for (int i = tid; i < p.limit - (p.keep - p.recent); i += kChoosers) kept[p.keep - p.recent + i] = i < p.recent ? others + i : -1;
+  const int others = len - p.recent, chosen = p.keep - p.recent;         // (recent <= keep <= limit < len)
+  for (int i = tid; i < p.limit - chosen; i += kChoosers) kept[chosen + i] = i < p.recent ? others + i : -1;
+  if (chosen == 0) return;
+  if (others <= 2 * kChoosers) choose<2>(p, lds, table, hk, others, kept);
+  else if (others <= 8 * kChoosers) choose<8>(p, lds, table, hk, others, kept);
+  else if (others <= 32 * kChoosers) choose<32>(p, lds, table, hk, others, kept);
+  else choose<0>(p, lds, table, hk, others, kept);
 }
 
-constexpr int kMovers = 256;
-
-// LANES lanes take a row, of up to 16 bytes each; a workgroup moves 256 / LANES rows at once and `DEEP` times as many with their loads in flight together.
-template <int LANES, int DEEP, bool APART>
-__global__ __launch_bounds__(kMovers) void paged_evict_move(const Evict p, const int tiles) {
-  constexpr int kRows = kMovers / LANES, kTile = kRows * DEEP;
+// LANES lanes take a row, of up to 16 bytes each; a workgroup moves THREADS / LANES rows at once and DEEP times as many with their loads in flight
+// together (each kind of load stands before the first that waits for one: positions, pages, rows).
+template <int LANES, int DEEP, bool APART, int THREADS>
+__global__ __launch_bounds__(THREADS, DEEP == 4 ? 8 : 4) void paged_evict_move(const Evict p, const int tiles) {
+  constexpr int kRows = THREADS / LANES, kTile = kRows * DEEP;
   const int sub = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int half = blockIdx.x & 1;
   int item = blockIdx.x >> 1, tile = 0;
@@ -162,62 +256,71 @@ __global__ __launch_bounds__(kMovers) void paged_evict_move(const Evict p, const
   const int count = left < p.limit ? left : p.limit;
   const int* table = p.g.table + b * p.g.t_sb;
   const int* to_table = APART ? p.out_table + b * p.ot_sb : table;
-  uint8_t* rows = half ? p.v : p.k;
+  uint8_t* rows = (half ? p.v : p.k) + (int64_t)hk * p.c_sh + sub * 16;
   float* scales = half ? p.v_scales : p.k_scales;
   const bool real = sub * 16 < p.row;
+  // of a row's lanes the first moves its scales, and among the keys the second (there are four) what attention it has had
+  const bool scaled = sub == 0 && scales, weighted = sub == 1 && half == 0;
+  float* word = scaled ? scales + (int64_t)hk * p.s_sh : p.weights + (int64_t)hk * p.w_sh;
+  const int64_t word_sp = scaled ? p.s_sp : p.w_sp, word_ss = scaled ? p.s_ss : p.w_ss;
 
   for (int i0 = tile * kTile; i0 < count; i0 = APART ? count : i0 + kTile) {
     const int last = i0 + kTile < count ? i0 + kTile - 1 : count - 1;
     if (!APART && kept[last] == last) continue;  // (positions rise: every row of the tile is in its place)
-    u32x4 x[DEEP];
-    float scale[DEEP], weight[DEEP];
-    int64_t to_page[DEEP];
-    int to_slot[DEEP];
+    int at[DEEP], slot[DEEP], page[DEEP], to_slot[DEEP], to_page[DEEP];
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
       const int i = i0 + u * kRows + group;
-      const int at = i < count ? kept[i] : -1;
-      to_page[u] = -1;
+      at[u] = kept[i < count ? i : count - 1];
+      to_page[u] = to_table[p.g.by_page.quotient(i < count ? i : count - 1, to_slot[u])];
+      if (i >= count) to_page[u] = -1;
+    }
+    if (at[0] < 0) break;                        // (all of them: some page of the sequence is not here)
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) page[u] = table[p.g.by_page.quotient(at[u], slot[u])];
+    u32x4 x[DEEP];
+    uint32_t y[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
       x[u] = u32x4{};
-      scale[u] = weight[u] = 0.f;
-      if (at >= 0) {
-        int slot;
-        const int64_t page = table[p.g.by_page.quotient(at, slot)];
-        const int to = to_table[p.g.by_page.quotient(i, to_slot[u])];
-        if ((uint32_t)to < (uint32_t)p.g.pages) to_page[u] = to;
-        if (real) x[u] = *reinterpret_cast<const u32x4*>(rows + page * p.c_sp + (int64_t)slot * p.c_ss + (int64_t)hk * p.c_sh + sub * 16);
-        if (sub == 0 && scales) scale[u] = scales[page * p.s_sp + (int64_t)slot * p.s_ss + (int64_t)hk * p.s_sh];
-        if (sub == 0 && half == 0) weight[u] = p.weights[page * p.w_sp + (int64_t)slot * p.w_ss + (int64_t)hk * p.w_sh];
-      }
+      y[u] = 0;
+      if (real) x[u] = *reinterpret_cast<const u32x4*>(rows + (int64_t)page[u] * p.c_sp + (int64_t)slot[u] * p.c_ss);
+    }
+    if (scaled || weighted) {
+#pragma unroll
+      for (int u = 0; u < DEEP; ++u) y[u] = *reinterpret_cast<const uint32_t*>(word + (int64_t)page[u] * word_sp + (int64_t)slot[u] * word_ss);
     }
     if (!APART) {                                // what the tile writes over has been read by all
 #pragma unroll
-      for (int u = 0; u < DEEP; ++u) asm volatile("" : "+v"(x[u]), "+v"(scale[u]), "+v"(weight[u]));
+      for (int u = 0; u < DEEP; ++u) asm volatile("" : "+v"(x[u]), "+v"(y[u]));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      if (to_page[u] < 0) continue;
-      if (real) *reinterpret_cast<u32x4*>(rows + to_page[u] * p.c_sp + (int64_t)to_slot[u] * p.c_ss + (int64_t)hk * p.c_sh + sub * 16) = x[u];
-      if (sub == 0 && scales) scales[to_page[u] * p.s_sp + (int64_t)to_slot[u] * p.s_ss + (int64_t)hk * p.s_sh] = scale[u];
-      if (sub == 0 && half == 0) p.weights[to_page[u] * p.w_sp + (int64_t)to_slot[u] * p.w_ss + (int64_t)hk * p.w_sh] = weight[u];
+      if ((uint32_t)to_page[u] >= (uint32_t)p.g.pages) continue;
+      if (real) *reinterpret_cast<u32x4*>(rows + (int64_t)to_page[u] * p.c_sp + (int64_t)to_slot[u] * p.c_ss) = x[u];
+      if (scaled || weighted) *reinterpret_cast<uint32_t*>(word + (int64_t)to_page[u] * word_sp + (int64_t)to_slot[u] * word_ss) = y[u];
     }
   }
 }
 
-constexpr int kDeep = 8;
+// Rows of a lane at once, us, 8 / 4: into other pages 32 x 3000 .. 8192 tokens e4m3 H8 D128 to 2048 95.6 / 74.5, bf16 137 / 134, one row of 64
+// more than its 1024 5.3 / 4.0; in its own pages, where a tile is a round of its loads and a barrier, the first 52.2 / 64.4, 4 x 8192 to
+// 8000 55.9 / 68.1.  With few (sequence, K/V head) pairs workgroups of 1024 threads: 1 x 8192 H8 bf16 to 4096 101 us with 256, 46.4 with 1024.
+constexpr int kDeepApart = 4, kDeep = 8, kMovers = 256, kManyMovers = 1024;
 int lanes_of(int row) { return row <= 64 ? 4 : row <= 128 ? 8 : 16; }
 int64_t tiles_of(const Evict& p) {
-  const int tile = kMovers / lanes_of(p.row) * kDeep;
+  const int tile = kMovers / lanes_of(p.row) * kDeepApart;
   return p.out_table ? ((int64_t)p.limit + tile - 1) / tile : 1;
 }
 template <int LANES>
 void move(const Evict& p, int64_t items, hipStream_t st) {
   const int tiles = (int)tiles_of(p);
   const dim3 grid((unsigned)(items * 2 * tiles));
-  if (p.out_table) hipLaunchKernelGGL((paged_evict_move<LANES, kDeep, true>), grid, dim3(kMovers), 0, st, p, tiles);
-  else hipLaunchKernelGGL((paged_evict_move<LANES, kDeep, false>), grid, dim3(kMovers), 0, st, p, tiles);
+  if (p.out_table) hipLaunchKernelGGL((paged_evict_move<LANES, kDeepApart, true, kMovers>), grid, dim3(kMovers), 0, st, p, tiles);
+  else if (items <= 128) hipLaunchKernelGGL((paged_evict_move<LANES, kDeep, false, kManyMovers>), grid, dim3(kManyMovers), 0, st, p, tiles);
+  else hipLaunchKernelGGL((paged_evict_move<LANES, kDeep, false, kMovers>), grid, dim3(kMovers), 0, st, p, tiles);
 }
 
 }  // namespace

@@ -405,6 +405,32 @@ def test_long_sequences_and_pages_past_four_gigabytes():
         assert torch.equal(weights[at[:30000], slot[:30000], h], had[want, h])
 
 
+@pytest.mark.parametrize("pattern", ["spread", "equal", "few", "close", "two"])
+@pytest.mark.parametrize("length", [2048, 2049, 8193, 32768, 32800, 70000])
+def test_which_positions_of_long_sequences_stay(length, pattern):
+    """Every way a sequence's weights are held, with weights that share all, most or few of their bits."""
+    page, Hkv, D = 64, 2, 8
+    count = -(-length // page)
+    g = torch.Generator().manual_seed(length)
+    cache, _ = M.paged_cache(2 * count, page, Hkv, D)
+    table = torch.randperm(2 * count, generator=g)[:count].int().view(1, -1)
+    w = {"spread": torch.exp(4 * torch.randn(length, Hkv, generator=g)), "equal": torch.full((length, Hkv), 0.25),
+         "few": torch.randint(0, 3, (length, Hkv), generator=g).float(), "close": 1 + torch.rand(length, Hkv, generator=g) / 4,
+         "two": torch.where(torch.rand(length, Hkv, generator=g) < 0.5, -1.5, 1.5)}[pattern]
+    weights = M.paged_weights(2 * count, page, Hkv)
+    position = torch.arange(length)
+    at, slot = table[0][position // page].long().cuda(), (position % page).cuda()
+    weights[at, slot] = w.cuda()
+    out_table = torch.tensor([sorted(set(range(2 * count)) - set(table[0].tolist()))[:count]], dtype=torch.int32).cuda()
+    for keep, recent in ((length - 1, 0), (length // 3, 100), (101, 100), (200, 200)):
+        kept, left = M.paged_cache_evict(cache, table.cuda(), _ints([length]), weights, keep, recent=recent, out_table=out_table)
+        assert left.item() == keep
+        for h in range(Hkv):
+            order = torch.sort(w[:length - recent, h], descending=True, stable=True).indices[:keep - recent]
+            want = torch.cat([torch.sort(order).values, torch.arange(length - recent, length)])
+            assert torch.equal(kept[0, h].cpu(), want.int()), (keep, recent, h)
+
+
 @pytest.mark.parametrize("kind", KINDS, ids=NAMES)
 def test_a_serving_run_within_a_budget(kind):
     """Prompts by packed chunks, then token by token; every step writes, attends, adds up weights and evicts, captured once and
