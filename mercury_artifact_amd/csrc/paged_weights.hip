@@ -9,10 +9,11 @@
 // more than 16 rows) wavefronts on every CU, whose loads are in flight together; no LDS, no barrier, no atomics, so that results are the same in every run.
 //
 // paged_weights_many: for prompts, bound by the vector unit (an exponential, a multiply-add and an add for each 2 D operations of the matrix
-// unit).  Here the keys stay: a workgroup of four wavefronts holds 256 of a (sequence, K/V head), 64 to a wavefront, as the A operand of
-// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 32 queries of a head come through a ring in LDS, copied there without passing through
-// registers.  Lane (ln, lg) holds query ln, its keys' weights are added in registers, and over the lanes once in 64 tiles (which keeps
-// the sums short: 64 in a row, then 32 as a tree).  The tiles that see a key differ with the mask, so the tiles of all items are counted
+// unit).  Here the keys stay: a workgroup of eight wavefronts holds 256 of a (sequence, K/V head), 32 to a wavefront, as the A operand of
+// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 64 queries of a head come through a ring in LDS, copied there without passing through
+// registers.  Lane (ln, lg) holds queries ln and 32 + ln, its keys' weights are added in registers, and over the lanes once in 64 tiles
+// (which keeps the sums short: 128 in a row, then 32 as a tree).  Four wavefronts on a SIMD, so that one's exponentials have another's MFMAs
+// beside them.  The tiles that see a key differ with the mask, so the tiles of all items are counted
 // in closed form and dealt out evenly, in order; a workgroup whose share ends inside an item leaves partial sums, and
 // paged_weights_join adds those up in their order.
 #include "paged.hpp"
@@ -216,14 +217,18 @@ __global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Ga
 }
 
 // ---- prompts -------------------------------------------------------------------------------------------------------------------
-constexpr int kKeys = 256, kQueries = 32;        // of a workgroup's item, of a step
+constexpr int kKeys = 256, kQueries = 64;        // of a workgroup's item, of a step
+constexpr int kManyWaves = kKeys / 32;
 constexpr int kManyWorkers = 512;                // workgroups: two on a CU
 constexpr int kManyStages = 4;
-constexpr int kQueryTile = kQueries * 256, kStageBytes = kQueryTile + 4 * 256;      // rows of 256 bytes; each wavefront's copy of the rows' lse
+constexpr int kQueryTile = kQueries * 256, kStageBytes = kQueryTile + kManyWaves * 256;     // rows of 256 bytes; each wavefront's copy of the rows' lse
 constexpr int kPause = 4;                        // what entering an item costs, in steps
+constexpr int kFrags = 4;                        // LDS operand reads ahead of the MFMAs
+constexpr int kNoColumn = 0x7fff0000;            // vector offset out of every descriptor's range (spans stay below 2^31, see kFarRows)
+constexpr int64_t kFarRows = 1 << 23;            // elements from one token's row of q to the next one's that paged_weights_many takes
 constexpr int kFlush = 64;                       // steps whose weights are added up in a register
 
-// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 8 k + z) on (all, without a mask),
+// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 4 k + z) on (all, without a mask),
 // so its steps are G times the rest, behind kPause.
 struct Steps {
   int tiles, queries, G, flat, z;                // key tiles, query tiles, heads; key tiles that all query tiles see
@@ -232,32 +237,31 @@ struct Steps {
     tiles = (s.len + kKeys - 1) / kKeys;
     queries = (s.n + kQueries - 1) / kQueries;
     G = p.G;
-    z = p.causal ? (s.n - s.len) >> 5 : 0;       // (floor)
-    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 3) + 1;
+    z = p.causal ? (s.n - s.len) >> 6 : 0;       // (floor)
+    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 2) + 1;
     flat = flat < tiles ? flat : tiles;
     all = before(tiles);
   }
-  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 8 * k + z; }
+  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 4 * k + z; }
   __device__ __forceinline__ int of(int k) const { return queries > 0 ? (queries - first(k)) * G : 0; }
   __device__ __forceinline__ int64_t before(int k) const {       // what the key tiles before k count for
     int64_t sum = (int64_t)k * queries;
-    if (k > flat) sum -= 4 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)z * (k - flat);
+    if (k > flat) sum -= 2 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)z * (k - flat);
     return (queries > 0 ? sum * G : 0) + (int64_t)k * kPause;
   }
 };
 
-// Sums over the 32 lanes of a half-wavefront of 32 registers each, lane ln with that of register ln: 31 exchanges instead of 160.
-__device__ __forceinline__ float sums_of_lanes(float (&x)[32], int ln) {
+// Sums over the 32 lanes of a half-wavefront of 16 registers each, lanes ln and ln ^ 1 with that of register ln / 2: 16 exchanges instead of 80.
+template <int HALF = 8>
+__device__ __forceinline__ float sums_of_lanes(float (&x)[16], int ln) {
+  const bool upper = ln & (2 * HALF);
 #pragma unroll
-  for (int half = 16; half > 0; half >>= 1) {
-    const bool upper = ln & half;
-#pragma unroll
-    for (int i = 0; i < half; ++i) {
-      const float keep = upper ? x[i + half] : x[i], give = upper ? x[i] : x[i + half];
-      x[i] = keep + __shfl_xor(give, half);
-    }
+  for (int i = 0; i < HALF; ++i) {
+    const float keep = upper ? x[i + HALF] : x[i], give = upper ? x[i] : x[i + HALF];
+    x[i] = keep + __shfl_xor(give, 2 * HALF);
   }
-  return x[0];
+  if constexpr (HALF > 1) return sums_of_lanes<HALF / 2>(x, ln);
+  else return x[0] + __shfl_xor(x[0], 1);
 }
 
 // Where the weight of a key lies, if its page is here.
@@ -278,7 +282,7 @@ __device__ __forceinline__ void leave(const Gather& p, const PagedSeq& s, const 
 }
 
 template <int TYPE, int COLS>
-__global__ __launch_bounds__(256, 2) void paged_weights_many(const Gather p) {
+__global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const Gather p) {
   constexpr int KB = COLS / 16;                  // k-steps of 16 columns
   __shared__ __attribute__((aligned(16))) unsigned char smem[kManyStages * kStageBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -310,6 +314,12 @@ __global__ __launch_bounds__(256, 2) void paged_weights_many(const Gather p) {
   int q_a[KB];                                   // Q operand (B): lane (ln, lg) reads chunk 2 ks + lg of row ln
 #pragma unroll
   for (int ks = 0; ks < KB; ++ks) q_a[ks] = (int)lds + ln * 256 + (((2 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
+  int voff[2];                                   // copies: four rows each, columns past the last are zeros
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = wave * 8 + u * 4 + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(r);
+    voff[u] = chunk * 8 < p.D ? r * (int)p.q_ss * 2 + chunk * 16 : kNoColumn;
+  }
   typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8;
   typedef __attribute__((address_space(3))) const float* lds_float;
   float scale_log2 = p.scale_log2;
@@ -337,27 +347,25 @@ __global__ __launch_bounds__(256, 2) void paged_weights_many(const Gather p) {
     const int64_t start = lo - from;             // of the item
     lo += take;
     pos += take;
-    const int key_at = kt * kKeys + wave * 64;   // the wavefront's first key
+    const int key_at = kt * kKeys + wave * 32;   // the wavefront's first key
     if (count == 0 && (steps > 0 || from > 0)) continue;
 
     float total_sum = 0.f;
     if (count > 0) {
-      // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of keys ln and 32 + ln, scaled -----------------------
-      bf16x8 kf[2][KB];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int key = key_at + kb * 32 + ln;
-        const Place at = place_of(p, b, key, s.len);
+      // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of key ln, scaled --------------------------------------
+      bf16x8 kf[KB];
+      {
+        const Place at = place_of(p, b, key_at + ln, s.len);
         const uint8_t* row = p.k + ((int64_t)at.page * p.c_sp + (int64_t)at.slot * p.c_ss + (int64_t)hk * p.c_sh);
         const float* scale = p.k_scales + ((int64_t)at.page * p.s_sp + (int64_t)at.slot * p.s_ss + (int64_t)hk * p.s_sh);
 #pragma unroll
         for (int ks = 0; ks < KB; ++ks) {
           const int col = ks * 16 + lg * 8;
-          kf[kb][ks] = bf16x8{};
+          kf[ks] = bf16x8{};
           if (at.page >= 0 && col < p.D) {
             if constexpr (TYPE == MHIP_E2M1) {
               const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + col / 2);
-              kf[kb][ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
+              kf[ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
             } else if constexpr (TYPE == MHIP_E4M3) {
               // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
               const u32x2 codes = *reinterpret_cast<const u32x2*>(row + col);
@@ -368,93 +376,113 @@ __global__ __launch_bounds__(256, 2) void paged_weights_many(const Gather p) {
                 x[2 * h] = pack_bf16(a[0] * *scale, a[1] * *scale);
                 x[2 * h + 1] = pack_bf16(c[0] * *scale, c[1] * *scale);
               }
-              kf[kb][ks] = __builtin_bit_cast(bf16x8, x);
+              kf[ks] = __builtin_bit_cast(bf16x8, x);
             } else {
-              kf[kb][ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
+              kf[ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
             }
           }
         }
       }
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[kb][ks]));       // loaded before the first copy goes out
+      for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[ks]));             // loaded before the first copy goes out
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();              // (the item before is through with the ring)
+      const int qt0 = st.first(kt);
 
       // ---- query tiles: step i is tile qt of head h, tiles fastest ---------------------------------------------------------------
-      const int qt0 = st.first(kt), of_head = st.queries - qt0;
-      int copy_h = first / of_head, copy_qt = first - copy_h * of_head, left = count;      // of the next copies, those that are left
-      auto copy = [&](int stage) {
-        const int head = hk * p.G + copy_h, row0 = (qt0 + copy_qt) * kQueries;
-        const uint16_t* base = p.q + b * p.q_sb + (int64_t)head * p.q_sh;
+      const int of_head = st.queries - qt0;
+      int copy_h = first / of_head, copy_qt = qt0 + first - copy_h * of_head, left = count;      // of the next copies, those that are left
+      int qt = copy_qt;
+      const uint16_t* q_head = p.q + b * p.q_sb + (int64_t)s.start * p.q_ss + (int64_t)(hk * p.G + copy_h) * p.q_sh;
+      const float* l_head = p.lse + b * p.l_sb + s.start + (int64_t)(hk * p.G + copy_h) * p.l_sh;
+      auto copy = [&](int stage) __attribute__((always_inline)) {
+        const int row0 = copy_qt * kQueries, rows = s.n - row0 < kQueries ? s.n - row0 : kQueries;
+        const u32x4 rs = rsrc_words(q_head + (int64_t)row0 * p.q_ss, (uint32_t)(((rows - 1) * (int)p.q_ss + p.D) * 2));
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {            // (rows past the last repeat it, columns past the last are those of zeros in K)
-          const int r = wave * 8 + u * 4 + (lane >> 4), row = row0 + r < s.n ? row0 + r : s.n - 1, chunk = (lane & 15) ^ lds_row_swizzle(r);
-          copy16_to_lds(base + (int64_t)(s.start + row) * p.q_ss + (chunk * 8 < p.D ? chunk * 8 : 0), lds + stage * kStageBytes + (wave * 2 + u) * 1024);
-        }
-        const int row = row0 + ln < s.n ? row0 + ln : s.n - 1;
-        copy4_to_lds(p.lse + b * p.l_sb + (int64_t)head * p.l_sh + s.start + row, lds + stage * kStageBytes + kQueryTile + wave * 256);
+        for (int u = 0; u < 2; ++u) copy16_to_lds(rs, lds + stage * kStageBytes + (wave * 2 + u) * 1024, voff[u], 0);
+        copy4_to_lds(rsrc_words(l_head + row0, (uint32_t)rows * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, lane * 4, 0);
         if (left > 1) {                          // (past the share's last tile that one again)
           --left;
-          if (++copy_qt == of_head) { copy_qt = 0; ++copy_h; }
+          if (++copy_qt == st.queries) {
+            copy_qt = qt0;
+            q_head += p.q_sh;
+            l_head += p.l_sh;
+          }
         }
       };
-      int qt = qt0 + copy_qt;
+      const int old_keys = s.len - s.n;
+      float sum[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[j] = 0.f;
       copy(0);
       copy(1);
       copy(2);
-      float sum[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) sum[i] = 0.f;
-      const int old_keys = s.len - s.n;
       for (int i = 0; i < count; ++i) {
-        // the copies of step i are done, by this wavefront and then by all; the stage of step i - 1 has been read by all
+        // tile i has been copied, by this wavefront and then by all, and all have read tile i - 1, whose stage tile i + 3 takes
         asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         copy((i + 3) & 3);
         const int at = (i & 3) * kStageBytes;
-        const float lse = *(lds_float)(uintptr_t)(uint32_t)(lds + at + kQueryTile + wave * 256 + ln * 4);
+        auto read_q = [&](int e) {               // operand e: k-step e / 2 of queries 32 (e % 2) + ln
+          return *(lds_bf16x8)(uintptr_t)(uint32_t)(q_a[e >> 1] + at + (e & 1) * (32 * 256));
+        };
+        float lse[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) lse[r] = *(lds_float)(uintptr_t)(uint32_t)(lds + at + kQueryTile + wave * 256 + (r * 32 + ln) * 4);
+        bf16x8 frag[kFrags];
+#pragma unroll
+        for (int e = 0; e < kFrags; ++e) frag[e] = read_q(e);
         f32x16 sc[2];
 #pragma unroll
-        for (int ks = 0; ks < KB; ++ks) {
-          const bf16x8 qf = *(lds_bf16x8)(uintptr_t)(uint32_t)(q_a[ks] + at);
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][ks], qf, ks == 0 ? f32x16{} : sc[kb], 0, 0, 0);
+        for (int e = 0; e < 2 * KB; ++e) {
+          sc[e & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[e >> 1], frag[e % kFrags], e < 2 ? f32x16{} : sc[e & 1], 0, 0, 0);
+          if (e + kFrags < 2 * KB) frag[e % kFrags] = read_q(e + kFrags);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        // rows past the last, and those that saw no key, weigh nothing
         const int row = qt * kQueries + ln;
-        const bool counts = row < s.n && lse != -INFINITY;         // (a row that saw no key weighs nothing)
-        const float nlse = counts ? -lse * kLog2e : 0.f;
-        if ((p.causal && key_at + 63 > old_keys + qt * kQueries) || __builtin_amdgcn_ballot_w64(!counts) != 0) {
+        const bool counts[2] = {row < s.n && lse[0] != -INFINITY, row + 32 < s.n && lse[1] != -INFINITY};
+        float minus[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) minus[r] = counts[r] ? -lse[r] * kLog2e : 0.f;
+        if ((p.causal && key_at + 31 > old_keys + qt * kQueries) || __builtin_amdgcn_ballot_w64(!counts[0] || !counts[1]) != 0) {
           asm volatile("");
-          const int seen = counts ? (p.causal ? old_keys + row + 1 : s.len) - key_at - 4 * lg : 0x80000000;      // from the wavefront's first key
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int r = 0; r < 2; ++r) {          // keys that the row sees, from the lane's first one
+            const int seen = counts[r] ? (p.causal ? old_keys + row + 32 * r + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (kb * 32 + 8 * (j >> 2) + (j & 3) >= seen) sc[kb][j] = -INFINITY;
+            for (int j = 0; j < 16; ++j) {
+              if (8 * (j >> 2) + (j & 3) >= seen) sc[r][j] = -INFINITY;
+              if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) sum[kb * 16 + j] += fast_exp2(__builtin_fmaf(sc[kb][j], scale_log2, nlse));
+          for (int j = 0; j < 16; ++j) {
+            sum[j] += fast_exp2(__builtin_fmaf(sc[r][j], scale_log2, minus[r]));
+            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
         if (++qt == st.queries) qt = qt0;
         if ((i & (kFlush - 1)) == kFlush - 1) {
+          asm volatile("");
           total_sum += sums_of_lanes(sum, ln);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sum[e] = 0.f;
+          for (int j = 0; j < 16; ++j) sum[j] = 0.f;
         }
       }
       total_sum += sums_of_lanes(sum, ln);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // copies past the last step
     }
-    // lane (ln, lg) has the sum of register ln: key 32 (ln / 16) + 8 (ln % 16 / 4) + 4 lg + ln % 4
-    const int own = (ln >> 4) * 32 + ((ln >> 2) & 3) * 8 + lg * 4 + (ln & 3);
+    // lanes (ln, lg) and (ln ^ 1, lg) have the sum of register j = ln / 2, of key 8 (j / 4) + 4 lg + j % 4
+    const int own = (ln >> 3) * 8 + lg * 4 + ((ln >> 1) & 3);
     if (count == steps) {
+      if (ln & 1) continue;
       leave(p, s, place_of(p, b, key_at + own, s.len), hk, key_at + own, total_sum);
       continue;
     }
-    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 64 + own] = total_sum;
+    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 32 + own] = total_sum;         // (both of the same)
     if (first == 0 && threadIdx.x == 0) {
       const int last = (int)(((start + weight) * shares - 1) / total);           // the workgroup with its last unit
       p.shared[w * 4 + 1] = b;
@@ -480,9 +508,9 @@ __global__ __launch_bounds__(kKeys) void paged_weights_join(const Gather p) {
 
 template <int TYPE>
 void launch_many(const Gather& p, hipStream_t st) {
-  if (p.D <= 64) hipLaunchKernelGGL((paged_weights_many<TYPE, 64>), dim3(kManyWorkers), dim3(256), 0, st, p);
-  else if (p.D <= 96) hipLaunchKernelGGL((paged_weights_many<TYPE, 96>), dim3(kManyWorkers), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((paged_weights_many<TYPE, 128>), dim3(kManyWorkers), dim3(256), 0, st, p);
+  if (p.D <= 64) hipLaunchKernelGGL((paged_weights_many<TYPE, 64>), dim3(kManyWorkers), dim3(kManyWaves * 64), 0, st, p);
+  else if (p.D <= 96) hipLaunchKernelGGL((paged_weights_many<TYPE, 96>), dim3(kManyWorkers), dim3(kManyWaves * 64), 0, st, p);
+  else hipLaunchKernelGGL((paged_weights_many<TYPE, 128>), dim3(kManyWorkers), dim3(kManyWaves * 64), 0, st, p);
   hipLaunchKernelGGL(paged_weights_join, dim3(kManyWorkers), dim3(kKeys), 0, st, p);
 }
 
@@ -501,7 +529,7 @@ void launch_rows(const Gather& p, int64_t rows, hipStream_t st) {
 }
 template <int TYPE>
 void launch(const Gather& p, int64_t rows, hipStream_t st) {
-  if (rows > kFewRows) launch_many<TYPE>(p, st);
+  if (rows > kFewRows && p.q_ss <= kFarRows) launch_many<TYPE>(p, st);
   else if (p.D <= 64) launch_rows<TYPE, 64>(p, rows, st);
   else launch_rows<TYPE, 128>(p, rows, st);
 }
