@@ -9,11 +9,12 @@
 // more than 16 rows) wavefronts on every CU, whose loads are in flight together; no LDS, no barrier, no atomics, so that results are the same in every run.
 //
 // paged_weights_many: for prompts, bound by the vector unit (an exponential, a multiply-add and an add for each 2 D operations of the matrix
-// unit).  Here the keys stay: a workgroup of eight wavefronts holds 256 of a (sequence, K/V head), 32 to a wavefront, as the A operand of
-// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 64 queries of a head come through a ring in LDS, copied there without passing through
-// registers.  Lane (ln, lg) holds queries ln and 32 + ln, its keys' weights are added in registers, and over the lanes once in 64 tiles
-// (which keeps the sums short: 128 in a row, then 32 as a tree).  Four wavefronts on a SIMD, so that one's exponentials have another's MFMAs
-// beside them.  The tiles that see a key differ with the mask, so the tiles of all items are counted
+// unit).  Here the keys stay: a workgroup of four wavefronts holds 256 of a (sequence, K/V head), 64 to a wavefront, as the A operand of
+// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 32 queries of a head come through a ring in LDS, copied there without passing through
+// registers; each operand read from LDS feeds two MFMAs (with 32 keys to a wavefront, four wavefronts on a SIMD, a prompt of 8192
+// tokens H32/8 takes 292 us on 128 columns and 203 on 64, so 280 and 219).
+// Lane (ln, lg) holds query ln, its keys' weights are added in registers, and over the lanes once in 64 tiles (which keeps the sums short: 64
+// in a row, then 32 as a tree).  The exponentials of a tile stand between the MFMAs of the next one.  The tiles that see a key differ with the mask, so the tiles of all items are counted
 // in closed form and dealt out evenly, in order; a workgroup whose share ends inside an item leaves partial sums, and
 // paged_weights_join adds those up in their order.
 #include "paged.hpp"
@@ -42,15 +43,15 @@ struct Gather {
 template <int NR>
 constexpr int kFewWaves = NR == 1 ? 4 : 2;
 
-template <int TYPE>
-constexpr int kBlocksOf = TYPE == MHIP_BF16 ? 2 : 4;       // 16-key blocks of a unit
+template <int TYPE, int NR>
+constexpr int kBlocksOf = TYPE == MHIP_BF16 || NR == 4 ? 2 : 4;      // 16-key blocks of a unit
 
 template <int UNIT>
 __device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) { return (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv; }
 
 template <int TYPE, int COLS, int NR>
 __global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Gather p) {
-  constexpr int kBlocks = kBlocksOf<TYPE>, UNIT = 16 * kBlocks, ROWS = 16 * NR;
+  constexpr int kBlocks = kBlocksOf<TYPE, NR>, UNIT = 16 * kBlocks, ROWS = 16 * NR;
   constexpr bool E4M3 = TYPE == MHIP_E4M3, E2M1 = TYPE == MHIP_E2M1;
   constexpr int KB = COLS / 32, KR = E2M1 ? 1 : E4M3 ? KB / 2 : KB;      // k-steps of 32 columns, loads of a key's row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -217,19 +218,21 @@ __global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Ga
 }
 
 // ---- prompts -------------------------------------------------------------------------------------------------------------------
-constexpr int kKeys = 256, kQueries = 64;        // of a workgroup's item, of a step
-constexpr int kManyWaves = kKeys / 32;
+constexpr int kKeys = 256, kQueries = 32;        // of a workgroup's item, of a step
+constexpr int kManyWaves = kKeys / 64;
 constexpr int kManyWorkers = 512;                // workgroups: two on a CU
 constexpr int kManyStages = 4;
 constexpr int kQueryTile = kQueries * 256, kStageBytes = kQueryTile + kManyWaves * 256;     // rows of 256 bytes; each wavefront's copy of the rows' lse
-constexpr int kPause = 4;                        // what entering an item costs, in steps
+// What entering an item costs, in steps, and the eight query tiles that cut through an item's keys cost twice.  (A prompt of 8192 tokens H32/8
+// D128 with all steps alike: workgroups end after 217 to 331 us, 229 to 315 so.)
+constexpr int kPause = 4, kCut = 8;
 constexpr int kFrags = 4;                        // LDS operand reads ahead of the MFMAs
 constexpr int kNoColumn = 0x7fff0000;            // vector offset out of every descriptor's range (spans stay below 2^31, see kFarRows)
 constexpr int64_t kFarRows = 1 << 23;            // elements from one token's row of q to the next one's that paged_weights_many takes
 constexpr int kFlush = 64;                       // steps whose weights are added up in a register
 
-// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 4 k + z) on (all, without a mask),
-// so its steps are G times the rest, behind kPause.
+// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 8 k + z) on (all, without a mask),
+// so its steps are G times the rest.
 struct Steps {
   int tiles, queries, G, flat, z;                // key tiles, query tiles, heads; key tiles that all query tiles see
   int64_t all;                                   // of all key tiles
@@ -237,31 +240,32 @@ struct Steps {
     tiles = (s.len + kKeys - 1) / kKeys;
     queries = (s.n + kQueries - 1) / kQueries;
     G = p.G;
-    z = p.causal ? (s.n - s.len) >> 6 : 0;       // (floor)
-    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 2) + 1;
+    z = p.causal ? (s.n - s.len) >> 5 : 0;       // (floor)
+    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 3) + 1;
     flat = flat < tiles ? flat : tiles;
     all = before(tiles);
   }
-  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 4 * k + z; }
+  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 8 * k + z; }
   __device__ __forceinline__ int of(int k) const { return queries > 0 ? (queries - first(k)) * G : 0; }
+  __device__ __forceinline__ int cost(int k) const { return of(k) + (queries > 0 && k >= flat ? kCut * G : 0); }      // behind kPause
   __device__ __forceinline__ int64_t before(int k) const {       // what the key tiles before k count for
     int64_t sum = (int64_t)k * queries;
-    if (k > flat) sum -= 2 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)z * (k - flat);
+    if (k > flat) sum -= 4 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)(z - kCut) * (k - flat);
     return (queries > 0 ? sum * G : 0) + (int64_t)k * kPause;
   }
 };
 
-// Sums over the 32 lanes of a half-wavefront of 16 registers each, lanes ln and ln ^ 1 with that of register ln / 2: 16 exchanges instead of 80.
-template <int HALF = 8>
-__device__ __forceinline__ float sums_of_lanes(float (&x)[16], int ln) {
-  const bool upper = ln & (2 * HALF);
+// Sums over the 32 lanes of a half-wavefront of 32 registers each, lane ln with that of register ln: 31 exchanges instead of 160.
+template <int HALF = 16>
+__device__ __forceinline__ float sums_of_lanes(float (&x)[32], int ln) {
+  const bool upper = ln & HALF;
 #pragma unroll
   for (int i = 0; i < HALF; ++i) {
     const float keep = upper ? x[i + HALF] : x[i], give = upper ? x[i] : x[i + HALF];
-    x[i] = keep + __shfl_xor(give, 2 * HALF);
+    x[i] = keep + __shfl_xor(give, HALF);
   }
   if constexpr (HALF > 1) return sums_of_lanes<HALF / 2>(x, ln);
-  else return x[0] + __shfl_xor(x[0], 1);
+  else return x[0];
 }
 
 // Where the weight of a key lies, if its page is here.
@@ -282,7 +286,7 @@ __device__ __forceinline__ void leave(const Gather& p, const PagedSeq& s, const 
 }
 
 template <int TYPE, int COLS>
-__global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const Gather p) {
+__global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const Gather p) {
   constexpr int KB = COLS / 16;                  // k-steps of 16 columns
   __shared__ __attribute__((aligned(16))) unsigned char smem[kManyStages * kStageBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -314,6 +318,7 @@ __global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const G
   int q_a[KB];                                   // Q operand (B): lane (ln, lg) reads chunk 2 ks + lg of row ln
 #pragma unroll
   for (int ks = 0; ks < KB; ++ks) q_a[ks] = (int)lds + ln * 256 + (((2 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
+  const int lse_a = (int)lds + kQueryTile + wave * 256 + ln * 4;
   int voff[2];                                   // copies: four rows each, columns past the last are zeros
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -341,31 +346,33 @@ __global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const G
       if (st.before(kt + half) <= in_head) { kt += half; span -= half; }
       else span = half;
     }
-    const int steps = st.of(kt), weight = steps + kPause, from = (int)(in_head - st.before(kt));
+    const int steps = st.of(kt), cost = st.cost(kt), weight = cost + kPause, from = (int)(in_head - st.before(kt));
     const int take = (int)(weight - from < hi - lo ? weight - from : hi - lo);
-    const int first = from > kPause ? from - kPause : 0, count = from + take > kPause ? from + take - kPause - first : 0;
+    auto step_at = [&](int unit) { return unit > kPause ? (int)((int64_t)(unit - kPause) * steps / cost) : 0; };
+    const int first = step_at(from), count = step_at(from + take) - first;
     const int64_t start = lo - from;             // of the item
     lo += take;
     pos += take;
-    const int key_at = kt * kKeys + wave * 32;   // the wavefront's first key
-    if (count == 0 && (steps > 0 || from > 0)) continue;
+    const int key_at = kt * kKeys + wave * 64;   // the wavefront's first key
+    if (count == 0 && first == 0 && (steps > 0 || from > 0)) continue;      // (with steps before and behind it, it leaves sums of nothing)
 
     float total_sum = 0.f;
     if (count > 0) {
-      // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of key ln, scaled --------------------------------------
-      bf16x8 kf[KB];
-      {
-        const Place at = place_of(p, b, key_at + ln, s.len);
+      // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of keys ln and 32 + ln, scaled ------------------------
+      bf16x8 kf[2][KB];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const Place at = place_of(p, b, key_at + kb * 32 + ln, s.len);
         const uint8_t* row = p.k + ((int64_t)at.page * p.c_sp + (int64_t)at.slot * p.c_ss + (int64_t)hk * p.c_sh);
         const float* scale = p.k_scales + ((int64_t)at.page * p.s_sp + (int64_t)at.slot * p.s_ss + (int64_t)hk * p.s_sh);
 #pragma unroll
         for (int ks = 0; ks < KB; ++ks) {
           const int col = ks * 16 + lg * 8;
-          kf[ks] = bf16x8{};
+          kf[kb][ks] = bf16x8{};
           if (at.page >= 0 && col < p.D) {
             if constexpr (TYPE == MHIP_E2M1) {
               const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + col / 2);
-              kf[ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
+              kf[kb][ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
             } else if constexpr (TYPE == MHIP_E4M3) {
               // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
               const u32x2 codes = *reinterpret_cast<const u32x2*>(row + col);
@@ -376,15 +383,17 @@ __global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const G
                 x[2 * h] = pack_bf16(a[0] * *scale, a[1] * *scale);
                 x[2 * h + 1] = pack_bf16(c[0] * *scale, c[1] * *scale);
               }
-              kf[ks] = __builtin_bit_cast(bf16x8, x);
+              kf[kb][ks] = __builtin_bit_cast(bf16x8, x);
             } else {
-              kf[ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
+              kf[kb][ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
             }
           }
         }
       }
 #pragma unroll
-      for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[ks]));             // loaded before the first copy goes out
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[kb][ks]));       // loaded before the first copy goes out
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();              // (the item before is through with the ring)
       const int qt0 = st.first(kt);
@@ -400,7 +409,7 @@ __global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const G
         const u32x4 rs = rsrc_words(q_head + (int64_t)row0 * p.q_ss, (uint32_t)(((rows - 1) * (int)p.q_ss + p.D) * 2));
 #pragma unroll
         for (int u = 0; u < 2; ++u) copy16_to_lds(rs, lds + stage * kStageBytes + (wave * 2 + u) * 1024, voff[u], 0);
-        copy4_to_lds(rsrc_words(l_head + row0, (uint32_t)rows * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, lane * 4, 0);
+        copy4_to_lds(rsrc_words(l_head + row0, (uint32_t)rows * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, ln * 4, 0);
         if (left > 1) {                          // (past the share's last tile that one again)
           --left;
           if (++copy_qt == st.queries) {
@@ -411,78 +420,119 @@ __global__ __launch_bounds__(kManyWaves * 64, 4) void paged_weights_many(const G
         }
       };
       const int old_keys = s.len - s.n;
-      float sum[16];
+      float sum[32];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum[j] = 0.f;
+      for (int e = 0; e < 32; ++e) sum[e] = 0.f;
+      f32x16 sc[2][2];
+      float lse[2];
+      bf16x8 frag[kFrags];
+      // Of the tile in stage kStage: its rows' lse, and S^T with the operands kFrags reads ahead; between(m) goes behind MFMA m.
+      auto product = [&](auto stage_of, f32x16 (&to)[2], float& to_lse, auto&& between) __attribute__((always_inline)) {
+        constexpr int kAt = decltype(stage_of)::value * kStageBytes;
+        auto read_q = [&](int ks) { return *(lds_bf16x8)(uintptr_t)(uint32_t)(q_a[ks] + kAt); };
+        to_lse = *(lds_float)(uintptr_t)(uint32_t)(lse_a + kAt);
+#pragma unroll
+        for (int ks = 0; ks < kFrags; ++ks) frag[ks] = read_q(ks);
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            to[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][ks], frag[ks % kFrags], ks == 0 ? f32x16{} : to[kb], 0, 0, 0);
+            if (kb == 1 && ks + kFrags < KB) frag[ks % kFrags] = read_q(ks + kFrags);
+            between(2 * ks + kb);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      };
       copy(0);
       copy(1);
       copy(2);
-      for (int i = 0; i < count; ++i) {
-        // tile i has been copied, by this wavefront and then by all, and all have read tile i - 1, whose stage tile i + 3 takes
+      copy(3);
+      asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      product(std::integral_constant<int, 0>{}, sc[0], lse[0], [](int) {});
+      // Step i: the weights of tile i, and between them the product of tile i + 1 (past the share's last tile that one again), which
+      // has been copied, by this wavefront and then by all; all have read tile i, whose stage tile i + 4 takes.  The loop is
+      // written out four times, so that a stage is an immediate offset of the reads.
+      auto step = [&](auto stage_of, int i) __attribute__((always_inline)) {
+        constexpr int kStage = decltype(stage_of)::value;
+        f32x16 (&now)[2] = sc[kStage & 1];
         asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        copy((i + 3) & 3);
-        const int at = (i & 3) * kStageBytes;
-        auto read_q = [&](int e) {               // operand e: k-step e / 2 of queries 32 (e % 2) + ln
-          return *(lds_bf16x8)(uintptr_t)(uint32_t)(q_a[e >> 1] + at + (e & 1) * (32 * 256));
-        };
-        float lse[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) lse[r] = *(lds_float)(uintptr_t)(uint32_t)(lds + at + kQueryTile + wave * 256 + (r * 32 + ln) * 4);
-        bf16x8 frag[kFrags];
-#pragma unroll
-        for (int e = 0; e < kFrags; ++e) frag[e] = read_q(e);
-        f32x16 sc[2];
-#pragma unroll
-        for (int e = 0; e < 2 * KB; ++e) {
-          sc[e & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[e >> 1], frag[e % kFrags], e < 2 ? f32x16{} : sc[e & 1], 0, 0, 0);
-          if (e + kFrags < 2 * KB) frag[e % kFrags] = read_q(e + kFrags);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        copy(kStage);
         // rows past the last, and those that saw no key, weigh nothing
-        const int row = qt * kQueries + ln;
-        const bool counts[2] = {row < s.n && lse[0] != -INFINITY, row + 32 < s.n && lse[1] != -INFINITY};
-        float minus[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) minus[r] = counts[r] ? -lse[r] * kLog2e : 0.f;
-        if ((p.causal && key_at + 31 > old_keys + qt * kQueries) || __builtin_amdgcn_ballot_w64(!counts[0] || !counts[1]) != 0) {
+        const int row0 = qt * kQueries;
+        const float mine = lse[kStage & 1];
+        float minus = mine * -kLog2e;
+        if (++qt == st.queries) qt = qt0;
+        if (p.causal && key_at > old_keys + row0 + kQueries - 1) {       // nobody sees any of them
+          product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [](int) {});
+        } else {
+        if (__builtin_expect((p.causal && key_at + 63 > old_keys + row0) || row0 + kQueries > s.n ||
+                             __builtin_amdgcn_ballot_w64(mine == -INFINITY) != 0, 0)) {
           asm volatile("");
+          const bool counts = row0 + ln < s.n && mine != -INFINITY;
+          // keys that the row sees, from the lane's first one
+          const int seen = counts ? (p.causal ? old_keys + row0 + ln + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
+          if (!counts) minus = 0.f;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {          // keys that the row sees, from the lane's first one
-            const int seen = counts[r] ? (p.causal ? old_keys + row + 32 * r + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (8 * (j >> 2) + (j & 3) >= seen) sc[r][j] = -INFINITY;
-              if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            }
+          for (int e = 0; e < 32; ++e) {
+            if ((e >> 4) * 32 + 8 * (e >> 2 & 3) + (e & 3) >= seen) now[e >> 4][e & 15] = -INFINITY;
+            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
           }
         }
+        // Behind MFMA m the next weights' multiply-adds, the exponentials of those before, and the sums of those before them: none waits for another.
+        constexpr int kEach = (32 + 2 * KB - 3) / (2 * KB - 2);
+        auto ahead = [&](int e) __attribute__((always_inline)) {
+          if (e < 32) now[e >> 4][e & 15] = __builtin_fmaf(now[e >> 4][e & 15], scale_log2, minus);
+        };
+        auto power = [&](int e) __attribute__((always_inline)) {
+          if (e >= 0 && e < 32) now[e >> 4][e & 15] = fast_exp2(now[e >> 4][e & 15]);
+        };
+        auto add = [&](int e) __attribute__((always_inline)) {
+          if (e >= 0 && e < 32) sum[e] += now[e >> 4][e & 15];
+        };
+        product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+          for (int e = 0; e < kEach; ++e) power((m - 1) * kEach + e);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            sum[j] += fast_exp2(__builtin_fmaf(sc[r][j], scale_log2, minus[r]));
-            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-          }
-        if (++qt == st.queries) qt = qt0;
-        if ((i & (kFlush - 1)) == kFlush - 1) {
+          for (int e = 0; e < kEach; ++e) ahead(m * kEach + e);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) add((m - 2) * kEach + e);
+        });
+#pragma unroll
+        for (int e = (2 * KB - 2) * kEach; e < 32; ++e) add(e);
+        }
+        if (kStage == 3 && (i & (kFlush - 1)) == kFlush - 1) {
           asm volatile("");
           total_sum += sums_of_lanes(sum, ln);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) sum[j] = 0.f;
+          for (int e = 0; e < 32; ++e) sum[e] = 0.f;
         }
+      };
+      for (int i = 0; i < count; i += 4) {
+        // The two workgroups of a CU take turns in going first: otherwise the older one ends long before the other, which is slow alone (a prompt of
+        // 8192 tokens H32/8 D128 290 us, 280 with turns of 16 steps, 284 of four).
+        if ((i >> 4 ^ blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        step(std::integral_constant<int, 0>{}, i);
+        if (i + 1 == count) break;
+        step(std::integral_constant<int, 1>{}, i + 1);
+        if (i + 2 == count) break;
+        step(std::integral_constant<int, 2>{}, i + 2);
+        if (i + 3 == count) break;
+        step(std::integral_constant<int, 3>{}, i + 3);
       }
+      __builtin_amdgcn_s_setprio(0);
       total_sum += sums_of_lanes(sum, ln);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // copies past the last step
     }
-    // lanes (ln, lg) and (ln ^ 1, lg) have the sum of register j = ln / 2, of key 8 (j / 4) + 4 lg + j % 4
-    const int own = (ln >> 3) * 8 + lg * 4 + ((ln >> 1) & 3);
+    // lane (ln, lg) has the sum of register ln: key 32 (ln / 16) + 8 (ln % 16 / 4) + 4 lg + ln % 4
+    const int own = (ln >> 4) * 32 + ((ln >> 2) & 3) * 8 + lg * 4 + (ln & 3);
     if (count == steps) {
-      if (ln & 1) continue;
       leave(p, s, place_of(p, b, key_at + own, s.len), hk, key_at + own, total_sum);
       continue;
     }
-    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 32 + own] = total_sum;         // (both of the same)
+    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 64 + own] = total_sum;
     if (first == 0 && threadIdx.x == 0) {
       const int last = (int)(((start + weight) * shares - 1) / total);           // the workgroup with its last unit
       p.shared[w * 4 + 1] = b;
