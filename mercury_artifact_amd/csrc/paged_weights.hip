@@ -10,7 +10,7 @@
 //
 // paged_weights_many: for prompts, bound by the vector unit (an exponential, a multiply-add and an add for each 2 D operations of the matrix
 // unit).  Here the keys stay: a workgroup of four wavefronts holds 256 of a (sequence, K/V head), 64 to a wavefront, as the A operand of
-// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 32 queries of a head come through a ring in LDS, copied there without passing through
+// S^T = K Q^T (v_mfma_f32_32x32x16_bf16), and tiles of 32 queries come through a ring in LDS, copied there without passing through
 // registers; each operand read from LDS feeds two MFMAs (with 32 keys to a wavefront, four wavefronts on a SIMD, a prompt of 8192
 // tokens H32/8 takes 292 us on 128 columns and 203 on 64, so 280 and 219).
 // Lane (ln, lg) holds query ln, its keys' weights are added in registers, and over the lanes once in 64 tiles (which keeps the sums short: 64
@@ -36,6 +36,7 @@ struct Gather {
   int Hkv, G, D, causal;
   float scale_log2, decay;
   Divisor by_group;
+  int fold;                                      // paged_weights_many: log2 of the heads in a query tile
   float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
 };
 
@@ -223,35 +224,37 @@ constexpr int kManyWaves = kKeys / 64;
 constexpr int kManyWorkers = 512;                // workgroups: two on a CU
 constexpr int kManyStages = 4;
 constexpr int kQueryTile = kQueries * 256, kStageBytes = kQueryTile + kManyWaves * 256;     // rows of 256 bytes; each wavefront's copy of the rows' lse
-// What entering an item costs, in steps, and the eight query tiles that cut through an item's keys cost twice.  (A prompt of 8192 tokens H32/8
+// What entering an item costs, in steps, and the query tiles (eight, of one head) that cut through an item's keys cost twice.  (A prompt of 8192 tokens H32/8
 // D128 with all steps alike: workgroups end after 217 to 331 us, 229 to 315 so.)
 constexpr int kPause = 4, kCut = 8;
 constexpr int kFrags = 4;                        // LDS operand reads ahead of the MFMAs
 constexpr int kNoColumn = 0x7fff0000;            // vector offset out of every descriptor's range (spans stay below 2^31, see kFarRows)
-constexpr int64_t kFarRows = 1 << 23;            // elements from one token's row of q to the next one's that paged_weights_many takes
+constexpr int64_t kFarRows = 1 << 23, kFarHeads = 1 << 24;       // elements between tokens, and between the heads of a tile, that paged_weights_many takes
 constexpr int kFlush = 64;                       // steps whose weights are added up in a register
 
-// Items of a sequence and K/V head: tiles of 256 keys.  Key tile k is seen by the query tiles from max(0, 8 k + z) on (all, without a mask),
-// so its steps are G times the rest.
+// Items of a sequence and K/V head: tiles of 256 keys.  A query tile is 32 / F tokens of F heads, so that short chunks of grouped heads
+// fill it too (F: the largest power of two up to 32 that divides G).  Key tile k is seen by the query tiles from max(0, 8 F k + z) on
+// (all, without a mask), and its steps are those of G / F groups of heads.
 struct Steps {
-  int tiles, queries, G, flat, z;                // key tiles, query tiles, heads; key tiles that all query tiles see
+  int tiles, queries, fold, groups, flat, z;     // key tiles, query tiles of a group, log2 F, groups; key tiles that all query tiles see
   int64_t all;                                   // of all key tiles
   __device__ __forceinline__ Steps(const Gather& p, const PagedSeq& s) {
     tiles = (s.len + kKeys - 1) / kKeys;
-    queries = (s.n + kQueries - 1) / kQueries;
-    G = p.G;
-    z = p.causal ? (s.n - s.len) >> 5 : 0;       // (floor)
-    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> 3) + 1;
+    fold = p.fold;
+    queries = (int)((((int64_t)s.n << fold) + kQueries - 1) / kQueries);
+    groups = p.G >> fold;
+    z = p.causal ? (s.n - s.len) >> (5 - fold) : 0;        // (floor)
+    flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> (3 + fold)) + 1;
     flat = flat < tiles ? flat : tiles;
     all = before(tiles);
   }
-  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : 8 * k + z; }
-  __device__ __forceinline__ int of(int k) const { return queries > 0 ? (queries - first(k)) * G : 0; }
-  __device__ __forceinline__ int cost(int k) const { return of(k) + (queries > 0 && k >= flat ? kCut * G : 0); }      // behind kPause
+  __device__ __forceinline__ int first(int k) const { return k < flat ? 0 : (k << (3 + fold)) + z; }
+  __device__ __forceinline__ int of(int k) const { return queries > 0 ? (queries - first(k)) * groups : 0; }
+  __device__ __forceinline__ int cost(int k) const { return of(k) + (queries > 0 && k >= flat ? (kCut << fold) * groups : 0); }      // behind kPause
   __device__ __forceinline__ int64_t before(int k) const {       // what the key tiles before k count for
     int64_t sum = (int64_t)k * queries;
-    if (k > flat) sum -= 4 * ((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) + (int64_t)(z - kCut) * (k - flat);
-    return (queries > 0 ? sum * G : 0) + (int64_t)k * kPause;
+    if (k > flat) sum -= (((int64_t)k * (k - 1) - (int64_t)flat * (flat - 1)) << (2 + fold)) + (int64_t)(z - (kCut << fold)) * (k - flat);
+    return (queries > 0 ? sum * groups : 0) + (int64_t)k * kPause;
   }
 };
 
@@ -319,12 +322,15 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
 #pragma unroll
   for (int ks = 0; ks < KB; ++ks) q_a[ks] = (int)lds + ln * 256 + (((2 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
   const int lse_a = (int)lds + kQueryTile + wave * 256 + ln * 4;
-  int voff[2];                                   // copies: four rows each, columns past the last are zeros
+  // copies of a query tile, row r of which is token r / F and head r % F: four rows each, columns past the last are zeros
+  const int heads = (1 << p.fold) - 1, tokens = kQueries >> p.fold;
+  int voff[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int r = wave * 8 + u * 4 + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(r);
-    voff[u] = chunk * 8 < p.D ? r * (int)p.q_ss * 2 + chunk * 16 : kNoColumn;
+    voff[u] = chunk * 8 < p.D ? ((r >> p.fold) * (int)p.q_ss + (r & heads) * (int)p.q_sh) * 2 + chunk * 16 : kNoColumn;
   }
+  const int l_off = ((ln >> p.fold) + (ln & heads) * (int)p.l_sh) * 4;
   typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8;
   typedef __attribute__((address_space(3))) const float* lds_float;
   float scale_log2 = p.scale_log2;
@@ -398,24 +404,26 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
       __builtin_amdgcn_s_barrier();              // (the item before is through with the ring)
       const int qt0 = st.first(kt);
 
-      // ---- query tiles: step i is tile qt of head h, tiles fastest ---------------------------------------------------------------
-      const int of_head = st.queries - qt0;
-      int copy_h = first / of_head, copy_qt = qt0 + first - copy_h * of_head, left = count;      // of the next copies, those that are left
+      // ---- query tiles: step i is tile qt of a group of heads, tiles fastest -------------------------------------------------------
+      const int of_group = st.queries - qt0, group0 = first / of_group;
+      int copy_qt = qt0 + first - group0 * of_group, left = count;       // of the next copies, those that are left
       int qt = copy_qt;
-      const uint16_t* q_head = p.q + b * p.q_sb + (int64_t)s.start * p.q_ss + (int64_t)(hk * p.G + copy_h) * p.q_sh;
-      const float* l_head = p.lse + b * p.l_sb + s.start + (int64_t)(hk * p.G + copy_h) * p.l_sh;
+      const int head0 = hk * p.G + (group0 << p.fold);
+      const uint16_t* q_group = p.q + b * p.q_sb + (int64_t)s.start * p.q_ss + (int64_t)head0 * p.q_sh;
+      const float* l_group = p.lse + b * p.l_sb + s.start + (int64_t)head0 * p.l_sh;
+      // (tokens past the last: zeros, or a row that there is, where q lies by heads; they are masked)
       auto copy = [&](int stage) __attribute__((always_inline)) {
-        const int row0 = copy_qt * kQueries, rows = s.n - row0 < kQueries ? s.n - row0 : kQueries;
-        const u32x4 rs = rsrc_words(q_head + (int64_t)row0 * p.q_ss, (uint32_t)(((rows - 1) * (int)p.q_ss + p.D) * 2));
+        const int token0 = copy_qt * tokens, here = s.n - token0 < tokens ? s.n - token0 : tokens;
+        const u32x4 rs = rsrc_words(q_group + (int64_t)token0 * p.q_ss, (uint32_t)(((here - 1) * (int)p.q_ss + heads * (int)p.q_sh + p.D) * 2));
 #pragma unroll
         for (int u = 0; u < 2; ++u) copy16_to_lds(rs, lds + stage * kStageBytes + (wave * 2 + u) * 1024, voff[u], 0);
-        copy4_to_lds(rsrc_words(l_head + row0, (uint32_t)rows * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, ln * 4, 0);
+        copy4_to_lds(rsrc_words(l_group + token0, (uint32_t)(heads * (int)p.l_sh + here) * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, l_off, 0);
         if (left > 1) {                          // (past the share's last tile that one again)
           --left;
           if (++copy_qt == st.queries) {
             copy_qt = qt0;
-            q_head += p.q_sh;
-            l_head += p.l_sh;
+            q_group += p.q_sh << p.fold;
+            l_group += p.l_sh << p.fold;
           }
         }
       };
@@ -460,19 +468,19 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
         __builtin_amdgcn_s_barrier();
         copy(kStage);
         // rows past the last, and those that saw no key, weigh nothing
-        const int row0 = qt * kQueries;
+        const int token0 = qt * tokens, token = token0 + (ln >> p.fold);
         const float mine = lse[kStage & 1];
         float minus = mine * -kLog2e;
         if (++qt == st.queries) qt = qt0;
-        if (p.causal && key_at > old_keys + row0 + kQueries - 1) {       // nobody sees any of them
+        if (p.causal && key_at > old_keys + token0 + tokens - 1) {       // nobody sees any of them
           product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [](int) {});
         } else {
-        if (__builtin_expect((p.causal && key_at + 63 > old_keys + row0) || row0 + kQueries > s.n ||
+        if (__builtin_expect((p.causal && key_at + 63 > old_keys + token0) || token0 + tokens > s.n ||
                              __builtin_amdgcn_ballot_w64(mine == -INFINITY) != 0, 0)) {
           asm volatile("");
-          const bool counts = row0 + ln < s.n && mine != -INFINITY;
+          const bool counts = token < s.n && mine != -INFINITY;
           // keys that the row sees, from the lane's first one
-          const int seen = counts ? (p.causal ? old_keys + row0 + ln + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
+          const int seen = counts ? (p.causal ? old_keys + token + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
           if (!counts) minus = 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -637,6 +645,9 @@ extern "C" int mhip_paged_attn_weights(const void* q, const void* k_cache, const
     if (!aligned16(workspace)) return MHIP_EALIGN;
     p.parts = static_cast<float*>(workspace);
     p.shared = reinterpret_cast<int*>(p.parts + (int64_t)kManyWorkers * 2 * kKeys);
+    // (heads share query tiles where the tokens of one would be few: 16 tokens of 16 heads on one at 8 x 4000 keys 33.0 us, 17.9 so, one of 64 89.2, 16.8;
+    // a prompt of 8192 274 and 280)
+    while (p.fold < 5 && ((int64_t)most_new << p.fold) < 4 * kQueries && (p.G >> p.fold) % 2 == 0 && (q_sh << (p.fold + 1)) <= kFarHeads && (p.l_sh << (p.fold + 1)) <= kFarHeads) ++p.fold;
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == MHIP_E2M1) launch<MHIP_E2M1>(p, rows, st);
