@@ -152,10 +152,14 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
     const int row = u * kCopyRows + lane / kChunks, chunk = (lane % kChunks) ^ swizzle<ROWB>(row);
     voff[u] = chunk * 16 < row_bytes(TYPE, p.D) ? row * (int)p.c_ss16 * 16 + chunk * 16 : kNoColumn;
   }
+  // Scales: lanes 0 .. 31 copy the keys', 16 of each half, the others the values'.  (Without a page there is nothing that could be read but q.)
+  const float* scales_of_lane = reinterpret_cast<const float*>(p.q);
+  if (SCALED && p.g.pages > 0) scales_of_lane = (lane >> 5 ? p.v_scales : p.k_scales) + ln * p.s_ss;
   // K operand: 16 bytes of row ln; in e4m3 they serve two k-steps of 32 columns; in e2m1 all four of 128 columns, and 8 bytes both of 64, and they
   // are of one block of 32 columns
   constexpr int KR = E2M1 ? 1 : E4M3 ? KB / 2 : KB;    // reads of a K row
   const int k_block = COLS == 128 ? lg : lg >> 1;      // (e2m1)
+  const int k_byte_a = (int)ring + 2 * kTileBytes + ln * 4 + k_block;
   int k_a[KR];
   if constexpr (E2M1) k_a[0] = (int)ring + ln * ROWB + ((k_block ^ swizzle<ROWB>(ln)) << 4) + (COLS == 128 ? 0 : (lg & 1) * 8);
   else {
@@ -268,10 +272,11 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
       }
     };
     auto copy_k = [&](int stage) {
-      if constexpr (SCALED) {
-        const int h = (lane >> 4) & 1, row = ln < held[h] ? ln : held[h] - 1;
-        const float* at = (lane >> 5 ? p.v_scales : p.k_scales) + (page[h] * p.s_sp + (slot[h] + row) * p.s_ss + hk * p.s_sh);
-        copy4_to_lds(held[h] > 0 ? static_cast<const void*>(at) : p.q, ring + stage * kStage + 2 * kTileBytes);
+      if constexpr (SCALED) {                          // (of all 16 rows: past the last key the page has them too)
+        int64_t from[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) from[h] = held[h] > 0 ? page[h] * p.s_sp + slot[h] * p.s_ss + hk * p.s_sh : 0;
+        copy4_to_lds(scales_of_lane + (lane & 16 ? from[1] : from[0]), ring + stage * kStage + 2 * kTileBytes);
       }
       copy(p.k, stage * kStage);
     };
@@ -315,37 +320,51 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
 #pragma unroll
       for (int r0 = 0; r0 < NR; r0 += kPair) {
         f32x4 sc[2][kPair];
+        if constexpr (E2M1) {
+          // (everything that is read comes in one round, and the two halves' products take turns: neither waits for its own)
+          u32x4 w[2];
+          uint32_t byte[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          if constexpr (E2M1) {
-            u32x4 w{};
-            if constexpr (COLS == 128) w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[0] + at + kb * 16 * ROWB);
+          for (int kb = 0; kb < 2; ++kb) {
+            w[kb] = u32x4{};
+            if constexpr (COLS == 128) w[kb] = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[0] + at + kb * 16 * ROWB);
             else {
               const u32x2 x = *(lds_u32x2)(uintptr_t)(uint32_t)(k_a[0] + at + kb * 16 * ROWB);
-              w[0] = x[0];
-              w[1] = x[1];
+              w[kb][0] = x[0];
+              w[kb][1] = x[1];
             }
-            const uint32_t byte = *(lds_byte)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + (kb * 16 + ln) * 4 + k_block);
-            const float scale = k_block * 32 < p.D ? e8m0(byte) : 1.f;         // (past the last column there may be anything)
-#pragma unroll
-            for (int ks = 0; ks < KB; ++ks) {
-              const bf16x8 kf = __builtin_bit_cast(bf16x8, e2m1_to_bf16(w[ks], scale));
-#pragma unroll
-              for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
-            }
-          } else
-#pragma unroll
-          for (int i = 0; i < KR; ++i) {
-            const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
-#pragma unroll
-            for (int e = 0; e < KB / KR; ++e) {
-              const bf16x8 kf = E4M3 ? e4m3_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
-              const int ks = E4M3 ? 2 * i + e : i;
-#pragma unroll
-              for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
-            }
+            byte[kb] = *(lds_byte)(uintptr_t)(uint32_t)(k_byte_a + at + kb * 64);
+            if (r0 == 0) v_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + 128 + kb * 64 + lg * 16);
           }
-        if (SCALED && r0 == 0)
+          float scale[2];                              // (past the last column there may be anything)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) scale[kb] = k_block * 32 < p.D ? e8m0(byte[kb]) : 1.f;
+#pragma unroll
+          for (int ks = 0; ks < KB; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              const bf16x8 kf = __builtin_bit_cast(bf16x8, e2m1_to_bf16(w[kb][ks], scale[kb]));
+#pragma unroll
+              for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
+            }
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) asm volatile("" : "+v"(v_scale[kb]));
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+              const u32x4 w = *(lds_u32x4)(uintptr_t)(uint32_t)(k_a[i] + at + kb * 16 * ROWB);
+#pragma unroll
+              for (int e = 0; e < KB / KR; ++e) {
+                const bf16x8 kf = E4M3 ? e4m3_to_bf16(w[2 * e], w[2 * e + 1]) : __builtin_bit_cast(bf16x8, w);
+                const int ks = E4M3 ? 2 * i + e : i;
+#pragma unroll
+                for (int r = 0; r < kPair; ++r) sc[kb][r] = mfma(kf, qf[r0 + r][ks], ks == 0 ? f32x4{} : sc[kb][r]);
+              }
+            }
+        }
+        if (E4M3 && r0 == 0)
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             k_scale[kb] = *(lds_f32x4)(uintptr_t)(uint32_t)(ring + at + 2 * kTileBytes + kb * 64 + lg * 16);
@@ -439,6 +458,9 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
                 for (int j = 0; j < 4; ++j) quads[r][kb][j] = j < left ? quads[r][kb][j] : 0u;
               }
             }
+          i32x2 codes[VR];
+#pragma unroll
+          for (int c = 0; c < VR; ++c) codes[c] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2)(uintptr_t)(uint32_t)(v_a[c] + at));
 #pragma unroll
           for (int c = 0; c < VR; ++c) {
 #pragma unroll
@@ -450,10 +472,9 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
 #pragma unroll
               for (int i = 0; i < 4; ++i) pw[r][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
             }
-            const i32x2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2)(uintptr_t)(uint32_t)(v_a[c] + at));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const bf16x8 vf = __builtin_bit_cast(bf16x8, e2m1_to_bf16((uint32_t)codes[e], 1.f));
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, e2m1_to_bf16((uint32_t)codes[c][e], 1.f));
 #pragma unroll
               for (int r = 0; r < kPair; ++r) weigh(2 * c + e, r0 + r, vf, pw[r], pl[r]);
             }
