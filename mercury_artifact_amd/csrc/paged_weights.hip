@@ -475,40 +475,42 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
         if (p.causal && key_at > old_keys + token0 + tokens - 1) {       // nobody sees any of them
           product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [](int) {});
         } else {
-        if (__builtin_expect((p.causal && key_at + 63 > old_keys + token0) || token0 + tokens > s.n ||
-                             __builtin_amdgcn_ballot_w64(mine == -INFINITY) != 0, 0)) {
-          asm volatile("");
-          const bool counts = token < s.n && mine != -INFINITY;
-          // keys that the row sees, from the lane's first one
-          const int seen = counts ? (p.causal ? old_keys + token + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
-          if (!counts) minus = 0.f;
+          if (__builtin_expect((p.causal && key_at + 63 > old_keys + token0) || token0 + tokens > s.n ||
+                               __builtin_amdgcn_ballot_w64(mine == -INFINITY) != 0, 0)) {
+            asm volatile("");
+            const bool counts = token < s.n && mine != -INFINITY;
+            // keys that the row sees, from the lane's first one
+            const int seen = counts ? (p.causal ? old_keys + token + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
+            // (an lse that is no number is that of the keys that the row sees, not of the others: they stay at -inf)
+            const float odd = counts && !(minus < INFINITY) ? minus : 0.f;
+            if (!counts || odd != 0.f) minus = 0.f;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if ((e >> 4) * 32 + 8 * (e >> 2 & 3) + (e & 3) >= seen) now[e >> 4][e & 15] = -INFINITY;
-            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < 32; ++e) {
+              now[e >> 4][e & 15] = (e >> 4) * 32 + 8 * (e >> 2 & 3) + (e & 3) >= seen ? -INFINITY : now[e >> 4][e & 15] + odd;
+              if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
           }
-        }
-        // Behind MFMA m the next weights' multiply-adds, the exponentials of those before, and the sums of those before them: none waits for another.
-        constexpr int kEach = (32 + 2 * KB - 3) / (2 * KB - 2);
-        auto ahead = [&](int e) __attribute__((always_inline)) {
-          if (e < 32) now[e >> 4][e & 15] = __builtin_fmaf(now[e >> 4][e & 15], scale_log2, minus);
-        };
-        auto power = [&](int e) __attribute__((always_inline)) {
-          if (e >= 0 && e < 32) now[e >> 4][e & 15] = fast_exp2(now[e >> 4][e & 15]);
-        };
-        auto add = [&](int e) __attribute__((always_inline)) {
-          if (e >= 0 && e < 32) sum[e] += now[e >> 4][e & 15];
-        };
-        product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [&](int m) __attribute__((always_inline)) {
+          // Behind MFMA m the next weights' multiply-adds, the exponentials of those before, and the sums of those before them: none waits for another.
+          constexpr int kEach = (32 + 2 * KB - 3) / (2 * KB - 2);
+          auto ahead = [&](int e) __attribute__((always_inline)) {
+            if (e < 32) now[e >> 4][e & 15] = __builtin_fmaf(now[e >> 4][e & 15], scale_log2, minus);
+          };
+          auto power = [&](int e) __attribute__((always_inline)) {
+            if (e >= 0 && e < 32) now[e >> 4][e & 15] = fast_exp2(now[e >> 4][e & 15]);
+          };
+          auto add = [&](int e) __attribute__((always_inline)) {
+            if (e >= 0 && e < 32) sum[e] += now[e >> 4][e & 15];
+          };
+          product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-          for (int e = 0; e < kEach; ++e) power((m - 1) * kEach + e);
+            for (int e = 0; e < kEach; ++e) power((m - 1) * kEach + e);
 #pragma unroll
-          for (int e = 0; e < kEach; ++e) ahead(m * kEach + e);
+            for (int e = 0; e < kEach; ++e) ahead(m * kEach + e);
 #pragma unroll
-          for (int e = 0; e < kEach; ++e) add((m - 2) * kEach + e);
-        });
+            for (int e = 0; e < kEach; ++e) add((m - 2) * kEach + e);
+          });
 #pragma unroll
-        for (int e = (2 * KB - 2) * kEach; e < 32; ++e) add(e);
+          for (int e = (2 * KB - 2) * kEach; e < 32; ++e) add(e);
         }
         if (kStage == 3 && (i & (kFlush - 1)) == kFlush - 1) {
           asm volatile("");

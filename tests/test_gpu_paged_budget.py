@@ -243,6 +243,97 @@ def test_weights_are_the_same_in_every_call():
         assert abs(total - 3 * new * 8) <= 3 * new * 8 * 1e-4
 
 
+@pytest.mark.parametrize("new", [1, 20, 100])
+def test_a_row_whose_lse_is_no_number_counts_for_the_keys_that_it_sees(new):
+    """Queries that are no numbers, and weights past the largest: the keys behind the row's token have nothing of them."""
+    s = Setting(torch.bfloat16, [230, 90], 2, 64, seed=4)
+    q = torch.randn(2, new, 4, 64, generator=s.g).bfloat16()
+    lse = _lse(s, q, 0.1)
+    for b, h, i, what in ((0, 1, 0, math.nan), (1, 2, new // 2, -2.0 ** 127), (1, 0, max(new - 11, 0), math.nan)):
+        lse[b, h, i] = what
+        if math.isnan(what):
+            q[b, i, h] = what
+    before = s.weights.cpu()
+    got = _weigh(s, q, lse, 0.1)
+    _check(got, s, q, lse, 0.1, before)
+    assert new == 1 or torch.isfinite(got[s.table[0][-1]]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAMES)
+@pytest.mark.parametrize("lengths,new,G,D,causal", [
+    ([300, 41], 41, 3, 64, True),
+    ([300, 41], 41, 6, 128, True),
+    ([290, 530], 12, 6, 96, False),
+    ([290, 9], 9, 16, 64, True),
+    ([260, 517], 2, 64, 128, True),
+    ([70, 31], 31, 64, 64, False),
+    ([5, 257], 33, 32, 32, True),                    # more new tokens than keys
+    ([513], 129, 2, 64, True),
+])
+@pytest.mark.parametrize("by_heads", [False, True], ids=["by_tokens", "by_heads"])
+def test_weights_of_chunks_of_grouped_heads(lengths, new, G, D, causal, by_heads, kind):
+    """A tile of rows is of several tokens and heads, whichever of them lies farther apart."""
+    print(f"case {lengths} new {new} G{G} D{D} causal {causal} {kind} by heads {by_heads}", flush=True)
+    s = Setting(kind, lengths, 2, D, seed=G + new)
+    q = torch.randn(len(lengths), new, 2 * G, D, generator=s.g).bfloat16()
+    lse, before = _lse(s, q, D ** -0.5, causal), s.weights.cpu()
+    laid = q.cuda().transpose(1, 2).contiguous().transpose(1, 2) if by_heads else q.cuda()
+    _check(_weigh(s, laid, lse, D ** -0.5, causal), s, q, lse, D ** -0.5, before, causal)
+
+
+@pytest.mark.parametrize("new,Hq", [(70, 2), (5, 32)])
+@pytest.mark.parametrize("far", [(1 << 23) + 8, (1 << 20) + 8])
+def test_weights_of_queries_that_lie_far_apart(new, Hq, far):
+    """Tokens, then heads, whose distances pass what a descriptor spans."""
+    s = Setting(torch.bfloat16, [200], 1, 64, seed=new)
+    q = torch.randn(1, new, Hq, 64, generator=s.g).bfloat16()
+    lse, before = _lse(s, q, 0.125), s.weights.cpu()
+    for steps in ((far, 64), (64, far)):
+        laid = torch.empty((new if steps[0] == far else Hq) * far, dtype=torch.bfloat16, device="cuda")
+        laid = laid.as_strided((1, new, Hq, 64), (far, *steps, 1)).copy_(q)
+        out = torch.zeros_like(s.weights)
+        M.paged_attn_weights(laid, s.dev, *s.tables(), 0.125, lse.cuda(), s.weights, out=out)
+        held = torch.zeros(before.shape, dtype=torch.bool)
+        for j in range(200):
+            held[s.table[0][j // 16], j % 16] = True
+        _check(torch.where(held, out.cpu(), before), s, q, lse, 0.125, before)
+
+
+@pytest.mark.parametrize("new", [3, 90])
+def test_weights_of_e4m3_keys_whose_scales_are_any_numbers(new):
+    """Long chunks take scale times code rounded to bf16, off by up to 2^-8 of each product, and a weight by as much of their sum."""
+    s = Setting(E4M3, [190], 2, 64, seed=new)
+    times = torch.rand(s.scales.shape, generator=s.g) * 0.9 + 0.55
+    s.scales.mul_(times.cuda())
+    dense = M.paged_cache_read(s.dev.view(torch.uint8).clone().view(E4M3), *s.tables(), 190, scales=torch.ones_like(s.scales)).cpu().double()
+    scales = s.scales.cpu().double()
+    for j in range(190):
+        at = s.table[0][j // 16], j % 16
+        s.values[:, at[0], at[1]] = dense[:, 0, j] * scales[:, at[0], at[1]].view(2, 2, 1)
+    q = torch.randn(1, new, 4, 64, generator=s.g).bfloat16()
+    lse, before = _lse(s, q, 0.125), s.weights.cpu()
+    got = _weigh(s, q, lse, 0.125, decay=0.0)
+    want, off = P.paged_weights(q, s.values, s.table, s.lengths, 0.125, lse, before, True, None, 0.0)
+    x = torch.stack([s.values[0, s.table[0][j // 16], j % 16] for j in range(190)])                  # (190, 2, 64)
+    for h in range(4):
+        for i in range(new):
+            sees = 190 - new + i + 1
+            score, size = x[:sees, h // 2] @ q[0, i, h].double() * 0.125, x[:sees, h // 2].abs() @ q[0, i, h].double().abs() * 0.125
+            more = torch.exp(score - lse[0, h, i].double()) * (torch.exp(size * 2.0 ** -8) - 1)
+            for j in range(sees):
+                off[s.table[0][j // 16], j % 16, h // 2] += more[j]
+    assert ((got.double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("lengths,new,Hq,Hkv", [([1500], [1500], 2, 1), ([1300, 290, 40], [900, 33, 40], 4, 2), ([2050], [130], 8, 1)])
+def test_weights_of_prompts_that_many_workgroups_share(lengths, new, Hq, Hkv):
+    s = Setting(torch.bfloat16, lengths, Hkv, 64, seed=Hq)
+    starts = [sum(new[:b]) for b in range(len(new) + 1)]
+    q = torch.randn(starts[-1], Hq, 64, generator=s.g).bfloat16()
+    lse, before = _lse(s, q, 0.125, starts=starts), s.weights.cpu()
+    _check(_weigh(s, q, lse, 0.125, starts=starts), s, q, lse, 0.125, before, starts=starts)
+
+
 # ---- eviction ------------------------------------------------------------------------------------------------------------------
 
 def _rows(s, table, kept):
