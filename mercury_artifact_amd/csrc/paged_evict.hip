@@ -35,6 +35,28 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// Lane l's with those of lanes 0 .. l - 1, by f; `none` takes no part in it.  (In registers: a shuffle is a trip through LDS.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved_lanes(uint32_t x, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <class F>
+__device__ __forceinline__ uint32_t up_to_lane(uint32_t x, uint32_t none, F&& f) {
+  x = f(x, moved_lanes<0x111, 0xf>(x, none));    // 1, 2, 4 and 8 lanes further up within rows of 16
+  x = f(x, moved_lanes<0x112, 0xf>(x, none));
+  x = f(x, moved_lanes<0x114, 0xf>(x, none));
+  x = f(x, moved_lanes<0x118, 0xf>(x, none));
+  x = f(x, moved_lanes<0x142, 0xa>(x, none));    // the last of rows 0 and 2 to rows 1 and 3
+  return f(x, moved_lanes<0x143, 0xc>(x, none)); // lane 31 to rows 2 and 3
+}
+// Of what the wavefronts have left, the sum over those before this one.
+__device__ __forceinline__ uint32_t before_wave(const uint32_t (&waves)[kChooserWaves], int wave) {
+  uint32_t sum = 0;
+#pragma unroll
+  for (int v = 0; v < kChooserWaves; ++v) sum += v < wave ? waves[v] : 0u;
+  return sum;
+}
+
 constexpr int kDigits = 2048, kListed = 24576;
 struct ChooserLds {
   uint32_t count[kDigits];
@@ -87,17 +109,15 @@ __device__ __forceinline__ void choose(const Evict& p, ChooserLds& lds, const in
       high = real && v > high ? v : high;
       low = real && v < low ? v : low;
     });
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const uint32_t h = __shfl_xor(high, off), l = __shfl_xor(low, off);
-      high = h > high ? h : high;
-      low = l < low ? l : low;
-    }
-    if (lane == 0) {
+    high = up_to_lane(high, 0u, [](uint32_t a, uint32_t c) { return a > c ? a : c; });
+    low = up_to_lane(low, 0xffffffffu, [](uint32_t a, uint32_t c) { return a < c ? a : c; });
+    if (lane == 63) {
       lds.waves[0][wave] = high;
       lds.waves[1][wave] = low;
     }
     __syncthreads();
+    high = 0;
+    low = 0xffffffffu;
 #pragma unroll
     for (int v = 0; v < kChooserWaves; ++v) {
       high = lds.waves[0][v] > high ? lds.waves[0][v] : high;
@@ -128,16 +148,10 @@ __device__ __forceinline__ void choose(const Evict& p, ChooserLds& lds, const in
     __syncthreads();
     // thread t has the digits 2047 - 2 t and 2046 - 2 t: how many are above them, and in which of them the last one kept is
     const uint32_t c0 = lds.count[kDigits - 1 - 2 * tid], c1 = lds.count[kDigits - 2 - 2 * tid];
-    uint32_t higher = c0 + c1;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t v = __shfl_up(higher, off);
-      if (lane >= off) higher += v;
-    }
+    uint32_t higher = up_to_lane(c0 + c1, 0u, [](uint32_t a, uint32_t c) { return a + c; });
     if (lane == 63) lds.waves[0][wave] = higher;
     __syncthreads();
-    for (int v = 0; v < wave; ++v) higher += lds.waves[0][v];
-    higher -= c0 + c1;
+    higher += before_wave(lds.waves[0], wave) - c0 - c1;
     if (higher < need && need <= higher + c0 + c1) {
       const bool upper = need <= higher + c0;
       lds.found[0] = kDigits - 1 - 2 * tid - (upper ? 0 : 1);
@@ -192,11 +206,8 @@ __device__ __forceinline__ void choose(const Evict& p, ChooserLds& lds, const in
     }
   }
   __syncthreads();
-  above = equal = 0;
-  for (int v = 0; v < wave; ++v) {
-    above += lds.waves[0][v];
-    equal += lds.waves[1][v];
-  }
+  above = before_wave(lds.waves[0], wave);
+  equal = before_wave(lds.waves[1], wave);
   const uint64_t below = (1ull << lane) - 1;
   all([&](int at, uint32_t v, bool real) {
     const uint64_t mask_above = __builtin_amdgcn_ballot_w64(real && v > last), mask_equal = __builtin_amdgcn_ballot_w64(real && v == last);
