@@ -36,7 +36,7 @@ struct Gather {
   int Hkv, G, D, causal;
   float scale_log2, decay;
   Divisor by_group;
-  int fold;                                      // paged_weights_many: log2 of the heads in a query tile
+  int most_fold;                                 // paged_weights_many: log2 of the heads that a query tile may have
   float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
 };
 
@@ -232,17 +232,27 @@ constexpr int kNoColumn = 0x7fff0000;            // vector offset out of every d
 constexpr int64_t kFarRows = 1 << 23, kFarHeads = 1 << 24;       // elements between tokens, and between the heads of a tile, that paged_weights_many takes
 constexpr int kFlush = 64;                       // steps whose weights are added up in a register
 
-// Items of a sequence and K/V head: tiles of 256 keys.  A query tile is 32 / F tokens of F heads, so that short chunks of grouped heads
-// fill it too (F: the largest power of two up to 32 that divides G).  Key tile k is seen by the query tiles from max(0, 8 F k + z) on
-// (all, without a mask), and its steps are those of G / F groups of heads.
+// Items of a sequence and K/V head: tiles of 256 keys.  A query tile is 32 / F tokens of F heads, F a power of two, so that short chunks of
+// grouped heads fill it too; heads past the last of a K/V head are masked.  F grows while the query tiles become no more and a group of heads
+// has less than four.  Key tile k is seen by the query tiles from max(0, 8 F k + z) on (all, without a mask), of each group of heads.
 struct Steps {
   int tiles, queries, fold, groups, flat, z;     // key tiles, query tiles of a group, log2 F, groups; key tiles that all query tiles see
   int64_t all;                                   // of all key tiles
+  __device__ __forceinline__ Steps() {}
   __device__ __forceinline__ Steps(const Gather& p, const PagedSeq& s) {
     tiles = (s.len + kKeys - 1) / kKeys;
-    fold = p.fold;
-    queries = (int)((((int64_t)s.n << fold) + kQueries - 1) / kQueries);
-    groups = p.G >> fold;
+    auto tiles_of = [&](int f) { return (int)((((int64_t)s.n << f) + kQueries - 1) / kQueries); };
+    auto groups_of = [&](int f) { return (p.G + (1 << f) - 1) >> f; };
+    fold = 0;
+    queries = tiles_of(0);
+    groups = p.G;
+    while (fold < p.most_fold && (int64_t)s.n << fold < 4 * kQueries && groups > 1) {
+      const int q = tiles_of(fold + 1), g = groups_of(fold + 1);
+      if (q * g > queries * groups) break;       // (both below 128 or G: far below 2^31)
+      queries = q;
+      groups = g;
+      ++fold;
+    }
     z = p.causal ? (s.n - s.len) >> (5 - fold) : 0;        // (floor)
     flat = !p.causal ? tiles : z > 0 ? 0 : (-z >> (3 + fold)) + 1;
     flat = flat < tiles ? flat : tiles;
@@ -279,13 +289,11 @@ __device__ __forceinline__ Place place_of(const Gather& p, int b, int key, int l
   if ((uint32_t)at.page >= (uint32_t)p.g.pages) at.page = -1;
   return at;
 }
-__device__ __forceinline__ void leave(const Gather& p, const PagedSeq& s, const Place& at, int hk, int key, float sum) {
-  if (at.page < 0) return;
-  if ((s.n == 0 || p.decay != 0.f) && key < (s.n == 0 ? s.len : s.len - s.n)) {
-    const float old = p.old[(int64_t)at.page * p.w_sp + (int64_t)at.slot * p.w_ss + (int64_t)hk * p.w_sh];
-    sum += s.n == 0 ? old : p.decay * old;
-  }
-  p.out[(int64_t)at.page * p.o_sp + (int64_t)at.slot * p.o_ss + (int64_t)hk * p.o_sh] = sum;
+// What a key had of its weight that counts on.
+__device__ __forceinline__ float had_before(const Gather& p, const PagedSeq& s, const Place& at, int hk, int key) {
+  if (at.page < 0 || (s.n > 0 && p.decay == 0.f) || key >= (s.n == 0 ? s.len : s.len - s.n)) return 0.f;
+  const float old = p.old[(int64_t)at.page * p.w_sp + (int64_t)at.slot * p.w_ss + (int64_t)hk * p.w_sh];
+  return s.n == 0 ? old : p.decay * old;
 }
 
 template <int TYPE, int COLS>
@@ -322,108 +330,168 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
 #pragma unroll
   for (int ks = 0; ks < KB; ++ks) q_a[ks] = (int)lds + ln * 256 + (((2 * ks + lg) ^ lds_row_swizzle(ln)) << 4);
   const int lse_a = (int)lds + kQueryTile + wave * 256 + ln * 4;
-  // copies of a query tile, row r of which is token r / F and head r % F: four rows each, columns past the last are zeros
-  const int heads = (1 << p.fold) - 1, tokens = kQueries >> p.fold;
-  int voff[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r = wave * 8 + u * 4 + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(r);
-    voff[u] = chunk * 8 < p.D ? ((r >> p.fold) * (int)p.q_ss + (r & heads) * (int)p.q_sh) * 2 + chunk * 16 : kNoColumn;
-  }
-  const int l_off = ((ln >> p.fold) + (ln & heads) * (int)p.l_sh) * 4;
   typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8;
   typedef __attribute__((address_space(3))) const float* lds_float;
   float scale_log2 = p.scale_log2;
   asm volatile("" : "+s"(scale_log2));
 
-  while (lo < hi) {
-    const PagedSeq s = paged_seq<true>(p.g, b);
-    const Steps st(p, s);
-    if (pos >= st.all * p.Hkv) {
-      pos -= st.all * p.Hkv;
-      ++b;
-      continue;
+  PagedSeq s{};
+  Steps st;
+  int heads = 0, tokens = 0, voff[2] = {}, l_off = 0;
+  int hk = 0, kt = 0, from = 0;                  // the next item, and the units of it that lie in shares before this one
+  for (bool enters = true; lo < hi;) {
+    if (enters) {                                // sequence b, `pos` units behind its first
+      s = paged_seq<true>(p.g, b);
+      st = Steps(p, s);
+      if (pos >= st.all * p.Hkv) {
+        pos -= st.all * p.Hkv;
+        ++b;
+        continue;
+      }
+      enters = false;
+      hk = kt = from = 0;
+      if (pos > 0) {
+        hk = (int)(pos / st.all);
+        const int64_t in_head = pos - hk * st.all;
+        for (int span = st.tiles; span > 1;) {   // the last key tile that begins at or before in_head
+          const int half = span / 2;
+          if (st.before(kt + half) <= in_head) { kt += half; span -= half; }
+          else span = half;
+        }
+        from = (int)(in_head - st.before(kt));
+      }
+      // copies of a query tile, row r of which is token r / F and head r % F: four rows each, columns past the last are zeros
+      heads = (1 << st.fold) - 1;
+      tokens = kQueries >> st.fold;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = wave * 8 + u * 4 + (lane >> 4), chunk = (lane & 15) ^ lds_row_swizzle(r);
+        voff[u] = chunk * 8 < p.D ? ((r >> st.fold) * (int)p.q_ss + (r & heads) * (int)p.q_sh) * 2 + chunk * 16 : kNoColumn;
+      }
+      l_off = ((ln >> st.fold) + (ln & heads) * (int)p.l_sh) * 4;
     }
-    const int hk = (int)(pos / st.all);
-    const int64_t in_head = pos - hk * st.all;
-    int kt = 0;                                  // the last key tile that begins at or before in_head
-    for (int span = st.tiles; span > 1;) {
-      const int half = span / 2;
-      if (st.before(kt + half) <= in_head) { kt += half; span -= half; }
-      else span = half;
-    }
-    const int steps = st.of(kt), cost = st.cost(kt), weight = cost + kPause, from = (int)(in_head - st.before(kt));
+    const int item_b = b, item_hk = hk, item_kt = kt;
+    const int steps = st.of(kt), cost = st.cost(kt), weight = cost + kPause;
     const int take = (int)(weight - from < hi - lo ? weight - from : hi - lo);
-    auto step_at = [&](int unit) { return unit > kPause ? (int)((int64_t)(unit - kPause) * steps / cost) : 0; };
-    const int first = step_at(from), count = step_at(from + take) - first;
+    int first = 0, count = steps;                // steps of this share
+    if (take < weight) {
+      auto step_at = [&](int unit) { return unit > kPause ? (int)((int64_t)(unit - kPause) * steps / cost) : 0; };
+      first = step_at(from);
+      count = step_at(from + take) - first;
+    }
     const int64_t start = lo - from;             // of the item
+    const bool leaves_none = count == 0 && first == 0 && (steps > 0 || from > 0);        // (with steps before and behind it, it leaves sums of nothing)
     lo += take;
-    pos += take;
-    const int key_at = kt * kKeys + wave * 64;   // the wavefront's first key
-    if (count == 0 && first == 0 && (steps > 0 || from > 0)) continue;      // (with steps before and behind it, it leaves sums of nothing)
+    from = 0;
+    if (++kt == st.tiles) {
+      kt = 0;
+      if (++hk == p.Hkv) {
+        ++b;
+        pos = 0;
+        enters = true;
+      }
+    }
+    if (leaves_none) continue;
+    const int key_at = item_kt * kKeys + wave * 64;          // the wavefront's first key
+    // lane (ln, lg) ends with the sum of register ln: key 32 (ln / 16) + 8 (ln % 16 / 4) + 4 lg + ln % 4, which what it had is read for now
+    const int own = key_at + (ln >> 4) * 32 + ((ln >> 2) & 3) * 8 + lg * 4 + (ln & 3);
+    const Place own_at = place_of(p, item_b, own, s.len);
+    float had = count == steps ? had_before(p, s, own_at, item_hk, own) : 0.f;
 
     float total_sum = 0.f;
     if (count > 0) {
       // ---- keys: A operand, lane (ln, lg) holds columns 16 ks + 8 lg .. +7 of keys ln and 32 + ln, scaled ------------------------
-      bf16x8 kf[2][KB];
+      // (all loads go out before the first is waited for; what is not here reads something that is, and is nothing)
+      constexpr int kCodes = TYPE == MHIP_E2M1 ? 1 : TYPE == MHIP_E4M3 ? 2 : 4;          // words of eight columns
+      uint32_t codes[2][KB][kCodes], scales[2] = {};
+      bool here[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const Place at = place_of(p, b, key_at + kb * 32 + ln, s.len);
-        const uint8_t* row = p.k + ((int64_t)at.page * p.c_sp + (int64_t)at.slot * p.c_ss + (int64_t)hk * p.c_sh);
-        const float* scale = p.k_scales + ((int64_t)at.page * p.s_sp + (int64_t)at.slot * p.s_ss + (int64_t)hk * p.s_sh);
+        const Place at = place_of(p, item_b, key_at + kb * 32 + ln, s.len);
+        here[kb] = at.page >= 0;
+        const int64_t page = here[kb] ? at.page : 0, slot = here[kb] ? at.slot : 0;
+        const uint8_t* row = p.k + (page * p.c_sp + slot * p.c_ss + (int64_t)item_hk * p.c_sh);
+        if constexpr (TYPE != MHIP_BF16)
+          scales[kb] = *reinterpret_cast<const uint32_t*>(p.k_scales + (page * p.s_sp + slot * p.s_ss + (int64_t)item_hk * p.s_sh));
 #pragma unroll
         for (int ks = 0; ks < KB; ++ks) {
           const int col = ks * 16 + lg * 8;
-          kf[kb][ks] = bf16x8{};
-          if (at.page >= 0 && col < p.D) {
-            if constexpr (TYPE == MHIP_E2M1) {
-              const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + col / 2);
-              kf[kb][ks] = __builtin_bit_cast(bf16x8, e2m1_to_bf16(codes, e8m0(reinterpret_cast<const uint8_t*>(scale)[col / 32])));
-            } else if constexpr (TYPE == MHIP_E4M3) {
-              // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
-              const u32x2 codes = *reinterpret_cast<const u32x2*>(row + col);
-              u32x4 x;
+          typedef __attribute__((__vector_size__(kCodes * sizeof(uint32_t)))) uint32_t Words;
+          const Words w = *reinterpret_cast<const Words*>(row + (col < p.D ? col : 0) * kCodes / 2);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], true);
-                x[2 * h] = pack_bf16(a[0] * *scale, a[1] * *scale);
-                x[2 * h + 1] = pack_bf16(c[0] * *scale, c[1] * *scale);
-              }
-              kf[kb][ks] = __builtin_bit_cast(bf16x8, x);
-            } else {
-              kf[kb][ks] = *reinterpret_cast<const bf16x8*>(row + col * 2);
-            }
-          }
+          for (int i = 0; i < kCodes; ++i) codes[kb][ks][i] = w[i];
         }
       }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks)
+#pragma unroll
+          for (int i = 0; i < kCodes; ++i) asm volatile("" : "+v"(codes[kb][ks][i]));
+      bf16x8 kf[2][KB];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KB; ++ks) {
+          const uint32_t (&c)[kCodes] = codes[kb][ks];
+          u32x4 x;
+          if constexpr (TYPE == MHIP_E2M1) {
+            x = e2m1_to_bf16(c[0], e8m0(scales[kb] >> (ks / 2 * 8) & 255u));
+          } else if constexpr (TYPE == MHIP_E4M3) {
+            // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
+            const float scale = __builtin_bit_cast(float, scales[kb]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[h], true);
+              x[2 * h] = pack_bf16(lo[0] * scale, lo[1] * scale);
+              x[2 * h + 1] = pack_bf16(hi[0] * scale, hi[1] * scale);
+            }
+          } else {
+            x = u32x4{c[0], c[1], c[2], c[3]};
+          }
+          const bool real = here[kb] && ks * 16 + lg * 8 < p.D;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = real ? x[i] : 0u;
+          kf[kb][ks] = __builtin_bit_cast(bf16x8, x);
+        }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int ks = 0; ks < KB; ++ks) asm volatile("" : "+v"(kf[kb][ks]));       // loaded before the first copy goes out
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();              // (the item before is through with the ring)
-      const int qt0 = st.first(kt);
+      const int qt0 = st.first(item_kt);
 
       // ---- query tiles: step i is tile qt of a group of heads, tiles fastest -------------------------------------------------------
-      const int of_group = st.queries - qt0, group0 = first / of_group;
+      const int of_group = st.queries - qt0, group0 = first == 0 ? 0 : first / of_group;
       int copy_qt = qt0 + first - group0 * of_group, left = count;       // of the next copies, those that are left
       int qt = copy_qt;
-      const int head0 = hk * p.G + (group0 << p.fold);
-      const uint16_t* q_group = p.q + b * p.q_sb + (int64_t)s.start * p.q_ss + (int64_t)head0 * p.q_sh;
-      const float* l_group = p.lse + b * p.l_sb + s.start + (int64_t)head0 * p.l_sh;
-      // (tokens past the last: zeros, or a row that there is, where q lies by heads; they are masked)
+      const int head0 = item_hk * p.G + (group0 << st.fold);
+      int copy_last = p.G - 1 - (group0 << st.fold), here_last = copy_last;        // of the copies' heads, of the next step's: the last there is
+      int q_tail, l_tail;                        // bytes of a copy's descriptors besides those of its tokens
+      auto tails = [&]() __attribute__((always_inline)) {
+        const int top = copy_last < heads ? copy_last : heads;
+        q_tail = (top * (int)p.q_sh + p.D - (int)p.q_ss) * 2;
+        l_tail = top * (int)p.l_sh * 4;
+      };
+      tails();
+      const uint16_t* q_group = p.q + item_b * p.q_sb + (int64_t)s.start * p.q_ss + (int64_t)head0 * p.q_sh;
+      const float* l_group = p.lse + item_b * p.l_sb + s.start + (int64_t)head0 * p.l_sh;
+      // (tokens and heads past the last: zeros, or a row that there is; they are masked)
       auto copy = [&](int stage) __attribute__((always_inline)) {
         const int token0 = copy_qt * tokens, here = s.n - token0 < tokens ? s.n - token0 : tokens;
-        const u32x4 rs = rsrc_words(q_group + (int64_t)token0 * p.q_ss, (uint32_t)(((here - 1) * (int)p.q_ss + heads * (int)p.q_sh + p.D) * 2));
+        const u32x4 rs = rsrc_words(q_group + (int64_t)token0 * p.q_ss, (uint32_t)(here * (int)p.q_ss * 2 + q_tail));
 #pragma unroll
         for (int u = 0; u < 2; ++u) copy16_to_lds(rs, lds + stage * kStageBytes + (wave * 2 + u) * 1024, voff[u], 0);
-        copy4_to_lds(rsrc_words(l_group + token0, (uint32_t)(heads * (int)p.l_sh + here) * 4), lds + stage * kStageBytes + kQueryTile + wave * 256, l_off, 0);
+        copy4_to_lds(rsrc_words(l_group + token0, (uint32_t)(here * 4 + l_tail)), lds + stage * kStageBytes + kQueryTile + wave * 256, l_off, 0);
         if (left > 1) {                          // (past the share's last tile that one again)
           --left;
           if (++copy_qt == st.queries) {
             copy_qt = qt0;
-            q_group += p.q_sh << p.fold;
-            l_group += p.l_sh << p.fold;
+            q_group += p.q_sh << st.fold;
+            l_group += p.l_sh << st.fold;
+            copy_last -= heads + 1;
+            tails();
           }
         }
       };
@@ -468,17 +536,20 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
         __builtin_amdgcn_s_barrier();
         copy(kStage);
         // rows past the last, and those that saw no key, weigh nothing
-        const int token0 = qt * tokens, token = token0 + (ln >> p.fold);
+        const int token0 = qt * tokens, token = token0 + (ln >> st.fold), top = here_last;
         const float mine = lse[kStage & 1];
         float minus = mine * -kLog2e;
-        if (++qt == st.queries) qt = qt0;
+        if (++qt == st.queries) {
+          qt = qt0;
+          here_last -= heads + 1;
+        }
         if (p.causal && key_at > old_keys + token0 + tokens - 1) {       // nobody sees any of them
           product(std::integral_constant<int, (kStage + 1) & 3>{}, sc[(kStage + 1) & 1], lse[(kStage + 1) & 1], [](int) {});
         } else {
-          if (__builtin_expect((p.causal && key_at + 63 > old_keys + token0) || token0 + tokens > s.n ||
+          if (__builtin_expect((p.causal && key_at + 63 > old_keys + token0) || token0 + tokens > s.n || top < heads ||
                                __builtin_amdgcn_ballot_w64(mine == -INFINITY) != 0, 0)) {
             asm volatile("");
-            const bool counts = token < s.n && mine != -INFINITY;
+            const bool counts = token < s.n && (ln & heads) <= top && mine != -INFINITY;
             // keys that the row sees, from the lane's first one
             const int seen = counts ? (p.causal ? old_keys + token + 1 : s.len) - key_at - 4 * lg : (int)0x80000000;
             // (an lse that is no number is that of the keys that the row sees, not of the others: they stay at -inf)
@@ -536,18 +607,16 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
       total_sum += sums_of_lanes(sum, ln);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // copies past the last step
     }
-    // lane (ln, lg) has the sum of register ln: key 32 (ln / 16) + 8 (ln % 16 / 4) + 4 lg + ln % 4
-    const int own = (ln >> 4) * 32 + ((ln >> 2) & 3) * 8 + lg * 4 + (ln & 3);
     if (count == steps) {
-      leave(p, s, place_of(p, b, key_at + own, s.len), hk, key_at + own, total_sum);
+      if (own_at.page >= 0) p.out[(int64_t)own_at.page * p.o_sp + (int64_t)own_at.slot * p.o_ss + (int64_t)item_hk * p.o_sh] = had + total_sum;
       continue;
     }
-    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + wave * 64 + own] = total_sum;
+    p.parts[(2 * (int64_t)w + (first == 0 ? 1 : 0)) * kKeys + own - item_kt * kKeys] = total_sum;
     if (first == 0 && threadIdx.x == 0) {
       const int last = (int)(((start + weight) * shares - 1) / total);           // the workgroup with its last unit
-      p.shared[w * 4 + 1] = b;
-      p.shared[w * 4 + 2] = hk;
-      p.shared[w * 4 + 3] = kt;
+      p.shared[w * 4 + 1] = item_b;
+      p.shared[w * 4 + 2] = item_hk;
+      p.shared[w * 4 + 3] = item_kt;
       p.shared[w * 4] = last - w + 1;
     }
   }
@@ -563,7 +632,7 @@ __global__ __launch_bounds__(kKeys) void paged_weights_join(const Gather p) {
   float sum = p.parts[(2 * (int64_t)w + 1) * kKeys + threadIdx.x];
 #pragma unroll 8
   for (int i = 1; i < parts; ++i) sum += p.parts[2 * (int64_t)(w + i) * kKeys + threadIdx.x];
-  leave(p, s, at, hk, key, sum);
+  if (at.page >= 0) p.out[(int64_t)at.page * p.o_sp + (int64_t)at.slot * p.o_ss + (int64_t)hk * p.o_sh] = had_before(p, s, at, hk, key) + sum;
 }
 
 template <int TYPE>
@@ -649,7 +718,7 @@ extern "C" int mhip_paged_attn_weights(const void* q, const void* k_cache, const
     p.shared = reinterpret_cast<int*>(p.parts + (int64_t)kManyWorkers * 2 * kKeys);
     // (heads share query tiles where the tokens of one would be few: 16 tokens of 16 heads on one at 8 x 4000 keys 33.0 us, 17.9 so, one of 64 89.2, 16.8;
     // a prompt of 8192 274 and 280)
-    while (p.fold < 5 && ((int64_t)most_new << p.fold) < 4 * kQueries && (p.G >> p.fold) % 2 == 0 && (q_sh << (p.fold + 1)) <= kFarHeads && (p.l_sh << (p.fold + 1)) <= kFarHeads) ++p.fold;
+    while (p.most_fold < 5 && (q_sh << (p.most_fold + 1)) <= kFarHeads && (p.l_sh << (p.most_fold + 1)) <= kFarHeads) ++p.most_fold;
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == MHIP_E2M1) launch<MHIP_E2M1>(p, rows, st);
