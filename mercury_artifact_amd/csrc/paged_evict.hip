@@ -8,6 +8,8 @@
 //   workgroup that reads a tile of rows whole, and then writes it, has read whatever it writes over, and rows of later tiles
 //   lie behind everything that it writes: one workgroup walks each (sequence, K/V head, half) from the first row on.  Into other
 //   pages rows are independent, and many workgroups share them.
+// Measured, us: one sequence of 1040 tokens, four heads, to 1024: 7 and 4 (both chains of dependent loads); 32 x 3000 .. 8192 e4m3 H8 D128 to
+// 2048: 13 and 74, the rows at 4.5 TB/s of reading and writing.
 #include "paged.hpp"
 
 namespace mhip {
@@ -69,36 +71,49 @@ struct ChooserLds {
 // The keep - recent with the largest weights of the first `others` positions into kept, in order.  A wavefront has 64 HELD positions in a
 // row in registers.  HELD = 0: as many as there are, read anew each time, three times if all goes well: to count the first digits; to put
 // those with the digit of the last one kept into a list, their other bits and which wavefront's they are; and to leave the positions.
-// (4 x 131072 tokens to 100000, 2 heads: 237 us when every digit was counted over all, 149 so.)
+// (4 x 131072 tokens to 100000, 2 heads: 237 us when every digit was counted over all, 149 so,
+// 115 with the runs below.)
 template <int HELD>
 __device__ __forceinline__ void choose(const Evict& p, ChooserLds& lds, const int* table, int hk, int others, int* kept) {
-  constexpr int kAtOnce = HELD > 0 ? HELD : 16;
+  constexpr int kAtOnce = HELD > 0 && HELD < 16 ? HELD : 16, kRegisters = HELD > 0 ? HELD : kAtOnce;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int each = HELD > 0 ? HELD : (others + kChoosers * kAtOnce - 1) / (kChoosers * kAtOnce) * kAtOnce;
   const int first = wave * each * 64 + lane;
-  uint32_t x[kAtOnce];
-  auto read = [&](int u0) {
-    int slot[kAtOnce], page[kAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int at = first + (u0 + u) * 64;
-      page[u] = table[p.g.by_page.quotient(at < others ? at : others - 1, slot[u])];
-    }
+  // The wavefront's positions from 64 u0 on.  Runs of 16 lie in one page: a lane finds where run `lane` begins, and all take from there
+  // what they need, so that the table is read and the strides are multiplied once for 16 positions.
+  uint32_t x[kRegisters];
+  const float* weights_of_lane = p.weights + ((int64_t)hk * p.w_sh + (lane & 15) * p.w_ss);
+  auto read = [&](int u0, uint32_t* to) __attribute__((always_inline)) {
+    const int run = wave * each * 64 + u0 * 64 + lane * 16;
+    int slot;
+    const int page = table[p.g.by_page.quotient(run < others ? run : (others - 1) & ~15, slot)];
+    const int64_t at = (int64_t)page * p.w_sp + (int64_t)slot * p.w_ss;
     float w[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u)
-      w[u] = p.weights[(int64_t)page[u] * p.w_sp + (int64_t)slot[u] * p.w_ss + (int64_t)hk * p.w_sh];
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int from = (u * 4 + (lane >> 4)) * 4;
+      const uint32_t lo = __builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)at), hi = __builtin_amdgcn_ds_bpermute(from, (int)(at >> 32));
+      w[u] = weights_of_lane[(int64_t)((uint64_t)hi << 32 | lo)];
+    }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) x[u] = order_of(w[u]);
+    for (int u = 0; u < kAtOnce; ++u) to[u] = order_of(w[u]);
   };
   auto all = [&](auto&& f) __attribute__((always_inline)) {              // f(position, its number, whether it is one)
-    for (int u0 = 0; u0 < each; u0 += kAtOnce) {
-      if (HELD == 0) read(u0);
+    if constexpr (HELD > 0) {
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) f(first + (u0 + u) * 64, x[u], first + (u0 + u) * 64 < others);
+      for (int u = 0; u < HELD; ++u) f(first + u * 64, x[u], first + u * 64 < others);
+    } else {
+      for (int u0 = 0; u0 < each; u0 += kAtOnce) {
+        read(u0, x);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) f(first + (u0 + u) * 64, x[u], first + (u0 + u) * 64 < others);
+      }
     }
   };
-  if (HELD > 0) read(0);
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int u0 = 0; u0 < HELD; u0 += kAtOnce) read(u0, x + u0);
+  }
 
   // ---- the bits that all have in common (of many they are not looked for) -----------------------------------------------------
   uint32_t last = 0, need = p.keep - p.recent;
