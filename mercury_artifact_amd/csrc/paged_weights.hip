@@ -5,8 +5,9 @@
 // paged_weights_few: bound by memory, a key's row is read once.  No softmax is left to do, so keys are independent of one another: a
 // wavefront takes a run of units of 32 (bf16) or 64 keys, whose rows go from memory into registers as the B operand of S = Q K^T
 // (v_mfma_f32_16x16x32_bf16) while the queries (A) stay in registers for the run.  Lane (ln, lg) then holds rows 4 lg .. +3 of key ln: their
-// exponentials are added in the lane and over the four lane groups.  The units of all sequences are dealt out evenly to 16 (8 with
-// more than 16 rows) wavefronts on every CU, whose loads are in flight together; no LDS, no barrier, no atomics, so that results are the same in every run.
+// exponentials are added in the lane and over the four lane groups.  The units of all sequences are dealt out evenly to 16 (e4m3 12; 8 with
+// more than 16 rows) wavefronts on every CU, and a unit's loads go out together (4 x 131072 in e2m1, waiting for each scale byte in
+// turn, 93 us, 83 so); no LDS, no barrier, no atomics, so that results are the same in every run.
 //
 // paged_weights_many: for prompts, bound by the vector unit (an exponential, a multiply-add and an add for each 2 D operations of the matrix
 // unit).  Here the keys stay: a workgroup of four wavefronts holds 256 of a (sequence, K/V head), 64 to a wavefront, as the A operand of
@@ -18,8 +19,8 @@
 // the mask, so the tiles of all items are counted in closed form and dealt out evenly, in order; a workgroup whose share ends inside an
 // item leaves partial sums, and paged_weights_join adds those up in their order.
 //
-// Measured, us: a step of 32 x 300 .. 16384 tokens H32/8 D128 in bf16 123 (4.9 TB/s of keys and weights); 64 x 100 .. 2048, five tokens each of
-// H16/8, in e2m1 19.5; a prompt of 8192 tokens H32/8 D128 283 (970 TFLOP/s, with an exponential for each 256 operations).
+// Measured, us: a step of 32 x 300 .. 16384 tokens H32/8 D128 in bf16 122 (4.8 TB/s of keys and weights); 64 x 100 .. 2048, five tokens each of
+// H16/8, in e2m1 19; a prompt of 8192 tokens H32/8 D128 283 (970 TFLOP/s, with an exponential for each 256 operations).
 #include "paged.hpp"
 
 #include <math.h>
@@ -43,9 +44,10 @@ struct Gather {
   float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
 };
 
-// Wavefronts on a SIMD: four where there are registers for them.
-template <int NR>
-constexpr int kFewWaves = NR == 1 ? 4 : 2;
+// Wavefronts on a SIMD: four where there are registers for them; units of e4m3 take more (us, four / three: 4 x 131072 H32/8 154 / 131,
+// 64 x 100 .. 2048 32 / 20; e2m1, which has them, 83 / 86).
+template <int TYPE, int NR>
+constexpr int kFewWaves = NR > 1 ? 2 : TYPE == MHIP_E4M3 ? 3 : 4;
 
 template <int TYPE, int NR>
 constexpr int kBlocksOf = TYPE == MHIP_BF16 || NR == 4 ? 2 : 4;      // 16-key blocks of a unit
@@ -54,7 +56,7 @@ template <int UNIT>
 __device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) { return (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv; }
 
 template <int TYPE, int COLS, int NR>
-__global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Gather p) {
+__global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(const Gather p) {
   constexpr int kBlocks = kBlocksOf<TYPE, NR>, UNIT = 16 * kBlocks, ROWS = 16 * NR;
   constexpr bool E4M3 = TYPE == MHIP_E4M3, E2M1 = TYPE == MHIP_E2M1;
   constexpr int KB = COLS / 32, KR = E2M1 ? 1 : E4M3 ? KB / 2 : KB;      // k-steps of 32 columns, loads of a key's row
@@ -138,50 +140,73 @@ __global__ __launch_bounds__(256, kFewWaves<NR>) void paged_weights_few(const Ga
     };
     if (rows <= ROWS) load_rows(0);
 
-    for (int t = t0; t < t0 + run; ++t) {
-      const int key0 = t * UNIT;
-      u32x4 w4[kBlocks][KR];
-      float mult[kBlocks];
+    // where a lane's columns begin in a row (within the row there is), and its row's scales
+    const int64_t row_of_lane = ln * p.c_ss + (E2M1 ? (k_block * 32 < p.D ? lg * (COLS == 128 ? 16 : 8) : 0) : lg * 16);
+    const int64_t scale_of_lane = ln * p.s_ss;
+    // The table's entries of a unit: the wavefront's blocks', and of the lane's own key.  They are on their way while the unit before is worked on.
+    struct Entries { int page[kBlocks], own; } next;
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+      int slot;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        const int key = key0 + 16 * i;
-        int slot = 0, page = -1;
-        if (key < s.len) page = uniform_load(table, p.g.by_page.quotient(key, slot));
-        mult[i] = p.scale_log2;
+        const int key = t * UNIT + 16 * i;
+        next.page[i] = uniform_load(table, p.g.by_page.quotient(key < s.len ? key : s.len - 1, slot));
+      }
+      const int own = t * UNIT + lane;
+      next.own = table[p.g.by_page.quotient(own < s.len ? own : s.len - 1, slot)];
+    };
+    look_up(t0);
+    for (int t = t0; t < t0 + run; ++t) {
+      const int key0 = t * UNIT;
+      const Entries here = next;
+      // (all loads go out before the first is waited for; a key that is not here reads one that is, and its sum goes nowhere)
+      u32x4 w4[kBlocks][KR];
+      float mult[kBlocks];
+      uint32_t scales[kBlocks];
 #pragma unroll
-        for (int u = 0; u < KR; ++u) w4[i][u] = u32x4{};
-        if ((uint32_t)page < (uint32_t)p.g.pages) {
-          const uint8_t* row = p.k + (int64_t)page * p.c_sp + (int64_t)(slot + ln) * p.c_ss + (int64_t)hk * p.c_sh;
-          const float* scale = p.k_scales + ((int64_t)page * p.s_sp + (int64_t)(slot + ln) * p.s_ss + (int64_t)hk * p.s_sh);
-          if constexpr (E2M1) {
-            if (k_block * 32 < p.D) {
-              if constexpr (COLS == 128) w4[i][0] = *reinterpret_cast<const u32x4*>(row + lg * 16);
-              else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(row + lg * 8);
-                w4[i][0][0] = x[0];
-                w4[i][0][1] = x[1];
-              }
-              mult[i] = e8m0(reinterpret_cast<const uint8_t*>(scale)[k_block]);
-            } else {
-              mult[i] = 1.f;
-            }
-          } else {
-            if constexpr (E4M3) mult[i] = *scale;
+      for (int i = 0; i < kBlocks; ++i) {
+        int slot;
+        p.g.by_page.quotient(key0 + 16 * i, slot);
+        const bool held = key0 + 16 * i < s.len && (uint32_t)here.page[i] < (uint32_t)p.g.pages;
+        const int64_t page = held ? here.page[i] : 0;
+        if (!held) slot = 0;
+        const uint8_t* row = p.k + (page * p.c_sp + (int64_t)slot * p.c_ss + (int64_t)hk * p.c_sh) + row_of_lane;
+        const float* scale = p.k_scales + (page * p.s_sp + (int64_t)slot * p.s_ss + (int64_t)hk * p.s_sh) + scale_of_lane;
+        if constexpr (E2M1) {
+          if constexpr (COLS == 128) w4[i][0] = *reinterpret_cast<const u32x4*>(row);
+          else {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(row);
+            w4[i][0] = u32x4{x[0], x[1], 0u, 0u};
+          }
+          scales[i] = *reinterpret_cast<const uint32_t*>(scale);
+        } else {
+          if constexpr (E4M3) scales[i] = *reinterpret_cast<const uint32_t*>(scale);
 #pragma unroll
-            for (int u = 0; u < KR; ++u)
-              if ((u * 4 + lg) * 16 < row_bytes(TYPE, p.D)) w4[i][u] = *reinterpret_cast<const u32x4*>(row + (u * 4 + lg) * 16);
+          for (int u = 0; u < KR; ++u) {
+            w4[i][u] = u32x4{};
+            if ((u * 4 + lg) * 16 < row_bytes(TYPE, p.D)) w4[i][u] = *reinterpret_cast<const u32x4*>(row + u * 64);
           }
         }
       }
       // the lane's own key, key0 + lane: what it had, and where it goes
       const int own = key0 + lane;
-      int own_slot = 0, own_page = -1;
-      if (lane < UNIT && own < s.len) own_page = table[p.g.by_page.quotient(own, own_slot)];
+      int own_slot;
+      p.g.by_page.quotient(own, own_slot);
+      const int own_page = lane < UNIT && own < s.len ? here.own : -1;
       const bool held = (uint32_t)own_page < (uint32_t)p.g.pages;
       float had = 0.f;
       if (held && reads_old && own < (s.n == 0 ? s.len : old_keys))
         had = decay * p.old[(int64_t)own_page * p.w_sp + (int64_t)own_slot * p.w_ss + (int64_t)hk * p.w_sh];
 
+      if (t + 1 < t0 + run) look_up(t + 1);
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {          // columns past the last are nothing
+        mult[i] = E4M3 ? __builtin_bit_cast(float, scales[i]) : p.scale_log2;
+        if constexpr (E2M1) {
+          mult[i] = k_block * 32 < p.D ? e8m0(scales[i] >> (k_block * 8) & 255u) : 1.f;
+          if (k_block * 32 >= p.D) w4[i][0] = u32x4{};
+        }
+      }
       float sum[kBlocks] = {};
       for (int row0 = 0; row0 < rows; row0 += ROWS) {
         const int row_end = row0 + ROWS < rows ? row0 + ROWS : rows;
@@ -238,7 +263,8 @@ constexpr int kFlush = 64;                       // steps whose weights are adde
 // Items of a sequence and K/V head: tiles of 256 keys.  A query tile is 32 / F tokens of F heads, F a power of two, so that short chunks of
 // grouped heads fill it too; heads past the last of a K/V head are masked.  F grows while the query tiles become no more and a group of heads
 // has less than four.  (us, one head to a tile / so: 8 x 4000 keys, 16 tokens of 16 heads on one 33.0 / 17.9, one token of 64 89.2 / 16.8;
-// 84 x 1300, up to 16 tokens of seven heads on one 249 / 157; a prompt of 8192 tokens H32/8, which has tiles enough, 274 / 280.)  Key tile k is seen by the query tiles from max(0, 8 F k + z) on (all, without a mask), of each group of heads.
+// 84 x 1300, up to 16 tokens of seven heads on one 249 / 157; a prompt of 8192 tokens H32/8, which has tiles enough, 274 / 280.)  Key tile k is seen
+// by the query tiles from max(0, 8 F k + z) on (all, without a mask), of each group of heads.
 struct Steps {
   int tiles, queries, fold, groups, flat, z;     // key tiles, query tiles of a group, log2 F, groups; key tiles that all query tiles see
   int64_t all;                                   // of all key tiles
@@ -652,7 +678,7 @@ constexpr int64_t kManyBytes = (int64_t)kManyWorkers * (2 * kKeys * 4 + 16);
 
 template <int TYPE, int COLS, int NR>
 void launch_few(const Gather& p, hipStream_t st) {
-  hipLaunchKernelGGL((paged_weights_few<TYPE, COLS, NR>), dim3(256 * kFewWaves<NR>), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_weights_few<TYPE, COLS, NR>), dim3(256 * kFewWaves<TYPE, NR>), dim3(256), 0, st, p);
 }
 template <int TYPE, int COLS>
 void launch_rows(const Gather& p, int64_t rows, hipStream_t st) {
