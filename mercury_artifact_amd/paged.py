@@ -261,7 +261,8 @@ def paged_attn_weights(q: torch.Tensor, cache: torch.Tensor, page_table: torch.T
     nothing for the keys of the new tokens -- plus the key's weight in the attention of every new token that sees it, summed over the
     query heads of its K/V head.  ``q``, ``lse`` and the other arguments are those of ``paged_attn_fwd``; ``lse`` may be merged over the
     ranks that hold parts of a sequence.  Rows whose ``lse`` is -inf weigh nothing, sequences without new tokens keep their weights, and
-    entries that belong to no key are left as they are.  ``out``: takes the results in place of ``weights`` (and is returned)."""
+    entries that belong to no key are left as they are.  No two sequences of a call may share a page.  ``out``: takes the results in
+    place of ``weights`` (and is returned)."""
     done = N.host.paged_attn_weights(q, cache, page_table, lengths, softmax_scale, lse, weights, causal, scales, starts, most_new, decay, out)
     if done is not None:
         return done
@@ -305,7 +306,7 @@ def paged_cache_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: to
     last tokens and, of the others, those with the largest ``weights`` (NaN above all, of equal ones the first).  They move, in their
     order, with values, scales and weights, to the first rows of the sequence -- in its own pages, which no two sequences may share, or
     in those of ``out_table`` ``(B, at least limit / page_size)``, where the rows of sequences that are not cut go too; no page of it
-    may hold a sequence's rows.  Returns their old positions, ``kept`` ``(B, Hkv, limit)`` in int32 with -1 behind them, and the new
+    may hold a sequence's rows or be there twice.  Returns their old positions, ``kept`` ``(B, Hkv, limit)`` in int32 with -1 behind them, and the new
     lengths, ``left`` ``(B,)``; ``lengths`` itself is not written.  A sequence of which a page is not here is left as it is, with -1
     in all of ``kept``."""
     limit = keep if limit is None else limit

@@ -630,6 +630,48 @@ def test_on_other_streams_and_two_at_once():
         assert left.tolist() == n and kept.tolist() == stay
 
 
+def test_weights_of_two_prompts_at_once_on_two_streams():
+    """Each call has partial sums of its own."""
+    calls = []
+    for i, (lengths, new) in enumerate((([2100, 300], 300), ([900, 1700, 64], 64))):
+        s = Setting(torch.bfloat16, lengths, 2, 128, seed=50 + i)
+        q = torch.randn(len(lengths), new, 8, 128, generator=s.g).bfloat16().cuda()
+        _, lse = M.paged_attn_fwd(q, s.dev, *s.tables(), 0.1)
+        calls.append((s, q, lse, s.tables(), torch.zeros_like(s.weights)))
+    alone = [M.paged_attn_weights(q, s.dev, *tables, 0.1, lse, s.weights, out=torch.zeros_like(out)) for s, q, lse, tables, out in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for (s, q, lse, tables, out), stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                M.paged_attn_weights(q, s.dev, *tables, 0.1, lse, s.weights, out=out)
+    torch.cuda.synchronize()
+    for (*_, out), want in zip(calls, alone):
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("lengths,page", [([1999, 63, 5000], 48), ([8300, 17000, 300], 64), ([33100, 40007], 112)])
+def test_which_positions_stay_whatever_the_strides(lengths, page):
+    """Weights that lie by tokens, inside a wider tensor, and pages that end inside a wavefront's run of positions."""
+    g = torch.Generator().manual_seed(page)
+    counts = [-(-n // page) for n in lengths]
+    pages, keep, recent = sum(counts), 200, 37
+    order = torch.randperm(pages, generator=g).tolist()
+    table = [order[sum(counts[:b]):sum(counts[:b + 1])] for b in range(len(lengths))]
+    wide = torch.randn(pages, page + 1, 5, generator=g).cuda()
+    weights = wide[:, 1:, 1:4:2]
+    assert weights.stride() == ((page + 1) * 5, 5, 2)
+    cache, _ = M.paged_cache(pages, page, 2, 8)
+    cache.zero_()
+    want, left = P.evicted(weights.cpu(), table, lengths, pages, keep, recent)
+    rows = _ints([row + [-1] * (max(counts) - len(row)) for row in table])
+    kept, now = M.paged_cache_evict(cache, rows, _ints(lengths), weights, keep, recent=recent)
+    assert now.tolist() == left
+    for b, n in enumerate(left):
+        for h in range(2):
+            assert kept[b, h, :n].tolist() == want[b][h] and (kept[b, h, n:] == -1).all()
+
+
 def test_the_interpreters_path_gives_the_same(monkeypatch):
     def run():
         s = Setting(E2M1, [140, 95], 2, 64, seed=3, spare=20)
