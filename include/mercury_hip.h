@@ -411,7 +411,8 @@ int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache,
  * and came out of mhip_paged_attn_fwd, or an lse merged over the parts of a sequence.  Rows with lse = -inf weigh nothing.  A
  * sequence without new tokens keeps its weights.  decay: 0 (weights are not read then) or a finite positive number.  Entries that belong
  * to no key stay as they are.  No two sequences of a call may share a page (each would write its entries).  most_new as for
- * mhip_paged_attn_fwd.  `workspace`: 16-byte aligned,
+ * mhip_paged_attn_fwd; with the same one, scores are rounded as its are: e4m3 keys times their scales to bf16 for sequences with many new tokens
+ * (exact for powers of two; not where q_ss passes 2^23), in fp32 for the others.  `workspace`: 16-byte aligned,
  * mhip_paged_attn_weights_workspace_bytes(n, T, most_new, whether there are starts, Hq, Hkv) bytes of device memory (may be NULL where
  * that is 0); calls that overlap in time need one each.
  */

@@ -82,6 +82,11 @@ __device__ __forceinline__ u32x4 e2m1_to_bf16(uint32_t codes, float scale) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
 }
 
+// Rows (new tokens times query heads) of a sequence and K/V head that the kernels for few rows take, attention's and weights' alike, and the tile
+// of 16, 32 or 64 that holds so many.
+constexpr int kFewRows = 64;
+constexpr int few_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
 // What the entry points ask of tables, lengths and starts, and of the cache: MHIP_OK, or the code to return.
 int paged_geometry(PagedGeom& g, const int* table, const int* lengths, const int* starts, int64_t t_sb, int B, int n, int T, int pages,
                    int page, int width);

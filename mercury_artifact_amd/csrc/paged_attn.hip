@@ -35,7 +35,6 @@ template <int TYPE, int COLS, int NR>
 constexpr int kRingOf = NR == 1 && row_bytes(TYPE, COLS) <= 128 ? 16384 : 32768;
 constexpr int kNoColumn = 0x7fff0000;      // vector offset out of every descriptor's range (spans stay below 2^30)
 constexpr int kWavefronts = 1024;          // of a launch with rings of 32 KB: four on a CU, in workgroups of four or two
-constexpr int kFewRows = 64;               // rows of a sequence and K/V head that paged_attn_few takes, else paged_attn_chunk
 
 // Row tiles of a sequence and K/V head, units of each, and what an item counts for: its units behind `pause` more, the time in which a
 // workgroup that enters it does not read.  Without it a workgroup with many short items ends last; where there are fewer items than
@@ -589,7 +588,7 @@ __global__ __launch_bounds__(WAVES * 64, (32768 / kRingOf<TYPE, COLS, NR>)) void
 }
 
 // Tiles of 16, 32 or 64 rows: the least that holds the rows of a sequence with `most` new tokens.
-int row_blocks(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int row_blocks(int64_t rows) { return few_tile(rows) / 16; }
 // Workgroups of four wavefronts, one to a CU, or of two, two to a CU: the pair covers the one's pauses between items (Q, the first tiles,
 // the wavefronts' results) with the other's reading, and costs twice as many partial results.  Items to a workgroup decide; us, four / two:
 //   items   8: 1 x 131072 H32/8 88.0 / 89.4, e4m3 57.5 / 61.2, 8 tokens at 32768 33.1 / 37.8    16: 8 x 8192 H16/2 D64 e4m3 16.9 / 20.8
@@ -698,7 +697,7 @@ extern "C" int mhip_paged_attn_fwd(const void* q, const void* k_cache, const voi
   } else {
     // Packed sequences may be of either kind, such as generate a token at a time and such as take a chunk: two pairs of launches, one
     // after the other on the stream, share the workspace.
-    p.few_rows = starts && p.G <= kFewRows ? 16 * row_blocks(p.G) : -1;
+    p.few_rows = starts && p.G <= kFewRows ? few_tile(p.G) : -1;
     if (p.few_rows > 0) launch(p, dtype, p.few_rows, st);
     paged_attn_chunk_launch(p, dtype, st);
   }

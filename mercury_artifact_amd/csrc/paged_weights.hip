@@ -40,6 +40,7 @@ struct Gather {
   int Hkv, G, D, causal;
   float scale_log2, decay;
   Divisor by_group;
+  int few_rows;                                  // sequences of up to so many rows are paged_weights_few's, the others paged_weights_many's
   int most_fold;                                 // paged_weights_many: log2 of the heads that a query tile may have
   float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
 };
@@ -53,7 +54,9 @@ template <int TYPE, int NR>
 constexpr int kBlocksOf = TYPE == MHIP_BF16 || NR == 4 ? 2 : 4;      // 16-key blocks of a unit
 
 template <int UNIT>
-__device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) { return (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv; }
+__device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) {
+  return s.n * p.G > p.few_rows ? 0 : (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv;
+}
 
 template <int TYPE, int COLS, int NR>
 __global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(const Gather p) {
@@ -91,7 +94,7 @@ __global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(
 
   while (lo < hi) {
     const PagedSeq s = paged_seq<true>(p.g, b);
-    const int tiles = (s.len + UNIT - 1) / UNIT, rows = s.n * p.G;
+    const int rows = s.n * p.G, tiles = rows > p.few_rows ? 0 : (s.len + UNIT - 1) / UNIT;
     if (tiles == 0 || pos >= (int64_t)tiles * p.Hkv) {
       pos -= (int64_t)tiles * p.Hkv;
       ++b;
@@ -270,7 +273,7 @@ struct Steps {
   int64_t all;                                   // of all key tiles
   __device__ __forceinline__ Steps() {}
   __device__ __forceinline__ Steps(const Gather& p, const PagedSeq& s) {
-    tiles = (s.len + kKeys - 1) / kKeys;
+    tiles = s.n * p.G > p.few_rows ? (s.len + kKeys - 1) / kKeys : 0;
     auto tiles_of = [&](int f) { return (int)((((int64_t)s.n << f) + kQueries - 1) / kQueries); };
     auto groups_of = [&](int f) { return (p.G + (1 << f) - 1) >> f; };
     fold = 0;
@@ -468,7 +471,7 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
           if constexpr (TYPE == MHIP_E2M1) {
             x = e2m1_to_bf16(c[0], e8m0(scales[kb] >> (ks / 2 * 8) & 255u));
           } else if constexpr (TYPE == MHIP_E4M3) {
-            // (times the scale, rounded to bf16: exact for powers of two, and what attention of such prompts takes)
+            // (times the scale, rounded to bf16: exact for powers of two, and what attention takes for the sequences that come here, see few_rows_of)
             const float scale = __builtin_bit_cast(float, scales[kb]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -673,7 +676,6 @@ void launch_many(const Gather& p, hipStream_t st) {
   hipLaunchKernelGGL(paged_weights_join, dim3(kManyWorkers), dim3(kKeys), 0, st, p);
 }
 
-constexpr int kFewRows = 64;                     // rows of a sequence and K/V head that paged_weights_few takes
 constexpr int64_t kManyBytes = (int64_t)kManyWorkers * (2 * kKeys * 4 + 16);
 
 template <int TYPE, int COLS, int NR>
@@ -686,11 +688,23 @@ void launch_rows(const Gather& p, int64_t rows, hipStream_t st) {
   else if (rows <= 32) launch_few<TYPE, COLS, 2>(p, st);
   else launch_few<TYPE, COLS, 4>(p, st);
 }
+
+// Which sequences are paged_weights_few's: all up to kFewRows rows, else none, but of packed e4m3 those whose attention takes the keys' scales in
+// fp32, so that every sequence's scores are those that its lse was made of.  (Another launch, and generating sequences in the form that reads keys
+// once.  us, all with paged_weights_many / so: two short sequences 11.5 / 17.2, 16 of 600 .. 8192 keys H32/4 D96 that take 1 .. 512 tokens 122 / 112, 84 x 1300
+// H112/16 up to 16 tokens 166 / 138, eight prompts of 1500 .. 2500 H32/8 212 / 208.  The other formats' keys are exact in both.)
+int few_rows_of(const Gather& p, int64_t rows, int dtype, bool packed) {
+  if (rows <= kFewRows || p.q_ss > kFarRows) return 0x7fffffff;
+  return packed && dtype == MHIP_E4M3 && p.G <= kFewRows ? few_tile(p.G) : -1;
+}
 template <int TYPE>
 void launch(const Gather& p, int64_t rows, hipStream_t st) {
-  if (rows > kFewRows && p.q_ss <= kFarRows) launch_many<TYPE>(p, st);
-  else if (p.D <= 64) launch_rows<TYPE, 64>(p, rows, st);
-  else launch_rows<TYPE, 128>(p, rows, st);
+  if (p.few_rows > 0) {
+    const int64_t few = p.few_rows < rows ? p.few_rows : rows;
+    if (p.D <= 64) launch_rows<TYPE, 64>(p, few, st);
+    else launch_rows<TYPE, 128>(p, few, st);
+  }
+  if (p.few_rows < 0x7fffffff) launch_many<TYPE>(p, st);
 }
 
 }  // namespace
@@ -741,6 +755,7 @@ extern "C" int mhip_paged_attn_weights(const void* q, const void* k_cache, const
   p.decay = decay;
   p.by_group = Divisor(p.G);
   const int64_t rows = (int64_t)most_new * p.G;
+  p.few_rows = few_rows_of(p, rows, dtype, starts != nullptr);
   if (rows > kFewRows) {
     if (!workspace) return MHIP_EINVAL;
     if (!aligned16(workspace)) return MHIP_EALIGN;

@@ -261,8 +261,9 @@ def paged_attn_weights(q: torch.Tensor, cache: torch.Tensor, page_table: torch.T
     nothing for the keys of the new tokens -- plus the key's weight in the attention of every new token that sees it, summed over the
     query heads of its K/V head.  ``q``, ``lse`` and the other arguments are those of ``paged_attn_fwd``; ``lse`` may be merged over the
     ranks that hold parts of a sequence.  Rows whose ``lse`` is -inf weigh nothing, sequences without new tokens keep their weights, and
-    entries that belong to no key are left as they are.  No two sequences of a call may share a page.  ``out``: takes the results in
-    place of ``weights`` (and is returned)."""
+    entries that belong to no key are left as they are.  No two sequences of a call may share a page.  Scores are rounded as those of
+    ``paged_attn_fwd`` with the same ``most_new``: where that rounds a row times its scale to bfloat16 (exact for powers of two), this does, too.
+    ``out``: takes the results in place of ``weights`` (and is returned)."""
     done = N.host.paged_attn_weights(q, cache, page_table, lengths, softmax_scale, lse, weights, causal, scales, starts, most_new, decay, out)
     if done is not None:
         return done
