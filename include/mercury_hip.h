@@ -410,7 +410,7 @@ int mhip_paged_attn_fwd(const void* q, const void* k_cache, const void* v_cache,
  * over the new tokens that see it (mask as for mhip_paged_attn_fwd) and the query heads of its K/V head; q and lse as they went into
  * and came out of mhip_paged_attn_fwd, or an lse merged over the parts of a sequence.  Rows with lse = -inf weigh nothing.  A
  * sequence without new tokens keeps its weights.  decay: 0 (weights are not read then) or a finite positive number.  Entries that belong
- * to no key stay as they are.  No two sequences of a call may share a page (each would write its entries).  most_new as for
+ * to no key stay as they are.  No two sequences of a call may share a page, nor one have it twice (each would write its entries).  most_new as for
  * mhip_paged_attn_fwd; with the same one, scores are rounded as its are: e4m3 keys times their scales to bf16 for sequences with many new tokens
  * (exact for powers of two; not where q_ss passes 2^23), in fp32 for the others.  `workspace`: 16-byte aligned,
  * mhip_paged_attn_weights_workspace_bytes(n, T, most_new, whether there are starts, Hq, Hkv) bytes of device memory (may be NULL where
@@ -433,7 +433,10 @@ int mhip_paged_attn_weights(const void* q, const void* k_cache, const void* k_sc
  * sequence of which some page is not here stays as it is (left its length, kept -1).  out_table NULL: in the sequences' own pages,
  * which no two sequences may share.  Else out_table (B, out_pages), stride ot_sb, names the pages that all kept rows go to, also those
  * of sequences that are not cut; out_pages * page_size >= limit, none of them may be in page_table up to a sequence's length or be named
- * twice, and rows of entries outside [0, pages) are dropped.  weights as for mhip_paged_attn_weights.
+ * twice, and rows of entries outside [0, pages) are dropped.  weights as for mhip_paged_attn_weights.  A sequence that stays as it is for a page
+ * that is not here has no rows in out_table's pages: its rows are where they were (kept tells: -1 in all of it).
+ * MHIP_EUNSUPPORTED before anything is launched: limit past 0x7fff0000, B * Hkv from 2^22 on, and with out_table B * Hkv * ceil(limit / t) from 2^23
+ * on, where t is 256 for rows of the cache of up to 64 bytes, 128 up to 128, else 64.
  */
 int mhip_paged_cache_evict(void* k_cache, void* v_cache, void* k_scales, void* v_scales, const int* page_table, const int* out_table,
                            const int* lengths, float* weights, int* kept, int* left,

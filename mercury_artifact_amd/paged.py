@@ -309,7 +309,7 @@ def paged_cache_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: to
     in those of ``out_table`` ``(B, at least limit / page_size)``, where the rows of sequences that are not cut go too; no page of it
     may hold a sequence's rows or be there twice.  Returns their old positions, ``kept`` ``(B, Hkv, limit)`` in int32 with -1 behind them, and the new
     lengths, ``left`` ``(B,)``; ``lengths`` itself is not written.  A sequence of which a page is not here is left as it is, with -1
-    in all of ``kept``."""
+    in all of ``kept``: it has no rows in the pages of ``out_table`` either, so it goes on with its row of ``page_table``."""
     limit = keep if limit is None else limit
     done = N.host.paged_cache_evict(cache, page_table, lengths, weights, keep, recent, limit, scales, out_table)
     if done is not None:
