@@ -40,9 +40,9 @@ struct Gather {
   int Hkv, G, D, causal;
   float scale_log2, decay;
   Divisor by_group;
-  int few_rows;                                  // sequences of up to so many rows are paged_weights_few's, the others paged_weights_many's
   int most_fold;                                 // paged_weights_many: log2 of the heads that a query tile may have
   float* parts; int* shared;                     // paged_weights_many: two partial results of each workgroup; items that begin in it and end elsewhere
+  int few_rows;                                  // sequences of up to so many rows are paged_weights_few's, the others paged_weights_many's
 };
 
 // Wavefronts on a SIMD: four where there are registers for them; units of e4m3 take more (us, four / three: 4 x 131072 H32/8 154 / 131,
@@ -53,9 +53,12 @@ constexpr int kFewWaves = NR > 1 ? 2 : TYPE == MHIP_E4M3 ? 3 : 4;
 template <int TYPE, int NR>
 constexpr int kBlocksOf = TYPE == MHIP_BF16 || NR == 4 ? 2 : 4;      // 16-key blocks of a unit
 
-template <int UNIT>
+// Whether a sequence has few rows: asked where a call's sequences may be of both kinds, in e4m3 (see few_rows_of).
+__device__ __forceinline__ bool is_few(const Gather& p, const PagedSeq& s) { return s.n * p.G <= p.few_rows; }
+
+template <int TYPE, int UNIT>
 __device__ __forceinline__ int64_t units_of(const Gather& p, const PagedSeq& s) {
-  return s.n * p.G > p.few_rows ? 0 : (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv;
+  return TYPE != MHIP_E4M3 || is_few(p, s) ? (int64_t)((s.len + UNIT - 1) / UNIT) * p.Hkv : 0;
 }
 
 template <int TYPE, int COLS, int NR>
@@ -71,7 +74,7 @@ __global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(
   const int per = (p.g.B + 63) / 64;
   int64_t mine = 0;
   for (int j = 0; j < per; ++j)
-    if (lane * per + j < p.g.B) mine += units_of<UNIT>(p, paged_seq<false>(p.g, lane * per + j));
+    if (lane * per + j < p.g.B) mine += units_of<TYPE, UNIT>(p, paged_seq<false>(p.g, lane * per + j));
   int64_t before = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -86,7 +89,7 @@ __global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(
   const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo >= before && lo < before + mine));
   int b = owner * per;
   int64_t pos = lo - uniform64(__shfl((long long)before, owner));        // inside sequence b
-  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<UNIT>(p, paged_seq<true>(p.g, b))); ++b) pos -= u;
+  for (int64_t u; b + 1 < p.g.B && pos >= (u = units_of<TYPE, UNIT>(p, paged_seq<true>(p.g, b))); ++b) pos -= u;
 
   const int k_block = COLS == 128 ? lg : lg >> 1;                        // (e2m1: the 32 columns that the lane's are of)
   auto col_of = [&](int ks) { return E2M1 ? (lg * KB + ks) * 8 : E4M3 ? (ks >> 1) * 64 + lg * 16 + (ks & 1) * 8 : ks * 32 + lg * 8; };
@@ -94,9 +97,10 @@ __global__ __launch_bounds__(256, (kFewWaves<TYPE, NR>)) void paged_weights_few(
 
   while (lo < hi) {
     const PagedSeq s = paged_seq<true>(p.g, b);
-    const int rows = s.n * p.G, tiles = rows > p.few_rows ? 0 : (s.len + UNIT - 1) / UNIT;
-    if (tiles == 0 || pos >= (int64_t)tiles * p.Hkv) {
-      pos -= (int64_t)tiles * p.Hkv;
+    const int tiles = (s.len + UNIT - 1) / UNIT, rows = s.n * p.G;
+    const bool here = !E4M3 || is_few(p, s);
+    if (!here || tiles == 0 || pos >= (int64_t)tiles * p.Hkv) {
+      if (here) pos -= (int64_t)tiles * p.Hkv;
       ++b;
       continue;
     }
@@ -273,7 +277,7 @@ struct Steps {
   int64_t all;                                   // of all key tiles
   __device__ __forceinline__ Steps() {}
   __device__ __forceinline__ Steps(const Gather& p, const PagedSeq& s) {
-    tiles = s.n * p.G > p.few_rows ? (s.len + kKeys - 1) / kKeys : 0;
+    tiles = (s.len + kKeys - 1) / kKeys;
     auto tiles_of = [&](int f) { return (int)((((int64_t)s.n << f) + kQueries - 1) / kQueries); };
     auto groups_of = [&](int f) { return (p.G + (1 << f) - 1) >> f; };
     fold = 0;
@@ -341,7 +345,10 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
   const int per = (p.g.B + 63) / 64;
   int64_t mine = 0;
   for (int j = 0; j < per; ++j)
-    if (lane * per + j < p.g.B) mine += Steps(p, paged_seq<false>(p.g, lane * per + j)).all * p.Hkv;
+    if (lane * per + j < p.g.B) {
+      const PagedSeq s = paged_seq<false>(p.g, lane * per + j);
+      if (TYPE != MHIP_E4M3 || !is_few(p, s)) mine += Steps(p, s).all * p.Hkv;
+    }
   int64_t before = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -376,6 +383,7 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void paged_weights_many(const G
     if (enters) {                                // sequence b, `pos` units behind its first
       s = paged_seq<true>(p.g, b);
       st = Steps(p, s);
+      if (TYPE == MHIP_E4M3 && is_few(p, s)) st.all = 0;
       if (pos >= st.all * p.Hkv) {
         pos -= st.all * p.Hkv;
         ++b;
@@ -691,8 +699,8 @@ void launch_rows(const Gather& p, int64_t rows, hipStream_t st) {
 
 // Which sequences are paged_weights_few's: all up to kFewRows rows, else none, but of packed e4m3 those whose attention takes the keys' scales in
 // fp32, so that every sequence's scores are those that its lse was made of.  (Another launch, and generating sequences in the form that reads keys
-// once.  us, all with paged_weights_many / so: two short sequences 11.5 / 17.2, 16 of 600 .. 8192 keys H32/4 D96 that take 1 .. 512 tokens 122 / 112, 84 x 1300
-// H112/16 up to 16 tokens 166 / 138, eight prompts of 1500 .. 2500 H32/8 212 / 208.  The other formats' keys are exact in both.)
+// once.  us, all with paged_weights_many / so: two short sequences 11.5 / 17.2, 16 of 600 .. 8192 keys H32/4 D96 that take 1 .. 512 tokens 122 / 110, 84 x 1300
+// H112/16 up to 16 tokens 165 / 132, eight prompts of 1500 .. 2500 H32/8 210 / 214.  The other formats' keys are exact in both.)
 int few_rows_of(const Gather& p, int64_t rows, int dtype, bool packed) {
   if (rows <= kFewRows || p.q_ss > kFarRows) return 0x7fffffff;
   return packed && dtype == MHIP_E4M3 && p.G <= kFewRows ? few_tile(p.G) : -1;
