@@ -164,6 +164,9 @@ def test_weights_of_a_prompt_with_hundreds_of_steps_to_a_workgroup(kind, D, Hq, 
     (E2M1, _spread(900, 1500, 100), _spread(12, 30, 100, 0.414214), 32, 4, 96, True, 1.0),      # tiles of several heads, of 3 to 5 steps
     (E2M1, _spread(2000, 5000, 24), [900 if b % 3 else 1 for b in range(24)], 12, 4, 128, True, 0.0),
     (BF16, [6000, 6000, 6000], [700, 700, 700], 14, 2, 64, False, 1.0),
+    (E4M3, _spread(2000, 5000, 24), [900 if b % 3 else 1 for b in range(24)], 12, 4, 128, True, 0.5),            # divided among both kernels
+    (E4M3, _spread(300, 9000, 150), [200 if b % 4 == 0 else b % 6 for b in range(150)], 32, 4, 96, True, 1.0),
+    (E4M3, _spread(300, 9000, 100), [70 if b % 9 == 0 else b % 3 for b in range(100)], 48, 2, 64, False, 0.0),
 ])
 def test_weights_of_many_items_to_a_workgroup(kind, lengths, new, Hq, Hkv, D, causal, decay):
     print(f"case {kind} H{Hq}/{Hkv} D{D} causal {causal}", flush=True)
